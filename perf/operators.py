@@ -330,12 +330,12 @@ def _own(s):
             capi.check(lib.fz_expert_combine_backward(at(out["drows"]), at(out["dw"]), at(s["dout"]), at(s["rows_in"]), at(s["w"]), at(s["slot"]), at(s["src"]), t, k, r, d, stream))
         return out
     z, r, v, k, tlse = s["z"], s["rows"], s["vocab"], s["k"], s.get("tlse")
-    loss, lse, tail = new(r), new(r), new(r) if s["tail"] else None
-    capi.check(lib.fz_distill(at(loss), at(lse), at(tail), at(z), v, at(s["ids"]), at(s["t"]), at(tlse), r, v, k, s["temp"], stream))
+    loss, stats = new(r), new(r, 4)
+    capi.check(lib.fz_distill(at(loss), at(stats), at(z), v, at(s["ids"]), at(s["t"]), at(tlse), r, v, k, s["temp"], stream))
     if not s["grad"]:
         return {"loss": loss}
     dz = torch.empty_like(z)
-    capi.check(lib.fz_distill_backward(at(dz), v, at(s["dloss"]), at(lse), at(tail), at(z), v, at(s["ids"]), at(s["t"]), at(tlse), r, v, k, s["temp"], stream))
+    capi.check(lib.fz_distill_backward(at(dz), v, at(s["dloss"]), at(stats), at(z), v, at(s["ids"]), at(s["t"]), at(tlse), r, v, k, s["temp"], stream))
     return {"loss": loss, "dz": dz}
 
 
