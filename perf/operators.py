@@ -271,7 +271,7 @@ def _distill(s):
     if s["grad"]:
         dz = mass[:, None] * torch.exp(z / tau - lse)
         if s["tail"]:
-            dz = dz - torch.where(some_tail[:, None], p_tail[:, None] * torch.exp(outside / tau - tail_lse), torch.zeros_like(lse))
+            dz = dz - torch.where(some_tail[:, None], p_tail[:, None] * torch.exp(outside / tau - tail_lse).masked_fill(inside, 0.0), torch.zeros_like(lse))
         dz = dz.scatter_add(1, at, torch.where(valid, -p, zero))
         out["dz"] = torch.where(some[:, None], (tau * s["dloss"])[:, None] * dz, torch.zeros_like(lse))
     return out
@@ -457,7 +457,7 @@ def _exact_distill(s):
         outside = torch.where(torch.isinf(spread), logq, torch.full_like(logq, -math.inf))
         log_rest = torch.logsumexp(outside, 1)
         loss = loss + torch.where(rest > 0, rest * (torch.log(rest) - log_rest), torch.zeros_like(rest))
-        dz = dz + rest[:, None] * (q - torch.where((rest > 0)[:, None], torch.exp(outside - log_rest[:, None]), torch.zeros_like(q)))
+        dz = dz + rest[:, None] * (q - torch.where((rest > 0)[:, None] & torch.isinf(spread), torch.exp(outside - log_rest[:, None]), torch.zeros_like(q)))
     zero = torch.zeros((), dtype=torch.float64, device=z.device)
     out = {"loss": torch.where(some, tau * tau * loss, zero)}
     if s["grad"]:
