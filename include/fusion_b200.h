@@ -381,6 +381,125 @@ int fz_philox_uniform(float *out, int64_t n, uint64_t seed, uint64_t offset, flo
 int fz_philox_dropout(float *out, const float *x, int64_t n, float rate, float keep, uint64_t seed,
                       uint64_t offset, void *stream);
 
+/* ---- normalisation ---------------------------------------------------------- */
+
+/* Activation that fz_group_norm applies to its result v: v itself, v > 0 ? v : 0 (Nova's
+ * ReLU, maximum(0): a NaN gives 0), v / (1 + exp(-v)), or v * Phi(v) with the normal
+ * distribution's Phi (erf form). */
+enum fz_activation { FZ_ACT_NONE = 0, FZ_ACT_RELU = 1, FZ_ACT_SILU = 2, FZ_ACT_GELU = 3 };
+
+/* Group norm with an activation over channels-last data (Nova's activations are
+ * [batch, ..., features]); no reference counterpart. x is a contiguous
+ * [batch, len, channels] view, its channels in `groups` groups of c = channels / groups
+ * (channels a multiple of groups). Per (b, g), over the len * c values: mean, biased
+ * variance var, rstd = 1 / sqrt(var + eps); y = act(gamma * (x - mean) * rstd + beta).
+ * gamma / beta hold `channels` values; NULL means ones / zeros. mean and rstd
+ * ([batch, groups], both or neither NULL) are written for the backward. Statistics are
+ * held in fp32 and joined by mean and centred sum of squares, so a large common offset
+ * of x costs no digits beyond those x itself lost. y may not overlap x.
+ * workspace: at least fz_group_norm_workspace(..., backward = 0, ...) bytes, 16-byte
+ * aligned, free for reuse once the call's work on `stream` is done (calls that overlap
+ * need one each); NULL when that is 0. eps >= 0. */
+int fz_group_norm(float *y, float *mean, float *rstd, const float *x, const float *gamma,
+                  const float *beta, int64_t batch, int64_t len, int64_t channels, int64_t groups,
+                  float eps, int act, void *workspace, size_t workspace_bytes, void *stream);
+/* Gradients of fz_group_norm from dy and the mean and rstd it wrote:
+ * dv = dy * act'(v), a = dv * gamma, xh = (x - mean) * rstd,
+ * dx = rstd * (a - (sum a + xh * sum(a * xh)) / (len * c)), sums over (b, g);
+ * dgamma = sum dv * xh and dbeta = sum dv over batch and len (either may be NULL).
+ * Sums are in a fixed order: results do not depend on scheduling. dx may not overlap x
+ * or dy. Workspace as above with backward = 1. */
+int fz_group_norm_backward(float *dx, float *dgamma, float *dbeta, const float *dy, const float *x,
+                           const float *mean, const float *rstd, const float *gamma,
+                           const float *beta, int64_t batch, int64_t len, int64_t channels,
+                           int64_t groups, int act, void *workspace, size_t workspace_bytes,
+                           void *stream);
+/* Bytes of workspace that fz_group_norm (backward = 0) or fz_group_norm_backward (1) needs
+ * on the current device for these sizes (0: none). */
+int fz_group_norm_workspace(int64_t batch, int64_t len, int64_t channels, int64_t groups,
+                            int backward, size_t *bytes);
+
+/* ---- mixture of experts -------------------------------------------------------- */
+
+/* No reference counterpart. A token's k choices are ids[t * k + j], j < k; an id outside
+ * [0, experts) is no choice (padding). Row and choice numbers are int32: tokens * k and
+ * the number of rows stay below 2^31; offsets into the data are 64-bit. */
+#define FZ_MAX_EXPERTS 1024
+#define FZ_MAX_CHOICES 32 /* k of fz_route */
+
+/* The router's gate: per token the k largest of `experts` logits, largest first (ties:
+ * the lowest expert; NaN ranks above every number), and their weights: renormalize != 0,
+ * softmax over the chosen logits; 0, the softmax over all logits at the chosen ones. A
+ * logit of -inf is never chosen: where fewer than k others are left, the id is -1 and the
+ * weight 0. logits [tokens, experts], weights and ids [tokens, k]; 1 <= k <= experts,
+ * k <= FZ_MAX_CHOICES, experts <= FZ_MAX_EXPERTS. */
+int fz_route(float *weights, int32_t *ids, const float *logits, int64_t tokens, int64_t experts,
+             int64_t k, int renormalize, void *stream);
+/* dlogits [tokens, experts] from dweights, and the weights and ids that fz_route gave for
+ * these logits: renormalized, w * (dw - sum w dw) at the chosen experts and 0 elsewhere;
+ * else p * (dw at the chosen experts - sum w dw), p the softmax over all logits. */
+int fz_route_backward(float *dlogits, const float *dweights, const float *weights,
+                      const int32_t *ids, const float *logits, int64_t tokens, int64_t experts,
+                      int64_t k, int renormalize, void *stream);
+
+/* Sort the choices by expert, stably (token by token, choice by choice). Expert e's rows
+ * begin at offsets[e]: capacity = 0 packs them (rows = tokens * k, offsets[experts] = the
+ * number of choices, the rows behind it are empty); capacity > 0 gives every expert
+ * `capacity` rows (rows = experts * capacity, offsets[e] = e * capacity, the layout of a
+ * batched product over experts) and drops an expert's later choices once they are full.
+ * slot [tokens, k]: a choice's row, -1 if it has none; src [rows]: the choice t * k + j in
+ * a row, -1 if empty; counts [experts]: choices that named the expert, dropped ones
+ * included; offsets [experts + 1]. */
+int fz_expert_sort(int32_t *slot, int32_t *src, int32_t *counts, int32_t *offsets,
+                   const int32_t *ids, int64_t tokens, int64_t k, int64_t experts,
+                   int64_t capacity, void *stream);
+/* rows[slot[t, j]] = x[t]; rows that src marks empty are zeroed. x [tokens, width], rows
+ * [num_rows, width], slot and src as fz_expert_sort wrote them (a slot outside
+ * [0, num_rows) is passed over). Its gradient is fz_expert_combine without weights. */
+int fz_expert_dispatch(float *rows, const float *x, const int32_t *slot, const int32_t *src,
+                       int64_t tokens, int64_t k, int64_t num_rows, int64_t width, void *stream);
+/* out[t] = sum_j weights[t, j] * rows[slot[t, j]] over the choices that have a row, in the
+ * order of j (a token without any gives zeros). weights [tokens, k]; NULL means ones. */
+int fz_expert_combine(float *out, const float *rows, const float *weights, const int32_t *slot,
+                      int64_t tokens, int64_t k, int64_t num_rows, int64_t width, void *stream);
+/* Gradients of fz_expert_combine: drows[slot[t, j]] = weights[t, j] * dout[t], empty rows
+ * zeroed; dweights[t, j] = <dout[t], rows[slot[t, j]]>, 0 for a choice without a row. weights
+ * NULL means ones; dweights may be NULL (rows is then not read and may be NULL). */
+int fz_expert_combine_backward(float *drows, float *dweights, const float *dout,
+                               const float *rows, const float *weights, const int32_t *slot,
+                               const int32_t *src, int64_t tokens, int64_t k, int64_t num_rows,
+                               int64_t width, void *stream);
+
+/* ---- distillation ---------------------------------------------------------------- */
+
+#define FZ_MAX_TEACHER 1024 /* entries of a teacher's list */
+
+/* Distillation from a teacher's top logits; no reference counterpart (Nova's only loss is
+ * the mean squared error). Per row r: z = logits[r, 0..vocab) (row pitch ld >= vocab), the
+ * teacher's k entries (ids[r, i], teacher[r, i]); an entry whose id lies outside
+ * [0, vocab) is padding. With tau = temperature > 0, q = softmax(z / tau) and
+ *   teacher_lse NULL: p = softmax(teacher / tau) over the row's entries;
+ *   else: p = exp(teacher / tau - teacher_lse[r]) (the logsumexp of the teacher's whole
+ *   vocabulary over tau), the rest pT = max(0, 1 - sum p) on one bucket, against the
+ *   student's qT = sum of q outside the row's entries;
+ *   loss[r] = tau^2 * (sum_i p_i (log p_i - log q_i) + pT (log pT - log qT)),
+ * a term with p = 0 counting 0. A row without entries (with teacher_lse NULL also one whose
+ * entries are all -inf) has loss 0 whatever its logits hold. For the backward, stats
+ * [rows, 4] receives the maximum of z and log sum exp((z - max) / tau), then, with
+ * teacher_lse, the same two over the logits outside the entries.
+ * k <= FZ_MAX_TEACHER, vocab <= 2^23; an id named twice counts its p each time. */
+int fz_distill(float *loss, float *stats, const float *logits, int64_t ld, const int32_t *ids,
+               const float *teacher, const float *teacher_lse, int64_t rows, int64_t vocab,
+               int64_t k, float temperature, void *stream);
+/* dlogits (row pitch ldd >= vocab; columns from vocab on are left alone) from dloss [rows]
+ * and the stats that fz_distill wrote. With P = sum p + pT and c = tau * dloss[r]:
+ * c * (P q_v - sum of p of the entries that name v), and for v outside the entries
+ * c * (P - pT / qT) q_v; rows without entries get zeros. dlogits may not overlap logits. */
+int fz_distill_backward(float *dlogits, int64_t ldd, const float *dloss, const float *stats,
+                        const float *logits, int64_t ld, const int32_t *ids, const float *teacher,
+                        const float *teacher_lse, int64_t rows, int64_t vocab, int64_t k,
+                        float temperature, void *stream);
+
 /* ---- collectives (data-parallel MLP step) -------------------------------- */
 
 #define FZ_UNIQUE_ID_BYTES 128

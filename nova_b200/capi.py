@@ -22,6 +22,7 @@ FZ_MAX_NODES = 48
 FZ_MAX_OUTPUTS = 4
 
 BINOPS = {"add": 0, "sub": 1, "mul": 2, "div": 3, "pow": 4, "maximum": 5, "gt": 6, "ge": 7}
+ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3}
 UNOPS = {"exp": 0, "log": 1, "sqrt": 2, "copy": 3, "tf32_lo": 4}
 REDOPS = {"sum": 0, "mean": 1, "max": 2}
 NODE_BINARY, NODE_UNARY, NODE_CONST = 0, 1, 2
@@ -132,6 +133,18 @@ def lib() -> C.CDLL:
         L.fz_gemm_stats.argtypes = [C.POINTER(C.c_int64)]
         L.fz_gemm_timing.argtypes = [C.c_int]
         L.fz_gemm_timing_read.argtypes = [C.POINTER(GemmTimingRec), C.c_int, C.POINTER(C.c_int)]
+        sz = C.c_size_t
+        L.fz_group_norm.argtypes = [vp] * 6 + [i64] * 4 + [f, C.c_int, vp, sz, vp]
+        L.fz_group_norm_backward.argtypes = [vp] * 9 + [i64] * 4 + [C.c_int, vp, sz, vp]
+        L.fz_group_norm_workspace.argtypes = [i64] * 4 + [C.c_int, C.POINTER(sz)]
+        L.fz_route.argtypes = [vp] * 3 + [i64] * 3 + [C.c_int, vp]
+        L.fz_route_backward.argtypes = [vp] * 5 + [i64] * 3 + [C.c_int, vp]
+        L.fz_expert_sort.argtypes = [vp] * 5 + [i64] * 4 + [vp]
+        L.fz_expert_dispatch.argtypes = [vp] * 4 + [i64] * 4 + [vp]
+        L.fz_expert_combine.argtypes = [vp] * 4 + [i64] * 4 + [vp]
+        L.fz_expert_combine_backward.argtypes = [vp] * 7 + [i64] * 4 + [vp]
+        L.fz_distill.argtypes = [vp] * 3 + [i64] + [vp] * 3 + [i64] * 3 + [f, vp]
+        L.fz_distill_backward.argtypes = [vp, i64] + [vp] * 3 + [i64] + [vp] * 3 + [i64] * 3 + [f, vp]
         L.fz_comm_init.argtypes = [C.POINTER(C.c_void_p), C.c_int, C.c_int, C.c_char_p]
         L.fz_comm_allreduce.argtypes = [vp, vp, vp, i64, f, vp]
         L.fz_comm_broadcast.argtypes = [vp, vp, i64, C.c_int, vp]
@@ -213,6 +226,14 @@ def make_plan(out_shape, operand_shapes) -> EwisePlan:
         for d in range(nd):
             p.stride_bytes[k][d] = st[d]
     return p
+
+
+def group_norm_workspace(batch: int, length: int, channels: int, groups: int,
+                         backward: bool = False) -> int:
+    """Bytes of workspace a group norm call of these sizes needs (fz_group_norm_workspace)."""
+    n = C.c_size_t()
+    check(lib().fz_group_norm_workspace(batch, length, channels, groups, int(backward), C.byref(n)))
+    return n.value
 
 
 def gemm_timing_read(max_records: int = 4096) -> list:

@@ -1,0 +1,629 @@
+// Mixture of experts: the router's gate, tokens sorted by expert and back, and their
+// gradients. All are bound by memory (or, for a handful of tokens, by launch latency):
+// every kernel reads its inputs once and writes its outputs once, with no atomics on
+// floating-point values, so results do not depend on scheduling.
+#include <cooperative_groups.h>
+
+#include <climits>
+#include <cstdint>
+
+#include "fz_common.cuh"
+
+namespace cg = cooperative_groups;
+
+namespace {
+
+constexpr unsigned kFull = 0xffffffffu;
+
+bool aligned16(const void *a, const void *b = nullptr, const void *c = nullptr) {
+  return (((uintptr_t)a | (uintptr_t)b | (uintptr_t)c) & 15) == 0;
+}
+
+// ---------------------------------------------------------------- router
+
+// Logits as unsigned keys in the same order: NaN above all, -0 equal to +0, and 0 free
+// to mark what has been taken.
+__device__ __forceinline__ uint32_t order_key(float v) {
+  if (v != v) return 0xffffffffu;
+  const uint32_t u = __float_as_uint(__fadd_rn(v, 0.0f));
+  return u ^ ((u >> 31) ? 0xffffffffu : 0x80000000u);
+}
+constexpr uint32_t kKeyMinusInf = 0x007fffffu;
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) v = __fadd_rn(v, __shfl_xor_sync(kFull, v, d));
+  return v;
+}
+
+// One warp per token, expert e = lane + 32 i in register i of lane `lane`. Each pick is
+// two warp-wide integer reductions: the largest key, then the lowest expert that has it.
+template <int NE>
+__global__ void __launch_bounds__(256) route_kernel(float *__restrict__ weights, int32_t *__restrict__ ids,
+                                                    const float *__restrict__ logits, int64_t tokens, int experts,
+                                                    int k, int renormalize) {
+  pdl_wait();
+  const int lane = threadIdx.x & 31;
+  const int64_t warps = (int64_t)gridDim.x * (blockDim.x >> 5);
+  for (int64_t t = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); t < tokens; t += warps) {
+    const float *row = logits + t * experts;
+    float v[NE];
+    uint32_t key[NE];
+#pragma unroll
+    for (int i = 0; i < NE; ++i) {
+      const int e = lane + 32 * i;
+      v[i] = e < experts ? row[e] : 0.0f;
+      key[i] = e < experts ? order_key(v[i]) : 0u;
+    }
+    float mine = 0.0f;  // lane j: the j-th pick's logit
+    int my_id = -1;
+    for (int j = 0; j < k; ++j) {
+      uint32_t best = key[0];
+      int at = 0;
+#pragma unroll
+      for (int i = 1; i < NE; ++i)
+        if (key[i] > best) {
+          best = key[i];
+          at = i;
+        }
+      const uint32_t top = __reduce_max_sync(kFull, best);
+      if (top <= kKeyMinusInf) break;  // only -inf (or nothing) left
+      const int e = (int)__reduce_min_sync(kFull, best == top ? (unsigned)(lane + 32 * at) : 0xffffffffu);
+      const int owner = e & 31, slot = e >> 5;
+      float picked = 0.0f;
+#pragma unroll
+      for (int i = 0; i < NE; ++i)
+        if (i == slot) {
+          picked = v[i];
+          if (lane == owner) key[i] = 0u;
+        }
+      picked = __shfl_sync(kFull, picked, owner);
+      if (lane == j) {
+        mine = picked;
+        my_id = e;
+      }
+    }
+    const float top = __shfl_sync(kFull, mine, 0);
+    const float num = my_id >= 0 ? expf(__fsub_rn(mine, top)) : 0.0f;
+    float den;
+    if (renormalize) {
+      den = warp_sum(num);
+    } else {
+      float s = 0.0f;
+#pragma unroll
+      for (int i = 0; i < NE; ++i)
+        if (lane + 32 * i < experts) s = __fadd_rn(s, expf(__fsub_rn(v[i], top)));
+      den = warp_sum(s);
+    }
+    if (lane < k) {
+      weights[t * k + lane] = my_id >= 0 ? __fdiv_rn(num, den) : 0.0f;
+      ids[t * k + lane] = my_id;
+    }
+  }
+}
+
+// One warp per token; the chosen experts' upstream gradients are spread over a row in
+// shared memory, which the warp then turns into the row of dlogits.
+template <int NE>
+__global__ void __launch_bounds__(256) route_backward_kernel(float *__restrict__ dlogits,
+                                                             const float *__restrict__ dweights,
+                                                             const float *__restrict__ weights,
+                                                             const int32_t *__restrict__ ids,
+                                                             const float *__restrict__ logits, int64_t tokens,
+                                                             int experts, int k, int renormalize) {
+  pdl_wait();
+  __shared__ float rows[8][NE * 32];
+  const int lane = threadIdx.x & 31;
+  float *up = rows[threadIdx.x >> 5];
+  const int64_t warps = (int64_t)gridDim.x * (blockDim.x >> 5);
+  for (int64_t t = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); t < tokens; t += warps) {
+    int id = -1;
+    float w = 0.0f, dw = 0.0f;
+    if (lane < k) {
+      id = ids[t * k + lane];
+      if (id >= 0 && id < experts) {
+        w = weights[t * k + lane];
+        dw = dweights[t * k + lane];
+      } else {
+        id = -1;
+      }
+    }
+    const float dot = warp_sum(__fmul_rn(w, dw));
+    const bool any = __any_sync(kFull, id >= 0);
+#pragma unroll
+    for (int i = 0; i < NE; ++i) up[lane + 32 * i] = 0.0f;
+    __syncwarp();
+    if (id >= 0) up[id] = renormalize ? __fmul_rn(w, __fsub_rn(dw, dot)) : dw;
+    __syncwarp();
+    float *out = dlogits + t * experts;
+    if (renormalize || !any) {
+#pragma unroll
+      for (int i = 0; i < NE; ++i) {
+        const int e = lane + 32 * i;
+        if (e < experts) out[e] = up[e];
+      }
+    } else {
+      const float *row = logits + t * experts;
+      float v[NE], top = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < NE; ++i) {
+        const int e = lane + 32 * i;
+        v[i] = e < experts ? row[e] : -INFINITY;
+        top = fmaxf(top, v[i]);
+      }
+#pragma unroll
+      for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(kFull, top, d));
+      float s = 0.0f;
+#pragma unroll
+      for (int i = 0; i < NE; ++i) {
+        v[i] = expf(__fsub_rn(v[i], top));
+        s = __fadd_rn(s, v[i]);
+      }
+      const float den = warp_sum(s);
+#pragma unroll
+      for (int i = 0; i < NE; ++i) {
+        const int e = lane + 32 * i;
+        if (e < experts) out[e] = __fmul_rn(__fdiv_rn(v[i], den), __fsub_rn(up[e], dot));
+      }
+    }
+    __syncwarp();
+  }
+}
+
+// ---------------------------------------------------------------- sort by expert
+
+// One cluster sorts everything (a counting sort): each warp owns a contiguous run of
+// choices and counts them per expert in shared memory; the CTAs exchange their totals
+// through distributed shared memory; then each warp places its run, in order, from its
+// own first place per expert. Equal experts within a warp's 32 choices are ranked by
+// match_any, so the order is stable whatever the scheduling.
+__global__ void __launch_bounds__(1024) sort_kernel(int32_t *__restrict__ slot, int32_t *__restrict__ src,
+                                                    int32_t *__restrict__ counts, int32_t *__restrict__ offsets,
+                                                    const int32_t *__restrict__ ids, int n, int experts,
+                                                    int capacity, int rows, int per_warp) {
+  pdl_wait();
+  cg::cluster_group cluster = cg::this_cluster();
+  const int rank = (int)cluster.block_rank(), ctas = (int)cluster.num_blocks();
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nwarps = blockDim.x >> 5;
+  extern __shared__ int32_t sh[];
+  int32_t *hist = sh;                       // [nwarps][experts]: counts, then the next place in the expert
+  int32_t *total = sh + nwarps * experts;   // [experts]: this CTA's counts
+  int32_t *start = total + experts;         // [experts]: the expert's first row
+  int32_t *all = start + experts;           // [experts]: counts over the cluster
+  __shared__ int32_t scan[32];
+
+  for (int i = tid; i < nwarps * experts; i += blockDim.x) hist[i] = 0;
+  __syncthreads();
+  const int64_t first = ((int64_t)rank * nwarps + warp) * per_warp;
+  const int end = (int)(first + per_warp < n ? first + per_warp : n);
+  int32_t *mine = hist + warp * experts;
+  for (int64_t i = first + lane; i < end; i += 32) {
+    const int e = ids[i];
+    if (e >= 0 && e < experts) atomicAdd(&mine[e], 1);
+  }
+  __syncthreads();
+  // exclusive sums over this CTA's warps
+  for (int e = tid; e < experts; e += blockDim.x) {
+    int s = 0;
+    for (int w = 0; w < nwarps; ++w) {
+      const int c = hist[w * experts + e];
+      hist[w * experts + e] = s;
+      s += c;
+    }
+    total[e] = s;
+  }
+  cluster.sync();
+  // counts over the cluster, and those of the CTAs before this one
+  for (int e = tid; e < experts; e += blockDim.x) {
+    int s = 0, before = 0;
+    for (int r = 0; r < ctas; ++r) {
+      const int c = cluster.map_shared_rank(total, r)[e];
+      if (r < rank) before += c;
+      s += c;
+    }
+    all[e] = s;
+    start[e] = before;
+  }
+  // the experts' first rows: e * capacity, or the exclusive sum of the counts
+  // (experts <= 1024 = one value a thread over up to 1024 threads; fewer threads loop)
+  __syncthreads();
+  int carry = 0;
+  for (int e0 = 0; e0 < experts; e0 += blockDim.x) {
+    const int e = e0 + tid;
+    const int c = e < experts ? all[e] : 0;
+    int x = c;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int y = __shfl_up_sync(kFull, x, d);
+      if (lane >= d) x += y;
+    }
+    if (lane == 31) scan[warp] = x;
+    __syncthreads();
+    int before = 0, sum = 0;
+    for (int w = 0; w < nwarps; ++w) {
+      if (w < warp) before += scan[w];
+      sum += scan[w];
+    }
+    if (e < experts) {
+      const int begin = capacity ? e * capacity : carry + before + x - c;
+      const int ahead = start[e];
+      start[e] = begin;
+      for (int w = 0; w < nwarps; ++w) hist[w * experts + e] += ahead;
+      if (rank == 0) {
+        counts[e] = c;
+        offsets[e] = begin;
+      }
+    }
+    carry += sum;
+    __syncthreads();
+  }
+  if (rank == 0 && tid == 0) offsets[experts] = capacity ? experts * capacity : carry;
+  // empty rows
+  if (capacity) {
+    for (int r = rank * (int)blockDim.x + tid; r < rows; r += ctas * (int)blockDim.x)
+      if (r % capacity >= all[r / capacity]) src[r] = -1;
+  } else {
+    for (int r = carry + rank * (int)blockDim.x + tid; r < rows; r += ctas * (int)blockDim.x) src[r] = -1;
+  }
+  // places
+  for (int64_t i0 = first; i0 < end; i0 += 32) {
+    const int64_t i = i0 + lane;
+    int e = i < end ? ids[i] : -1;
+    if (e < 0 || e >= experts) e = -1;
+    const unsigned peers = __match_any_sync(kFull, e);
+    int at = -1;
+    if (e >= 0) {
+      at = mine[e] + __popc(peers & ((1u << lane) - 1u));
+      at = capacity && at >= capacity ? -1 : start[e] + at;
+    }
+    __syncwarp();
+    if (e >= 0 && lane == __ffs(peers) - 1) mine[e] += __popc(peers);
+    __syncwarp();
+    if (i < end) {
+      slot[i] = at;
+      if (at >= 0) src[at] = (int)i;
+    }
+  }
+  cluster.sync();  // no CTA leaves while another may read its totals
+}
+
+// ---------------------------------------------------------------- rows to experts and back
+
+// Work is cut into pieces of one token and kChunk vectors a lane; a warp takes a piece.
+// VEC = 4: rows of float4 (width a multiple of 4, 16-byte aligned buffers), else 1.
+constexpr int kUnroll = 4;
+
+template <int VEC>
+struct Vec;
+template <>
+struct Vec<4> {
+  using T = float4;
+  static __device__ __forceinline__ T zero() { return make_float4(0.0f, 0.0f, 0.0f, 0.0f); }
+  static __device__ __forceinline__ T fma(float w, T y, T a) {
+    return make_float4(__fmaf_rn(w, y.x, a.x), __fmaf_rn(w, y.y, a.y), __fmaf_rn(w, y.z, a.z),
+                       __fmaf_rn(w, y.w, a.w));
+  }
+  static __device__ __forceinline__ T scale(float w, T y) {
+    return make_float4(__fmul_rn(w, y.x), __fmul_rn(w, y.y), __fmul_rn(w, y.z), __fmul_rn(w, y.w));
+  }
+  static __device__ __forceinline__ float dot(T a, T b, float s) {
+    return __fmaf_rn(a.w, b.w, __fmaf_rn(a.z, b.z, __fmaf_rn(a.y, b.y, __fmaf_rn(a.x, b.x, s))));
+  }
+};
+template <>
+struct Vec<1> {
+  using T = float;
+  static __device__ __forceinline__ T zero() { return 0.0f; }
+  static __device__ __forceinline__ T fma(float w, T y, T a) { return __fmaf_rn(w, y, a); }
+  static __device__ __forceinline__ T scale(float w, T y) { return __fmul_rn(w, y); }
+  static __device__ __forceinline__ float dot(T a, T b, float s) { return __fmaf_rn(a, b, s); }
+};
+
+// Zero the piece [c0, c0 + 32 * kUnroll) of the empty ones among 32 rows from r0.
+template <int VEC>
+__device__ __forceinline__ void zero_empty(typename Vec<VEC>::T *rows, const int32_t *src, int64_t r0,
+                                           int64_t num_rows, int64_t nvec, int64_t c0, int lane) {
+  const int64_t r = r0 + lane;
+  unsigned empty = __ballot_sync(kFull, r < num_rows && src[r < num_rows ? r : 0] < 0);
+  while (empty) {
+    const int b = __ffs(empty) - 1;
+    empty &= empty - 1;
+    typename Vec<VEC>::T *row = rows + (r0 + b) * nvec;
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const int64_t c = c0 + u * 32 + lane;
+      if (c < nvec) row[c] = Vec<VEC>::zero();
+    }
+  }
+}
+
+template <int VEC>
+__global__ void __launch_bounds__(256) dispatch_kernel(typename Vec<VEC>::T *__restrict__ rows,
+                                                       const typename Vec<VEC>::T *__restrict__ x,
+                                                       const int32_t *__restrict__ slot,
+                                                       const int32_t *__restrict__ src, int64_t tokens, int64_t k,
+                                                       int64_t num_rows, int64_t nvec, int64_t chunks) {
+  using V = Vec<VEC>;
+  pdl_wait();
+  const int lane = threadIdx.x & 31;
+  const int64_t work = tokens * chunks, all = work + (num_rows + 31) / 32 * chunks;
+  const int64_t warps = (int64_t)gridDim.x * (blockDim.x >> 5);
+  for (int64_t p = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); p < all; p += warps) {
+    if (p >= work) {
+      const int64_t q = p - work, g = q / chunks;
+      zero_empty<VEC>(rows, src, g * 32, num_rows, nvec, (q - g * chunks) * 32 * kUnroll, lane);
+      continue;
+    }
+    const int64_t t = p / chunks, c0 = (p - t * chunks) * 32 * kUnroll;
+    typename V::T v[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const int64_t c = c0 + u * 32 + lane;
+      v[u] = c < nvec ? x[t * nvec + c] : V::zero();
+    }
+    for (int64_t j = 0; j < k; ++j) {
+      const int64_t r = slot[t * k + j];
+      if (r < 0 || r >= num_rows) continue;
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) {
+        const int64_t c = c0 + u * 32 + lane;
+        if (c < nvec) rows[r * nvec + c] = v[u];
+      }
+    }
+  }
+}
+
+template <int VEC>
+__global__ void __launch_bounds__(256) combine_kernel(typename Vec<VEC>::T *__restrict__ out,
+                                                      const typename Vec<VEC>::T *__restrict__ rows,
+                                                      const float *__restrict__ weights,
+                                                      const int32_t *__restrict__ slot, int64_t tokens, int64_t k,
+                                                      int64_t num_rows, int64_t nvec, int64_t chunks) {
+  using V = Vec<VEC>;
+  pdl_wait();
+  const int lane = threadIdx.x & 31;
+  const int64_t work = tokens * chunks, warps = (int64_t)gridDim.x * (blockDim.x >> 5);
+  for (int64_t p = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); p < work; p += warps) {
+    const int64_t t = p / chunks, c0 = (p - t * chunks) * 32 * kUnroll;
+    typename V::T acc[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) acc[u] = V::zero();
+    for (int64_t j = 0; j < k; ++j) {
+      const int64_t r = slot[t * k + j];
+      if (r < 0 || r >= num_rows) continue;
+      const float w = weights ? weights[t * k + j] : 1.0f;
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) {
+        const int64_t c = c0 + u * 32 + lane;
+        if (c < nvec) acc[u] = V::fma(w, rows[r * nvec + c], acc[u]);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const int64_t c = c0 + u * 32 + lane;
+      if (c < nvec) out[t * nvec + c] = acc[u];
+    }
+  }
+}
+
+// A warp takes one choice: its row of drows and its dweight.
+template <int VEC>
+__global__ void __launch_bounds__(256) combine_backward_kernel(
+    typename Vec<VEC>::T *__restrict__ drows, float *__restrict__ dweights,
+    const typename Vec<VEC>::T *__restrict__ dout, const typename Vec<VEC>::T *__restrict__ rows,
+    const float *__restrict__ weights, const int32_t *__restrict__ slot, const int32_t *__restrict__ src,
+    int64_t tokens, int64_t k, int64_t num_rows, int64_t nvec, int64_t chunks) {
+  using V = Vec<VEC>;
+  pdl_wait();
+  const int lane = threadIdx.x & 31;
+  const int64_t work = tokens * k, all = work + (num_rows + 31) / 32 * chunks;
+  const int64_t warps = (int64_t)gridDim.x * (blockDim.x >> 5);
+  for (int64_t p = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); p < all; p += warps) {
+    if (p >= work) {
+      const int64_t q = p - work, g = q / chunks;
+      zero_empty<VEC>(drows, src, g * 32, num_rows, nvec, (q - g * chunks) * 32 * kUnroll, lane);
+      continue;
+    }
+    const int64_t r = slot[p];
+    float s = 0.0f;
+    if (r >= 0 && r < num_rows) {
+      const float w = weights ? weights[p] : 1.0f;
+      const typename V::T *g = dout + p / k * nvec;
+      for (int64_t c0 = 0; c0 < nvec; c0 += 32 * kUnroll) {
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) {
+          const int64_t c = c0 + u * 32 + lane;
+          if (c < nvec) {
+            const typename V::T d = g[c];
+            if (dweights) s = V::dot(d, rows[r * nvec + c], s);
+            drows[r * nvec + c] = V::scale(w, d);
+          }
+        }
+      }
+    }
+    if (dweights) {
+      s = warp_sum(s);
+      if (lane == 0) dweights[p] = s;
+    }
+  }
+}
+
+// Arguments that dispatch, combine and its backward share.
+int check_rows(const char *who, int64_t tokens, int64_t k, int64_t num_rows, int64_t width) {
+  const std::string name(who);
+  FZ_REQUIRE(tokens >= 0 && k >= 1 && num_rows >= 0 && width >= 0, name + ": negative size or k < 1");
+  FZ_REQUIRE(k <= INT_MAX && tokens <= INT_MAX / k && num_rows <= INT_MAX,
+             name + ": tokens * k and the rows must be below 2^31");
+  FZ_REQUIRE(width <= INT_MAX, name + ": width must be below 2^31");
+  return FZ_OK;
+}
+
+template <int VEC>
+int64_t chunks_of(int64_t width) {
+  const int64_t per = (int64_t)32 * kUnroll * VEC;
+  return (width + per - 1) / per;
+}
+
+unsigned warps_grid(int64_t pieces) { return fz::grid_for(pieces, 8, 8, 4); }
+
+template <int NE>
+int launch_route(float *w, int32_t *ids, const float *logits, int64_t tokens, int experts, int k, int renorm,
+                 cudaStream_t s) {
+  FZ_CUDA(fz::launch_pdl(route_kernel<NE>, dim3(warps_grid(tokens)), dim3(256), 0, s, w, ids, logits, tokens,
+                         experts, k, renorm));
+  FZ_CHECK_LAUNCH();
+  return FZ_OK;
+}
+template <int NE>
+int launch_route_backward(float *dl, const float *dw, const float *w, const int32_t *ids, const float *logits,
+                          int64_t tokens, int experts, int k, int renorm, cudaStream_t s) {
+  FZ_CUDA(fz::launch_pdl(route_backward_kernel<NE>, dim3(warps_grid(tokens)), dim3(256), 0, s, dl, dw, w, ids,
+                         logits, tokens, experts, k, renorm));
+  FZ_CHECK_LAUNCH();
+  return FZ_OK;
+}
+
+int check_route(const char *who, int64_t tokens, int64_t experts, int64_t k) {
+  const std::string name(who);
+  FZ_REQUIRE(tokens >= 0 && experts >= 1 && k >= 1, name + ": negative or zero size");
+  FZ_REQUIRE(experts <= FZ_MAX_EXPERTS, name + ": more than FZ_MAX_EXPERTS experts");
+  FZ_REQUIRE(k <= experts && k <= FZ_MAX_CHOICES, name + ": k must be at most experts and FZ_MAX_CHOICES");
+  FZ_REQUIRE(tokens <= INT_MAX / k, name + ": tokens * k must be below 2^31");
+  return FZ_OK;
+}
+
+}  // namespace
+
+extern "C" int fz_route(float *weights, int32_t *ids, const float *logits, int64_t tokens, int64_t experts,
+                        int64_t k, int renormalize, void *stream) {
+  if (int rc = check_route("fz_route", tokens, experts, k)) return rc;
+  if (tokens == 0) return FZ_OK;
+  FZ_REQUIRE(weights && ids && logits, "fz_route: null pointer");
+  cudaStream_t s = fz::resolve(stream);
+  const int e = (int)experts, kk = (int)k, rn = renormalize != 0;
+  if (e <= 32) return launch_route<1>(weights, ids, logits, tokens, e, kk, rn, s);
+  if (e <= 64) return launch_route<2>(weights, ids, logits, tokens, e, kk, rn, s);
+  if (e <= 128) return launch_route<4>(weights, ids, logits, tokens, e, kk, rn, s);
+  if (e <= 256) return launch_route<8>(weights, ids, logits, tokens, e, kk, rn, s);
+  if (e <= 512) return launch_route<16>(weights, ids, logits, tokens, e, kk, rn, s);
+  return launch_route<32>(weights, ids, logits, tokens, e, kk, rn, s);
+}
+
+extern "C" int fz_route_backward(float *dlogits, const float *dweights, const float *weights, const int32_t *ids,
+                                 const float *logits, int64_t tokens, int64_t experts, int64_t k,
+                                 int renormalize, void *stream) {
+  if (int rc = check_route("fz_route_backward", tokens, experts, k)) return rc;
+  if (tokens == 0) return FZ_OK;
+  FZ_REQUIRE(dlogits && dweights && weights && ids && logits, "fz_route_backward: null pointer");
+  cudaStream_t s = fz::resolve(stream);
+  const int e = (int)experts, kk = (int)k, rn = renormalize != 0;
+  if (e <= 32) return launch_route_backward<1>(dlogits, dweights, weights, ids, logits, tokens, e, kk, rn, s);
+  if (e <= 64) return launch_route_backward<2>(dlogits, dweights, weights, ids, logits, tokens, e, kk, rn, s);
+  if (e <= 128) return launch_route_backward<4>(dlogits, dweights, weights, ids, logits, tokens, e, kk, rn, s);
+  if (e <= 256) return launch_route_backward<8>(dlogits, dweights, weights, ids, logits, tokens, e, kk, rn, s);
+  if (e <= 512) return launch_route_backward<16>(dlogits, dweights, weights, ids, logits, tokens, e, kk, rn, s);
+  return launch_route_backward<32>(dlogits, dweights, weights, ids, logits, tokens, e, kk, rn, s);
+}
+
+extern "C" int fz_expert_sort(int32_t *slot, int32_t *src, int32_t *counts, int32_t *offsets, const int32_t *ids,
+                              int64_t tokens, int64_t k, int64_t experts, int64_t capacity, void *stream) {
+  FZ_REQUIRE(tokens >= 0 && k >= 1 && experts >= 1 && capacity >= 0, "fz_expert_sort: negative or zero size");
+  FZ_REQUIRE(experts <= FZ_MAX_EXPERTS, "fz_expert_sort: more than FZ_MAX_EXPERTS experts");
+  FZ_REQUIRE(k <= INT_MAX && tokens <= INT_MAX / k && capacity <= INT_MAX / experts,
+             "fz_expert_sort: tokens * k and experts * capacity must be below 2^31");
+  const int64_t n = tokens * k, rows = capacity ? experts * capacity : n;
+  FZ_REQUIRE(counts && offsets, "fz_expert_sort: null pointer");
+  FZ_REQUIRE((n == 0 || (slot && ids)) && (rows == 0 || src), "fz_expert_sort: null pointer");
+  // Few choices: one CTA of few warps (fewer histograms to scan); many: a cluster of 8.
+  const int ctas = n > 8192 || rows > 65536 ? 8 : 1;
+  const int threads = n > 1024 || experts > 256 || ctas > 1 ? 1024 : 256;
+  const int warps = ctas * threads / 32;
+  const int per_warp = (int)((n + warps - 1) / warps);
+  const size_t smem = sizeof(int32_t) * (size_t)experts * (threads / 32 + 3);
+  FZ_CUDA(cudaFuncSetAttribute(sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                               (int)(sizeof(int32_t) * FZ_MAX_EXPERTS * (1024 / 32 + 3))));
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(ctas);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = fz::resolve(stream);
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = (unsigned)ctas;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  FZ_CUDA(cudaLaunchKernelEx(&cfg, sort_kernel, slot, src, counts, offsets, ids, (int)n, (int)experts,
+                             (int)capacity, (int)rows, per_warp));
+  FZ_CHECK_LAUNCH();
+  return FZ_OK;
+}
+
+extern "C" int fz_expert_dispatch(float *rows, const float *x, const int32_t *slot, const int32_t *src,
+                                  int64_t tokens, int64_t k, int64_t num_rows, int64_t width, void *stream) {
+  if (int rc = check_rows("fz_expert_dispatch", tokens, k, num_rows, width)) return rc;
+  if (num_rows == 0 || width == 0) return FZ_OK;
+  FZ_REQUIRE(rows && src && (tokens == 0 || (x && slot)), "fz_expert_dispatch: null pointer");
+  cudaStream_t s = fz::resolve(stream);
+  const int64_t groups = (num_rows + 31) / 32;
+  if (width % 4 == 0 && aligned16(rows, x)) {
+    const int64_t chunks = chunks_of<4>(width);
+    FZ_CUDA(fz::launch_pdl(dispatch_kernel<4>, dim3(warps_grid((tokens + groups) * chunks)), dim3(256), 0, s,
+                           (float4 *)rows, (const float4 *)x, slot, src, tokens, k, num_rows, width / 4, chunks));
+  } else {
+    const int64_t chunks = chunks_of<1>(width);
+    FZ_CUDA(fz::launch_pdl(dispatch_kernel<1>, dim3(warps_grid((tokens + groups) * chunks)), dim3(256), 0, s,
+                           rows, x, slot, src, tokens, k, num_rows, width, chunks));
+  }
+  FZ_CHECK_LAUNCH();
+  return FZ_OK;
+}
+
+extern "C" int fz_expert_combine(float *out, const float *rows, const float *weights, const int32_t *slot,
+                                 int64_t tokens, int64_t k, int64_t num_rows, int64_t width, void *stream) {
+  if (int rc = check_rows("fz_expert_combine", tokens, k, num_rows, width)) return rc;
+  if (tokens == 0 || width == 0) return FZ_OK;
+  FZ_REQUIRE(out && slot && (num_rows == 0 || rows), "fz_expert_combine: null pointer");
+  cudaStream_t s = fz::resolve(stream);
+  if (width % 4 == 0 && aligned16(out, rows)) {
+    const int64_t chunks = chunks_of<4>(width);
+    FZ_CUDA(fz::launch_pdl(combine_kernel<4>, dim3(warps_grid(tokens * chunks)), dim3(256), 0, s, (float4 *)out,
+                           (const float4 *)rows, weights, slot, tokens, k, num_rows, width / 4, chunks));
+  } else {
+    const int64_t chunks = chunks_of<1>(width);
+    FZ_CUDA(fz::launch_pdl(combine_kernel<1>, dim3(warps_grid(tokens * chunks)), dim3(256), 0, s, out, rows,
+                           weights, slot, tokens, k, num_rows, width, chunks));
+  }
+  FZ_CHECK_LAUNCH();
+  return FZ_OK;
+}
+
+extern "C" int fz_expert_combine_backward(float *drows, float *dweights, const float *dout, const float *rows,
+                                          const float *weights, const int32_t *slot, const int32_t *src,
+                                          int64_t tokens, int64_t k, int64_t num_rows, int64_t width,
+                                          void *stream) {
+  if (int rc = check_rows("fz_expert_combine_backward", tokens, k, num_rows, width)) return rc;
+  if (tokens == 0 && (num_rows == 0 || width == 0)) return FZ_OK;
+  const bool data = num_rows > 0 && width > 0;
+  FZ_REQUIRE((!data || (drows && src && (tokens == 0 || dout))) && (tokens == 0 || slot) &&
+                 (!dweights || !data || tokens == 0 || rows),
+             "fz_expert_combine_backward: null pointer");
+  cudaStream_t s = fz::resolve(stream);
+  const int64_t groups = (num_rows + 31) / 32;
+  if (width % 4 == 0 && aligned16(drows, dout, rows)) {
+    const int64_t chunks = chunks_of<4>(width);
+    FZ_CUDA(fz::launch_pdl(combine_backward_kernel<4>, dim3(warps_grid(tokens * k + groups * chunks)), dim3(256),
+                           0, s, (float4 *)drows, dweights, (const float4 *)dout, (const float4 *)rows, weights,
+                           slot, src, tokens, k, num_rows, width / 4, chunks));
+  } else {
+    const int64_t chunks = chunks_of<1>(width);
+    FZ_CUDA(fz::launch_pdl(combine_backward_kernel<1>, dim3(warps_grid(tokens * k + groups * chunks)), dim3(256),
+                           0, s, drows, dweights, dout, rows, weights, slot, src, tokens, k, num_rows, width,
+                           chunks));
+  }
+  FZ_CHECK_LAUNCH();
+  return FZ_OK;
+}

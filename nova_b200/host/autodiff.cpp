@@ -55,6 +55,11 @@ const char *op_name(OpKind k) {
     case OpKind::Mean: return "Mean";
     case OpKind::SwapAxes: return "SwapAxes";
     case OpKind::Dropout: return "Dropout";
+    case OpKind::GroupNorm: return "GroupNorm";
+    case OpKind::Route: return "Route";
+    case OpKind::ExpertDispatch: return "ExpertDispatch";
+    case OpKind::ExpertCombine: return "ExpertCombine";
+    case OpKind::Distill: return "Distill";
   }
   return "?";
 }
@@ -73,6 +78,10 @@ static void allow_scalar_binary(const RawTensor &a, const RawTensor &b, const ch
     throw std::runtime_error(os.str());
   }
 }
+
+// The value of t as it is now: a later in-place write through t leaves it alone, so that a
+// backward reads the values that its saved statistics belong to.
+static RawTensor snapshot(const RawTensor &t) { return RawTensor(t.expr(), t.dtype(), t.device()); }
 
 // Forward/backward formulas of fusion/src/Fusion/autodiff/registry/** restated.
 std::vector<RawTensor> op_forward(OpKind k, OpContext &ctx, const std::vector<RawTensor> &in,
@@ -148,6 +157,47 @@ std::vector<RawTensor> op_forward(OpKind k, OpContext &ctx, const std::vector<Ra
       ctx.ints["axis1"] = p.axis1;
       ctx.ints["axis2"] = p.axis2;
       return {x.swapaxes(p.axis1, p.axis2)};
+    case OpKind::GroupNorm: {
+      ctx.param = p;
+      const RawTensor gamma = in.size() > 1 ? in.at(1) : RawTensor(), beta = in.size() > 1 ? in.at(2) : RawTensor();
+      GroupNormStats s = math::group_norm(x, gamma, beta, p.learn->groups, p.learn->eps, p.learn->act);
+      ctx.saved["x"] = snapshot(x);
+      if (in.size() > 1) {
+        ctx.saved["gamma"] = snapshot(gamma);
+        ctx.saved["beta"] = snapshot(beta);
+      }
+      ctx.saved["mean"] = s.mean;
+      ctx.saved["rstd"] = s.rstd;
+      return {s.y};
+    }
+    case OpKind::Route: {
+      auto [weights, ids] = math::route(x, p.learn->k, p.learn->renormalize);
+      p.learn->ids = ids;
+      ctx.param = p;
+      ctx.saved["x"] = snapshot(x);
+      ctx.saved["weights"] = snapshot(weights);
+      return {weights};
+    }
+    case OpKind::ExpertDispatch:
+      ctx.param = p;
+      ctx.saved["x"] = snapshot(x);  // its shape
+      return {math::expert_dispatch(x, *p.learn->plan)};
+    case OpKind::ExpertCombine: {
+      ctx.param = p;
+      const RawTensor weights = in.size() > 1 ? in.at(1) : RawTensor();
+      RawTensor out = math::expert_combine(x, weights, *p.learn->plan, p.learn->shape);
+      ctx.saved["rows"] = snapshot(x);
+      if (in.size() > 1) ctx.saved["weights"] = snapshot(weights);
+      return {out};
+    }
+    case OpKind::Distill: {
+      ctx.param = p;
+      const LearnParam &l = *p.learn;
+      DistillStats s = math::distill(x, l.ids, l.teacher, l.teacher_lse, l.temperature);
+      ctx.saved["x"] = snapshot(x);
+      ctx.saved["stats"] = s.stats;
+      return {s.loss};
+    }
   }
   throw std::runtime_error("unknown op");
 }
@@ -215,6 +265,35 @@ std::vector<RawTensor> op_backward(OpKind k, OpContext &ctx, const RawTensor &g0
       // (signed zeros and NaNs included): the same kernel redraws the same mask
       const OpParam &q = ctx.param;
       return {math::dropout(g0, q.rate, q.keep, q.rng_seed, q.rng_offset)};
+    }
+    case OpKind::GroupNorm: {
+      const LearnParam &l = *ctx.param.learn;
+      const bool affine = ctx.saved.count("gamma") > 0;
+      const RawTensor gamma = affine ? ctx.load("gamma") : RawTensor(), beta = affine ? ctx.load("beta") : RawTensor();
+      const GroupNormStats s{RawTensor(), ctx.load("mean"), ctx.load("rstd")};
+      std::vector<RawTensor> r = math::group_norm_backward(g0, ctx.load("x"), s, gamma, beta, l.groups, l.act,
+                                                           affine && (want(1) || want(2)));
+      if (!affine) r.resize(1);
+      return r;
+    }
+    case OpKind::Route: {
+      const LearnParam &l = *ctx.param.learn;
+      return {math::route_backward(g0, ctx.load("weights"), l.ids, ctx.load("x"), l.renormalize)};
+    }
+    case OpKind::ExpertDispatch:
+      return {math::expert_combine(g0, RawTensor(), *ctx.param.learn->plan, ctx.load("x").shape())};
+    case OpKind::ExpertCombine: {
+      const bool weighted = ctx.saved.count("weights") > 0;
+      const RawTensor weights = weighted ? ctx.load("weights") : RawTensor();
+      std::vector<RawTensor> r = math::expert_combine_backward(g0, ctx.load("rows"), weights,
+                                                               *ctx.param.learn->plan, weighted && want(1));
+      if (!weighted) r.resize(1);
+      return r;
+    }
+    case OpKind::Distill: {
+      const LearnParam &l = *ctx.param.learn;
+      return {math::distill_backward(g0, ctx.load("stats"), ctx.load("x"), l.ids, l.teacher, l.teacher_lse,
+                                     l.temperature)};
     }
   }
   throw std::runtime_error("unknown op");
@@ -494,6 +573,26 @@ ADTensor ADTensor::unary_op(OpKind k, const OpParam &p) const {
   ValueID vx = const_cast<ADTensor *>(this)->ensure_vid();
   ValueID out = eng.apply(k, {raw_}, {vx}, p);
   ADTensor r(eng.materialise(out), requires_grad_);
+  r.set_vid(out);
+  return r;
+}
+
+ADTensor ADTensor::nary_op(OpKind k, const std::vector<ADTensor *> &ins, const OpParam &p) {
+  bool any = false;
+  std::vector<RawTensor> raws;
+  for (const ADTensor *t : ins) {
+    any = any || t->requires_grad_;
+    raws.push_back(t->raw_);
+  }
+  if (!grad_enabled() || !any || !engine_instance()) {
+    OpContext ctx;
+    return ADTensor(op_forward(k, ctx, raws, p).at(0), any);
+  }
+  Engine &eng = current_engine();
+  std::vector<ValueID> vids;
+  for (ADTensor *t : ins) vids.push_back(t->ensure_vid());
+  const ValueID out = eng.apply(k, raws, vids, p);
+  ADTensor r(eng.materialise(out), any);
   r.set_vid(out);
   return r;
 }

@@ -29,6 +29,7 @@
 #include <unordered_set>
 #include <vector>
 
+#include "learn.hpp"
 #include "tensor.hpp"
 
 namespace fusion_b200 {
@@ -44,6 +45,7 @@ struct OpParam {
   // the divisor keep = fp32(1 - rate)
   uint64_t rng_seed = 0, rng_offset = 0;
   float rate = 0.0f, keep = 1.0f;
+  std::shared_ptr<LearnParam> learn;  // GroupNorm .. Distill (learn.hpp)
 };
 
 struct OpContext {
@@ -56,7 +58,9 @@ struct OpContext {
 enum class OpKind {
   Add, Subtract, Multiply, Divide, Pow, Maximum, GreaterThan, GreaterThanEqual,
   MatMul, Exp, Log, Sqrt, Sum, Mean, SwapAxes,
-  Dropout  // no reference op: Nova's Dropout composition with a device-drawn mask
+  Dropout,  // no reference op: Nova's Dropout composition with a device-drawn mask
+  // no reference ops: the language-model training operators of learn.hpp
+  GroupNorm, Route, ExpertDispatch, ExpertCombine, Distill
 };
 const char *op_name(OpKind k);
 
@@ -182,6 +186,9 @@ class ADTensor {
   ADTensor binary_op(OpKind k, const ADTensor &other) const;
   ADTensor binary_scalar(OpKind k, float s) const;
   ADTensor unary_op(OpKind k, const OpParam &p = {}) const;
+  // An op of any number of inputs, traced under the same rule as the others (learn.hpp's
+  // operators).
+  static ADTensor nary_op(OpKind k, const std::vector<ADTensor *> &ins, const OpParam &p);
 
  private:
   RawTensor raw_;

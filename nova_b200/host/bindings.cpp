@@ -8,6 +8,7 @@
 #include <pybind11/pybind11.h>
 #include <pybind11/stl.h>
 
+#include <cmath>
 #include <numeric>
 #include <optional>
 #include <random>
@@ -78,6 +79,88 @@ RawTensor raw_from_array(const std::vector<size_t> &shape, py::array_t<float, py
   size_t total = prod(shape);
   if ((size_t)a.size() != total) throw std::invalid_argument("shape* must equal data.size()");
   return RawTensor(shape, a.data(), dt, dev);
+}
+
+Indices indices_from_array(py::object values, Device dev) {
+  py::array a = py::array::ensure(values);
+  if (!a) throw py::error_already_set();
+  const char kind = a.dtype().kind();
+  if (kind != 'i' && kind != 'u')
+    throw std::invalid_argument("Indices: an array of whole numbers is needed");
+  auto v = py::array_t<int64_t, py::array::c_style | py::array::forcecast>::ensure(a);
+  if (!v) throw py::error_already_set();
+  std::vector<size_t> shape;
+  for (ssize_t d = 0; d < v.ndim(); ++d) shape.push_back((size_t)v.shape(d));
+  std::vector<int32_t> host((size_t)v.size());
+  for (size_t i = 0; i < host.size(); ++i) {
+    const int64_t x = v.data()[i];
+    if (x < INT32_MIN || x > INT32_MAX) throw std::invalid_argument("Indices: a value does not fit int32");
+    host[i] = (int32_t)x;
+  }
+  return Indices(shape, host, dev);
+}
+
+py::array_t<int32_t> indices_to_numpy(const Indices &t) {
+  std::vector<ssize_t> sh(t.shape().begin(), t.shape().end());
+  py::array_t<int32_t> arr(sh);
+  t.to_host(static_cast<int32_t *>(arr.request().ptr));
+  return arr;
+}
+
+OpParam learn_param(LearnParam l) {
+  OpParam p;
+  p.learn = std::make_shared<LearnParam>(std::move(l));
+  return p;
+}
+
+ADTensor group_norm(ADTensor &x, int64_t groups, ADTensor *gamma, ADTensor *beta, float eps, const std::string &act) {
+  if (!gamma != !beta) throw std::invalid_argument("group_norm: gamma and beta go together");
+  LearnParam l;
+  l.groups = groups;
+  l.eps = eps;
+  l.act = activation_code(act);
+  std::vector<ADTensor *> ins{&x};
+  if (gamma) ins.push_back(gamma), ins.push_back(beta);
+  return ADTensor::nary_op(OpKind::GroupNorm, ins, learn_param(std::move(l)));
+}
+
+py::tuple route(ADTensor &logits, int64_t k, bool renormalize) {
+  LearnParam l;
+  l.k = k;
+  l.renormalize = renormalize;
+  OpParam p = learn_param(std::move(l));
+  ADTensor w = ADTensor::nary_op(OpKind::Route, {&logits}, p);
+  return py::make_tuple(w, p.learn->ids);
+}
+
+ADTensor expert_dispatch(ADTensor &x, std::shared_ptr<ExpertPlan> plan) {
+  LearnParam l;
+  l.plan = std::move(plan);
+  return ADTensor::nary_op(OpKind::ExpertDispatch, {&x}, learn_param(std::move(l)));
+}
+
+ADTensor expert_combine(ADTensor &rows, std::shared_ptr<ExpertPlan> plan, ADTensor *weights) {
+  LearnParam l;
+  l.shape = plan->token_shape();
+  if (rows.rank()) l.shape.push_back(rows.shape().back());
+  l.plan = std::move(plan);
+  std::vector<ADTensor *> ins{&rows};
+  if (weights) ins.push_back(weights);
+  return ADTensor::nary_op(OpKind::ExpertCombine, ins, learn_param(std::move(l)));
+}
+
+// The teacher's values are constants: no gradient reaches them.
+ADTensor distill(ADTensor &logits, const Indices &ids, const ADTensor &teacher, float temperature,
+                 const ADTensor *teacher_lse) {
+  if (!(temperature > 0.0f) || std::isinf(temperature))
+    throw std::invalid_argument("distill: temperature must be positive and finite");
+  auto value = [](const ADTensor &t) { return RawTensor(t.raw().expr(), t.raw().dtype(), t.raw().device()); };
+  LearnParam l;
+  l.ids = ids;
+  l.teacher = value(teacher);
+  if (teacher_lse) l.teacher_lse = value(*teacher_lse);
+  l.temperature = temperature;
+  return ADTensor::nary_op(OpKind::Distill, {&logits}, learn_param(std::move(l)));
 }
 
 struct GradTape {
@@ -380,6 +463,53 @@ PYBIND11_MODULE(fusion, m) {
       py::arg("state") = py::none(),
       "Get or set whether autodiff is enabled for this thread. When enabled, a default "
       "Engine is installed in the EngineContext.");
+
+  // ---- operators for training language models (no reference counterpart) ----
+  py::class_<Indices>(m, "Indices", py::module_local(),
+                      "An immutable int32 array on the device: expert choices, rows, token ids.")
+      .def(py::init(&indices_from_array), py::arg("values"), py::arg("device") = Device(DeviceType::CPU, 0))
+      .def_property_readonly("shape", [](const Indices &t) { return t.shape(); })
+      .def_property_readonly("size", &Indices::size)
+      .def("to_numpy", &indices_to_numpy, "Return a NumPy copy (int32) of the values.");
+  py::class_<ExpertPlan, std::shared_ptr<ExpertPlan>>(
+      m, "ExpertPlan", py::module_local(),
+      "Choices ids [..., k] of a batch of tokens sorted by expert, stably: `slot` [..., k] is a choice's "
+      "row (-1: none), `src` [rows] the choice in a row (-1: empty), `counts` [experts] how many named an "
+      "expert, `offsets` [experts + 1] where its rows begin. capacity = 0 packs the rows; capacity > 0 gives "
+      "every expert that many (the layout of a batched product) and drops an expert's later choices once "
+      "they are full. Ids outside [0, experts) are no choice.")
+      .def(py::init<const Indices &, int64_t, int64_t>(), py::arg("ids"), py::arg("experts"), py::arg("capacity") = 0)
+      .def_readonly("ids", &ExpertPlan::ids)
+      .def_readonly("slot", &ExpertPlan::slot)
+      .def_readonly("src", &ExpertPlan::src)
+      .def_readonly("counts", &ExpertPlan::counts)
+      .def_readonly("offsets", &ExpertPlan::offsets)
+      .def_readonly("tokens", &ExpertPlan::tokens)
+      .def_readonly("k", &ExpertPlan::k)
+      .def_readonly("experts", &ExpertPlan::experts)
+      .def_readonly("capacity", &ExpertPlan::capacity)
+      .def_readonly("rows", &ExpertPlan::rows);
+  m.def("group_norm", &group_norm, py::arg("x"), py::arg("groups"), py::arg("gamma") = nullptr,
+        py::arg("beta") = nullptr, py::arg("eps") = 1e-5f, py::arg("activation") = "none",
+        "act(gamma * (x - mean) * rstd + beta) of x [batch, ..., channels], the statistics over each "
+        "sample's group of channels (and everything between batch and channels); gamma and beta [channels] or "
+        "both None; activation none, relu, silu or gelu. Traced by autodiff for x, gamma and beta.");
+  m.def("route", &route, py::arg("logits"), py::arg("k"), py::arg("renormalize") = true,
+        "The router's gate over logits [..., experts]: (weights, ids) of each token's k largest, largest first, "
+        "ties to the lowest expert; weights are the softmax over the chosen logits, or with renormalize=False "
+        "over all. A logit of -inf is never chosen (id -1, weight 0). weights is traced by autodiff.");
+  m.def("expert_dispatch", &expert_dispatch, py::arg("x"), py::arg("plan"),
+        "x [..., width] of the plan's tokens in the plan's rows, empty rows zero: [experts, capacity, width], "
+        "or [rows, width] packed. Traced by autodiff.");
+  m.def("expert_combine", &expert_combine, py::arg("rows"), py::arg("plan"), py::arg("weights") = nullptr,
+        "The way back: per token the sum of its choices' rows, times weights [..., k] (None: ones). Traced by "
+        "autodiff for rows and weights.");
+  m.def("distill", &distill, py::arg("logits"), py::arg("ids"), py::arg("teacher"), py::arg("temperature") = 1.0f,
+        py::arg("teacher_lse") = nullptr,
+        "Per row of logits [..., vocab], temperature^2 * KL(teacher || student) over the teacher's top logits "
+        "teacher [..., k] at ids [..., k] (ids outside the vocabulary are padding; a row without entries has "
+        "loss 0). teacher_lse None: the teacher is the softmax over its list; else the logsumexp of its whole "
+        "vocabulary over the temperature, with the remaining mass on one bucket. Traced by autodiff for logits.");
 
   // ---- backend controls (no reference counterpart) ------------------------
   m.def("set_device", [](int d) { fz_check(fz_set_device(d), "fz_set_device"); }, py::arg("index"),

@@ -383,6 +383,272 @@ int fz_philox_dropout(float *out, const float *x, int64_t n, float rate, float k
   return FZ_OK;
 }
 
+// Operators for training language models: plain loops in double, rounded once.
+static double act_of(int a, double v) {
+  if (a == FZ_ACT_RELU) return v > 0 ? v : 0.0;
+  if (a == FZ_ACT_SILU) return v / (1 + std::exp(-v));
+  if (a == FZ_ACT_GELU) return 0.5 * v * (1 + std::erf(v / std::sqrt(2.0)));
+  return v;
+}
+static double slope_of(int a, double v) {
+  if (a == FZ_ACT_RELU) return v > 0 ? 1.0 : 0.0;
+  if (a == FZ_ACT_SILU) {
+    const double s = 1 / (1 + std::exp(-v));
+    return s * (1 + v * (1 - s));
+  }
+  if (a == FZ_ACT_GELU)
+    return 0.5 * (1 + std::erf(v / std::sqrt(2.0))) + v * std::exp(-0.5 * v * v) * 0.3989422804014327;
+  return 1.0;
+}
+int fz_group_norm_workspace(int64_t, int64_t, int64_t channels, int64_t groups, int, size_t *bytes) {
+  *bytes = 64;
+  return groups >= 1 && channels % groups == 0 ? FZ_OK : fail(FZ_ERR_INVALID, "fz_group_norm_workspace: bad sizes");
+}
+int fz_group_norm(float *y, float *mean, float *rstd, const float *x, const float *gamma, const float *beta,
+                  int64_t batch, int64_t len, int64_t channels, int64_t groups, float eps, int act, void *work,
+                  size_t bytes, void *) {
+  if (!work || bytes < 64) return fail(FZ_ERR_INVALID, "fz_group_norm: workspace too small");
+  const int64_t c = channels / groups;
+  for (int64_t b = 0; b < batch; ++b)
+    for (int64_t g = 0; g < groups; ++g) {
+      double m = 0, v = 0;
+      auto at = [&](int64_t l, int64_t i) { return (b * len + l) * channels + g * c + i; };
+      for (int64_t l = 0; l < len; ++l)
+        for (int64_t i = 0; i < c; ++i) m += x[at(l, i)];
+      m /= (double)(len * c);
+      for (int64_t l = 0; l < len; ++l)
+        for (int64_t i = 0; i < c; ++i) v += (x[at(l, i)] - m) * (x[at(l, i)] - m);
+      const double r = 1 / std::sqrt(v / (double)(len * c) + eps);
+      if (mean) mean[b * groups + g] = (float)m, rstd[b * groups + g] = (float)r;
+      for (int64_t l = 0; l < len; ++l)
+        for (int64_t i = 0; i < c; ++i) {
+          const double ga = gamma ? gamma[g * c + i] : 1.0, be = beta ? beta[g * c + i] : 0.0;
+          y[at(l, i)] = (float)act_of(act, (x[at(l, i)] - m) * r * ga + be);
+        }
+    }
+  ++g_launches;
+  return FZ_OK;
+}
+int fz_group_norm_backward(float *dx, float *dgamma, float *dbeta, const float *dy, const float *x,
+                           const float *mean, const float *rstd, const float *gamma, const float *beta,
+                           int64_t batch, int64_t len, int64_t channels, int64_t groups, int act, void *work,
+                           size_t bytes, void *) {
+  if (!work || bytes < 64) return fail(FZ_ERR_INVALID, "fz_group_norm_backward: workspace too small");
+  const int64_t c = channels / groups;
+  std::vector<double> dg(channels, 0.0), db(channels, 0.0);
+  for (int64_t b = 0; b < batch; ++b)
+    for (int64_t g = 0; g < groups; ++g) {
+      const double m = mean[b * groups + g], r = rstd[b * groups + g];
+      double s1 = 0, s2 = 0;
+      for (int pass = 0; pass < 2; ++pass)
+        for (int64_t l = 0; l < len; ++l)
+          for (int64_t i = 0; i < c; ++i) {
+            const int64_t at = (b * len + l) * channels + g * c + i, ch = g * c + i;
+            const double ga = gamma ? gamma[ch] : 1.0, xh = (x[at] - m) * r;
+            const double dv = dy[at] * slope_of(act, xh * ga + (beta ? beta[ch] : 0.0)), a = dv * ga;
+            if (!pass) {
+              s1 += a;
+              s2 += a * xh;
+              dg[ch] += dv * xh;
+              db[ch] += dv;
+            } else {
+              dx[at] = (float)(r * (a - (s1 + xh * s2) / (double)(len * c)));
+            }
+          }
+    }
+  for (int64_t ch = 0; ch < channels; ++ch) {
+    if (dgamma) dgamma[ch] = (float)dg[ch];
+    if (dbeta) dbeta[ch] = (float)db[ch];
+  }
+  ++g_launches;
+  return FZ_OK;
+}
+int fz_route(float *w, int32_t *ids, const float *logits, int64_t tokens, int64_t experts, int64_t k, int renorm,
+             void *) {
+  for (int64_t t = 0; t < tokens; ++t) {
+    const float *z = logits + t * experts;
+    std::vector<bool> taken(experts, false);
+    double den = 0;
+    float top = -INFINITY;
+    for (int64_t j = 0; j < k; ++j) {
+      int64_t best = -1;
+      for (int64_t e = 0; e < experts; ++e) {
+        if (taken[e] || z[e] == -INFINITY) continue;
+        if (best < 0 || (z[e] != z[e] && z[best] == z[best]) || z[e] > z[best]) best = e;
+      }
+      if (j == 0 && best >= 0) {
+        top = z[best];
+        if (!renorm)
+          for (int64_t e = 0; e < experts; ++e) den += std::exp((double)z[e] - top);
+      }
+      ids[t * k + j] = (int32_t)best;
+      const double num = best >= 0 ? std::exp((double)z[best] - top) : 0.0;
+      if (best >= 0) taken[best] = true;
+      if (renorm) den += num;
+    }
+    for (int64_t j = 0; j < k; ++j) {
+      const int32_t e = ids[t * k + j];
+      w[t * k + j] = e < 0 ? 0.0f : (float)(std::exp((double)z[e] - top) / den);
+    }
+  }
+  ++g_launches;
+  return FZ_OK;
+}
+int fz_route_backward(float *dl, const float *dw, const float *w, const int32_t *ids, const float *logits,
+                      int64_t tokens, int64_t experts, int64_t k, int renorm, void *) {
+  for (int64_t t = 0; t < tokens; ++t) {
+    double dot = 0, den = 0, top = -INFINITY;
+    bool any = false;
+    for (int64_t j = 0; j < k; ++j)
+      if (ids[t * k + j] >= 0) {
+        dot += (double)w[t * k + j] * dw[t * k + j];
+        any = true;
+      }
+    const float *z = logits + t * experts;
+    for (int64_t e = 0; e < experts; ++e) top = z[e] > top ? z[e] : top;
+    for (int64_t e = 0; e < experts; ++e) den += std::exp(z[e] - top);
+    for (int64_t e = 0; e < experts; ++e) {
+      double up = 0;
+      for (int64_t j = 0; j < k; ++j)
+        if (ids[t * k + j] == e) up = renorm ? w[t * k + j] * (dw[t * k + j] - dot) : dw[t * k + j];
+      dl[t * experts + e] = (float)(renorm || !any ? up : std::exp(z[e] - top) / den * (up - dot));
+    }
+  }
+  ++g_launches;
+  return FZ_OK;
+}
+int fz_expert_sort(int32_t *slot, int32_t *src, int32_t *counts, int32_t *offsets, const int32_t *ids,
+                   int64_t tokens, int64_t k, int64_t experts, int64_t capacity, void *) {
+  const int64_t n = tokens * k, rows = capacity ? experts * capacity : n;
+  for (int64_t e = 0; e < experts; ++e) counts[e] = 0;
+  for (int64_t i = 0; i < n; ++i)
+    if (ids[i] >= 0 && ids[i] < experts) ++counts[ids[i]];
+  offsets[0] = 0;
+  for (int64_t e = 0; e < experts; ++e) offsets[e + 1] = offsets[e] + (int32_t)(capacity ? capacity : counts[e]);
+  std::vector<int32_t> used(experts, 0);
+  for (int64_t r = 0; r < rows; ++r) src[r] = -1;
+  for (int64_t i = 0; i < n; ++i) {
+    slot[i] = -1;
+    const int32_t e = ids[i];
+    if (e < 0 || e >= experts) continue;
+    const int32_t place = used[e]++;
+    if (capacity && place >= capacity) continue;
+    slot[i] = offsets[e] + place;
+    src[slot[i]] = (int32_t)i;
+  }
+  ++g_launches;
+  return FZ_OK;
+}
+int fz_expert_dispatch(float *rows, const float *x, const int32_t *, const int32_t *src, int64_t, int64_t k,
+                       int64_t num_rows, int64_t width, void *) {
+  for (int64_t r = 0; r < num_rows; ++r)
+    for (int64_t c = 0; c < width; ++c) rows[r * width + c] = src[r] < 0 ? 0.0f : x[src[r] / k * width + c];
+  ++g_launches;
+  return FZ_OK;
+}
+int fz_expert_combine(float *out, const float *rows, const float *w, const int32_t *slot, int64_t tokens, int64_t k,
+                      int64_t, int64_t width, void *) {
+  for (int64_t t = 0; t < tokens; ++t)
+    for (int64_t c = 0; c < width; ++c) {
+      double s = 0;
+      for (int64_t j = 0; j < k; ++j) {
+        const int64_t r = slot[t * k + j];
+        if (r >= 0) s += (w ? (double)w[t * k + j] : 1.0) * rows[r * width + c];
+      }
+      out[t * width + c] = (float)s;
+    }
+  ++g_launches;
+  return FZ_OK;
+}
+int fz_expert_combine_backward(float *drows, float *dw, const float *dout, const float *rows, const float *w,
+                               const int32_t *slot, const int32_t *src, int64_t tokens, int64_t k, int64_t num_rows,
+                               int64_t width, void *) {
+  for (int64_t r = 0; r < num_rows; ++r)
+    for (int64_t c = 0; c < width; ++c)
+      drows[r * width + c] = src[r] < 0 ? 0.0f : (w ? w[src[r]] : 1.0f) * dout[src[r] / k * width + c];
+  for (int64_t i = 0; dw && i < tokens * k; ++i) {
+    double s = 0;
+    for (int64_t c = 0; slot[i] >= 0 && c < width; ++c) s += (double)dout[i / k * width + c] * rows[slot[i] * width + c];
+    dw[i] = (float)s;
+  }
+  ++g_launches;
+  return FZ_OK;
+}
+// p (per entry, 0 for padding), the teacher's mass and tail; false if the row has no entries.
+static bool teacher_of(const int32_t *ids, const float *t, const float *lse, int64_t vocab, int64_t k, double tau,
+                       std::vector<double> &p, std::vector<double> &logp, double &mass, double &tail) {
+  double top = -INFINITY, sum = 0;
+  bool any = false;
+  for (int64_t i = 0; i < k; ++i)
+    if (ids[i] >= 0 && ids[i] < vocab && (lse || t[i] != -INFINITY)) {
+      any = true;
+      top = t[i] > top ? t[i] : top;
+    }
+  mass = tail = 0;
+  if (!any) return false;
+  for (int64_t i = 0; i < k; ++i)
+    if (ids[i] >= 0 && ids[i] < vocab) sum += std::exp((t[i] - top) / tau);
+  for (int64_t i = 0; i < k; ++i) {
+    const bool ok = ids[i] >= 0 && ids[i] < vocab;
+    logp[i] = lse ? t[i] / tau - *lse : (t[i] - top) / tau - std::log(sum);
+    p[i] = ok ? std::exp(logp[i]) : 0.0;
+    mass += p[i];
+  }
+  if (lse && mass < 1) tail = 1 - mass;
+  mass += tail;
+  return true;
+}
+int fz_distill(float *loss, float *stats, const float *logits, int64_t ld, const int32_t *ids, const float *teacher,
+               const float *lse, int64_t rows, int64_t vocab, int64_t k, float tau, void *) {
+  std::vector<double> p(k), logp(k);
+  for (int64_t r = 0; r < rows; ++r) {
+    double mass, tail, l = 0;
+    const float *z = logits + r * ld;
+    float *st = stats + r * 4;
+    loss[r] = st[0] = st[1] = st[2] = st[3] = 0.0f;
+    if (!teacher_of(ids + r * k, teacher + r * k, lse ? lse + r : nullptr, vocab, k, tau, p, logp, mass, tail)) continue;
+    std::set<int64_t> inside;
+    for (int64_t i = 0; i < k; ++i) inside.insert(ids[r * k + i]);
+    double m = -INFINITY, tm = -INFINITY, s = 0, ts = 0;
+    for (int64_t v = 0; v < vocab; ++v) {
+      m = z[v] > m ? z[v] : m;
+      if (!inside.count(v)) tm = z[v] > tm ? z[v] : tm;
+    }
+    for (int64_t v = 0; v < vocab; ++v) {
+      s += std::exp((z[v] - m) / tau);
+      if (!inside.count(v)) ts += std::exp((z[v] - tm) / tau);
+    }
+    for (int64_t i = 0; i < k; ++i)
+      if (p[i] != 0) l += p[i] * (logp[i] - ((z[ids[r * k + i]] - m) / tau - std::log(s)));
+    if (tail != 0) l += tail * (std::log(tail) - ((tm - m) / tau + std::log(ts) - std::log(s)));
+    loss[r] = (float)(tau * tau * l);
+    st[0] = (float)m, st[1] = (float)std::log(s), st[2] = (float)tm, st[3] = (float)std::log(ts);
+  }
+  ++g_launches;
+  return FZ_OK;
+}
+int fz_distill_backward(float *dz, int64_t ldd, const float *dloss, const float *stats, const float *logits,
+                        int64_t ld, const int32_t *ids, const float *teacher, const float *lse, int64_t rows,
+                        int64_t vocab, int64_t k, float tau, void *) {
+  std::vector<double> p(k), logp(k);
+  for (int64_t r = 0; r < rows; ++r) {
+    double mass, tail;
+    const float *z = logits + r * ld, *st = stats + r * 4;
+    const bool any = teacher_of(ids + r * k, teacher + r * k, lse ? lse + r : nullptr, vocab, k, tau, p, logp, mass, tail);
+    std::map<int64_t, double> inside;
+    for (int64_t i = 0; any && i < k; ++i)
+      if (ids[r * k + i] >= 0) inside[ids[r * k + i]] += p[i];
+    for (int64_t v = 0; v < vocab; ++v) {
+      double g = any ? mass * std::exp((z[v] - (double)st[0]) / tau - st[1]) : 0.0;
+      if (inside.count(v)) g -= inside[v];
+      else if (tail != 0) g -= tail * std::exp((z[v] - (double)st[2]) / tau - st[3]);
+      dz[r * ldd + v] = any ? (float)(tau * dloss[r] * g) : 0.0f;
+    }
+  }
+  ++g_launches;
+  return FZ_OK;
+}
+
 int fz_comm_unique_id(unsigned char id[FZ_UNIQUE_ID_BYTES]) { std::memset(id, 0, FZ_UNIQUE_ID_BYTES); return FZ_OK; }
 int fz_comm_init(void **c, int world, int, const unsigned char *) {
   if (world != 1 && !g_transport) return fail(FZ_ERR_UNSUPPORTED, "host test double: world must be 1");

@@ -1,0 +1,781 @@
+"""The language-model training operators' kernels through the C ABI, against the 64-bit
+implementations of learn_oracle, at the sizes, alignments and masks where they can go
+wrong; the same operators through the `fusion` module (learn_cases).
+
+Bounds: u = 2^-24 is the largest relative error of one fp32 rounding, and every bound below
+counts the roundings of the operator's formula to first order, with D sequential additions
+for a sum of m values spread over at least 32 lanes (D = m / 32 + 32). CUDA's expf, erff
+and logf and the hardware's 2^x are within 2 ulp = 4 u of their result.
+"""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+import learn_cases
+import learn_oracle as O
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+GUARD = 64
+SENTINEL = np.float32(-12345.678)
+
+
+class Out:
+    """A device array of `shape` between two guard zones, `off` floats off 16-byte alignment;
+    get() checks that the zones were left alone."""
+
+    def __init__(self, capi, shape, off=0, dtype=np.float32):
+        self.shape, self.n, self.off, self.dtype = tuple(shape), int(np.prod(shape)), off, dtype
+        self.host = np.full(self.n + 2 * GUARD, SENTINEL, np.float32)
+        self.d = capi.DeviceArray.from_numpy(self.host)
+        self.ptr = self.d.ptr + 4 * (GUARD + off)
+
+    def get(self):
+        a = self.d.numpy()
+        lo, hi = GUARD + self.off, GUARD + self.off + self.n
+        assert np.all(a[:lo] == SENTINEL) and np.all(a[hi:] == SENTINEL), "wrote outside its output"
+        return a[lo:hi].view(self.dtype).reshape(self.shape).copy()
+
+
+class In:
+    def __init__(self, capi, a, off=0):
+        a = np.ascontiguousarray(a)
+        a = a.astype(np.int32).view(np.float32) if a.dtype.kind in "iu" else a.astype(np.float32)
+        self.d = capi.DeviceArray.from_numpy(np.concatenate([np.zeros(off, np.float32), a.ravel()]))
+        self.ptr = self.d.ptr + 4 * off
+
+
+def ptr(x):
+    return None if x is None else x.ptr
+
+
+def close(got, want, bound, what):
+    got = got.astype(np.float64)
+    same_nan = np.isnan(got) & np.isnan(want)
+    with np.errstate(invalid="ignore"):
+        ok = (np.abs(got - want) <= bound) | same_nan | (got == want)
+    if not ok.all():
+        i = np.unravel_index(int(np.argmin(ok)), ok.shape)
+        raise AssertionError(f"{what}: {int((~ok).sum())} values off; at {i}: {got[i]!r} for {want[i]!r}, "
+                             f"bound {np.broadcast_to(bound, ok.shape)[i]!r}")
+
+
+# ---------------------------------------------------------------- group norm
+
+
+def norm_bounds(x, gamma, beta, groups, eps, act, dy=None):
+    """First-order bounds of y, mean, rstd (and dx, dgamma, dbeta)."""
+    x = x.astype(np.float64)
+    b, n, c = x.shape
+    cg, m = c // groups, n * c // groups
+    D = m / 32 + 32
+    ga = np.ones(c) if gamma is None else gamma.astype(np.float64)
+    be = np.zeros(c) if beta is None else beta.astype(np.float64)
+    spread = lambda s: np.repeat(s, cg, axis=-1)[:, None, :]  # noqa: E731  [b, groups] -> [b, 1, c]
+    over = lambda v: v.reshape(b, n, groups, cg).mean(axis=(1, 3))  # noqa: E731
+    mean, var = over(x), None
+    d = x - spread(mean)
+    var = over(d * d)
+    e_mean = (D + 3) * U * over(np.abs(x))
+    e_d = spread(e_mean) + U * np.abs(d)
+    with np.errstate(divide="ignore", invalid="ignore"):
+        rstd = 1 / np.sqrt(var + eps)
+        r_rstd = 0.5 * (over(2 * np.abs(d) * e_d + e_d * e_d) + (D + 3) * U * var) / (var + eps) + 4 * U
+    xh = d * spread(rstd)
+    e_xh = spread(rstd) * e_d + np.abs(xh) * (spread(r_rstd) + 2 * U)
+    v = xh * ga + be
+    e_v = np.abs(ga) * e_xh + 3 * U * (np.abs(ga * xh) + np.abs(be))
+    res = [1.13 * e_v + 16 * U * np.abs(v), e_mean, rstd * r_rstd]
+    if dy is None:
+        return res, e_v, v
+    dy = dy.astype(np.float64)
+    slope = O.act_slope(v, act)
+    e_slope = 0.0 if act in ("none", "relu") else 1.2 * e_v + 24 * U
+    dv, a = dy * slope, dy * slope * ga
+    e_dv = np.abs(dy) * e_slope + 2 * U * np.abs(dv)
+    e_a = e_dv * np.abs(ga) + 2 * U * np.abs(a)
+    k1, k2 = np.abs(over(a)), np.abs(over(a * xh))
+    e_k1 = over(e_a) + (D + 3) * U * over(np.abs(a))
+    e_k2 = over(e_a * np.abs(xh) + np.abs(a) * e_xh) + (D + 3) * U * over(np.abs(a * xh))
+    parts = np.abs(a) + spread(k1) + np.abs(xh) * spread(k2)
+    e_dx = spread(rstd) * (e_a + spread(e_k1) + e_xh * spread(k2) + np.abs(xh) * spread(e_k2) + 4 * U * parts) \
+        + spread(rstd) * parts * (spread(r_rstd) + 2 * U)
+    chain = b * n / 8 + 64
+    e_dg = (e_dv * np.abs(xh) + np.abs(dv) * e_xh).sum(axis=(0, 1)) + chain * U * np.abs(dv * xh).sum(axis=(0, 1))
+    e_db = e_dv.sum(axis=(0, 1)) + chain * U * np.abs(dv).sum(axis=(0, 1))
+    return res + [e_dx, e_dg, e_db], e_v, v
+
+
+def run_norm(capi, x, gamma, beta, groups, eps, act, dy=None, off=0, params=True):
+    L = capi.lib()
+    b, n, c = x.shape
+    a = capi.ACTIVATIONS[act]
+    dx_, dg, db = In(capi, x, off), gamma is not None and In(capi, gamma, off), beta is not None and In(capi, beta, off)
+    pg, pb = (ptr(dg) if dg else None), (ptr(db) if db else None)
+    y, mean, rstd = Out(capi, x.shape, off), Out(capi, (b, groups)), Out(capi, (b, groups))
+    size = capi.group_norm_workspace(b, n, c, groups)
+    work = Out(capi, ((size + 3) // 4,))
+    capi.check(L.fz_group_norm(y.ptr, mean.ptr, rstd.ptr, dx_.ptr, pg, pb, b, n, c, groups, eps, a, work.ptr, size, None))
+    res = [y.get(), mean.get(), rstd.get()]
+    work.get()
+    if dy is None:
+        return res
+    size = capi.group_norm_workspace(b, n, c, groups, True)
+    work = Out(capi, ((size + 3) // 4,))
+    dd = In(capi, dy, off)
+    gx, gg, gb = Out(capi, x.shape, off), Out(capi, (c,), off), Out(capi, (c,), off)
+    capi.check(L.fz_group_norm_backward(gx.ptr, gg.ptr if params else None, gb.ptr if params else None, dd.ptr,
+                                        dx_.ptr, mean.ptr, rstd.ptr, pg, pb, b, n, c, groups, a, work.ptr, size, None))
+    work.get()
+    return res + [gx.get()] + ([gg.get(), gb.get()] if params else [])
+
+
+# (batch, len, channels, groups): one value; odd groups; the MLP's rows; 10, 3, 2 and 1 channels a
+# group; groups of 4 and more than one CTA holds; one group of many channels; many small samples;
+# more samples than CTAs; a long sample with few channels, and a large one
+NORM_SHAPES = [(1, 1, 1, 1), (3, 1, 8, 2), (2, 5, 12, 4), (4, 1, 4096, 32), (2, 37, 320, 32), (1, 1, 3, 1),
+               (3, 100, 6, 6), (2, 4096, 64, 8), (1, 16384, 8, 2), (65, 1, 100, 1), (5, 7, 36, 9), (2, 130, 1000, 1),
+               (1, 3, 20000, 2), (1000, 3, 8, 1), (4000, 1, 64, 4), (1, 30011, 16, 4), (2, 1024, 256, 32),
+               (1, 65536, 32, 1), (3, 257, 68, 17), (9, 33, 1024, 64), (1, 2, 40000, 1), (300, 2, 2048, 1)]
+
+
+@pytest.mark.parametrize("shape", NORM_SHAPES, ids=str)
+@pytest.mark.parametrize("act,affine,off", [("silu", True, 0), ("gelu", True, 1), ("none", False, 0)])
+def test_group_norm(capi, shape, act, affine, off):
+    b, n, c, groups = shape
+    rng = np.random.default_rng(b * 7 + n * 3 + c)
+    x = (rng.standard_normal((b, n, c)) * 1.5 + 0.7).astype(np.float32)
+    dy = rng.standard_normal((b, n, c)).astype(np.float32)
+    gamma = (1 + 0.3 * rng.standard_normal(c)).astype(np.float32) if affine else None
+    beta = (0.2 * rng.standard_normal(c)).astype(np.float32) if affine else None
+    got = run_norm(capi, x, gamma, beta, groups, 1e-5, act, dy, off)
+    want = O.group_norm(x, gamma, beta, groups, 1e-5, act, dy)
+    bounds, _, _ = norm_bounds(x, gamma, beta, groups, 1e-5, act, dy)
+    for name, g, w, e in zip(("y", "mean", "rstd", "dx", "dgamma", "dbeta"), got, want, bounds):
+        close(g, w, e, name)
+    again = run_norm(capi, x, gamma, beta, groups, 1e-5, act, dy, off)
+    for g, h in zip(got, again):
+        np.testing.assert_array_equal(g.view(np.uint32), h.view(np.uint32))
+
+
+@pytest.mark.parametrize("shape", [(4, 1, 4096, 32), (2, 37, 320, 32), (1, 16384, 8, 2)], ids=str)
+def test_group_norm_relu(capi, shape):
+    """ReLU's slope jumps at zero: the inputs keep away from it by more than v's error."""
+    b, n, c, groups = shape
+    rng = np.random.default_rng(11)
+    x = rng.standard_normal((b, n, c)).astype(np.float32)
+    dy = rng.standard_normal((b, n, c)).astype(np.float32)
+    gamma, beta = np.ones(c, np.float32), np.zeros(c, np.float32)
+    for _ in range(4):  # move values near zero away from it
+        bounds, e_v, v = norm_bounds(x, gamma, beta, groups, 1e-5, "relu", dy)
+        x = np.where(np.abs(v) < 1e-2, x + np.float32(0.05), x)
+    bounds, e_v, v = norm_bounds(x, gamma, beta, groups, 1e-5, "relu", dy)
+    assert np.all(np.abs(v) > 2 * e_v)
+    got = run_norm(capi, x, gamma, beta, groups, 1e-5, "relu", dy)
+    want = O.group_norm(x, gamma, beta, groups, 1e-5, "relu", dy)
+    for name, g, w, e in zip(("y", "mean", "rstd", "dx", "dgamma", "dbeta"), got, want, bounds):
+        close(g, w, e, name)
+
+
+@pytest.mark.parametrize("shape", [(4, 1, 256, 4), (3, 600, 64, 2), (1, 40000, 8, 1)], ids=str)
+def test_group_norm_offset_and_constant(capi, shape):
+    """A large common offset costs no more digits than x lost by it; a constant group has
+    variance 0, and its result is beta."""
+    b, n, c, groups = shape
+    rng = np.random.default_rng(12)
+    x = (rng.standard_normal((b, n, c)) + 1000).astype(np.float32)
+    x[0, :, : c // groups] = 3.25
+    beta = rng.standard_normal(c).astype(np.float32)
+    gamma = np.ones(c, np.float32)
+    got = run_norm(capi, x, gamma, beta, groups, 1e-5, "none")
+    want = O.group_norm(x, gamma, beta, groups, 1e-5, "none")
+    bounds, _, _ = norm_bounds(x, gamma, beta, groups, 1e-5, "none")
+    for name, g, w, e in zip(("y", "mean", "rstd"), got, want, bounds):
+        close(g, w, e, name)
+    # variance 3.25 is exact in every order of summation, so is the group's mean
+    np.testing.assert_array_equal(got[0][0, :, : c // groups], np.broadcast_to(beta[: c // groups], (n, c // groups)))
+
+
+@pytest.mark.parametrize("shape", [(6, 1, 64, 4), (3, 50, 40, 4), (2, 9000, 16, 2)], ids=str)
+def test_group_norm_nan_stays_in_its_group(capi, shape):
+    b, n, c, groups = shape
+    rng = np.random.default_rng(13)
+    x = rng.standard_normal((b, n, c)).astype(np.float32)
+    clean = run_norm(capi, x, None, None, groups, 1e-5, "silu")[0]
+    x[1, n // 2, 0] = np.nan
+    x[0, 0, c - 1] = np.inf
+    y = run_norm(capi, x, None, None, groups, 1e-5, "silu")[0]
+    hit = np.zeros((b, n, c), bool)
+    hit[1, :, : c // groups] = True
+    hit[0, :, c - c // groups:] = True
+    assert np.isnan(y[1, :, : c // groups]).all() and np.isnan(y[0, :, c - c // groups:]).any()
+    np.testing.assert_array_equal(y[~hit], clean[~hit])
+
+
+def test_group_norm_partial_results(capi):
+    """mean and rstd, and the parameters' gradients, are optional; an empty batch has zero
+    gradients."""
+    L = capi.lib()
+    rng = np.random.default_rng(14)
+    x, dy = rng.standard_normal((2, 3, 8)).astype(np.float32), rng.standard_normal((2, 3, 8)).astype(np.float32)
+    y, d = Out(capi, x.shape), In(capi, x)
+    size = capi.group_norm_workspace(2, 3, 8, 2)
+    work = Out(capi, ((size + 3) // 4,))
+    capi.check(L.fz_group_norm(y.ptr, None, None, d.ptr, None, None, 2, 3, 8, 2, 1e-5, 0, work.ptr, size, None))
+    full = run_norm(capi, x, None, None, 2, 1e-5, "none", dy)
+    np.testing.assert_array_equal(y.get(), full[0])
+    np.testing.assert_array_equal(run_norm(capi, x, None, None, 2, 1e-5, "none", dy, params=False)[3], full[3])
+    dg, db = Out(capi, (8,)), Out(capi, (8,))
+    size = capi.group_norm_workspace(0, 3, 8, 2, True)
+    work = Out(capi, ((size + 3) // 4,))
+    capi.check(L.fz_group_norm_backward(None, dg.ptr, db.ptr, None, None, None, None, None, None, 0, 3, 8, 2, 0,
+                                        work.ptr, size, None))
+    assert not dg.get().any() and not db.get().any()
+
+
+def test_group_norm_gradient_by_differences(capi):
+    """<dx, h> against the central difference of the kernel's own forward along h."""
+    rng = np.random.default_rng(15)
+    shape, groups, eps = (3, 20, 24), 4, 1e-3
+    x, dy, h = (rng.standard_normal(shape).astype(np.float32) for _ in range(3))
+    gamma, beta = rng.standard_normal(24).astype(np.float32), rng.standard_normal(24).astype(np.float32)
+    step = np.float32(2.0 ** -6)
+    dx = run_norm(capi, x, gamma, beta, groups, eps, "gelu", dy)[3].astype(np.float64)
+    hi, lo = x + step * h, x - step * h
+    f = lambda z: (run_norm(capi, z, gamma, beta, groups, eps, "gelu")[0].astype(np.float64) * dy).sum()  # noqa: E731
+    slope = (f(hi) - f(lo)) / (2 * float(step))
+    # the difference's own error: its third-order term, measured at a doubled step in 64 bits,
+    # and the forward's roundings over the step
+    g = lambda s: ((O.group_norm(x + s * h, gamma, beta, groups, eps, "gelu")[0] - O.group_norm(  # noqa: E731
+        x - s * h, gamma, beta, groups, eps, "gelu")[0]) * dy).sum() / (2 * s)
+    curve = abs(g(2 * float(step)) - g(float(step)))
+    e_y = norm_bounds(x, gamma, beta, groups, eps, "gelu")[0][0]
+    bound = curve + 1.2 * (e_y * np.abs(dy)).sum() / float(step)
+    assert abs(slope - (dx * h).sum()) <= bound
+
+
+# ---------------------------------------------------------------- router
+
+
+def run_route(capi, z, k, renorm, dw=None):
+    L = capi.lib()
+    t, e = z.shape
+    d, w, ids = In(capi, z), Out(capi, (t, k)), Out(capi, (t, k), dtype=np.int32)
+    capi.check(L.fz_route(w.ptr, ids.ptr, d.ptr, t, e, k, renorm, None))
+    if dw is None:
+        return w.get(), ids.get()
+    g, dz = In(capi, dw), Out(capi, (t, e))
+    capi.check(L.fz_route_backward(dz.ptr, g.ptr, w.ptr, ids.ptr, d.ptr, t, e, k, renorm, None))
+    return w.get(), ids.get(), dz.get()
+
+
+@pytest.mark.parametrize("t,e,k", [(1, 1, 1), (5, 3, 3), (33, 32, 4), (7, 33, 2), (1000, 64, 8), (17, 100, 1),
+                                   (9, 256, 32), (4, 300, 5), (3, 513, 8), (2, 1024, 32), (70001, 8, 2)])
+@pytest.mark.parametrize("renorm", [True, False])
+def test_route(capi, t, e, k, renorm):
+    rng = np.random.default_rng(t + e)
+    z = (rng.standard_normal((t, e)) * 3).astype(np.float32)
+    z[: t // 2] = np.round(z[: t // 2])  # ties
+    z[rng.random((t, e)) < 0.1] = -np.inf
+    z[rng.random((t, e)) < 0.05] = -0.0
+    z[0] = -np.inf if t > 4 else z[0]
+    dw = rng.standard_normal((t, k)).astype(np.float32)
+    sample = slice(None) if t < 2000 else np.r_[0:500, t - 500:t]
+    w, ids, dz = (a[sample] for a in run_route(capi, z, k, renorm, dw))
+    w64, i64, dz64 = O.route(z[sample], k, renorm, dw[sample])
+    np.testing.assert_array_equal(ids, i64)
+    # exp's argument (exact to u |d|, |d| the distance below the largest), exp, a sum of at
+    # most E / 32 + 5 additions of such terms, the quotient
+    far = np.where(np.isfinite(z), np.nanmax(np.where(np.isfinite(z), z, -1e9), axis=1, keepdims=True) - z, 0)[sample].max()
+    rel = U * (2 * far + e / 32 + k + 24)
+    close(w, w64, rel * w64, "weights")
+    terms = (np.abs(w64) * np.abs(dw[sample])).sum(1, keepdims=True)
+    close(dz, dz64, (rel + (k + 8) * U) * (np.abs(dw[sample]).max(1, keepdims=True) + terms), "dlogits")
+    if renorm:
+        assert not dz[dz64 == 0].any()
+
+
+def test_route_specials(capi):
+    """NaN ranks first and makes its token's weights NaN, other tokens keep theirs; the
+    type's lowest value is a number like others; equal logits go to the lowest experts."""
+    low = np.finfo(np.float32).min
+    z = np.array([[0, np.nan, 1, 2], [low, low, low, low], [-np.inf, low, -np.inf, -np.inf], [5, 5, 5, 5],
+                  [-np.inf] * 4, [0.0, -0.0, 0.0, -0.0]], np.float32)
+    w, ids = run_route(capi, z, 2, True)
+    np.testing.assert_array_equal(ids, [[1, 3], [0, 1], [1, -1], [0, 1], [-1, -1], [0, 1]])
+    assert np.isnan(w[0]).all()
+    np.testing.assert_array_equal(w[1:], np.float32([[.5, .5], [1, 0], [.5, .5], [0, 0], [.5, .5]]))
+    w, ids, dz = run_route(capi, z, 2, False, np.ones((6, 2), np.float32))
+    assert np.isnan(dz[0]).all() and not np.isnan(dz[1:]).any() and not dz[4].any()
+
+
+def test_route_backward_ignores_foreign_ids(capi):
+    """Ids that name no expert take no part (and touch no memory outside the row)."""
+    L = capi.lib()
+    z, w = np.zeros((2, 4), np.float32), np.full((2, 2), 0.5, np.float32)
+    ids = np.array([[1, 1000000], [-7, 4]])
+    a = [In(capi, v) for v in (np.ones((2, 2)), w, ids, z)]
+    dz = Out(capi, (2, 4))
+    capi.check(L.fz_route_backward(dz.ptr, *[v.ptr for v in a], 2, 4, 2, 1, None))
+    np.testing.assert_array_equal(dz.get(), [[0, 0.25, 0, 0], [0, 0, 0, 0]])
+
+
+# ---------------------------------------------------------------- experts
+
+
+def run_sort(capi, ids, e, cap):
+    t, k = ids.shape
+    rows = e * cap if cap else t * k
+    d = In(capi, ids)
+    outs = [Out(capi, s, dtype=np.int32) for s in ((t, k), (rows,), (e,), (e + 1,))]
+    capi.check(capi.lib().fz_expert_sort(*[o.ptr for o in outs], d.ptr, t, k, e, cap, None))
+    return [o.get() for o in outs]
+
+
+@pytest.mark.parametrize("t,k,e,cap", [(1, 1, 1, 0), (1, 2, 4, 1), (16, 2, 64, 0), (31, 3, 7, 0), (1000, 4, 8, 300),
+                                       (1000, 4, 8, 700), (4097, 2, 5, 0), (9000, 8, 256, 250), (20000, 2, 1024, 0),
+                                       (5000, 1, 1024, 6), (300, 7, 1000, 0), (65536, 8, 64, 0), (64, 1, 3, 40000)])
+def test_expert_sort(capi, t, k, e, cap):
+    rng = np.random.default_rng(t + e)
+    ids = np.minimum((rng.random((t, k)) ** 2 * (e + 1)).astype(np.int64), e) - (rng.random((t, k)) < 0.1) * (e + 3)
+    for got, want, name in zip(run_sort(capi, ids, e, cap), O.expert_sort(ids, e, cap), ("slot", "src", "counts", "offsets")):
+        np.testing.assert_array_equal(got, want, err_msg=name)
+
+
+@pytest.mark.parametrize("ids", [np.full((70, 3), -1), np.full((70, 3), 2), np.full((5000, 2), 2 ** 31 - 1),
+                                 np.zeros((20000, 1), np.int64)], ids=["none", "one", "foreign", "first"])
+@pytest.mark.parametrize("cap", [0, 50])
+def test_expert_sort_one_sided(capi, ids, cap):
+    for got, want in zip(run_sort(capi, ids, 4, cap), O.expert_sort(ids, 4, cap)):
+        np.testing.assert_array_equal(got, want)
+
+
+def test_expert_sort_without_tokens(capi):
+    L = capi.lib()
+    for cap in (0, 5):
+        src, counts, offsets = (Out(capi, (n,), dtype=np.int32) for n in (15 if cap else 0, 3, 4))
+        capi.check(L.fz_expert_sort(None, src.ptr, counts.ptr, offsets.ptr, None, 0, 2, 3, cap, None))
+        assert (src.get() == -1).all() and not counts.get().any()
+        np.testing.assert_array_equal(offsets.get(), np.arange(4) * cap)
+
+
+EXPERT_SHAPES = [(1, 1, 1, 0, 1, 0), (16, 2, 8, 0, 4096, 0), (37, 3, 5, 11, 1001, 0), (100, 8, 16, 40, 64, 0),
+                 (5, 4, 4, 0, 516, 1), (300, 2, 3, 300, 8, 0), (64, 1, 4, 0, 2048, 0), (9, 2, 3, 2, 7, 3), (700, 5, 9, 0, 132, 0),
+                 (3, 40, 64, 2, 260, 0)]
+
+
+@pytest.mark.parametrize("t,k,e,cap,width,off", EXPERT_SHAPES)
+def test_dispatch_and_combine(capi, t, k, e, cap, width, off):
+    L = capi.lib()
+    rng = np.random.default_rng(t * 5 + width)
+    ids = rng.integers(-1, e, (t, k))
+    slot, src, _, _ = O.expert_sort(ids, e, cap)
+    n = len(src)
+    x, g = (rng.standard_normal((t, width)).astype(np.float32) for _ in range(2))
+    y = rng.standard_normal((n, width)).astype(np.float32)
+    y[src < 0] = np.nan  # rows that no choice has are never read into a result
+    w = rng.uniform(-1, 1, (t, k)).astype(np.float32)
+    dslot, dsrc = In(capi, slot), In(capi, src)
+    dx, dy, dg, dw = In(capi, x, off), In(capi, y, off), In(capi, g, off), In(capi, w)
+    rows = Out(capi, (n, width), off)
+    capi.check(L.fz_expert_dispatch(rows.ptr, dx.ptr, dslot.ptr, dsrc.ptr, t, k, n, width, None))
+    np.testing.assert_array_equal(rows.get(), O.dispatch(x, slot, n).astype(np.float32))
+
+    clean = np.where(np.isnan(y), 0, y)
+    out64, drows64, dw64 = O.combine(clean, w, slot, g)
+    held = (slot >= 0)[..., None]
+    terms = (np.abs(w)[..., None] * np.abs(clean)[np.maximum(slot, 0)] * held).sum(1)
+    out = Out(capi, (t, width), off)
+    capi.check(L.fz_expert_combine(out.ptr, dy.ptr, dw.ptr, dslot.ptr, t, k, n, width, None))
+    close(out.get(), out64, (k + 1) * U * terms, "out")
+    plain = Out(capi, (t, width), off)
+    capi.check(L.fz_expert_combine(plain.ptr, dy.ptr, None, dslot.ptr, t, k, n, width, None))
+    close(plain.get(), O.combine(clean, None, slot), (k + 1) * U * (np.abs(clean)[np.maximum(slot, 0)] * held).sum(1), "sum")
+
+    drows, dweights = Out(capi, (n, width), off), Out(capi, (t, k))
+    capi.check(L.fz_expert_combine_backward(drows.ptr, dweights.ptr, dg.ptr, dy.ptr, dw.ptr, dslot.ptr, dsrc.ptr, t, k, n,
+                                            width, None))
+    # one product, rounded once (a zero's sign aside)
+    want = np.zeros((n, width), np.float32)
+    for i, j in zip(*np.nonzero(slot >= 0)):
+        want[slot[i, j]] = w[i, j] * g[i]
+    np.testing.assert_array_equal(drows.get(), want)
+    prods = (np.abs(g)[:, None] * np.abs(clean)[np.maximum(slot, 0)] * held).sum(2)
+    close(dweights.get(), dw64, (width / 32 + 40) * U * prods, "dweights")
+    only = Out(capi, (n, width), off)
+    capi.check(L.fz_expert_combine_backward(only.ptr, None, dg.ptr, None, None, dslot.ptr, dsrc.ptr, t, k, n, width, None))
+    np.testing.assert_array_equal(only.get(), O.dispatch(g, slot, n).astype(np.float32))
+
+
+def test_combine_passes_over_foreign_slots(capi):
+    """A slot outside the rows is no choice: nothing is read or written for it."""
+    L = capi.lib()
+    slot, src = np.array([[0, 99], [-5, 1], [2 ** 31 - 1, 2]]), np.array([0, 3, 5])
+    x = np.arange(24, dtype=np.float32).reshape(3, 8)
+    a = {n: In(capi, v) for n, v in (("slot", slot), ("src", src), ("x", x), ("w", np.ones((3, 2))))}
+    rows, out, dw = Out(capi, (3, 8)), Out(capi, (3, 8)), Out(capi, (3, 2))
+    capi.check(L.fz_expert_dispatch(rows.ptr, a["x"].ptr, a["slot"].ptr, a["src"].ptr, 3, 2, 3, 8, None))
+    np.testing.assert_array_equal(rows.get(), x)
+    capi.check(L.fz_expert_combine(out.ptr, rows.ptr, a["w"].ptr, a["slot"].ptr, 3, 2, 3, 8, None))
+    np.testing.assert_array_equal(out.get(), x)
+    back = Out(capi, (3, 8))
+    capi.check(L.fz_expert_combine_backward(back.ptr, dw.ptr, a["x"].ptr, rows.ptr, a["w"].ptr, a["slot"].ptr, a["src"].ptr, 3, 2,
+                                            3, 8, None))
+    np.testing.assert_array_equal(back.get(), x)
+    np.testing.assert_array_equal(dw.get() != 0, [[True, False], [False, True], [False, True]])
+
+
+def test_rows_past_32_bit_offsets(capi):
+    """Rows whose element offsets pass 2^31 (2.2e9 floats, 8.6 GB each way)."""
+    L = capi.lib()
+    t, width, n = 64, 8192, 263000
+    rng = np.random.default_rng(3)
+    at = np.sort(rng.choice(n, t, replace=False))
+    at[-1] = n - 1
+    src = np.full(n, -1)
+    src[at] = np.arange(t)
+    x = rng.standard_normal((t, width)).astype(np.float32)
+    rows = capi.DeviceArray((n, width))
+    dx, dslot, dsrc = In(capi, x), In(capi, at[:, None]), In(capi, src)
+    out = Out(capi, (t, width))
+    capi.check(L.fz_expert_dispatch(rows.ptr, dx.ptr, dslot.ptr, dsrc.ptr, t, 1, n, width, None))
+    capi.check(L.fz_expert_combine(out.ptr, rows.ptr, None, dslot.ptr, t, 1, n, width, None))
+    np.testing.assert_array_equal(out.get(), x)
+    most = capi.DeviceArray((n,))
+    capi.check(L.fz_reduce(capi.REDOPS["max"], most.ptr, rows.ptr, n, width, 1, None))
+    m = most.numpy()
+    assert not m[src < 0].any()
+    np.testing.assert_array_equal(m[at], x.max(1))
+    rows.free()
+    capi.check(L.fz_pool_release())
+
+
+# ---------------------------------------------------------------- distillation
+
+
+def distill_bounds(z, ids, teacher, tau, lse, dloss):
+    """First-order bounds of the loss and dz, row by row; chains of at most V / 512 additions
+    and as many rescalings (6 u each) a thread."""
+    r, v = z.shape
+    k = ids.shape[1]
+    e_loss, e_dz = np.zeros(r), np.zeros((r, v))
+    for i in range(r):
+        held = (ids[i] >= 0) & (ids[i] < v)
+        at, t = ids[i][held], teacher[i][held].astype(np.float64)
+        if not held.any() or (lse is None and np.all(t == -np.inf)):
+            continue
+        z64 = z[i].astype(np.float64)
+
+        def log_sum(x):
+            m = x.max(initial=-np.inf)
+            arg = np.where(np.isfinite(x), (x - m) / tau, 0)
+            ex = np.where(np.isfinite(x), np.exp(arg), 0)
+            s = ex.sum()
+            err = U * ((ex * (4 * np.abs(arg) + 5)).sum() / s + v / 512 * 3 + 64) + 4 * U * abs(np.log(s))
+            return m, np.log(s), err
+
+        with np.errstate(all="ignore"):
+            m, ls, e_ls = log_sum(z64)
+            arg = np.where(np.isfinite(z64), (z64 - m) / tau, 0)
+            q, e_q = np.where(np.isfinite(z64), np.exp(arg - ls), 0), 4 * U * np.abs(arg) + e_ls + 8 * U
+            if lse is None:
+                tm, tls, e_tls = log_sum(t)
+                e_tls += k * U
+                logp = (t - tm) / tau - tls
+                e_p = np.where(np.isfinite(t), 4 * U * np.abs((t - tm) / tau) + e_tls + 4 * U, 0)
+            else:
+                logp = t / tau - np.float64(lse[i])
+                e_p = np.where(np.isfinite(t), 3 * U * (np.abs(t / tau) + abs(float(lse[i]))) + 4 * U, 0)
+            p = np.exp(logp)
+            logq = arg[at] - ls
+            gap = np.where(p > 0, np.abs(logp - logq), 0)
+            e = (p * ((e_p + 6 * U) * gap + e_p + e_q[at])).sum() + k * U * (p * gap).sum()
+            pt = 0.0
+            e_pt = (p * e_p).sum() + (k / 32 + 16) * U * p.sum()
+            g, e_g = np.zeros(v), np.zeros(v)
+            if lse is not None:
+                pt = max(0.0, 1 - p.sum())
+                out = np.ones(v, bool)
+                out[at] = False
+                if pt > 0:
+                    om, ol, e_ol = log_sum(z64[out])
+                    lqt = (om - m) / tau + ol - ls
+                    e += e_pt * (abs(np.log(pt) - lqt) + 1) + pt * (e_ol + e_ls + 8 * U * (abs(lqt) + abs(np.log(pt)) + 1))
+                    qt = np.exp(np.where(np.isfinite(z64), (z64 - om) / tau - ol, -np.inf))
+                    e_qt = 4 * U * np.abs(np.where(np.isfinite(z64), (z64 - om) / tau, 0)) + e_ol + 8 * U
+                    e_g[out] += (pt * qt * (e_qt + 4 * U) + e_pt * qt)[out]
+            mass = p.sum() + pt
+            e_g += mass * q * (e_q + 4 * U) + (e_pt + 2 * U) * q + (k / 32 + 16) * U * q
+            np.add.at(e_g, at, p * (e_p + (k + 4) * U))
+            g = mass * q
+            e_loss[i] = tau * tau * (e + 8 * U * (p * gap).sum())
+            e_dz[i] = tau * abs(float(dloss[i])) * (e_g + 4 * U * g)
+    return e_loss, e_dz
+
+
+def run_distill(capi, z, ids, teacher, tau, lse, dloss, off=0, pitch=0):
+    L = capi.lib()
+    r, v = z.shape
+    k = ids.shape[1]
+    ld = v + pitch
+    wide = np.full((r, ld), np.nan, np.float32)  # columns behind the vocabulary are never read
+    wide[:, :v] = z
+    a = [In(capi, wide, off), In(capi, ids), In(capi, teacher), In(capi, dloss)]
+    dl = None if lse is None else In(capi, lse)
+    loss, stats = Out(capi, (r,)), Out(capi, (r, 4))
+    capi.check(L.fz_distill(loss.ptr, stats.ptr, a[0].ptr, ld, a[1].ptr, a[2].ptr, ptr(dl), r, v, k, tau, None))
+    ldd = v + (pitch + 1 if pitch else 0)
+    dz = Out(capi, (r, ldd), off)
+    capi.check(L.fz_distill_backward(dz.ptr, ldd, a[3].ptr, stats.ptr, a[0].ptr, ld, a[1].ptr, a[2].ptr, ptr(dl), r, v, k,
+                                     tau, None))
+    got = dz.get()
+    assert np.all(got[:, v:] == SENTINEL), "columns behind the vocabulary were written"
+    return loss.get(), got[:, :v]
+
+
+def distill_inputs(rng, r, v, k, tau, tail):
+    z = (rng.standard_normal((r, v)) * 2).astype(np.float32)
+    ids = np.stack([rng.permutation(v)[:k] for _ in range(r)])
+    t = -np.sort(-(rng.standard_normal((r, k)) * 2 + 3).astype(np.float32))
+    ids[rng.random((r, k)) < 0.1] = -1
+    if r > 2:
+        ids[1] = -1
+        ids[2] = v + 5
+    lse = None
+    if tail:
+        inside = np.where((ids >= 0) & (ids < v), np.exp(t.astype(np.float64) / tau), 0).sum(1)
+        lse = np.log(np.maximum(inside, 1e-3) / rng.uniform(0.3, 0.99, r)).astype(np.float32)
+    return z, ids, t, lse, (rng.standard_normal(r)).astype(np.float32)
+
+
+# (rows, vocab, k, tau, alignment offset, extra pitch)
+DISTILL_SHAPES = [(1, 1, 1, 1.0, 0, 0), (4, 5, 5, 2.0, 0, 0), (3, 130, 7, 1.0, 1, 0), (5, 1000, 64, 0.5, 0, 3), (2, 50001, 33, 4.0, 2, 0),
+                  (1, 131072, 8, 1.0, 0, 0), (400, 515, 20, 2.0, 3, 2), (7, 32768, 256, 1.0, 0, 0), (3, 9000, 1024, 1.0, 0, 0),
+                  (320, 4099, 3, 1.0, 0, 0), (2, 262144, 100, 2.0, 1, 1)]
+
+
+@pytest.mark.parametrize("r,v,k,tau,off,pitch", DISTILL_SHAPES)
+@pytest.mark.parametrize("tail", [False, True])
+def test_distill(capi, r, v, k, tau, off, pitch, tail):
+    z, ids, t, lse, g = distill_inputs(np.random.default_rng(v + k), r, v, k, tau, tail)
+    loss, dz = run_distill(capi, z, ids, t, tau, lse, g, off, pitch)
+    loss64, dz64 = O.distill(z, ids, t, tau, lse, g)
+    e_loss, e_dz = distill_bounds(z, ids, t, tau, lse, g)
+    close(loss, loss64, e_loss, "loss")
+    close(dz, dz64, e_dz, "dz")
+    again = run_distill(capi, z, ids, t, tau, lse, g, off, pitch)
+    np.testing.assert_array_equal(loss.view(np.uint32), again[0].view(np.uint32))
+    np.testing.assert_array_equal(dz.view(np.uint32), again[1].view(np.uint32))
+
+
+@pytest.mark.parametrize("tail", [False, True])
+def test_distill_repeated_ids(capi, tail):
+    """An id named twice counts its p twice, and its logit once; results do not vary."""
+    rng = np.random.default_rng(21)
+    z, ids, t, lse, g = distill_inputs(rng, 6, 3000, 40, 1.0, tail)
+    ids = rng.integers(0, 12, ids.shape) * 250
+    if tail:
+        lse = np.log(np.exp(t.astype(np.float64)).sum(1) / 0.8).astype(np.float32)
+    loss, dz = run_distill(capi, z, ids, t, 1.0, lse, g)
+    loss64, dz64 = O.distill(z, ids, t, 1.0, lse, g)
+    e_loss, e_dz = distill_bounds(z, ids, t, 1.0, lse, g)
+    close(loss, loss64, e_loss, "loss")
+    close(dz, dz64, e_dz, "dz")
+    for _ in range(3):
+        again = run_distill(capi, z, ids, t, 1.0, lse, g)
+        np.testing.assert_array_equal(dz.view(np.uint32), again[1].view(np.uint32))
+
+
+@pytest.mark.parametrize("tail", [False, True])
+def test_distill_masks(capi, tail):
+    """Masked columns at -inf and at the type's lowest value; a row of nothing but the lowest
+    value (a uniform student); a common offset of 10^4; rows whose logits are NaN but have no
+    teacher; an entry of the teacher at -inf; a NaN in one row stays in it."""
+    rng = np.random.default_rng(22)
+    low = np.finfo(np.float32).min
+    r, v, k = 8, 5000, 16
+    z, ids, t, lse, g = distill_inputs(rng, r, v, k, 1.0, tail)
+    ids = np.stack([rng.permutation(v)[:k] for _ in range(r)])
+    keep = np.ones(v, bool)
+    keep[rng.choice(v, 500, replace=False)] = False
+    keep[ids[0]] = keep[ids[1]] = True
+    z[0, ~keep] = -np.inf
+    z[1, ~keep] = low
+    z[2] = low
+    z[3] += 10000
+    z[4] = np.nan
+    ids[4] = -1
+    t[5, 3:] = -np.inf
+    z[6, 17] = np.nan
+    ids[7, 1:] = -1
+    t[7] = -np.inf
+    if tail:
+        inside = np.where(ids >= 0, np.exp(t.astype(np.float64)), 0).sum(1)
+        lse = np.log(np.maximum(inside, 1e-3) / 0.7).astype(np.float32)
+    loss, dz = run_distill(capi, z, ids, t, 1.0, lse, g)
+    ok = np.array([0, 1, 2, 3, 4, 5, 7])
+    loss64, dz64 = O.distill(z[ok], ids[ok], t[ok], 1.0, None if lse is None else lse[ok], g[ok])
+    e_loss, e_dz = distill_bounds(z[ok], ids[ok], t[ok], 1.0, None if lse is None else lse[ok], g[ok])
+    close(loss[ok], loss64, e_loss, "loss")
+    close(dz[ok], dz64, e_dz, "dz")
+    assert loss[4] == 0 and not dz[4].any()
+    assert np.isnan(loss[6]) and np.isnan(dz[6]).all()
+    if not tail:
+        assert loss[7] == 0 and not dz[7].any()
+
+
+def test_distill_student_without_mass(capi):
+    """The student gives a teacher's entry no probability: the loss is infinite, the gradient
+    q - p is not."""
+    z = np.zeros((1, 6), np.float32)
+    z[0, 2] = -np.inf
+    loss, dz = run_distill(capi, z, np.array([[2, 3]]), np.zeros((1, 2), np.float32), 1.0, None, np.ones(1, np.float32))
+    assert loss[0] == np.inf
+    close(dz, np.array([[.2, .2, -.5, -.3, .2, .2]]), 8 * U, "dz")
+
+
+def test_distill_sure_student(capi):
+    """The tail's mass far below one rounding of the whole: its log and gradient keep their
+    digits."""
+    rng = np.random.default_rng(23)
+    z = (rng.standard_normal((3, 4000)) - 40).astype(np.float32)
+    ids = np.stack([rng.permutation(4000)[:4] for _ in range(3)])
+    np.put_along_axis(z, ids, np.float32(10), 1)
+    t = np.zeros((3, 4), np.float32)
+    lse = np.full(3, np.log(4 / 0.9), np.float32)
+    g = np.ones(3, np.float32)
+    loss, dz = run_distill(capi, z, ids, t, 1.0, lse, g)
+    loss64, dz64 = O.distill(z, ids, t, 1.0, lse, g)
+    e_loss, e_dz = distill_bounds(z, ids, t, 1.0, lse, g)
+    close(loss, loss64, e_loss, "loss")
+    close(dz, dz64, e_dz, "dz")
+    # the tail's part: qT = 4000 e^(-40 + 1/2) / (4 e^10), 0.1 (log 0.1 - log qT) = 4.03; the
+    # entries': 0.9 log(0.225 / 0.25) = -0.09
+    assert np.all(loss64 > 3.9)
+
+
+def test_distill_gradient_by_differences(capi):
+    rng = np.random.default_rng(24)
+    z, ids, t, lse, g = distill_inputs(rng, 4, 200, 6, 2.0, True)
+    h = rng.standard_normal(z.shape).astype(np.float32)
+    step = np.float32(2.0 ** -5)
+    dz = run_distill(capi, z, ids, t, 2.0, lse, g)[1].astype(np.float64)
+    f = lambda s: (run_distill(capi, z + s * h, ids, t, 2.0, lse, g)[0].astype(np.float64) * g).sum()  # noqa: E731
+    slope = (f(step) - f(-step)) / (2 * float(step))
+    f64 = lambda s: (O.distill(z + s * h.astype(np.float64), ids, t, 2.0, lse) * g).sum()  # noqa: E731
+    d = lambda s: (f64(s) - f64(-s)) / (2 * s)  # noqa: E731
+    s = float(step)
+    e_loss, _ = distill_bounds(z, ids, t, 2.0, lse, g)
+    # third-order term, the forward's roundings over the step, and the rounding of z + s h
+    # (u |z| a value, through the gradient)
+    bound = abs(d(2 * s) - d(s)) + 1.2 * (e_loss * np.abs(g)).sum() / s + U * (np.abs(dz) * (np.abs(z) + 1)).sum() / s
+    assert abs(slope - (dz * h).sum()) <= bound
+
+
+# ---------------------------------------------------------------- together
+
+
+@pytest.mark.parametrize("case", learn_cases.API_CASES, ids=lambda c: c.__name__)
+def test_api(capi, case):
+    import nova_b200
+
+    # the model case runs through the framework's 3xTF32 products, held to 1e-5 norm-wise each;
+    # four of them in a row, forward and back, add up
+    if case is learn_cases.model_step:
+        case(nova_b200.fusion, tol=4e-5)
+    else:
+        case(nova_b200.fusion)
+
+
+def test_api_refusals(capi):
+    import nova_b200
+
+    learn_cases.refusals(nova_b200.fusion)
+
+
+def test_two_streams_and_graph_replay(capi):
+    """The same calls on a stream of the caller's, and captured into a CUDA graph that is
+    replayed on new inputs, give the same bits as on the library's stream."""
+    torch = pytest.importorskip("torch")
+    L = capi.lib()
+    gen = torch.Generator("cuda").manual_seed(1)
+    b, n, c, g, t, e, k, v, kt = 4, 70, 64, 8, 200, 16, 2, 5000, 12
+    x = torch.randn(b, n, c, generator=gen, device="cuda")
+    z = torch.randn(t, e, generator=gen, device="cuda")
+    lg = torch.randn(t, v, generator=gen, device="cuda")
+    ids = torch.randint(0, v, (t, kt), generator=gen, device="cuda", dtype=torch.int32)
+    teach = torch.randn(t, kt, generator=gen, device="cuda")
+    size = max(capi.group_norm_workspace(b, n, c, g), capi.group_norm_workspace(b, n, c, g, True), 16)
+
+    def buffers():
+        f = lambda *s: torch.zeros(s, device="cuda")  # noqa: E731
+        i = lambda *s: torch.zeros(s, device="cuda", dtype=torch.int32)  # noqa: E731
+        return dict(y=f(b, n, c), mean=f(b, g), rstd=f(b, g), dx=f(b, n, c), work=f(size // 4 + 1), w=f(t, k), ids=i(t, k),
+                    slot=i(t, k), src=i(t * k), counts=i(e), offs=i(e + 1), rows=f(t * k, e), out=f(t, e), loss=f(t), stats=f(t, 4), dz=f(t, v),
+                    one=torch.ones(t, device="cuda"))
+
+    def work(o, s):
+        p = {a: q.data_ptr() for a, q in o.items()}
+        capi.check(L.fz_group_norm(p["y"], p["mean"], p["rstd"], x.data_ptr(), None, None, b, n, c, g, 1e-5, 2, p["work"], size, s))
+        capi.check(L.fz_group_norm_backward(p["dx"], None, None, p["y"], x.data_ptr(), p["mean"], p["rstd"], None, None, b, n, c, g, 2,
+                                            p["work"], size, s))
+        capi.check(L.fz_route(p["w"], p["ids"], z.data_ptr(), t, e, k, 1, s))
+        capi.check(L.fz_expert_sort(p["slot"], p["src"], p["counts"], p["offs"], p["ids"], t, k, e, 0, s))
+        capi.check(L.fz_expert_dispatch(p["rows"], z.data_ptr(), p["slot"], p["src"], t, k, t * k, e, s))
+        capi.check(L.fz_expert_combine(p["out"], p["rows"], p["w"], p["slot"], t, k, t * k, e, s))
+        capi.check(L.fz_distill(p["loss"], p["stats"], lg.data_ptr(), v, ids.data_ptr(), teach.data_ptr(), None, t, v, kt, 1.5, s))
+        capi.check(L.fz_distill_backward(p["dz"], v, p["one"], p["stats"], lg.data_ptr(), v, ids.data_ptr(), teach.data_ptr(), None, t, v,
+                                         kt, 1.5, s))
+
+    ref, side, cap = buffers(), buffers(), buffers()
+    torch.cuda.synchronize()
+    work(ref, None)
+    stream = torch.cuda.Stream()
+    work(side, stream.cuda_stream)
+    capi.check(L.fz_stream_sync(None))
+    torch.cuda.synchronize()
+    same = lambda p, q: all(torch.equal(p[a].view(torch.int32), q[a].view(torch.int32)) for a in p if a != "work")  # noqa: E731
+    assert same(ref, side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        work(cap, torch.cuda.current_stream().cuda_stream)
+    for seed in (5, 6):
+        for a in (x, z, lg, teach):
+            a.normal_(generator=gen)
+        torch.cuda.synchronize()
+        graph.replay()
+        work(ref, None)
+        capi.check(L.fz_stream_sync(None))
+        torch.cuda.synchronize()
+        assert same(ref, cap), seed
+    # release the graph before the test ends: nothing captured outlives its buffers
+    del graph
+
+
+def test_calls_from_two_threads(capi):
+    """Two host threads, each on its own stream, with their own buffers."""
+    import threading
+
+    rng = np.random.default_rng(30)
+    jobs = [distill_inputs(rng, 20, 3000, 10, 1.0, True) for _ in range(2)]
+    want = [run_distill(capi, z, i, t, 1.0, lse, g) for z, i, t, lse, g in jobs]
+    got, errors = [None, None], []
+
+    def work(q):
+        try:
+            capi.check(capi.lib().fz_set_device(0))
+            z, i, t, lse, g = jobs[q]
+            for _ in range(20):
+                got[q] = run_distill(capi, z, i, t, 1.0, lse, g)
+        except Exception as err:  # pragma: no cover
+            errors.append(err)
+
+    threads = [threading.Thread(target=work, args=(q,)) for q in range(2)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    assert not errors
+    for a, b in zip(got, want):
+        np.testing.assert_array_equal(a[0], b[0])
+        np.testing.assert_array_equal(a[1], b[1])
