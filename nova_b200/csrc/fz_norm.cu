@@ -26,6 +26,7 @@
 
 #include <climits>
 #include <cstdint>
+#include <mutex>
 
 #include "fz_common.cuh"
 
@@ -34,10 +35,12 @@ namespace cg = cooperative_groups;
 namespace {
 
 constexpr unsigned kFull = 0xffffffffu;
-constexpr int kRowThreads = 256;
-constexpr int kTileForward = 512, kTileBackward = 256;  // threads
-// Vectors of x a tile kernel's thread holds: what the registers of two CTAs an SM leave.
-__host__ __device__ constexpr int held(int v) { return v == 4 ? 8 : v == 2 ? 12 : 16; }
+constexpr int kRowThreads = 256, kTileThreads = 256;
+constexpr int kTileCtas = 2;  // resident an SM
+constexpr int kMaxTileGroups = 16;  // groups side by side in a tile
+// Vectors of x (backward: of x and of dy) a tile kernel's thread holds: what the registers of
+// two CTAs an SM leave.
+__host__ __device__ constexpr int held(int v, bool backward) { return (v == 4 ? 16 : 32) / (backward ? 2 : 1); }
 constexpr int kMaxCluster = 16;
 
 // ---------------------------------------------------------------- activations
@@ -53,107 +56,217 @@ __device__ __forceinline__ float rcp(float x) {
   return y;
 }
 
-__device__ __forceinline__ float sigmoid(float v) {
-  return rcp(__fadd_rn(1.0f, ex2(__fmul_rn(v, -1.4426950408889634f))));
+// Paired fp32 arithmetic: one instruction for two values, each rounded as the scalar
+// instruction rounds. The row kernels would otherwise be bound by instruction issue.
+using Pair = unsigned long long;
+__device__ __forceinline__ Pair pair(float a, float b) {
+  Pair r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ Pair both(float a) { return pair(a, a); }
+__device__ __forceinline__ void unpair(Pair p, float &a, float &b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p));
+}
+__device__ __forceinline__ Pair add2(Pair a, Pair b) {
+  Pair r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ Pair mul2(Pair a, Pair b) {
+  Pair r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
+  Pair r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
 }
 
-// Phi(v) and, through e, exp(-v^2 / 2). With h = Phi(-|v|) = exp(-v^2 / 2) R(t), t = 1 /
-// (1 + 0.3 |v|): R is a polynomial of degree 8 without constant term, fitted to the least
-// largest relative error on |v| <= 14 (Remez; 1.5e-7). erff would take the forward from
-// memory- to issue-bound.
-__device__ __forceinline__ float phi(float v, float *e) {
-  const float t = rcp(__fmaf_rn(fabsf(v), 0.3f, 1.0f));
-  *e = ex2(__fmul_rn(__fmul_rn(v, v), -0.72134752044448170f));
-  float r = __fmaf_rn(0.035674769431352615f, t, -0.1572030633687973f);
-  r = __fmaf_rn(r, t, 0.20635347068309784f);
-  r = __fmaf_rn(r, t, -0.05368361622095108f);
-  r = __fmaf_rn(r, t, 0.1285616159439087f);
-  r = __fmaf_rn(r, t, 0.09991349279880524f);
-  r = __fmaf_rn(r, t, 0.12075395882129669f);
-  r = __fmaf_rn(r, t, 0.11962930113077164f);
-  const float h = __fmul_rn(__fmul_rn(r, t), *e);
-  return v < 0.0f ? h : __fsub_rn(1.0f, h);  // NaN: h is NaN
+__device__ __forceinline__ Pair sigmoid2(Pair v) {
+  float a, b;
+  unpair(mul2(v, both(-1.4426950408889634f)), a, b);
+  unpair(add2(pair(ex2(a), ex2(b)), both(1.0f)), a, b);
+  return pair(rcp(a), rcp(b));
 }
 
-template <int V>
-__device__ __forceinline__ void activate(int act, float (&v)[V]) {
-  if (act == FZ_ACT_SILU) {
-#pragma unroll
-    for (int j = 0; j < V; ++j) v[j] = __fmul_rn(v[j], sigmoid(v[j]));
-  } else if (act == FZ_ACT_GELU) {
-    float e;
-#pragma unroll
-    for (int j = 0; j < V; ++j) v[j] = __fmul_rn(v[j], phi(v[j], &e));
-  } else if (act == FZ_ACT_RELU) {
-#pragma unroll
-    for (int j = 0; j < V; ++j) v[j] = v[j] > 0.0f ? v[j] : 0.0f;
+// Phi(v) and exp(-v^2 / 2). With h = Phi(-|v|) = exp(-v^2 / 2) R(t), t = 1 / (1 + 0.3 |v|):
+// R is a polynomial of degree 8 without constant term, fitted to the least largest relative
+// error on |v| <= 14 (Remez; 1.5e-7).
+__device__ __forceinline__ Pair phi2(Pair v, Pair *e) {
+  float a, b, c, d;
+  unpair(v, a, b);
+  unpair(fma2(pair(fabsf(a), fabsf(b)), both(0.3f), both(1.0f)), c, d);
+  const Pair t = pair(rcp(c), rcp(d));
+  unpair(mul2(mul2(v, v), both(-0.72134752044448170f)), c, d);
+  *e = pair(ex2(c), ex2(d));
+  Pair r = fma2(both(0.035674769431352615f), t, both(-0.1572030633687973f));
+  r = fma2(r, t, both(0.20635347068309784f));
+  r = fma2(r, t, both(-0.05368361622095108f));
+  r = fma2(r, t, both(0.1285616159439087f));
+  r = fma2(r, t, both(0.09991349279880524f));
+  r = fma2(r, t, both(0.12075395882129669f));
+  r = fma2(r, t, both(0.11962930113077164f));
+  const Pair h = mul2(mul2(r, t), *e);
+  float g, k;
+  unpair(h, c, d);
+  unpair(fma2(h, both(-1.0f), both(1.0f)), g, k);
+  return pair(a < 0.0f ? c : g, b < 0.0f ? d : k);  // NaN: both are
+}
+
+__device__ __forceinline__ Pair activate2(int act, Pair v) {
+  if (act == FZ_ACT_SILU) return mul2(v, sigmoid2(v));
+  if (act == FZ_ACT_GELU) {
+    Pair e;
+    return mul2(v, phi2(v, &e));
   }
+  if (act == FZ_ACT_RELU) {
+    float a, b;
+    unpair(v, a, b);
+    return pair(a > 0.0f ? a : 0.0f, b > 0.0f ? b : 0.0f);
+  }
+  return v;
 }
 
-// d *= act'(v)
-template <int V>
-__device__ __forceinline__ void times_slope(int act, float (&d)[V], const float (&v)[V]) {
+// d act'(v)
+__device__ __forceinline__ Pair times_slope2(int act, Pair d, Pair v) {
   if (act == FZ_ACT_SILU) {
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const float s = sigmoid(v[j]);
-      d[j] = __fmul_rn(d[j], __fmul_rn(s, __fmaf_rn(v[j], __fsub_rn(1.0f, s), 1.0f)));
-    }
-  } else if (act == FZ_ACT_GELU) {
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      float e;
-      const float p = phi(v[j], &e);
-      d[j] = __fmul_rn(d[j], __fmaf_rn(__fmul_rn(v[j], 0.39894228040143268f), e, p));
-    }
-  } else if (act == FZ_ACT_RELU) {
-#pragma unroll
-    for (int j = 0; j < V; ++j) d[j] = v[j] > 0.0f ? d[j] : 0.0f;
+    const Pair s = sigmoid2(v), rest = fma2(s, both(-1.0f), both(1.0f));
+    return mul2(d, mul2(s, fma2(v, rest, both(1.0f))));
   }
+  if (act == FZ_ACT_GELU) {
+    Pair e;
+    const Pair p = phi2(v, &e);
+    return mul2(d, fma2(mul2(v, both(0.39894228040143268f)), e, p));
+  }
+  if (act == FZ_ACT_RELU) {
+    float a, b, x, y;
+    unpair(v, a, b);
+    unpair(d, x, y);
+    return pair(a > 0.0f ? x : 0.0f, b > 0.0f ? y : 0.0f);
+  }
+  return d;
 }
 
 // ---------------------------------------------------------------- vectors
 
+// V floats in registers as pairs (V = 1: a pair whose second value is zero and never stored).
 template <int V>
-__device__ __forceinline__ void load(float (&r)[V], const float *p) {
-  if constexpr (V == 4) {
-    const float4 q = *reinterpret_cast<const float4 *>(p);
-    r[0] = q.x, r[1] = q.y, r[2] = q.z, r[3] = q.w;
-  } else if constexpr (V == 2) {
-    const float2 q = *reinterpret_cast<const float2 *>(p);
-    r[0] = q.x, r[1] = q.y;
-  } else {
-    r[0] = *p;
-  }
-}
+struct Vec {
+  static constexpr int N = V == 4 ? 2 : 1;
+  Pair p[N];
+};
 template <int V>
-__device__ __forceinline__ void store(float *p, const float (&r)[V]) {
-  if constexpr (V == 4) *reinterpret_cast<float4 *>(p) = make_float4(r[0], r[1], r[2], r[3]);
-  else if constexpr (V == 2) *reinterpret_cast<float2 *>(p) = make_float2(r[0], r[1]);
-  else *p = r[0];
-}
-template <int V>
-__device__ __forceinline__ void load_or(float (&r)[V], const float *p, float otherwise) {
-  if (p) {
-    load(r, p);
-  } else {
+__device__ __forceinline__ Vec<V> splat(float a) {
+  Vec<V> r;
 #pragma unroll
-    for (int j = 0; j < V; ++j) r[j] = otherwise;
+  for (int i = 0; i < Vec<V>::N; ++i) r.p[i] = V == 1 ? pair(a, 0.0f) : both(a);
+  return r;
+}
+template <int V>
+__device__ __forceinline__ Vec<V> load(const float *q) {
+  Vec<V> r;
+  if constexpr (V == 4) {
+    const float4 f = *reinterpret_cast<const float4 *>(q);
+    r.p[0] = pair(f.x, f.y);
+    r.p[1] = pair(f.z, f.w);
+  } else if constexpr (V == 2) {
+    const float2 f = *reinterpret_cast<const float2 *>(q);
+    r.p[0] = pair(f.x, f.y);
+  } else {
+    r.p[0] = pair(*q, 0.0f);
   }
+  return r;
+}
+template <int V>
+__device__ __forceinline__ void store(float *q, const Vec<V> &r) {
+  float a, b, c, d;
+  unpair(r.p[0], a, b);
+  if constexpr (V == 4) {
+    unpair(r.p[1], c, d);
+    *reinterpret_cast<float4 *>(q) = make_float4(a, b, c, d);
+  } else if constexpr (V == 2) {
+    *reinterpret_cast<float2 *>(q) = make_float2(a, b);
+  } else {
+    *q = a;
+  }
+}
+template <int V>
+__device__ __forceinline__ Vec<V> load_or(const float *q, float otherwise) {
+  return q ? load<V>(q) : splat<V>(otherwise);
+}
+// Tiles are fetched ahead through shared memory that each thread has to itself: it copies
+// the vectors that it will process a few tiles later, asynchronously, waits for its own
+// copies and reads them back, so no barrier is needed and no registers are held meanwhile.
+template <int V>
+__device__ __forceinline__ void copy_async(float *to, const float *from) {
+  const uint32_t dst = (uint32_t)__cvta_generic_to_shared(to);
+  if constexpr (V == 4) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(from) : "memory");
+  else if constexpr (V == 2) asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(from) : "memory");
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-// (n, mean, M2) of a union.
-struct Moments {
-  float n, mean, m2;
-};
-__device__ __forceinline__ Moments join(Moments a, Moments b) {
-  if (b.n == 0.0f) return a;
-  if (a.n == 0.0f) return b;
-  const float n = __fadd_rn(a.n, b.n), d = __fsub_rn(b.mean, a.mean), f = __fdiv_rn(b.n, n);
-  return {n, __fmaf_rn(d, f, a.mean), __fmaf_rn(__fmul_rn(d, d), __fmul_rn(a.n, f), __fadd_rn(a.m2, b.m2))};
+// The sum of a vector's values.
+template <int V>
+__device__ __forceinline__ float total(const Vec<V> &r) {
+  float a, b;
+  unpair(V == 4 ? add2(r.p[0], r.p[Vec<V>::N - 1]) : r.p[0], a, b);
+  return V == 1 ? a : __fadd_rn(a, b);
 }
-__device__ __forceinline__ float rstd_of(float m2, float m, float eps) {
-  return __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(__fdiv_rn(m2, m), eps)));
+// s += x; s += (x - mean)^2
+template <int V>
+__device__ __forceinline__ void sum_into(Vec<V> &s, const Vec<V> &x) {
+#pragma unroll
+  for (int i = 0; i < Vec<V>::N; ++i) s.p[i] = add2(s.p[i], x.p[i]);
+}
+template <int V>
+__device__ __forceinline__ void square_into(Vec<V> &s, const Vec<V> &x, Pair minus_mean) {
+#pragma unroll
+  for (int i = 0; i < Vec<V>::N; ++i) {
+    const Pair d = add2(x.p[i], minus_mean);
+    s.p[i] = fma2(d, d, s.p[i]);
+  }
+}
+// act(gamma (x - mean) rstd + beta)
+template <int V>
+__device__ __forceinline__ Vec<V> normalize(int act, const Vec<V> &x, Pair minus_mean, Pair rstd, const Vec<V> &gamma,
+                                            const Vec<V> &beta) {
+  Vec<V> r;
+#pragma unroll
+  for (int i = 0; i < Vec<V>::N; ++i)
+    r.p[i] = activate2(act, fma2(mul2(add2(x.p[i], minus_mean), rstd), gamma.p[i], beta.p[i]));
+  return r;
+}
+// x <- xh, d <- dv gamma; dv and dv xh are added to db and dg
+template <int V>
+__device__ __forceinline__ void gradient(int act, Vec<V> &x, Vec<V> &d, Vec<V> &db, Vec<V> &dg, Pair minus_mean,
+                                         Pair rstd, const Vec<V> &gamma, const Vec<V> &beta) {
+#pragma unroll
+  for (int i = 0; i < Vec<V>::N; ++i) {
+    x.p[i] = mul2(add2(x.p[i], minus_mean), rstd);
+    const Pair dv = times_slope2(act, d.p[i], fma2(x.p[i], gamma.p[i], beta.p[i]));
+    db.p[i] = add2(db.p[i], dv);
+    dg.p[i] = fma2(dv, x.p[i], dg.p[i]);
+    d.p[i] = mul2(dv, gamma.p[i]);
+  }
+}
+// rstd (d - k1 - xh k2)
+template <int V>
+__device__ __forceinline__ Vec<V> finish(const Vec<V> &xh, const Vec<V> &d, Pair minus_k1, Pair minus_k2, Pair rstd) {
+  Vec<V> r;
+#pragma unroll
+  for (int i = 0; i < Vec<V>::N; ++i) r.p[i] = mul2(rstd, fma2(xh.p[i], minus_k2, add2(d.p[i], minus_k1)));
+  return r;
+}
+
+__device__ __forceinline__ float rstd_of(float m2, float inv_m, float eps) {
+  return rsqrtf(__fmaf_rn(m2, inv_m, eps));
 }
 
 struct Norm {
@@ -165,26 +278,45 @@ struct Norm {
   float *stat;  // two-launch tiles: statistics of a group's tiles
   int64_t batch, len, channels;
   int groups, c;  // c: channels a group
-  float m, eps;
+  float m, inv_m, eps;  // inv_m = 1 / m
   int act;
 };
 
 // ---------------------------------------------------------------- row kernels
 
-// Sum over the P lanes (or, P = kRowThreads, threads) of a team.
-template <int P>
-__device__ __forceinline__ float team_sum(float v, float *sh) {
+// The sums of U values each over the P lanes (or, P = kRowThreads and U = 1, threads) of a
+// team. Four values go through one butterfly: after the two steps that halve how many
+// values a lane carries, lane l holds (a part of) value which(l), and `done` of its whole
+// sum is computed once for it; every lane then fetches all U.
+template <int P, int U, class Done>
+__device__ __forceinline__ void team_sums(float (&v)[U], float *sh, Done done) {
+  const int lane = threadIdx.x & 31;
+  if constexpr (U == 4 && P <= 32) {
+    const bool hi = lane & (P / 2), lo = lane & (P / 4);
+    float a = __fadd_rn(hi ? v[2] : v[0], __shfl_xor_sync(kFull, hi ? v[0] : v[2], P / 2));
+    float b = __fadd_rn(hi ? v[3] : v[1], __shfl_xor_sync(kFull, hi ? v[1] : v[3], P / 2));
+    a = __fadd_rn(lo ? b : a, __shfl_xor_sync(kFull, lo ? a : b, P / 4));
 #pragma unroll
-  for (int d = (P < 32 ? P : 32) / 2; d > 0; d >>= 1) v = __fadd_rn(v, __shfl_xor_sync(kFull, v, d));
-  if constexpr (P > 32) {
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = v;
-    __syncthreads();
-    v = sh[0];
+    for (int d = P / 8; d > 0; d >>= 1) a = __fadd_rn(a, __shfl_xor_sync(kFull, a, d));
+    a = done(a);
 #pragma unroll
-    for (int w = 1; w < P / 32; ++w) v = __fadd_rn(v, sh[w]);
+    for (int u = 0; u < 4; ++u) v[u] = __shfl_sync(kFull, a, (u >> 1) * (P / 2) + (u & 1) * (P / 4), P);
+  } else {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+#pragma unroll
+      for (int d = (P < 32 ? P : 32) / 2; d > 0; d >>= 1) v[u] = __fadd_rn(v[u], __shfl_xor_sync(kFull, v[u], d));
+      if constexpr (P > 32) {
+        __syncthreads();
+        if (lane == 0) sh[threadIdx.x >> 5] = v[u];
+        __syncthreads();
+        v[u] = sh[0];
+#pragma unroll
+        for (int w = 1; w < P / 32; ++w) v[u] = __fadd_rn(v[u], sh[w]);
+      }
+      v[u] = done(v[u]);
+    }
   }
-  return v;
 }
 
 // Teams id, id + stride, ... belong to P lanes each, stride a multiple of groups, so a
@@ -211,177 +343,245 @@ struct RowTeam {
     }
   }
 };
-
-template <int V, int P, int NV, int U>
-__global__ void __launch_bounds__(kRowThreads) norm_rows_kernel(const Norm a, int stride) {
-  pdl_wait();
-  __shared__ float sh[kRowThreads / 32];
-  const RowTeam<V, P, NV> t(a, stride);
-  const int parts = stride / a.groups;
-  const int64_t sample = a.len * a.channels;
-  for (int64_t b0 = 0; b0 < a.batch; b0 += (int64_t)parts * U) {
-    float x[U][NV][V], mean[U], rstd[U];
-    bool on[U];
-    int64_t base[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int64_t b = b0 + (int64_t)u * parts + t.part;
-      on[u] = t.on && b < a.batch;
-      base[u] = b * sample + (int64_t)t.g * a.c;
+// gamma and beta of a lane's vectors: in registers where there are few, else from L1
+template <int V, int NV>
+struct Affine {
+  static constexpr bool kKeep = NV <= 2;
+  Vec<V> gamma[kKeep ? NV : 1], beta[kKeep ? NV : 1];
+  __device__ Affine(const Norm &a, const int (&channel)[NV]) {
+    if constexpr (kKeep)
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
-        if (on[u] && t.at[i] >= 0) {
-          load(x[u][i], a.x + base[u] + t.at[i]);
-        } else {
-#pragma unroll
-          for (int j = 0; j < V; ++j) x[u][i][j] = 0.0f;
-        }
+        gamma[i] = load_or<V>(a.gamma ? a.gamma + channel[i] : nullptr, 1.0f);
+        beta[i] = load_or<V>(a.beta ? a.beta + channel[i] : nullptr, 0.0f);
       }
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      float s = 0.0f;
-#pragma unroll
-      for (int i = 0; i < NV; ++i)
-#pragma unroll
-        for (int j = 0; j < V; ++j) s = __fadd_rn(s, x[u][i][j]);
-      mean[u] = s;
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) mean[u] = __fdiv_rn(team_sum<P>(mean[u], sh), a.m);
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      float s = 0.0f;
-#pragma unroll
-      for (int i = 0; i < NV; ++i)
-        if (t.at[i] >= 0)
-#pragma unroll
-          for (int j = 0; j < V; ++j) {
-            const float d = __fsub_rn(x[u][i][j], mean[u]);
-            s = __fmaf_rn(d, d, s);
-          }
-      rstd[u] = s;
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) rstd[u] = rstd_of(team_sum<P>(rstd[u], sh), a.m, a.eps);
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      if (t.at[i] < 0) continue;
-      float ga[V], be[V];
-      load_or(ga, a.gamma ? a.gamma + t.channel[i] : nullptr, 1.0f);
-      load_or(be, a.beta ? a.beta + t.channel[i] : nullptr, 0.0f);
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        if (!on[u]) continue;
-        float v[V];
-#pragma unroll
-        for (int j = 0; j < V; ++j)
-          v[j] = __fmaf_rn(__fmul_rn(__fsub_rn(x[u][i][j], mean[u]), rstd[u]), ga[j], be[j]);
-        activate(a.act, v);
-        store(a.y + base[u] + t.at[i], v);
-      }
-    }
-    if (a.mean && threadIdx.x % P == 0)
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (on[u]) {
-          const int64_t team = (b0 + (int64_t)u * parts + t.part) * a.groups + t.g;
-          a.mean[team] = mean[u];
-          a.rstd[team] = rstd[u];
-        }
   }
+  __device__ __forceinline__ void get(const Norm &a, const int (&channel)[NV], int i, Vec<V> &ga, Vec<V> &be) const {
+    if constexpr (kKeep) {
+      ga = gamma[i];
+      be = beta[i];
+    } else {
+      ga = load_or<V>(a.gamma ? a.gamma + channel[i] : nullptr, 1.0f);
+      be = load_or<V>(a.beta ? a.beta + channel[i] : nullptr, 0.0f);
+    }
+  }
+};
+
+// The row kernels' shape by vectors a lane: teams in flight U, resident CTAs an SM, and
+// stages fetched ahead (about 190 KB an SM in all).
+__host__ __device__ constexpr int row_u(int p, int nv) { return p > 32 ? 1 : nv == 1 ? 4 : nv == 2 ? 2 : 1; }
+__host__ __device__ constexpr int row_ctas(bool backward, int nv) {
+  return backward ? (nv == 8 ? 1 : 2) : 3;
+}
+__host__ __device__ constexpr int row_stages(bool backward, int nv) { return backward ? 3 : nv == 8 ? 2 : 4; }
+__host__ __device__ constexpr int row_smem(bool backward, int p, int nv, int v) {
+  return row_stages(backward, nv) * (backward ? 2 : 1) * kRowThreads * row_u(p, nv) * nv * v * 4;
 }
 
-template <int V, int P, int NV, int U>
-__global__ void __launch_bounds__(kRowThreads) norm_rows_backward_kernel(const Norm a, int stride) {
+template <int V, int P, int NV>
+__global__ void __launch_bounds__(kRowThreads, row_ctas(false, NV)) norm_rows_kernel(const Norm a, int stride) {
   pdl_wait();
+  constexpr int U = row_u(P, NV), S = row_stages(false, NV);
+  extern __shared__ __align__(16) float fifo[];  // [S][U][NV][threads] vectors
   __shared__ float sh[kRowThreads / 32];
   const RowTeam<V, P, NV> t(a, stride);
-  const int parts = stride / a.groups;
-  const int64_t sample = a.len * a.channels;
-  float db[NV][V], dg[NV][V];
-#pragma unroll
-  for (int i = 0; i < NV; ++i)
-#pragma unroll
-    for (int j = 0; j < V; ++j) db[i][j] = dg[i][j] = 0.0f;
-  for (int64_t b0 = 0; b0 < a.batch; b0 += (int64_t)parts * U) {
-    float x[U][NV][V], d[U][NV][V], mean[U], rstd[U], s1[U], s2[U];
-    bool on[U];
-    int64_t base[U];
+  const Affine<V, NV> affine(a, t.channel);
+  const int parts = stride / a.groups, step = parts * U, batch = t.on ? (int)a.batch : 0;
+  const int64_t hop = (int64_t)parts * a.len * a.channels;  // floats from one team in flight to the next
+  const int64_t first = (int64_t)t.part * a.len * a.channels + (int64_t)t.g * a.c;
+  const float *from = a.x + first;
+  float *to = a.y + first;
+  int64_t team = (int64_t)t.part * a.groups + t.g;
+  float *mine = fifo + (int)threadIdx.x * V;
+  const auto fetch = [&](int s, int b) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int64_t b = b0 + (int64_t)u * parts + t.part;
-      on[u] = t.on && b < a.batch;
-      base[u] = b * sample + (int64_t)t.g * a.c;
-      mean[u] = on[u] ? a.mean_in[b * a.groups + t.g] : 0.0f;
-      rstd[u] = on[u] ? a.rstd_in[b * a.groups + t.g] : 0.0f;
+      if (b + u * parts < batch)
 #pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        if (on[u] && t.at[i] >= 0) {
-          load(x[u][i], a.x + base[u] + t.at[i]);
-          load(d[u][i], a.dy + base[u] + t.at[i]);
-        } else {
-#pragma unroll
-          for (int j = 0; j < V; ++j) x[u][i][j] = d[u][i][j] = 0.0f;
-        }
-      }
+        for (int i = 0; i < NV; ++i)
+          if (t.at[i] >= 0) copy_async<V>(mine + ((s * U + u) * NV + i) * kRowThreads * V, from + t.at[i]);
+      from += hop;
     }
-    // x <- xh, d <- dv gamma
+    copy_commit();
+  };
 #pragma unroll
-    for (int u = 0; u < U; ++u) s1[u] = s2[u] = 0.0f;
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      float ga[V], be[V];
-      load_or(ga, a.gamma ? a.gamma + t.channel[i] : nullptr, 1.0f);
-      load_or(be, a.beta ? a.beta + t.channel[i] : nullptr, 0.0f);
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        if (!on[u] || t.at[i] < 0) continue;
-        float v[V];
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-          x[u][i][j] = __fmul_rn(__fsub_rn(x[u][i][j], mean[u]), rstd[u]);
-          v[j] = __fmaf_rn(x[u][i][j], ga[j], be[j]);
-        }
-        times_slope(a.act, d[u][i], v);
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-          db[i][j] = __fadd_rn(db[i][j], d[u][i][j]);
-          dg[i][j] = __fmaf_rn(d[u][i][j], x[u][i][j], dg[i][j]);
-          d[u][i][j] = __fmul_rn(d[u][i][j], ga[j]);
-          s1[u] = __fadd_rn(s1[u], d[u][i][j]);
-          s2[u] = __fmaf_rn(d[u][i][j], x[u][i][j], s2[u]);
-        }
-      }
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      s1[u] = __fdiv_rn(team_sum<P>(s1[u], sh), a.m);
-      s2[u] = __fdiv_rn(team_sum<P>(s2[u], sh), a.m);
-    }
+  for (int s = 0; s < S; ++s) fetch(s, t.part + s * step);
+  int s = 0;
+  for (int b0 = 0; b0 < (int)a.batch; b0 += step, s = s + 1 < S ? s + 1 : 0) {
+    const int b = b0 + t.part;
+    Vec<V> x[U][NV];
+    float mean[U], rstd[U];
+    copy_wait<S - 1>();
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        if (!on[u] || t.at[i] < 0) continue;
-        float v[V];
+      for (int i = 0; i < NV; ++i)
+        x[u][i] = b + u * parts < batch && t.at[i] >= 0
+                      ? load<V>(mine + ((s * U + u) * NV + i) * kRowThreads * V)
+                      : splat<V>(0.0f);
+    fetch(s, b + S * step);
 #pragma unroll
-        for (int j = 0; j < V; ++j)
-          v[j] = __fmul_rn(rstd[u], __fsub_rn(__fsub_rn(d[u][i][j], s1[u]), __fmul_rn(x[u][i][j], s2[u])));
-        store(a.dx + base[u] + t.at[i], v);
+    for (int u = 0; u < U; ++u) {
+      Vec<V> q = x[u][0];
+#pragma unroll
+      for (int i = 1; i < NV; ++i) sum_into(q, x[u][i]);
+      mean[u] = total(q);
+    }
+    team_sums<P, U>(mean, sh, [&](float v) { return __fdiv_rn(v, a.m); });  // exact for a constant
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      Vec<V> q = splat<V>(0.0f);
+      const Pair minus = V == 1 ? pair(-mean[u], 0.0f) : both(-mean[u]);
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+        if (t.at[i] >= 0) square_into(q, x[u][i], minus);
+      rstd[u] = total(q);
+    }
+    team_sums<P, U>(rstd, sh, [&](float v) { return rstd_of(v, a.inv_m, a.eps); });
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (b + u * parts < batch) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+          if (t.at[i] >= 0) {
+            Vec<V> ga, be;
+            affine.get(a, t.channel, i, ga, be);
+            store(to + t.at[i], normalize(a.act, x[u][i], both(-mean[u]), both(rstd[u]), ga, be));
+          }
+        if (a.mean && threadIdx.x % P == 0) {
+          a.mean[team] = mean[u];
+          a.rstd[team] = rstd[u];
+        }
       }
+      to += hop;
+      team += stride;
+    }
   }
-  if (a.part && t.on) {
-    // [part][2][groups][len * c]: every vector of the team a column of its own
-    const int64_t row = (int64_t)a.groups * a.len * a.c;
-    float *p = a.part + (int64_t)t.part * 2 * row + (int64_t)t.g * a.len * a.c;
+  copy_wait<0>();
+}
+
+// fold: teams of a CTA that share a group and whose channel sums are added up in the CTA.
+template <int V, int P, int NV>
+__global__ void __launch_bounds__(kRowThreads, row_ctas(true, NV))
+    norm_rows_backward_kernel(const Norm a, int stride, int fold) {
+  pdl_wait();
+  constexpr int U = row_u(P, NV), S = row_stages(true, NV);
+  extern __shared__ __align__(16) float fifo[];  // [S][2][U][NV][threads] vectors, then the CTA's channel sums
+  __shared__ float sh[kRowThreads / 32];
+  const RowTeam<V, P, NV> t(a, stride);
+  const Affine<V, NV> affine(a, t.channel);
+  const int parts = stride / a.groups, step = parts * U, batch = t.on ? (int)a.batch : 0;
+  const int64_t hop = (int64_t)parts * a.len * a.channels;
+  const int64_t first = (int64_t)t.part * a.len * a.channels + (int64_t)t.g * a.c;
+  const float *from_x = a.x + first, *from_d = a.dy + first;
+  float *to = a.dx + first;
+  int64_t team = (int64_t)t.part * a.groups + t.g;
+  float *mine = fifo + (int)threadIdx.x * V;
+  const auto fetch = [&](int s, int b) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (b + u * parts < batch)
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+          if (t.at[i] >= 0) {
+            copy_async<V>(mine + ((s * 2 * U + u) * NV + i) * kRowThreads * V, from_x + t.at[i]);
+            copy_async<V>(mine + (((s * 2 + 1) * U + u) * NV + i) * kRowThreads * V, from_d + t.at[i]);
+          }
+      from_x += hop;
+      from_d += hop;
+    }
+    copy_commit();
+  };
+  float next_mean[U], next_rstd[U];
+  const auto fetch_stats = [&](int b) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      next_mean[u] = b + u * parts < batch ? a.mean_in[team] : 0.0f;
+      next_rstd[u] = b + u * parts < batch ? a.rstd_in[team] : 0.0f;
+      team += stride;
+    }
+  };
+#pragma unroll
+  for (int s = 0; s < S; ++s) fetch(s, t.part + s * step);
+  fetch_stats(t.part);
+  Vec<V> db[NV], dg[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) db[i] = dg[i] = splat<V>(0.0f);
+  int s = 0;
+  for (int b0 = 0; b0 < (int)a.batch; b0 += step, s = s + 1 < S ? s + 1 : 0) {
+    const int b = b0 + t.part;
+    Vec<V> x[U][NV], d[U][NV];
+    float rstd[U], s1[U], s2[U];
+    Pair minus[U];
+    copy_wait<S - 1>();
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      minus[u] = both(-next_mean[u]);
+      rstd[u] = next_rstd[u];
+      s1[u] = s2[u] = 0.0f;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const bool in = b + u * parts < batch && t.at[i] >= 0;
+        x[u][i] = in ? load<V>(mine + ((s * 2 * U + u) * NV + i) * kRowThreads * V) : splat<V>(0.0f);
+        d[u][i] = in ? load<V>(mine + (((s * 2 + 1) * U + u) * NV + i) * kRowThreads * V) : splat<V>(0.0f);
+      }
+    }
+    fetch(s, b + S * step);
+    fetch_stats(b + step);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      if (t.at[i] < 0) continue;
+      Vec<V> ga, be;
+      affine.get(a, t.channel, i, ga, be);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        // behind the batch x, d, mean and rstd are 0, and so is all that they give
+        gradient(a.act, x[u][i], d[u][i], db[i], dg[i], minus[u], both(rstd[u]), ga, be);
+        Vec<V> w;
+#pragma unroll
+        for (int j = 0; j < Vec<V>::N; ++j) w.p[j] = mul2(d[u][i].p[j], x[u][i].p[j]);
+        s1[u] = __fadd_rn(s1[u], total(d[u][i]));
+        s2[u] = __fadd_rn(s2[u], total(w));
+      }
+    }
+    const auto over_m = [&](float v) { return __fmul_rn(v, -a.inv_m); };
+    team_sums<P, U>(s1, sh, over_m);
+    team_sums<P, U>(s2, sh, over_m);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (b + u * parts < batch)
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+          if (t.at[i] >= 0)
+            store(to + t.at[i], finish(x[u][i], d[u][i], both(s1[u]), both(s2[u]), both(rstd[u])));
+      to += hop;
+    }
+  }
+  copy_wait<0>();
+  if (!a.part) return;
+  // Per channel, over the rows of the sample and the CTA's `fold` teams of the group, in
+  // order: part[row][2][channels]. The teams' sums (at most 8192 floats) take the place of
+  // the first stage.
+  constexpr int kTeams = kRowThreads / P;
+  const int id0 = (int)blockIdx.x * kTeams, wide = (int)a.len * a.c;
+  float *own = fifo + (int)(threadIdx.x / P) * wide;
+#pragma unroll
+  for (int which = 0; which < 2; ++which) {
+    __syncthreads();
 #pragma unroll
     for (int i = 0; i < NV; ++i)
-      if (t.at[i] >= 0) {
-        float *q = p + (i * P + (int64_t)(threadIdx.x % P)) * V;
-        store(q, db[i]);
-        store(q + row, dg[i]);
-      }
+      if (t.at[i] >= 0) store(own + (i * P + (int)(threadIdx.x % P)) * V, which ? dg[i] : db[i]);
+    __syncthreads();
+    const int first = kTeams / fold;  // teams with channels of their own
+    for (int i = threadIdx.x; i < first * a.c; i += kRowThreads) {
+      const int team = i / a.c, ch = i - team * a.c, id = id0 + team;
+      if (id >= stride) break;
+      float sum = 0.0f;
+      for (int f = 0; f < fold; ++f)
+        for (int l = 0; l < (int)a.len; ++l) sum = __fadd_rn(sum, fifo[(team + f * first) * wide + l * a.c + ch]);
+      const int row = id / (a.groups * fold), g = id % a.groups;
+      a.part[((int64_t)row * 2 + which) * a.channels + (int64_t)g * a.c + ch] = sum;
+    }
   }
 }
 
@@ -390,416 +590,415 @@ __global__ void __launch_bounds__(kRowThreads) norm_rows_backward_kernel(const N
 // How a launch cuts samples into tiles (see norm_plan).
 struct Tiling {
   int cols;      // vectors a tile is wide
+  int wide;      // the next power of two: thread columns
   int q;         // whole groups a tile holds (1 where a group is split)
   int split;     // tiles a group's columns are split into
   int bundles;   // tiles side by side over a sample's groups (without the split)
-  int ty;        // thread rows of a tile
   int rows;      // rows a tile
   int chunks;    // tiles one below the other
   int k;         // tiles that share statistics: split * chunks
+  int sets;      // sets of k tiles: batch * bundles
 };
 
-template <int V, int THREADS>
+// How a tile kernel gets the statistics of a set of tiles: kInCluster, one cluster a set
+// (k <= 16 tiles), each CTA pushing its share to all of them; or in two launches, kParts
+// leaving each tile's in the workspace and kWhole joining them. CTAs (clusters) are
+// resident and go through the tiles (sets) in turn, the next tile fetched ahead, so its
+// loads run while a set waits for its statistics.
+enum : int { kInCluster = 0, kParts = 1, kWhole = 2 };
+
+// One tile, as a thread sees it.
+template <int V>
 struct Tile {
-  int64_t b;
-  int k, chunk;
-  int q;             // groups in this tile
-  int g0;            // its first group
-  int cols;          // its vectors a row
-  int tx, ty;
-  bool on;           // this thread holds a column
-  int channel;       // its first channel
-  int group;         // its group, counted from g0
-  int row0, rows;    // its rows
-  int64_t base;
-  // share: which of the k tiles that share statistics; team: which set of them
-  __device__ Tile(const Norm &a, const Tiling &t, int64_t team, int share) {
-    b = team / t.bundles;
-    k = share;
-    const int bundle = (int)(team - b * t.bundles);
-    chunk = share / t.split;
-    const int piece = share - chunk * t.split, cv = a.c / V;
-    g0 = bundle * t.q;
-    q = min(t.q, a.groups - g0);
-    cols = t.split > 1 ? min(t.cols, cv - piece * t.cols) : q * cv;
-    tx = threadIdx.x % t.cols;
-    ty = threadIdx.x / t.cols;
-    on = ty < t.ty && tx < cols;
-    channel = g0 * a.c + (piece * t.cols + tx) * V;
-    group = t.split > 1 ? 0 : tx / cv;
-    row0 = chunk * t.rows;
-    rows = (int)min((int64_t)t.rows, a.len - row0);
-    base = (b * a.len + row0) * a.channels + channel;
+  int b, chunk, k;
+  int g0, q, cols;  // its first group, its groups, its vectors a row
+  int rows, mine;   // its rows, and those of this thread (0: none)
+  int channel;      // this thread's first channel
+  int64_t at;       // offset of this thread's first vector
+};
+
+// A CTA's walk over the tiles: (b, bundle, share) counted in mixed radix, since a division
+// a tile costs as much as a good part of its arithmetic. kWhole walks from the last tile.
+template <int V, int MODE>
+struct Walk {
+  int b, bundle, share, db, dbundle, dshare, left;
+  int tx, ty, shift;  // thread column and row, log2 of the thread rows
+  __device__ Walk(const Tiling &t, int rank) {
+    const int k = MODE == kInCluster ? 1 : t.k;
+    const int first = MODE == kInCluster ? (int)blockIdx.x / t.k : (int)blockIdx.x;
+    const int step = MODE == kInCluster ? (int)gridDim.x / t.k : (int)gridDim.x;
+    const int units = t.sets * k;
+    left = first < units ? (units - 1 - first) / step + 1 : 0;
+    share = MODE == kInCluster ? rank : first % k;
+    bundle = first / k % t.bundles;
+    b = first / k / t.bundles;
+    dshare = MODE == kInCluster ? 0 : step % k;
+    dbundle = step / k % t.bundles;
+    db = step / k / t.bundles;
+    tx = (int)threadIdx.x & (t.wide - 1);
+    ty = (int)threadIdx.x / t.wide;
+    shift = __ffs(kTileThreads / t.wide) - 1;
   }
-  // values of one group in the tile
-  __device__ float count(const Norm &a, const Tiling &t) const {
-    return (float)rows * (float)(t.split > 1 ? cols * V : a.c);
+  __device__ void advance(const Tiling &t) {
+    --left;
+    int carry = 0;
+    if (MODE != kInCluster) {
+      share += dshare;
+      carry = share >= t.k;
+      share -= carry ? t.k : 0;
+    }
+    bundle += dbundle + carry;
+    carry = bundle >= t.bundles;
+    bundle -= carry ? t.bundles : 0;
+    b += db + carry;
   }
-  // the same of another tile that shares the statistics
-  static __device__ float count_of(const Norm &a, const Tiling &t, int share) {
-    const int chunk = share / t.split, piece = share - chunk * t.split;
-    const float r = (float)min((int64_t)t.rows, a.len - (int64_t)chunk * t.rows);
-    return r * (float)(t.split > 1 ? min(t.cols, a.c / V - piece * t.cols) * V : a.c);
+  __device__ Tile<V> get(const Norm &a, const Tiling &t) const {
+    Tile<V> r;
+    const bool back = MODE == kWhole;
+    const int cv = a.c / V, at = back ? t.bundles - 1 - bundle : bundle;
+    r.b = back ? (int)a.batch - 1 - b : b;
+    r.k = back ? t.k - 1 - share : share;
+    r.chunk = t.split > 1 ? r.k / t.split : r.k;
+    const int piece = r.k - r.chunk * t.split;
+    r.g0 = at * t.q;
+    r.q = min(t.q, a.groups - r.g0);
+    r.cols = t.split > 1 ? min(t.cols, cv - piece * t.cols) : r.q * cv;
+    const int64_t row0 = (int64_t)r.chunk * t.rows;
+    r.rows = (int)min((int64_t)t.rows, a.len - row0);
+    r.channel = r.g0 * a.c + (piece * t.cols + tx) * V;
+    r.mine = tx < r.cols && ty < r.rows ? ((r.rows - 1 - ty) >> shift) + 1 : 0;
+    r.at = (r.b * a.len + row0 + ty) * a.channels + r.channel;
+    return r;
   }
 };
 
-// sums[g] of the threads' v over the tile's groups; sh holds a float a thread. A warp takes
-// a group at a time.
-template <int V, int THREADS>
-__device__ __forceinline__ void group_sums(float v, float *sh, float *sums, const Tile<V, THREADS> &me,
-                                           const Tiling &t, int cv) {
-  sh[threadIdx.x] = me.on ? v : 0.0f;
-  __syncthreads();
-  const int lane = threadIdx.x & 31, width = t.split > 1 ? me.cols : cv;
-  for (int g = threadIdx.x >> 5; g < me.q; g += THREADS / 32) {
-    float s = 0.0f;
-    for (int i = lane; i < width * t.ty; i += 32) {
-      const int y = i / width;
-      s = __fadd_rn(s, sh[y * t.cols + g * cv + (i - y * width)]);
-    }
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) s = __fadd_rn(s, __shfl_xor_sync(kFull, s, d));
-    if (lane == 0) sums[g] = s;
-  }
-  __syncthreads();
-}
-
-template <int V, int THREADS>
-__device__ __forceinline__ void load_tile(float (&x)[held(V)][V], const float *p, const Tile<V, THREADS> &me,
-                                          const Tiling &t, int64_t channels) {
-#pragma unroll
-  for (int i = 0; i < held(V); ++i) {
-    const int r = me.ty + i * t.ty;
-    if (me.on && r < me.rows) {
-      load(x[i], p + me.base + r * channels);
-    } else {
-#pragma unroll
-      for (int j = 0; j < V; ++j) x[i][j] = 0.0f;
-    }
-  }
-}
-
-// The tile's own mean and M2 per group, in shared memory.
-template <int V, int THREADS>
-__device__ __forceinline__ void tile_moments(const float (&x)[held(V)][V], float *sh, float *mean, float *m2,
-                                             const Norm &a, const Tile<V, THREADS> &me, const Tiling &t) {
-  const int cv = a.c / V;
-  float s = 0.0f;
-#pragma unroll
-  for (int i = 0; i < held(V); ++i)
-#pragma unroll
-    for (int j = 0; j < V; ++j) s = __fadd_rn(s, x[i][j]);
-  group_sums(s, sh, m2, me, t, cv);
-  const float n = me.count(a, t);
-  for (int g = threadIdx.x; g < me.q; g += THREADS) mean[g] = __fdiv_rn(m2[g], n);
-  __syncthreads();
-  const float mu = me.on ? mean[me.group] : 0.0f;
-  s = 0.0f;
-#pragma unroll
-  for (int i = 0; i < held(V); ++i)
-    if (me.ty + i * t.ty < me.rows)
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const float d = __fsub_rn(x[i][j], mu);
-        s = __fmaf_rn(d, d, s);
-      }
-  group_sums(s, sh, m2, me, t, cv);
-}
-
-template <int V, int THREADS>
-__device__ __forceinline__ void write_tile(const float (&x)[held(V)][V], float mean, float rstd, const Norm &a,
-                                           const Tile<V, THREADS> &me, const Tiling &t) {
-  if (!me.on) return;
-  float ga[V], be[V];
-  load_or(ga, a.gamma ? a.gamma + me.channel : nullptr, 1.0f);
-  load_or(be, a.beta ? a.beta + me.channel : nullptr, 0.0f);
-#pragma unroll
-  for (int i = 0; i < held(V); ++i) {
-    const int r = me.ty + i * t.ty;
-    if (r >= me.rows) break;
-    float v[V];
-#pragma unroll
-    for (int j = 0; j < V; ++j) v[j] = __fmaf_rn(__fmul_rn(__fsub_rn(x[i][j], mean), rstd), ga[j], be[j]);
-    activate(a.act, v);
-    store(a.y + me.base + r * a.channels, v);
-  }
-}
-
-// One cluster per set of tiles that share statistics.
+// Values of one group in tile `k` of a set.
 template <int V>
-__global__ void __launch_bounds__(kTileForward, 2) norm_tile_kernel(const Norm a, const Tiling t) {
-  pdl_wait();
-  constexpr int T = kTileForward;
-  cg::cluster_group cluster = cg::this_cluster();
-  __shared__ float sh[T], mean[T], m2[T], mean_all[T], rstd_all[T];
-  const Tile<V, T> me(a, t, blockIdx.x / t.k, (int)(blockIdx.x % t.k));
-  float x[held(V)][V];
-  load_tile(x, a.x, me, t, a.channels);
-  tile_moments(x, sh, mean, m2, a, me, t);
-  if (t.k > 1) cluster.sync();
-  for (int g = threadIdx.x; g < me.q; g += T) {
-    Moments s{0.0f, 0.0f, 0.0f};
-    if (t.k > 1) {
-      for (int r = 0; r < t.k; ++r)
-        s = join(s, {Tile<V, T>::count_of(a, t, r), cluster.map_shared_rank(mean, r)[g],
-                     cluster.map_shared_rank(m2, r)[g]});
-    } else {
-      s = {a.m, mean[g], m2[g]};
-    }
-    mean_all[g] = s.mean;
-    rstd_all[g] = rstd_of(s.m2, a.m, a.eps);
-    if (a.mean && me.k == 0) {
-      a.mean[me.b * a.groups + me.g0 + g] = s.mean;
-      a.rstd[me.b * a.groups + me.g0 + g] = rstd_all[g];
-    }
-  }
-  __syncthreads();
-  if (t.k > 1) cluster.barrier_arrive();
-  if (me.on) write_tile(x, mean_all[me.group], rstd_all[me.group], a, me, t);
-  if (t.k > 1) cluster.barrier_wait();  // no CTA leaves while its statistics may be read
+__device__ __forceinline__ float count_of(const Norm &a, const Tiling &t, int k) {
+  const int chunk = t.split > 1 ? k / t.split : k, piece = k - chunk * t.split;
+  const float rows = (float)min((int64_t)t.rows, a.len - (int64_t)chunk * t.rows);
+  return rows * (float)(t.split > 1 ? min(t.cols, a.c / V - piece * t.cols) * V : a.c);
 }
 
-// The two-launch form: statistics to stat[(b * groups + g) * k + tile] = (mean, M2) ...
-template <int V>
-__global__ void __launch_bounds__(kTileForward, 2) norm_tile_stats_kernel(const Norm a, const Tiling t) {
-  pdl_wait();
-  constexpr int T = kTileForward;
-  __shared__ float sh[T], mean[T], m2[T];
-  const Tile<V, T> me(a, t, blockIdx.x / t.k, (int)(blockIdx.x % t.k));
-  float x[held(V)][V];
-  load_tile(x, a.x, me, t, a.channels);
-  tile_moments(x, sh, mean, m2, a, me, t);
-  for (int g = threadIdx.x; g < me.q; g += T) {
-    float *s = a.stat + ((me.b * a.groups + me.g0 + g) * t.k + me.k) * 2;
-    s[0] = mean[g];
-    s[1] = m2[g];
+// A tile's vectors to a thread's place in shared memory ([held][threads] vectors), and back.
+template <int V, int N>
+__device__ __forceinline__ void fetch_tile(float *fifo, const float *p, const Tile<V> &me, int64_t step) {
+  const float *q = p + me.at;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    if (i < me.mine) copy_async<V>(fifo + (i * kTileThreads + (int)threadIdx.x) * V, q);
+    q += step;
   }
 }
-// ... and the result from them: a warp joins a group's tiles.
-template <int V>
-__global__ void __launch_bounds__(kTileForward, 2) norm_tile_apply_kernel(const Norm a, const Tiling t) {
-  pdl_wait();
-  constexpr int T = kTileForward;
-  __shared__ float mean_all[T], rstd_all[T];
-  const unsigned block = gridDim.x - 1 - blockIdx.x;
-  const Tile<V, T> me(a, t, block / t.k, (int)(block % t.k));
-  float x[held(V)][V];
-  load_tile(x, a.x, me, t, a.channels);
+template <int V, int N>
+__device__ __forceinline__ void take_tile(Vec<V> (&x)[N], const float *fifo, const Tile<V> &me) {
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    x[i] = i < me.mine ? load<V>(fifo + (i * kTileThreads + (int)threadIdx.x) * V) : splat<V>(0.0f);
+}
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) v = __fadd_rn(v, __shfl_xor_sync(kFull, v, d));
+  return v;
+}
+
+// The threads' v, one a thread column, summed over the thread rows of each warp (lanes a
+// multiple of `wide` apart) and put into sh[row][wide]; `slices` rows of it.
+__device__ __forceinline__ int slices_of(int wide) { return wide < 32 ? kTileThreads / 32 : kTileThreads / wide; }
+__device__ __forceinline__ void put_columns(float v, float *sh, int wide) {
+  for (int d = 16; d >= wide; d >>= 1) v = __fadd_rn(v, __shfl_xor_sync(kFull, v, d));
   const int lane = threadIdx.x & 31;
-  for (int g = threadIdx.x >> 5; g < me.q; g += T / 32) {
-    const int64_t team = me.b * a.groups + me.g0 + g;
-    Moments s{0.0f, 0.0f, 0.0f};
-    for (int r = lane; r < t.k; r += 32) {
-      const float2 p = *reinterpret_cast<const float2 *>(a.stat + (team * t.k + r) * 2);
-      s = join(s, {Tile<V, T>::count_of(a, t, r), p.x, p.y});
-    }
+  if (wide >= 32) sh[threadIdx.x] = v;
+  else if (lane < wide) sh[(threadIdx.x >> 5) * wide + lane] = v;
+}
+// A warp's sum over `width` columns from `col` on.
+__device__ __forceinline__ float take_columns(const float *sh, int wide, int col, int width) {
+  const int lane = threadIdx.x & 31, n = slices_of(wide) * width;
+  int y = lane / width, c = lane - y * width;
+  const int dy = 32 / width, dc = 32 - dy * width;
+  float s = 0.0f;
+  for (int i = lane; i < n; i += 32) {
+    s = __fadd_rn(s, sh[y * wide + col + c]);
+    y += dy;
+    c += dc;
+    if (c >= width) c -= width, ++y;
+  }
+  return warp_sum(s);
+}
+
+// The tile's own (mean, M2) per group, by the warp that goes on with the group.
+template <int V, int N>
+__device__ __forceinline__ void tile_moments(const Vec<V> (&x)[N], float *sh, float *sh2, float2 *moments,
+                                             const Norm &a, const Tile<V> &me, const Tiling &t, int tx) {
+  const int cv = a.c / V, width = t.split > 1 ? me.cols : cv, warp = threadIdx.x >> 5;
+  Vec<V> s = x[0];
 #pragma unroll
-    for (int d = 16; d > 0; d >>= 1) {
-      const Moments o{__shfl_down_sync(kFull, s.n, d), __shfl_down_sync(kFull, s.mean, d),
-                      __shfl_down_sync(kFull, s.m2, d)};
-      s = join(s, o);
+  for (int i = 1; i < N; ++i) sum_into(s, x[i]);
+  put_columns(total(s), sh, t.wide);
+  __syncthreads();
+  const float n = (float)me.rows * (float)(width * V);
+  for (int g = warp; g < me.q; g += kTileThreads / 32) {
+    const float mean = __fdiv_rn(take_columns(sh, t.wide, g * cv, width), n);
+    if ((threadIdx.x & 31) == 0) moments[g].x = mean;
+  }
+  __syncthreads();
+  const float mean = moments[me.mine ? (t.split > 1 ? 0 : tx / cv) : 0].x;
+  const Pair minus = V == 1 ? pair(-mean, 0.0f) : both(-mean);
+  s = splat<V>(0.0f);
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    if (i < me.mine) square_into(s, x[i], minus);
+  put_columns(total(s), sh2, t.wide);
+  __syncthreads();
+  for (int g = warp; g < me.q; g += kTileThreads / 32) {
+    const float m2 = take_columns(sh2, t.wide, g * cv, width);
+    if ((threadIdx.x & 31) == 0) moments[g].y = m2;
+  }
+}
+
+// mean and rstd of the union of lanes' (n, mean, M2); every lane gets them.
+__device__ __forceinline__ float2 join_lanes(float n, float2 p, const Norm &a) {
+  const float mean = __fdiv_rn(warp_sum(__fmul_rn(n, p.x)), a.m), d = __fsub_rn(p.x, mean);
+  const float m2 = warp_sum(n == 0.0f ? 0.0f : __fmaf_rn(__fmul_rn(d, d), n, p.y));
+  return make_float2(mean, rstd_of(m2, a.inv_m, a.eps));
+}
+
+template <int V, int MODE>
+__global__ void __launch_bounds__(kTileThreads, kTileCtas) norm_tile_kernel(const Norm a, const Tiling t) {
+  pdl_wait();
+  constexpr int N = held(V, false);
+  cg::cluster_group cluster = cg::this_cluster();
+  extern __shared__ __align__(16) float fifo[];
+  __shared__ float sh[kTileThreads], sh2[kTileThreads];
+  // by parity of the tile: a warp may be a tile ahead of one that still reads
+  __shared__ float2 moments[kMaxTileGroups], stats_by[2][kMaxTileGroups];
+  // the cluster's moments by parity of the tile, so that one barrier a tile is enough: a CTA
+  // writes a parity again only after a barrier that all have reached behind their reading it
+  __shared__ float2 all[2][kMaxCluster][kMaxTileGroups];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, cv = a.c / V;
+  const bool joined = MODE == kInCluster && t.k > 1;
+  Walk<V, MODE> walk(t, MODE == kInCluster ? (int)cluster.block_rank() : 0);
+  if (joined) cluster.barrier_arrive();
+  const int64_t step = (int64_t)(kTileThreads / t.wide) * a.channels;
+  const int column = t.split > 1 ? 0 : walk.tx / cv;  // this thread's group in the tile
+  const float share = joined && lane < t.k ? count_of<V>(a, t, lane) : 0.0f;
+  Tile<V> me, next;
+  if (walk.left) {
+    next = walk.get(a, t);
+    fetch_tile<V, N>(fifo, a.x, next, step);
+  }
+  copy_commit();
+  if (joined) cluster.barrier_wait();  // all of the cluster's CTAs run
+  for (int n = 0; walk.left; n ^= 1) {
+    me = next;
+    walk.advance(t);
+    Vec<V> x[N];
+    copy_wait<0>();
+    take_tile(x, fifo, me);
+    if (walk.left) {
+      next = walk.get(a, t);
+      fetch_tile<V, N>(fifo, a.x, next, step);
     }
-    if (lane == 0) {
-      mean_all[g] = s.mean;
-      rstd_all[g] = rstd_of(s.m2, a.m, a.eps);
-      if (a.mean && me.k == 0) {
-        a.mean[team] = s.mean;
-        a.rstd[team] = rstd_all[g];
+    copy_commit();
+    if (MODE != kWhole) tile_moments(x, sh, sh2, moments, a, me, t, walk.tx);
+    if (joined) {
+      for (int g = warp; g < me.q; g += kTileThreads / 32) {
+        __syncwarp();
+        if (lane < t.k) cluster.map_shared_rank(&all[n][me.k][g], lane)[0] = moments[g];
+      }
+      cluster.sync();
+    }
+    float2 *stats = stats_by[n];
+    for (int g = warp; g < me.q; g += kTileThreads / 32) {
+      const int64_t team = (int64_t)me.b * a.groups + me.g0 + g;
+      __syncwarp();
+      if (MODE == kParts) {
+        if (lane == 0) reinterpret_cast<float2 *>(a.stat)[team * t.k + me.k] = moments[g];
+        continue;
+      }
+      float2 r;
+      if (joined) {
+        r = join_lanes(share, lane < t.k ? all[n][lane][g] : make_float2(0.0f, 0.0f), a);
+      } else if (MODE == kInCluster) {
+        r = make_float2(moments[g].x, rstd_of(moments[g].y, a.inv_m, a.eps));
+      } else {
+        const float2 *q = reinterpret_cast<const float2 *>(a.stat) + team * t.k;
+        float u = 0.0f, w = 0.0f;
+        for (int i = lane; i < t.k; i += 32) u = __fmaf_rn(count_of<V>(a, t, i), q[i].x, u);
+        const float mean = __fdiv_rn(warp_sum(u), a.m);
+        for (int i = lane; i < t.k; i += 32) {
+          const float d = __fsub_rn(q[i].x, mean);
+          w = __fadd_rn(w, __fmaf_rn(__fmul_rn(d, d), count_of<V>(a, t, i), q[i].y));
+        }
+        r = make_float2(mean, rstd_of(warp_sum(w), a.inv_m, a.eps));
+      }
+      if (lane == 0) {
+        stats[g] = r;
+        if (a.mean && me.k == 0) {
+          a.mean[team] = r.x;
+          a.rstd[team] = r.y;
+        }
+      }
+    }
+    __syncthreads();
+    if (MODE != kParts && me.mine) {
+      const Vec<V> ga = load_or<V>(a.gamma ? a.gamma + me.channel : nullptr, 1.0f);
+      const Vec<V> be = load_or<V>(a.beta ? a.beta + me.channel : nullptr, 0.0f);
+      const Pair minus = both(-stats[column].x), rstd = both(stats[column].y);
+      float *q = a.y + me.at;
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        if (i < me.mine) store(q, normalize(a.act, x[i], minus, rstd, ga, be));
+        q += step;
       }
     }
   }
-  __syncthreads();
-  if (me.on) write_tile(x, mean_all[me.group], rstd_all[me.group], a, me, t);
+  copy_wait<0>();
 }
 
-// x <- xh, d <- dv gamma, and the column sums of dv and dv xh of this thread's rows.
-template <int V, int THREADS>
-__device__ __forceinline__ void tile_gradient(float (&x)[held(V)][V], float (&d)[held(V)][V], float (&db)[V],
-                                              float (&dg)[V], const Norm &a, const Tile<V, THREADS> &me,
-                                              const Tiling &t) {
+// The tile's sums of dv and dv xh: per channel into `part`, and gamma-weighted per group,
+// by the warp that goes on with the group. sh: [slices][2][wide * V].
+template <int V>
+__device__ __forceinline__ void tile_gradient_sums(Vec<V> db, Vec<V> dg, float *sh, float2 *sums, const Norm &a,
+                                                   const Tile<V> &me, const Tiling &t, int tx) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, row = t.wide * V, slices = slices_of(t.wide);
+  for (int d = 16; d >= t.wide; d >>= 1) {
 #pragma unroll
-  for (int j = 0; j < V; ++j) db[j] = dg[j] = 0.0f;
-  if (!me.on) return;
-  float ga[V], be[V];
-  load_or(ga, a.gamma ? a.gamma + me.channel : nullptr, 1.0f);
-  load_or(be, a.beta ? a.beta + me.channel : nullptr, 0.0f);
-  const int64_t team = me.b * a.groups + me.g0 + me.group;
-  const float mean = a.mean_in[team], rstd = a.rstd_in[team];
-#pragma unroll
-  for (int i = 0; i < held(V); ++i) {
-    if (me.ty + i * t.ty >= me.rows) break;
-    float v[V];
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      x[i][j] = __fmul_rn(__fsub_rn(x[i][j], mean), rstd);
-      v[j] = __fmaf_rn(x[i][j], ga[j], be[j]);
-    }
-    times_slope(a.act, d[i], v);
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      db[j] = __fadd_rn(db[j], d[i][j]);
-      dg[j] = __fmaf_rn(d[i][j], x[i][j], dg[j]);
-      d[i][j] = __fmul_rn(d[i][j], ga[j]);
+    for (int i = 0; i < Vec<V>::N; ++i) {
+      db.p[i] = add2(db.p[i], __shfl_xor_sync(kFull, db.p[i], d));
+      dg.p[i] = add2(dg.p[i], __shfl_xor_sync(kFull, dg.p[i], d));
     }
   }
-}
-
-// The tile's sums: per channel into `part`, and gamma-weighted per group into s1, s2
-// (shared memory). sh: 2 V floats a thread.
-template <int V, int THREADS>
-__device__ __forceinline__ void tile_gradient_sums(const float (&db)[V], const float (&dg)[V], float *sh, float *s1,
-                                                   float *s2, const Norm &a, const Tile<V, THREADS> &me,
-                                                   const Tiling &t) {
-  const int wide = t.cols * V;  // channels of a full tile
-#pragma unroll
-  for (int j = 0; j < V; ++j) {
-    if (me.ty < t.ty) {
-      sh[me.ty * wide + me.tx * V + j] = db[j];
-      sh[(t.ty + me.ty) * wide + me.tx * V + j] = dg[j];
-    }
+  if (t.wide >= 32 || lane < t.wide) {
+    float *q = sh + (t.wide >= 32 ? (int)threadIdx.x / t.wide : warp) * 2 * row + tx * V;
+    store(q, db);
+    store(q + row, dg);
   }
   __syncthreads();
-  const int n = me.cols * V, first = me.channel - me.tx * V;
-  for (int i = threadIdx.x; i < 2 * n; i += THREADS) {
-    const int which = i >= n, ch = i - which * n;
-    float *col = sh + which * t.ty * wide + ch;
-    float s = col[0];
-    for (int y = 1; y < t.ty; ++y) s = __fadd_rn(s, col[y * wide]);
-    col[0] = s;
-    if (a.part) a.part[((me.b * t.chunks + me.chunk) * 2 + which) * a.channels + first + ch] = s;
+  const int n = me.cols * V, first = me.channel - tx * V;
+  for (int i = threadIdx.x; i < 2 * n; i += kTileThreads) {
+    const int which = i >= n, ch = i - (which ? n : 0);
+    float *q = sh + which * row + ch;
+    float s = q[0];
+    for (int y = 1; y < slices; ++y) s = __fadd_rn(s, q[y * 2 * row]);
+    q[0] = s;
+    if (a.part) a.part[(((int64_t)me.b * t.chunks + me.chunk) * 2 + which) * a.channels + first + ch] = s;
   }
   __syncthreads();
-  const int lane = threadIdx.x & 31, width = t.split > 1 ? n : a.c;
-  for (int g = threadIdx.x >> 5; g < me.q; g += THREADS / 32) {
+  const int width = t.split > 1 ? n : a.c;
+  for (int g = warp; g < me.q; g += kTileThreads / 32) {
     float u = 0.0f, w = 0.0f;
     for (int i = lane; i < width; i += 32) {
       const float ga = a.gamma ? a.gamma[first + g * a.c + i] : 1.0f;
       u = __fmaf_rn(ga, sh[g * a.c + i], u);
-      w = __fmaf_rn(ga, sh[t.ty * wide + g * a.c + i], w);
+      w = __fmaf_rn(ga, sh[row + g * a.c + i], w);
     }
-#pragma unroll
-    for (int e = 16; e > 0; e >>= 1) {
-      u = __fadd_rn(u, __shfl_xor_sync(kFull, u, e));
-      w = __fadd_rn(w, __shfl_xor_sync(kFull, w, e));
-    }
-    if (lane == 0) {
-      s1[g] = u;
-      s2[g] = w;
-    }
-  }
-  __syncthreads();
-}
-
-template <int V, int THREADS>
-__device__ __forceinline__ void write_gradient(const float (&x)[held(V)][V], const float (&d)[held(V)][V],
-                                               float k1, float k2, const Norm &a, const Tile<V, THREADS> &me,
-                                               const Tiling &t) {
-  const float rstd = a.rstd_in[me.b * a.groups + me.g0 + me.group];
-#pragma unroll
-  for (int i = 0; i < held(V); ++i) {
-    const int r = me.ty + i * t.ty;
-    if (r >= me.rows) break;
-    float v[V];
-#pragma unroll
-    for (int j = 0; j < V; ++j)
-      v[j] = __fmul_rn(rstd, __fsub_rn(__fsub_rn(d[i][j], k1), __fmul_rn(x[i][j], k2)));
-    store(a.dx + me.base + r * a.channels, v);
+    u = warp_sum(u);
+    w = warp_sum(w);
+    if (lane == 0) sums[g] = make_float2(u, w);
   }
 }
 
-template <int V>
-__global__ void __launch_bounds__(kTileBackward, 2) norm_tile_backward_kernel(const Norm a, const Tiling t) {
+template <int V, int MODE>
+__global__ void __launch_bounds__(kTileThreads, kTileCtas) norm_tile_backward_kernel(const Norm a, const Tiling t) {
   pdl_wait();
-  constexpr int T = kTileBackward;
+  constexpr int N = held(V, true), kStage = N * kTileThreads * V;
   cg::cluster_group cluster = cg::this_cluster();
-  __shared__ float sh[2 * V * T], s1[T], s2[T], k1[T], k2[T];
-  const Tile<V, T> me(a, t, blockIdx.x / t.k, (int)(blockIdx.x % t.k));
-  float x[held(V)][V], d[held(V)][V], db[V], dg[V];
-  load_tile(x, a.x, me, t, a.channels);
-  load_tile(d, a.dy, me, t, a.channels);
-  tile_gradient(x, d, db, dg, a, me, t);
-  tile_gradient_sums(db, dg, sh, s1, s2, a, me, t);
-  if (t.k > 1) cluster.sync();
-  for (int g = threadIdx.x; g < me.q; g += T) {
-    float u = s1[g], w = s2[g];
-    if (t.k > 1) {
-      u = w = 0.0f;
-      for (int r = 0; r < t.k; ++r) {
-        u = __fadd_rn(u, cluster.map_shared_rank(s1, r)[g]);
-        w = __fadd_rn(w, cluster.map_shared_rank(s2, r)[g]);
+  extern __shared__ __align__(16) float fifo[];  // x and dy of one tile
+  __shared__ __align__(16) float sh[2 * V * kTileThreads];
+  __shared__ float2 sums[kMaxTileGroups], means_by[2][kMaxTileGroups];
+  __shared__ float2 all[2][kMaxCluster][kMaxTileGroups];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, cv = a.c / V;
+  const bool joined = MODE == kInCluster && t.k > 1;
+  Walk<V, MODE> walk(t, MODE == kInCluster ? (int)cluster.block_rank() : 0);
+  if (joined) cluster.barrier_arrive();
+  const int64_t step = (int64_t)(kTileThreads / t.wide) * a.channels;
+  const int column = t.split > 1 ? 0 : walk.tx / cv;
+  Tile<V> me, next;
+  float2 stat, next_stat = make_float2(0.0f, 0.0f);  // mean and rstd of this thread's group
+  const auto fetch = [&]() {
+    if (walk.left) {
+      next = walk.get(a, t);
+      fetch_tile<V, N>(fifo, a.x, next, step);
+      fetch_tile<V, N>(fifo + kStage, a.dy, next, step);
+      const int64_t team = (int64_t)next.b * a.groups + next.g0 + (next.mine ? column : 0);
+      next_stat = make_float2(a.mean_in[team], a.rstd_in[team]);
+    }
+    copy_commit();
+  };
+  fetch();
+  if (joined) cluster.barrier_wait();
+  for (int n = 0; walk.left; n ^= 1) {
+    me = next;
+    stat = next_stat;
+    walk.advance(t);
+    Vec<V> x[N], d[N], db = splat<V>(0.0f), dg = db;
+    copy_wait<0>();
+    take_tile(x, fifo, me);
+    take_tile(d, fifo + kStage, me);
+    fetch();
+    const Pair rstd = both(stat.y);
+    if (me.mine) {
+      const Vec<V> ga = load_or<V>(a.gamma ? a.gamma + me.channel : nullptr, 1.0f);
+      const Vec<V> be = load_or<V>(a.beta ? a.beta + me.channel : nullptr, 0.0f);
+      const Pair minus = both(-stat.x);
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (i < me.mine) gradient(a.act, x[i], d[i], db, dg, minus, rstd, ga, be);
+    }
+    if (MODE != kWhole) tile_gradient_sums(db, dg, sh, sums, a, me, t, walk.tx);
+    if (joined) {
+      for (int g = warp; g < me.q; g += kTileThreads / 32) {
+        __syncwarp();
+        if (lane < t.k) cluster.map_shared_rank(&all[n][me.k][g], lane)[0] = sums[g];
+      }
+      cluster.sync();
+    }
+    float2 *means = means_by[n];
+    for (int g = warp; g < me.q; g += kTileThreads / 32) {
+      const int64_t team = (int64_t)me.b * a.groups + me.g0 + g;
+      __syncwarp();
+      if (MODE == kParts) {
+        if (lane == 0) reinterpret_cast<float2 *>(a.stat)[team * t.k + me.k] = sums[g];
+        continue;
+      }
+      float u = 0.0f, w = 0.0f;
+      if (MODE == kWhole) {
+        const float2 *q = reinterpret_cast<const float2 *>(a.stat) + team * t.k;
+        for (int i = lane; i < t.k; i += 32) u = __fadd_rn(u, q[i].x), w = __fadd_rn(w, q[i].y);
+      } else if (lane < t.k) {
+        const float2 q = joined ? all[n][lane][g] : sums[g];
+        u = q.x, w = q.y;
+      }
+      u = __fmul_rn(warp_sum(u), -a.inv_m);
+      w = __fmul_rn(warp_sum(w), -a.inv_m);
+      if (lane == 0) means[g] = make_float2(u, w);
+    }
+    __syncthreads();
+    if (MODE != kParts && me.mine) {
+      const Pair k1 = both(means[column].x), k2 = both(means[column].y);
+      float *q = a.dx + me.at;
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        if (i < me.mine) store(q, finish(x[i], d[i], k1, k2, rstd));
+        q += step;
       }
     }
-    k1[g] = __fdiv_rn(u, a.m);
-    k2[g] = __fdiv_rn(w, a.m);
   }
-  __syncthreads();
-  if (t.k > 1) cluster.barrier_arrive();
-  if (me.on) write_gradient(x, d, k1[me.group], k2[me.group], a, me, t);
-  if (t.k > 1) cluster.barrier_wait();
-}
-
-template <int V>
-__global__ void __launch_bounds__(kTileBackward, 2) norm_tile_sums_kernel(const Norm a, const Tiling t) {
-  pdl_wait();
-  constexpr int T = kTileBackward;
-  __shared__ float sh[2 * V * T], s1[T], s2[T];
-  const Tile<V, T> me(a, t, blockIdx.x / t.k, (int)(blockIdx.x % t.k));
-  float x[held(V)][V], d[held(V)][V], db[V], dg[V];
-  load_tile(x, a.x, me, t, a.channels);
-  load_tile(d, a.dy, me, t, a.channels);
-  tile_gradient(x, d, db, dg, a, me, t);
-  tile_gradient_sums(db, dg, sh, s1, s2, a, me, t);
-  for (int g = threadIdx.x; g < me.q; g += T) {
-    float *s = a.stat + ((me.b * a.groups + me.g0 + g) * t.k + me.k) * 2;
-    s[0] = s1[g];
-    s[1] = s2[g];
-  }
-}
-
-template <int V>
-__global__ void __launch_bounds__(kTileBackward, 2) norm_tile_dx_kernel(const Norm a, const Tiling t) {
-  pdl_wait();
-  constexpr int T = kTileBackward;
-  __shared__ float k1[T], k2[T];
-  const unsigned block = gridDim.x - 1 - blockIdx.x;
-  const Tile<V, T> me(a, t, block / t.k, (int)(block % t.k));
-  float x[held(V)][V], d[held(V)][V], db[V], dg[V];
-  load_tile(x, a.x, me, t, a.channels);
-  load_tile(d, a.dy, me, t, a.channels);
-  const int lane = threadIdx.x & 31;
-  for (int g = threadIdx.x >> 5; g < me.q; g += T / 32) {
-    const int64_t team = me.b * a.groups + me.g0 + g;
-    float u = 0.0f, w = 0.0f;
-    for (int r = lane; r < t.k; r += 32) {
-      const float2 p = *reinterpret_cast<const float2 *>(a.stat + (team * t.k + r) * 2);
-      u = __fadd_rn(u, p.x);
-      w = __fadd_rn(w, p.y);
-    }
-#pragma unroll
-    for (int e = 16; e > 0; e >>= 1) {
-      u = __fadd_rn(u, __shfl_xor_sync(kFull, u, e));
-      w = __fadd_rn(w, __shfl_xor_sync(kFull, w, e));
-    }
-    if (lane == 0) {
-      k1[g] = __fdiv_rn(u, a.m);
-      k2[g] = __fdiv_rn(w, a.m);
-    }
-  }
-  tile_gradient(x, d, db, dg, a, me, t);
-  __syncthreads();
-  if (me.on) write_gradient(x, d, k1[me.group], k2[me.group], a, me, t);
+  copy_wait<0>();
 }
 
 // ---------------------------------------------------------------- the parameters' gradients
 
-// dbeta[c] and dgamma[c] from part[p][2][groups][len][c] (len = 1 for the tile kernels'
-// per-channel rows): 32 channels a CTA, the p x len rows over its warps and over the CTAs of
-// a cluster, which fold their sums through distributed shared memory in order.
+// dbeta[c] and dgamma[c] from part[rows][2][channels]: 32 channels a CTA, the rows over its
+// warps and over the CTAs of a cluster, which fold their sums through distributed shared
+// memory in order.
 constexpr int kFoldWarps = 16;
 __global__ void __launch_bounds__(kFoldWarps * 32) norm_fold_kernel(float *__restrict__ dgamma,
                                                                     float *__restrict__ dbeta,
-                                                                    const float *__restrict__ part, int64_t parts,
-                                                                    int64_t len, int64_t channels, int groups, int c) {
+                                                                    const float *__restrict__ part, int rows,
+                                                                    int64_t channels) {
   pdl_wait();
   cg::cluster_group cluster = cg::this_cluster();
   const int rank = (int)cluster.block_rank(), ctas = (int)cluster.num_blocks();
@@ -807,35 +1006,31 @@ __global__ void __launch_bounds__(kFoldWarps * 32) norm_fold_kernel(float *__res
   __shared__ float sum[2][32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t ch = (int64_t)(blockIdx.x / ctas) * 32 + lane;
-  float s[2] = {0.0f, 0.0f};
+  float u = 0.0f, w = 0.0f;
   if (ch < channels) {
-    const int64_t row = channels * len, g = ch / c, col = g * len * c + (ch - g * c);
-    const uint32_t n = (uint32_t)(parts * len), per = (uint32_t)len;
-#pragma unroll 4
-    for (uint32_t r = rank * kFoldWarps + warp; r < n; r += ctas * kFoldWarps) {
-      const uint32_t p = r / per, l = r - p * per;
-      const float *at = part + p * 2 * row + col + (int64_t)l * c;
-      s[0] = __fadd_rn(s[0], at[0]);
-      s[1] = __fadd_rn(s[1], at[row]);
+#pragma unroll 8
+    for (int r = rank * kFoldWarps + warp; r < rows; r += ctas * kFoldWarps) {
+      const float *at = part + (int64_t)r * 2 * channels + ch;
+      u = __fadd_rn(u, at[0]);
+      w = __fadd_rn(w, at[channels]);
     }
   }
-  sh[0][warp][lane] = s[0];
-  sh[1][warp][lane] = s[1];
+  sh[0][warp][lane] = u;
+  sh[1][warp][lane] = w;
   __syncthreads();
   if (warp < 2) {
-    float u = sh[warp][0][lane];
+    u = sh[warp][0][lane];
 #pragma unroll
-    for (int w = 1; w < kFoldWarps; ++w) u = __fadd_rn(u, sh[warp][w][lane]);
+    for (int i = 1; i < kFoldWarps; ++i) u = __fadd_rn(u, sh[warp][i][lane]);
     sum[warp][lane] = u;
   }
-  cluster.sync();
+  if (ctas > 1) cluster.sync();
   if (rank == 0 && warp < 2 && ch < channels) {
-    float u = 0.0f;
-    for (int r = 0; r < ctas; ++r) u = __fadd_rn(u, cluster.map_shared_rank(&sum[0][0], r)[warp * 32 + lane]);
+    for (int r = 1; r < ctas; ++r) u = __fadd_rn(u, cluster.map_shared_rank(&sum[0][0], r)[warp * 32 + lane]);
     float *out = warp ? dgamma : dbeta;
     if (out) out[ch] = u;
   }
-  cluster.sync();
+  if (ctas > 1) cluster.sync();
 }
 
 // ---------------------------------------------------------------- choosing a kernel
@@ -848,11 +1043,17 @@ struct Plan {
   unsigned grid;
   Tiling t;
   bool cluster;          // tile kernels: statistics within a cluster
-  int64_t parts, part_len;  // rows of the per-channel partial sums (backward)
+  int parts;             // rows of the per-channel partial sums (backward)
+  int fold;              // row kernels: teams a CTA adds up
   size_t part_floats, stat_floats;
 };
 
 int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b; }
+int64_t power_of_two(int64_t a) {
+  int64_t p = 1;
+  while (p < a) p *= 2;
+  return p;
+}
 
 Plan norm_plan(int64_t batch, int64_t len, int64_t channels, int64_t groups, int v, bool backward) {
   Plan p{};
@@ -868,47 +1069,58 @@ Plan norm_plan(int64_t batch, int64_t len, int64_t channels, int64_t groups, int
     p.nv = 1;
     while ((int64_t)p.nv * p.lanes < vectors) p.nv *= 2;
     const int64_t per_cta = kRowThreads / p.lanes;
-    // enough teams in flight to fill the SMs a few times over; a multiple of groups
-    int64_t want = (int64_t)fz::num_sms() * 16 * per_cta / (p.lanes > 32 ? 2 : 1);
+    // Teams in flight: what is resident, a multiple of groups.
+    int64_t want = (int64_t)fz::num_sms() * per_cta * row_ctas(backward, p.nv);
     if (want > teams) want = teams;
     want = want / groups * groups;
     if (want < groups) want = groups;
     p.stride = (int)want;
     p.grid = (unsigned)up(want, per_cta);
     if (backward) {
-      p.parts = want / groups;
-      p.part_len = len;
-      p.part_floats = (size_t)(p.parts * 2 * channels * len);
+      p.fold = per_cta % groups == 0 ? (int)(per_cta / groups) : 1;
+      p.parts = (int)up(want, groups * p.fold);
+      p.part_floats = (size_t)p.parts * 2 * channels;
     }
     return p;
   }
-  // Tiles: whole groups side by side until a row's piece has 128 bytes, or a part of one
-  // group where it has more vectors than a CTA has threads.
-  const int threads = backward ? kTileBackward : kTileForward;
+  // Tiles: whole groups side by side, or a part of one group where it has more vectors than a
+  // CTA has threads.
   Tiling &t = p.t;
   t.q = 1;
-  t.split = (int)up(cv, threads);
+  t.split = (int)up(cv, kTileThreads);
   if (t.split == 1) {
-    const int64_t want = up(32, c);
-    t.q = (int)(want < groups ? want : groups);
-    while (t.q > 1 && t.q * cv > threads) --t.q;
+    // of the numbers of groups that give 96 to 192 bytes, the one that wastes the fewest
+    // thread columns (their number is a power of two)
+    double best = 0.0;
+    for (int64_t q = 1; q <= groups && q <= kMaxTileGroups && q * cv <= kTileThreads; ++q) {
+      if (q > 1 && q * c > 48) break;
+      const double use = (double)(q * cv) / power_of_two(q * cv) * (q * c >= 24 ? 1.0 : (double)(q * c) / 24);
+      if (use >= best) best = use, t.q = (int)q;
+    }
     t.cols = (int)(t.q * cv);
   } else {
     t.cols = (int)up(cv, t.split);
   }
+  t.wide = (int)power_of_two(t.cols);
   t.bundles = (int)up(groups, t.q);
-  t.ty = threads / t.cols;
-  t.rows = t.ty * held(v);
-  if (t.rows > len) t.rows = (int)len;
+  t.sets = (int)(batch * t.bundles);
+  // Rows: as few tiles one below the other as hold the sample, or, where those would leave
+  // SMs idle, as many as a cluster takes and that keep four rows a thread.
+  const int64_t ty = kTileThreads / t.wide, most = ty * held(v, backward);
+  int64_t chunks = up(len, most);
+  const int64_t idle = up((int64_t)fz::num_sms() * kTileCtas, (int64_t)t.sets * t.split);
+  int64_t room = kMaxCluster / t.split;
+  if (room > up(len, ty * 4)) room = up(len, ty * 4);
+  if (room > idle) room = idle;
+  if (chunks < room) chunks = room;
+  t.rows = (int)up(len, chunks);
   t.chunks = (int)up(len, t.rows);
   const int64_t k = (int64_t)t.split * t.chunks;
   t.k = (int)k;
   p.cluster = k <= kMaxCluster;
-  p.grid = (unsigned)(batch * t.bundles * k);
   if (backward) {
-    p.parts = batch * t.chunks;
-    p.part_len = 1;
-    p.part_floats = (size_t)(p.parts * 2 * channels);
+    p.parts = (int)(batch * t.chunks);
+    p.part_floats = (size_t)p.parts * 2 * channels;
   }
   if (!p.cluster) p.stat_floats = (size_t)(teams * k * 2);
   return p;
@@ -920,15 +1132,12 @@ int vector_of(std::initializer_list<const void *> ptrs) {
   return (all & 15) == 0 ? 4 : (all & 7) == 0 ? 2 : 1;
 }
 
-// Launch `kernel` over clusters of `k` CTAs (k = 1: none).
-template <typename... KArgs, typename... Args>
-int launch_cluster(void (*kernel)(KArgs...), unsigned grid, int threads, int k, cudaStream_t s, Args... args) {
-  if (k > 8) FZ_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+cudaLaunchConfig_t config(unsigned grid, int threads, int smem, int k, cudaStream_t s, cudaLaunchAttribute *attr) {
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(grid);
   cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = (size_t)smem;
   cfg.stream = s;
-  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   attr[1].id = cudaLaunchAttributeClusterDimension;
@@ -937,58 +1146,101 @@ int launch_cluster(void (*kernel)(KArgs...), unsigned grid, int threads, int k, 
   attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
+  return cfg;
+}
+
+// Launch a kernel over clusters of `k` CTAs (k = 1: none).
+template <typename... KArgs, typename... Args>
+int launch_cluster(void (*kernel)(KArgs...), unsigned grid, int threads, int smem, int k, cudaStream_t s,
+                   Args... args) {
+  cudaLaunchAttribute attr[2];
+  const cudaLaunchConfig_t cfg = config(grid, threads, smem, k, s, attr);
   FZ_CUDA(cudaLaunchKernelEx(&cfg, kernel, args...));
   FZ_CHECK_LAUNCH();
   return FZ_OK;
 }
 
-using RowKernel = void (*)(const Norm, int);
-template <int V>
-RowKernel row_kernel(int lanes, int nv) {
-  if (lanes == 4) return norm_rows_kernel<V, 4, 1, 4>;
-  if (lanes == 8) return norm_rows_kernel<V, 8, 1, 4>;
-  if (lanes == 16) return norm_rows_kernel<V, 16, 1, 4>;
-  if (lanes == 32)
-    return nv == 1 ? norm_rows_kernel<V, 32, 1, 4> : nv == 2 ? norm_rows_kernel<V, 32, 2, 4>
-         : nv == 4 ? norm_rows_kernel<V, 32, 4, 2> : norm_rows_kernel<V, 32, 8, 1>;
-  return nv == 2 ? norm_rows_kernel<V, kRowThreads, 2, 1> : nv == 4 ? norm_rows_kernel<V, kRowThreads, 4, 1>
-       : norm_rows_kernel<V, kRowThreads, 8, 1>;
+// Shared memory and cluster sizes that a kernel asks for, and (tile kernels in clusters)
+// how many clusters of k CTAs are resident at once, asked for once a device, kernel and k.
+int resident_clusters(const void *kernel, int threads, int smem, int k, int *count) {
+  struct Entry {
+    const void *kernel;
+    int device, k, count;
+  };
+  static std::mutex mu;
+  static Entry known[512];
+  static int entries = 0;
+  int device = 0;
+  FZ_CUDA(cudaGetDevice(&device));
+  std::lock_guard<std::mutex> lock(mu);
+  for (int i = 0; i < entries; ++i)
+    if (known[i].kernel == kernel && known[i].device == device && known[i].k == k) {
+      *count = known[i].count;
+      return FZ_OK;
+    }
+  FZ_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  if (k > 8) FZ_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+  cudaLaunchAttribute attr[2];
+  const cudaLaunchConfig_t cfg = config((unsigned)k, threads, smem, k, nullptr, attr);
+  int n = 0;
+  FZ_CUDA(cudaOccupancyMaxActiveClusters(&n, kernel, &cfg));
+  FZ_REQUIRE(n > 0, "group norm: a cluster does not fit the device");
+  if (entries < 512) known[entries++] = {kernel, device, k, n};
+  *count = n;
+  return FZ_OK;
 }
-template <int V>
-RowKernel row_backward_kernel(int lanes, int nv) {
-  if (lanes == 4) return norm_rows_backward_kernel<V, 4, 1, 4>;
-  if (lanes == 8) return norm_rows_backward_kernel<V, 8, 1, 4>;
-  if (lanes == 16) return norm_rows_backward_kernel<V, 16, 1, 4>;
-  if (lanes == 32)
-    return nv == 1 ? norm_rows_backward_kernel<V, 32, 1, 4> : nv == 2 ? norm_rows_backward_kernel<V, 32, 2, 2>
-         : nv == 4 ? norm_rows_backward_kernel<V, 32, 4, 1> : norm_rows_backward_kernel<V, 32, 8, 1>;
-  return nv == 2 ? norm_rows_backward_kernel<V, kRowThreads, 2, 1>
-       : nv == 4 ? norm_rows_backward_kernel<V, kRowThreads, 4, 1> : norm_rows_backward_kernel<V, kRowThreads, 8, 1>;
+
+template <typename... KArgs, typename... Args>
+int launch_rows(void (*kernel)(KArgs...), unsigned grid, int smem, cudaStream_t s, Args... args) {
+  FZ_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  FZ_CUDA(fz::launch_pdl(kernel, dim3(grid), dim3(kRowThreads), (size_t)smem, s, args...));
+  FZ_CHECK_LAUNCH();
+  return FZ_OK;
+}
+
+template <int V, int P, int NV>
+int run_row(const Norm &a, const Plan &p, bool backward, cudaStream_t s) {
+  if (backward)
+    return launch_rows(norm_rows_backward_kernel<V, P, NV>, p.grid, row_smem(true, P, NV, V), s, a, p.stride, p.fold);
+  return launch_rows(norm_rows_kernel<V, P, NV>, p.grid, row_smem(false, P, NV, V), s, a, p.stride);
 }
 
 template <int V>
-int run_forward(const Norm &a, const Plan &p, cudaStream_t s) {
-  if (p.lanes) {
-    FZ_CUDA(fz::launch_pdl(row_kernel<V>(p.lanes, p.nv), dim3(p.grid), dim3(kRowThreads), 0, s, a, p.stride));
-    FZ_CHECK_LAUNCH();
-    return FZ_OK;
+int run_rows(const Norm &a, const Plan &p, bool backward, cudaStream_t s) {
+  switch (p.lanes) {
+    case 4: return run_row<V, 4, 1>(a, p, backward, s);
+    case 8: return run_row<V, 8, 1>(a, p, backward, s);
+    case 16: return run_row<V, 16, 1>(a, p, backward, s);
+    case 32:
+      return p.nv == 1   ? run_row<V, 32, 1>(a, p, backward, s)
+             : p.nv == 2 ? run_row<V, 32, 2>(a, p, backward, s)
+             : p.nv == 4 ? run_row<V, 32, 4>(a, p, backward, s)
+                         : run_row<V, 32, 8>(a, p, backward, s);
+    default:
+      return p.nv == 2   ? run_row<V, kRowThreads, 2>(a, p, backward, s)
+             : p.nv == 4 ? run_row<V, kRowThreads, 4>(a, p, backward, s)
+                         : run_row<V, kRowThreads, 8>(a, p, backward, s);
   }
-  if (p.cluster) return launch_cluster(norm_tile_kernel<V>, p.grid, kTileForward, p.t.k, s, a, p.t);
-  if (int rc = launch_cluster(norm_tile_stats_kernel<V>, p.grid, kTileForward, 1, s, a, p.t)) return rc;
-  return launch_cluster(norm_tile_apply_kernel<V>, p.grid, kTileForward, 1, s, a, p.t);
+}
+
+template <int V, int MODE>
+int run_tile(const Norm &a, const Plan &p, bool backward, cudaStream_t s) {
+  const auto kernel = backward ? norm_tile_backward_kernel<V, MODE> : norm_tile_kernel<V, MODE>;
+  const int smem = held(V, backward) * kTileThreads * V * 4 * (backward ? 2 : 1);
+  const int k = MODE == kInCluster ? p.t.k : 1;
+  int resident = 0;
+  if (int rc = resident_clusters((const void *)kernel, kTileThreads, smem, k, &resident)) return rc;
+  const int64_t units = (int64_t)p.t.sets * (MODE == kInCluster ? 1 : p.t.k);
+  const int64_t grid = (units < resident ? units : resident) * k;
+  return launch_cluster(kernel, (unsigned)grid, kTileThreads, smem, k, s, a, p.t);
 }
 
 template <int V>
-int run_backward(const Norm &a, const Plan &p, cudaStream_t s) {
-  if (p.lanes) {
-    FZ_CUDA(fz::launch_pdl(row_backward_kernel<V>(p.lanes, p.nv), dim3(p.grid), dim3(kRowThreads), 0, s, a,
-                           p.stride));
-    FZ_CHECK_LAUNCH();
-    return FZ_OK;
-  }
-  if (p.cluster) return launch_cluster(norm_tile_backward_kernel<V>, p.grid, kTileBackward, p.t.k, s, a, p.t);
-  if (int rc = launch_cluster(norm_tile_sums_kernel<V>, p.grid, kTileBackward, 1, s, a, p.t)) return rc;
-  return launch_cluster(norm_tile_dx_kernel<V>, p.grid, kTileBackward, 1, s, a, p.t);
+int run(const Norm &a, const Plan &p, bool backward, cudaStream_t s) {
+  if (p.lanes) return run_rows<V>(a, p, backward, s);
+  if (p.cluster) return run_tile<V, kInCluster>(a, p, backward, s);
+  if (int rc = run_tile<V, kParts>(a, p, backward, s)) return rc;
+  return run_tile<V, kWhole>(a, p, backward, s);
 }
 
 int check_sizes(const char *who, int64_t batch, int64_t len, int64_t channels, int64_t groups) {
@@ -1037,9 +1289,9 @@ extern "C" int fz_group_norm(float *y, float *mean, float *rstd, const float *x,
   a.x = x, a.gamma = gamma, a.beta = beta, a.y = y, a.mean = mean, a.rstd = rstd;
   a.stat = (float *)workspace;
   a.batch = batch, a.len = len, a.channels = channels, a.groups = (int)groups, a.c = (int)(channels / groups);
-  a.m = (float)(len * a.c), a.eps = eps, a.act = act;
+  a.m = (float)(len * a.c), a.inv_m = (float)(1.0 / (double)(len * a.c)), a.eps = eps, a.act = act;
   cudaStream_t s = fz::resolve(stream);
-  return p.v == 4 ? run_forward<4>(a, p, s) : p.v == 2 ? run_forward<2>(a, p, s) : run_forward<1>(a, p, s);
+  return p.v == 4 ? run<4>(a, p, false, s) : p.v == 2 ? run<2>(a, p, false, s) : run<1>(a, p, false, s);
 }
 
 extern "C" int fz_group_norm_backward(float *dx, float *dgamma, float *dbeta, const float *dy, const float *x,
@@ -1065,15 +1317,14 @@ extern "C" int fz_group_norm_backward(float *dx, float *dgamma, float *dbeta, co
   a.stat = (float *)workspace;
   a.part = dgamma || dbeta ? (float *)workspace + p.stat_floats : nullptr;
   a.batch = batch, a.len = len, a.channels = channels, a.groups = (int)groups, a.c = (int)(channels / groups);
-  a.m = (float)(len * a.c), a.act = act;
-  if (int rc = p.v == 4 ? run_backward<4>(a, p, s) : p.v == 2 ? run_backward<2>(a, p, s) : run_backward<1>(a, p, s))
+  a.m = (float)(len * a.c), a.inv_m = (float)(1.0 / (double)(len * a.c)), a.act = act;
+  if (int rc = p.v == 4 ? run<4>(a, p, true, s) : p.v == 2 ? run<2>(a, p, true, s) : run<1>(a, p, true, s))
     return rc;
   if (!a.part) return FZ_OK;
   // CTAs a block of 32 channels: as many as have 4 rows a warp, until the SMs are filled
   const int64_t blocks = up(channels, 32);
   int ctas = 1;
-  while (ctas < 8 && blocks * ctas < fz::num_sms() && p.parts * p.part_len > (int64_t)ctas * 2 * kFoldWarps * 4)
-    ctas *= 2;
-  return launch_cluster(norm_fold_kernel, (unsigned)(blocks * ctas), kFoldWarps * 32, ctas, s, dgamma, dbeta,
-                        (const float *)a.part, p.parts, p.part_len, channels, (int)groups, a.c);
+  while (ctas < 8 && blocks * ctas < fz::num_sms() && p.parts > ctas * 2 * kFoldWarps * 4) ctas *= 2;
+  return launch_cluster(norm_fold_kernel, (unsigned)(blocks * ctas), kFoldWarps * 32, 0, ctas, s, dgamma, dbeta,
+                        (const float *)a.part, p.parts, channels);
 }
