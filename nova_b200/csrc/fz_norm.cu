@@ -703,58 +703,68 @@ __device__ __forceinline__ float warp_sum(float v) {
   return v;
 }
 
-// The threads' v, one a thread column, summed over the thread rows of each warp (lanes a
-// multiple of `wide` apart) and put into sh[row][wide]; `slices` rows of it.
+// A tile's thread rows come in slices: the thread rows of a warp where a warp holds several
+// (wide < 32), else one thread row each.
 __device__ __forceinline__ int slices_of(int wide) { return wide < 32 ? kTileThreads / 32 : kTileThreads / wide; }
-__device__ __forceinline__ void put_columns(float v, float *sh, int wide) {
+// The sum of v over the lanes of a warp that share a thread column.
+__device__ __forceinline__ float over_rows(float v, int wide) {
   for (int d = 16; d >= wide; d >>= 1) v = __fadd_rn(v, __shfl_xor_sync(kFull, v, d));
-  const int lane = threadIdx.x & 31;
-  if (wide >= 32) sh[threadIdx.x] = v;
-  else if (lane < wide) sh[(threadIdx.x >> 5) * wide + lane] = v;
+  return v;
 }
-// A warp's sum over `width` columns from `col` on.
-__device__ __forceinline__ float take_columns(const float *sh, int wide, int col, int width) {
-  const int lane = threadIdx.x & 31, n = slices_of(wide) * width;
-  int y = lane / width, c = lane - y * width;
-  const int dy = 32 / width, dc = 32 - dy * width;
-  float s = 0.0f;
-  for (int i = lane; i < n; i += 32) {
-    s = __fadd_rn(s, sh[y * wide + col + c]);
-    y += dy;
-    c += dc;
-    if (c >= width) c -= width, ++y;
-  }
-  return warp_sum(s);
+// Rows of the tile that slice y holds.
+__device__ __forceinline__ int rows_of_slice(int y, int rows, int wide, int shift) {
+  const int tall = wide < 32 ? 32 / wide : 1, rest = rows & ((1 << shift) - 1);
+  return (rows >> shift) * tall + min(max(rest - y * tall, 0), tall);
 }
 
-// The tile's own (mean, M2) per group, by the warp that goes on with the group.
+// The tile's own (mean, M2) of group g in every lane of the warp that asks, after the
+// barrier in here. Each slice reduces a column to its mean and the sum of squares about it;
+// the warp joins the group's columns: M2 = sum of theirs + n_column (mean_column - mean)^2.
 template <int V, int N>
-__device__ __forceinline__ void tile_moments(const Vec<V> (&x)[N], float *sh, float *sh2, float2 *moments,
-                                             const Norm &a, const Tile<V> &me, const Tiling &t, int tx) {
-  const int cv = a.c / V, width = t.split > 1 ? me.cols : cv, warp = threadIdx.x >> 5;
+__device__ __forceinline__ void column_moments(const Vec<V> (&x)[N], float2 *sh, const Tile<V> &me, const Tiling &t,
+                                               int shift) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int slice = t.wide < 32 ? warp : (int)threadIdx.x / t.wide;
   Vec<V> s = x[0];
 #pragma unroll
   for (int i = 1; i < N; ++i) sum_into(s, x[i]);
-  put_columns(total(s), sh, t.wide);
-  __syncthreads();
-  const float n = (float)me.rows * (float)(width * V);
-  for (int g = warp; g < me.q; g += kTileThreads / 32) {
-    const float mean = __fdiv_rn(take_columns(sh, t.wide, g * cv, width), n);
-    if ((threadIdx.x & 31) == 0) moments[g].x = mean;
-  }
-  __syncthreads();
-  const float mean = moments[me.mine ? (t.split > 1 ? 0 : tx / cv) : 0].x;
+  const float n = (float)(rows_of_slice(slice, me.rows, t.wide, shift) * V);
+  const float mean = __fdiv_rn(over_rows(total(s), t.wide), n);  // n = 0: not read
   const Pair minus = V == 1 ? pair(-mean, 0.0f) : both(-mean);
   s = splat<V>(0.0f);
 #pragma unroll
   for (int i = 0; i < N; ++i)
     if (i < me.mine) square_into(s, x[i], minus);
-  put_columns(total(s), sh2, t.wide);
+  const float m2 = over_rows(total(s), t.wide);
+  if (t.wide >= 32) sh[threadIdx.x] = make_float2(mean, m2);
+  else if (lane < t.wide) sh[warp * t.wide + lane] = make_float2(mean, m2);
   __syncthreads();
-  for (int g = warp; g < me.q; g += kTileThreads / 32) {
-    const float m2 = take_columns(sh2, t.wide, g * cv, width);
-    if ((threadIdx.x & 31) == 0) moments[g].y = m2;
+}
+template <int V>
+__device__ __forceinline__ float2 group_moments(const float2 *sh, int g, const Norm &a, const Tile<V> &me,
+                                                const Tiling &t, int shift) {
+  const int lane = threadIdx.x & 31, cv = a.c / V, width = t.split > 1 ? me.cols : cv;
+  const int total = slices_of(t.wide) * width, dy = 32 / width, dc = 32 - dy * width;
+  const int y0 = lane / width, c0 = lane - y0 * width;
+  float u = 0.0f, w = 0.0f;
+  for (int i = lane, y = y0, c = c0; i < total; i += 32) {
+    const int n = rows_of_slice(y, me.rows, t.wide, shift) * V;
+    if (n) u = __fmaf_rn((float)n, sh[y * t.wide + g * cv + c].x, u);
+    y += dy, c += dc;
+    if (c >= width) c -= width, ++y;
   }
+  const float mean = __fdiv_rn(warp_sum(u), (float)me.rows * (float)(width * V));
+  for (int i = lane, y = y0, c = c0; i < total; i += 32) {
+    const int n = rows_of_slice(y, me.rows, t.wide, shift) * V;
+    if (n) {
+      const float2 p = sh[y * t.wide + g * cv + c];
+      const float d = __fsub_rn(p.x, mean);
+      w = __fadd_rn(w, __fmaf_rn(__fmul_rn(d, d), (float)n, p.y));
+    }
+    y += dy, c += dc;
+    if (c >= width) c -= width, ++y;
+  }
+  return make_float2(mean, warp_sum(w));
 }
 
 // mean and rstd of the union of lanes' (n, mean, M2); every lane gets them.
@@ -770,9 +780,9 @@ __global__ void __launch_bounds__(kTileThreads, kTileCtas) norm_tile_kernel(cons
   constexpr int N = held(V, false);
   cg::cluster_group cluster = cg::this_cluster();
   extern __shared__ __align__(16) float fifo[];
-  __shared__ float sh[kTileThreads], sh2[kTileThreads];
+  __shared__ float2 sh[kTileThreads];
   // by parity of the tile: a warp may be a tile ahead of one that still reads
-  __shared__ float2 moments[kMaxTileGroups], stats_by[2][kMaxTileGroups];
+  __shared__ float2 stats_by[2][kMaxTileGroups];
   // the cluster's moments by parity of the tile, so that one barrier a tile is enough: a CTA
   // writes a parity again only after a barrier that all have reached behind their reading it
   __shared__ float2 all[2][kMaxCluster][kMaxTileGroups];
@@ -801,27 +811,28 @@ __global__ void __launch_bounds__(kTileThreads, kTileCtas) norm_tile_kernel(cons
       fetch_tile<V, N>(fifo, a.x, next, step);
     }
     copy_commit();
-    if (MODE != kWhole) tile_moments(x, sh, sh2, moments, a, me, t, walk.tx);
+    if (MODE != kWhole) column_moments(x, sh, me, t, walk.shift);
     if (joined) {
       for (int g = warp; g < me.q; g += kTileThreads / 32) {
-        __syncwarp();
-        if (lane < t.k) cluster.map_shared_rank(&all[n][me.k][g], lane)[0] = moments[g];
+        const float2 m = group_moments(sh, g, a, me, t, walk.shift);
+        if (lane < t.k) cluster.map_shared_rank(&all[n][me.k][g], lane)[0] = m;
       }
       cluster.sync();
     }
     float2 *stats = stats_by[n];
     for (int g = warp; g < me.q; g += kTileThreads / 32) {
       const int64_t team = (int64_t)me.b * a.groups + me.g0 + g;
-      __syncwarp();
       if (MODE == kParts) {
-        if (lane == 0) reinterpret_cast<float2 *>(a.stat)[team * t.k + me.k] = moments[g];
+        const float2 m = group_moments(sh, g, a, me, t, walk.shift);
+        if (lane == 0) reinterpret_cast<float2 *>(a.stat)[team * t.k + me.k] = m;
         continue;
       }
       float2 r;
       if (joined) {
         r = join_lanes(share, lane < t.k ? all[n][lane][g] : make_float2(0.0f, 0.0f), a);
       } else if (MODE == kInCluster) {
-        r = make_float2(moments[g].x, rstd_of(moments[g].y, a.inv_m, a.eps));
+        r = group_moments(sh, g, a, me, t, walk.shift);
+        r.y = rstd_of(r.y, a.inv_m, a.eps);
       } else {
         const float2 *q = reinterpret_cast<const float2 *>(a.stat) + team * t.k;
         float u = 0.0f, w = 0.0f;
@@ -857,12 +868,15 @@ __global__ void __launch_bounds__(kTileThreads, kTileCtas) norm_tile_kernel(cons
   copy_wait<0>();
 }
 
-// The tile's sums of dv and dv xh: per channel into `part`, and gamma-weighted per group,
-// by the warp that goes on with the group. sh: [slices][2][wide * V].
+// The tile's sums of dv and dv xh. column_sums: per slice and channel to sh[slices][2][wide * V],
+// with a barrier at the end. Then, a warp a group, group_sums adds up the slices, leaves the
+// channels' sums in `part` and gives the gamma-weighted sums over the group to every lane.
+// Groups of many channels are added up over the slices by all threads first.
+constexpr int kNarrow = 32;  // channels a group up to which a warp adds up the slices alone
 template <int V>
-__device__ __forceinline__ void tile_gradient_sums(Vec<V> db, Vec<V> dg, float *sh, float2 *sums, const Norm &a,
-                                                   const Tile<V> &me, const Tiling &t, int tx) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, row = t.wide * V, slices = slices_of(t.wide);
+__device__ __forceinline__ void column_sums(Vec<V> db, Vec<V> dg, float *sh, const Norm &a, const Tile<V> &me,
+                                            const Tiling &t, int tx) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, row = t.wide * V;
   for (int d = 16; d >= t.wide; d >>= 1) {
 #pragma unroll
     for (int i = 0; i < Vec<V>::N; ++i) {
@@ -876,28 +890,36 @@ __device__ __forceinline__ void tile_gradient_sums(Vec<V> db, Vec<V> dg, float *
     store(q + row, dg);
   }
   __syncthreads();
-  const int n = me.cols * V, first = me.channel - tx * V;
-  for (int i = threadIdx.x; i < 2 * n; i += kTileThreads) {
-    const int which = i >= n, ch = i - (which ? n : 0);
-    float *q = sh + which * row + ch;
+  if (a.c > kNarrow) {
+    const int n = me.cols * V, slices = slices_of(t.wide);
+    for (int i = threadIdx.x; i < 2 * n; i += kTileThreads) {
+      const int which = i >= n, ch = i - (which ? n : 0);
+      float *q = sh + which * row + ch;
+      float s = q[0];
+      for (int y = 1; y < slices; ++y) s = __fadd_rn(s, q[y * 2 * row]);
+      q[0] = s;
+    }
+    __syncthreads();
+  }
+}
+template <int V>
+__device__ __forceinline__ float2 group_sums(const float *sh, int g, const Norm &a, const Tile<V> &me,
+                                             const Tiling &t, int tx) {
+  const int lane = threadIdx.x & 31, row = t.wide * V, slices = a.c > kNarrow ? 1 : slices_of(t.wide);
+  const int width = t.split > 1 ? me.cols * V : a.c, first = me.channel - tx * V + g * a.c;
+  float *part = a.part ? a.part + ((int64_t)me.b * t.chunks + me.chunk) * 2 * a.channels + first : nullptr;
+  float u = 0.0f, w = 0.0f;
+  for (int i = lane; i < 2 * width; i += 32) {
+    const int which = i >= width, ch = i - (which ? width : 0);
+    const float *q = sh + which * row + g * a.c + ch;
     float s = q[0];
     for (int y = 1; y < slices; ++y) s = __fadd_rn(s, q[y * 2 * row]);
-    q[0] = s;
-    if (a.part) a.part[(((int64_t)me.b * t.chunks + me.chunk) * 2 + which) * a.channels + first + ch] = s;
+    if (part) part[which * a.channels + ch] = s;
+    s = __fmul_rn(a.gamma ? a.gamma[first + ch] : 1.0f, s);
+    if (which) w = __fadd_rn(w, s);
+    else u = __fadd_rn(u, s);
   }
-  __syncthreads();
-  const int width = t.split > 1 ? n : a.c;
-  for (int g = warp; g < me.q; g += kTileThreads / 32) {
-    float u = 0.0f, w = 0.0f;
-    for (int i = lane; i < width; i += 32) {
-      const float ga = a.gamma ? a.gamma[first + g * a.c + i] : 1.0f;
-      u = __fmaf_rn(ga, sh[g * a.c + i], u);
-      w = __fmaf_rn(ga, sh[row + g * a.c + i], w);
-    }
-    u = warp_sum(u);
-    w = warp_sum(w);
-    if (lane == 0) sums[g] = make_float2(u, w);
-  }
+  return make_float2(warp_sum(u), warp_sum(w));
 }
 
 template <int V, int MODE>
@@ -907,7 +929,7 @@ __global__ void __launch_bounds__(kTileThreads, kTileCtas) norm_tile_backward_ke
   cg::cluster_group cluster = cg::this_cluster();
   extern __shared__ __align__(16) float fifo[];  // x and dy of one tile
   __shared__ __align__(16) float sh[2 * V * kTileThreads];
-  __shared__ float2 sums[kMaxTileGroups], means_by[2][kMaxTileGroups];
+  __shared__ float2 means_by[2][kMaxTileGroups];
   __shared__ float2 all[2][kMaxCluster][kMaxTileGroups];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, cv = a.c / V;
   const bool joined = MODE == kInCluster && t.k > 1;
@@ -947,32 +969,33 @@ __global__ void __launch_bounds__(kTileThreads, kTileCtas) norm_tile_backward_ke
       for (int i = 0; i < N; ++i)
         if (i < me.mine) gradient(a.act, x[i], d[i], db, dg, minus, rstd, ga, be);
     }
-    if (MODE != kWhole) tile_gradient_sums(db, dg, sh, sums, a, me, t, walk.tx);
+    if (MODE != kWhole) column_sums(db, dg, sh, a, me, t, walk.tx);
     if (joined) {
       for (int g = warp; g < me.q; g += kTileThreads / 32) {
-        __syncwarp();
-        if (lane < t.k) cluster.map_shared_rank(&all[n][me.k][g], lane)[0] = sums[g];
+        const float2 m = group_sums(sh, g, a, me, t, walk.tx);
+        if (lane < t.k) cluster.map_shared_rank(&all[n][me.k][g], lane)[0] = m;
       }
       cluster.sync();
     }
     float2 *means = means_by[n];
     for (int g = warp; g < me.q; g += kTileThreads / 32) {
       const int64_t team = (int64_t)me.b * a.groups + me.g0 + g;
-      __syncwarp();
+      float2 m = make_float2(0.0f, 0.0f);
+      if (MODE == kParts || (MODE == kInCluster && !joined)) m = group_sums(sh, g, a, me, t, walk.tx);
       if (MODE == kParts) {
-        if (lane == 0) reinterpret_cast<float2 *>(a.stat)[team * t.k + me.k] = sums[g];
+        if (lane == 0) reinterpret_cast<float2 *>(a.stat)[team * t.k + me.k] = m;
         continue;
       }
-      float u = 0.0f, w = 0.0f;
+      float u = m.x, w = m.y;
       if (MODE == kWhole) {
         const float2 *q = reinterpret_cast<const float2 *>(a.stat) + team * t.k;
         for (int i = lane; i < t.k; i += 32) u = __fadd_rn(u, q[i].x), w = __fadd_rn(w, q[i].y);
-      } else if (lane < t.k) {
-        const float2 q = joined ? all[n][lane][g] : sums[g];
-        u = q.x, w = q.y;
+      } else if (joined && lane < t.k) {
+        u = all[n][lane][g].x, w = all[n][lane][g].y;
       }
-      u = __fmul_rn(warp_sum(u), -a.inv_m);
-      w = __fmul_rn(warp_sum(w), -a.inv_m);
+      if (MODE == kWhole || joined) u = warp_sum(u), w = warp_sum(w);
+      u = __fmul_rn(u, -a.inv_m);
+      w = __fmul_rn(w, -a.inv_m);
       if (lane == 0) means[g] = make_float2(u, w);
     }
     __syncthreads();
@@ -1089,12 +1112,16 @@ Plan norm_plan(int64_t batch, int64_t len, int64_t channels, int64_t groups, int
   t.q = 1;
   t.split = (int)up(cv, kTileThreads);
   if (t.split == 1) {
-    // of the numbers of groups that give 96 to 192 bytes, the one that wastes the fewest
-    // thread columns (their number is a power of two)
+    // Of the numbers of groups that give 48 to 192 bytes a row, the one that wastes the fewest
+    // thread columns (their number is a power of two), the larger of equals; tiles of less
+    // than 96 bytes only where they bring the cluster to 8 CTAs.
     double best = 0.0;
     for (int64_t q = 1; q <= groups && q <= kMaxTileGroups && q * cv <= kTileThreads; ++q) {
       if (q > 1 && q * c > 48) break;
-      const double use = (double)(q * cv) / power_of_two(q * cv) * (q * c >= 24 ? 1.0 : (double)(q * c) / 24);
+      const int64_t wide = power_of_two(q * cv), tall = kTileThreads / wide * held(v, backward);
+      double use = (double)(q * cv) / wide;
+      if (q * c < 24) use *= q * c / 24.0;
+      if (up(len, tall) > 8 && up(len, tall) <= 2 * kMaxCluster) use *= 0.6;
       if (use >= best) best = use, t.q = (int)q;
     }
     t.cols = (int)(t.q * cv);
