@@ -23,7 +23,6 @@ namespace {
 
 constexpr int kThreads = 512;
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLn2 = 0.69314718055994531f;
 
 // 2^x to within 2 ulp (results below the normal range flush to 0, next to sums that are
 // at least 1).

@@ -280,6 +280,7 @@ struct Norm {
   int groups, c;  // c: channels a group
   float m, inv_m, eps;  // inv_m = 1 / m
   int act;
+  int *err;  // where a wait that gave up is recorded, or null
 };
 
 // ---------------------------------------------------------------- row kernels
@@ -774,6 +775,71 @@ __device__ __forceinline__ float2 join_lanes(float n, float2 p, const Norm &a) {
   return make_float2(mean, rstd_of(m2, a.inv_m, a.eps));
 }
 
+// The statistics that a cluster's CTAs push to one another: all[parity][CTA][group]. Each
+// push is an asynchronous store that counts its bytes on the receiving CTA's mbarrier of that
+// parity, so a tile costs neither a cluster barrier nor the fence that comes with one (which
+// would wait for the tile's own stores to memory). Parities suffice: a CTA pushes tile n + 2
+// only after it got all of tile n + 1, which the others push after they have read tile n.
+constexpr unsigned long long kWaitNs = 4000000000ull;  // 4 s
+constexpr int kErrNormExchange = 16;
+struct Exchange {
+  float2 all[2][kMaxCluster][kMaxTileGroups];
+  uint64_t bar[2];
+  int gave_up;
+};
+__device__ __forceinline__ uint32_t shared_address(const void *p) {
+  return (uint32_t)__cvta_generic_to_shared(p);
+}
+__device__ __forceinline__ void exchange_init(Exchange &x) {
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2; ++i)
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(shared_address(&x.bar[i])) : "memory");
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    x.gave_up = 0;
+  }
+}
+// One thread: this tile's bytes are to come.
+__device__ __forceinline__ void exchange_expect(Exchange &x, int parity, int bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(shared_address(&x.bar[parity])),
+               "r"(bytes)
+               : "memory");
+}
+// Lane r < k: group g's pair to CTA r.
+__device__ __forceinline__ void exchange_push(Exchange &x, int parity, int from, int g, int to, float2 v) {
+  uint32_t slot, bar;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(slot) : "r"(shared_address(&x.all[parity][from][g])), "r"(to));
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(bar) : "r"(shared_address(&x.bar[parity])), "r"(to));
+  asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.b64 [%0], %1, [%2];" ::"r"(slot),
+               "l"(pair(v.x, v.y)), "r"(bar)
+               : "memory");
+}
+// Until this tile's pairs are there. A wait that takes 4 s is given up and recorded; the CTA
+// then waits no more and runs to its end.
+__device__ __forceinline__ void exchange_wait(Exchange &x, int parity, int phase, int *err) {
+  const auto ready = [&]() {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.b32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(shared_address(&x.bar[parity])), "r"(phase)
+        : "memory");
+    return ok != 0;
+  };
+  if (ready()) return;
+  volatile int *gave_up = &x.gave_up;
+  uint64_t t0, t;
+  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t0));
+  while (!ready() && !*gave_up) {
+    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+    if (t - t0 > kWaitNs) {
+      *gave_up = 1;
+      if (err) atomicCAS(err, 0, kErrNormExchange);
+    }
+  }
+}
+
 template <int V, int MODE>
 __global__ void __launch_bounds__(kTileThreads, kTileCtas) norm_tile_kernel(const Norm a, const Tiling t) {
   pdl_wait();
@@ -783,13 +849,15 @@ __global__ void __launch_bounds__(kTileThreads, kTileCtas) norm_tile_kernel(cons
   __shared__ float2 sh[kTileThreads];
   // by parity of the tile: a warp may be a tile ahead of one that still reads
   __shared__ float2 stats_by[2][kMaxTileGroups];
-  // the cluster's moments by parity of the tile, so that one barrier a tile is enough: a CTA
-  // writes a parity again only after a barrier that all have reached behind their reading it
-  __shared__ float2 all[2][kMaxCluster][kMaxTileGroups];
+  __shared__ Exchange exchange;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, cv = a.c / V;
   const bool joined = MODE == kInCluster && t.k > 1;
   Walk<V, MODE> walk(t, MODE == kInCluster ? (int)cluster.block_rank() : 0);
-  if (joined) cluster.barrier_arrive();
+  if (joined) {
+    exchange_init(exchange);
+    __syncthreads();
+    cluster.barrier_arrive();
+  }
   const int64_t step = (int64_t)(kTileThreads / t.wide) * a.channels;
   const int column = t.split > 1 ? 0 : walk.tx / cv;  // this thread's group in the tile
   const float share = joined && lane < t.k ? count_of<V>(a, t, lane) : 0.0f;
@@ -800,7 +868,8 @@ __global__ void __launch_bounds__(kTileThreads, kTileCtas) norm_tile_kernel(cons
   }
   copy_commit();
   if (joined) cluster.barrier_wait();  // all of the cluster's CTAs run
-  for (int n = 0; walk.left; n ^= 1) {
+  for (int i = 0; walk.left; ++i) {
+    const int n = i & 1;
     me = next;
     walk.advance(t);
     Vec<V> x[N];
@@ -813,11 +882,12 @@ __global__ void __launch_bounds__(kTileThreads, kTileCtas) norm_tile_kernel(cons
     copy_commit();
     if (MODE != kWhole) column_moments(x, sh, me, t, walk.shift);
     if (joined) {
+      if (threadIdx.x == kTileThreads - 1) exchange_expect(exchange, n, t.k * me.q * (int)sizeof(float2));
       for (int g = warp; g < me.q; g += kTileThreads / 32) {
         const float2 m = group_moments(sh, g, a, me, t, walk.shift);
-        if (lane < t.k) cluster.map_shared_rank(&all[n][me.k][g], lane)[0] = m;
+        if (lane < t.k) exchange_push(exchange, n, me.k, g, lane, m);
       }
-      cluster.sync();
+      if (warp < me.q) exchange_wait(exchange, n, i >> 1 & 1, a.err);
     }
     float2 *stats = stats_by[n];
     for (int g = warp; g < me.q; g += kTileThreads / 32) {
@@ -829,7 +899,7 @@ __global__ void __launch_bounds__(kTileThreads, kTileCtas) norm_tile_kernel(cons
       }
       float2 r;
       if (joined) {
-        r = join_lanes(share, lane < t.k ? all[n][lane][g] : make_float2(0.0f, 0.0f), a);
+        r = join_lanes(share, lane < t.k ? exchange.all[n][lane][g] : make_float2(0.0f, 0.0f), a);
       } else if (MODE == kInCluster) {
         r = group_moments(sh, g, a, me, t, walk.shift);
         r.y = rstd_of(r.y, a.inv_m, a.eps);
@@ -930,11 +1000,15 @@ __global__ void __launch_bounds__(kTileThreads, kTileCtas) norm_tile_backward_ke
   extern __shared__ __align__(16) float fifo[];  // x and dy of one tile
   __shared__ __align__(16) float sh[2 * V * kTileThreads];
   __shared__ float2 means_by[2][kMaxTileGroups];
-  __shared__ float2 all[2][kMaxCluster][kMaxTileGroups];
+  __shared__ Exchange exchange;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, cv = a.c / V;
   const bool joined = MODE == kInCluster && t.k > 1;
   Walk<V, MODE> walk(t, MODE == kInCluster ? (int)cluster.block_rank() : 0);
-  if (joined) cluster.barrier_arrive();
+  if (joined) {
+    exchange_init(exchange);
+    __syncthreads();
+    cluster.barrier_arrive();
+  }
   const int64_t step = (int64_t)(kTileThreads / t.wide) * a.channels;
   const int column = t.split > 1 ? 0 : walk.tx / cv;
   Tile<V> me, next;
@@ -951,7 +1025,8 @@ __global__ void __launch_bounds__(kTileThreads, kTileCtas) norm_tile_backward_ke
   };
   fetch();
   if (joined) cluster.barrier_wait();
-  for (int n = 0; walk.left; n ^= 1) {
+  for (int i = 0; walk.left; ++i) {
+    const int n = i & 1;
     me = next;
     stat = next_stat;
     walk.advance(t);
@@ -971,11 +1046,12 @@ __global__ void __launch_bounds__(kTileThreads, kTileCtas) norm_tile_backward_ke
     }
     if (MODE != kWhole) column_sums(db, dg, sh, a, me, t, walk.tx);
     if (joined) {
+      if (threadIdx.x == kTileThreads - 1) exchange_expect(exchange, n, t.k * me.q * (int)sizeof(float2));
       for (int g = warp; g < me.q; g += kTileThreads / 32) {
         const float2 m = group_sums(sh, g, a, me, t, walk.tx);
-        if (lane < t.k) cluster.map_shared_rank(&all[n][me.k][g], lane)[0] = m;
+        if (lane < t.k) exchange_push(exchange, n, me.k, g, lane, m);
       }
-      cluster.sync();
+      if (warp < me.q) exchange_wait(exchange, n, i >> 1 & 1, a.err);
     }
     float2 *means = means_by[n];
     for (int g = warp; g < me.q; g += kTileThreads / 32) {
@@ -991,7 +1067,7 @@ __global__ void __launch_bounds__(kTileThreads, kTileCtas) norm_tile_backward_ke
         const float2 *q = reinterpret_cast<const float2 *>(a.stat) + team * t.k;
         for (int i = lane; i < t.k; i += 32) u = __fadd_rn(u, q[i].x), w = __fadd_rn(w, q[i].y);
       } else if (joined && lane < t.k) {
-        u = all[n][lane][g].x, w = all[n][lane][g].y;
+        u = exchange.all[n][lane][g].x, w = exchange.all[n][lane][g].y;
       }
       if (MODE == kWhole || joined) u = warp_sum(u), w = warp_sum(w);
       u = __fmul_rn(u, -a.inv_m);
@@ -1251,7 +1327,15 @@ int run_rows(const Norm &a, const Plan &p, bool backward, cudaStream_t s) {
 }
 
 template <int V, int MODE>
-int run_tile(const Norm &a, const Plan &p, bool backward, cudaStream_t s) {
+int run_tile(Norm a, const Plan &p, bool backward, cudaStream_t s) {
+  // the word for waits that give up; not allocated while the stream is being captured
+  a.err = fz::device_error_word_if_any();
+  if (!a.err && MODE == kInCluster) {
+    cudaStreamCaptureStatus capture;
+    FZ_CUDA(cudaStreamIsCapturing(s, &capture));
+    if (capture == cudaStreamCaptureStatusNone)
+      if (int rc = fz::device_error_word(&a.err)) return rc;
+  }
   const auto kernel = backward ? norm_tile_backward_kernel<V, MODE> : norm_tile_kernel<V, MODE>;
   const int smem = held(V, backward) * kTileThreads * V * 4 * (backward ? 2 : 1);
   const int k = MODE == kInCluster ? p.t.k : 1;

@@ -108,6 +108,12 @@ int device_error_word(int **word) {
   return FZ_OK;
 }
 
+int *device_error_word_if_any() {
+  int d = current_device();
+  std::lock_guard<std::mutex> lk(g_err_mu);
+  return g_err_word[d];
+}
+
 int num_sms() {
   int d = current_device();
   if (!g_dev[d].sms) setup_device(d);
