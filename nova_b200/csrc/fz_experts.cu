@@ -36,8 +36,44 @@ __device__ __forceinline__ float warp_sum(float v) {
   return v;
 }
 
-// One warp per token, expert e = lane + 32 i in register i of lane `lane`. Each pick is
-// two warp-wide integer reductions: the largest key, then the lowest expert that has it.
+__device__ __forceinline__ float exp_below(float v, float top) {  // e^(v - top)
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(__fmul_rn(__fsub_rn(v, top), 1.4426950408889634f)));
+  return y;
+}
+
+// Descending sort of a lane's N keys: Batcher's odd-even merge network.
+template <int N>
+__device__ __forceinline__ void sort_keys(uint32_t (&key)[N]) {
+#pragma unroll
+  for (int p = 1; p < N; p *= 2)
+#pragma unroll
+    for (int q = p; q > 0; q /= 2)
+#pragma unroll
+      for (int j = q % p; j + q < N; j += 2 * q)
+#pragma unroll
+        for (int i = 0; i < q; ++i)
+          if (i + j + q < N && (i + j) / (2 * p) == (i + j + q) / (2 * p)) {
+            const uint32_t x = key[i + j], y = key[i + j + q];
+            key[i + j] = max(x, y);
+            key[i + j + q] = min(x, y);
+          }
+}
+
+template <int NE>
+__device__ __forceinline__ void load_row(float (&v)[NE], const float *row, int lane, int experts) {
+#pragma unroll
+  for (int i = 0; i < NE; ++i) v[i] = lane + 32 * i < experts ? row[lane + 32 * i] : -INFINITY;
+}
+
+// One warp per token, expert e = lane + 32 i in register i of lane `lane`, the next token's
+// logits fetched ahead. Bound by instruction issue, so experts are picked by their keys
+// alone: every lane sorts its own keys once, a pick is the largest of the lanes' heads (one
+// warp-wide reduction) and its lane moves its list up. Then the experts whose keys were
+// picked are found in ascending order, each taking the first open pick of its key: ties go
+// to the lowest experts, and those that are too many find none. (Keeping each expert's
+// number with its key, and removing it from an unsorted list, cost 2.4 times as many
+// instructions at 256 experts and 8 picks.)
 template <int NE>
 __global__ void __launch_bounds__(256) route_kernel(float *__restrict__ weights, int32_t *__restrict__ ids,
                                                     const float *__restrict__ logits, int64_t tokens, int experts,
@@ -45,59 +81,62 @@ __global__ void __launch_bounds__(256) route_kernel(float *__restrict__ weights,
   pdl_wait();
   const int lane = threadIdx.x & 31;
   const int64_t warps = (int64_t)gridDim.x * (blockDim.x >> 5);
-  for (int64_t t = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); t < tokens; t += warps) {
-    const float *row = logits + t * experts;
-    float v[NE];
+  int64_t t = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+  float v[NE], next[NE];
+  if (t < tokens) load_row(next, logits + t * experts, lane, experts);
+  for (; t < tokens; t += warps) {
     uint32_t key[NE];
 #pragma unroll
     for (int i = 0; i < NE; ++i) {
-      const int e = lane + 32 * i;
-      v[i] = e < experts ? row[e] : 0.0f;
-      key[i] = e < experts ? order_key(v[i]) : 0u;
+      v[i] = next[i];
+      key[i] = order_key(v[i]);
     }
-    float mine = 0.0f;  // lane j: the j-th pick's logit
-    int my_id = -1;
+    if (t + warps < tokens) load_row(next, logits + (t + warps) * experts, lane, experts);
+    sort_keys(key);
+    uint32_t mine = 0;  // lane j: the j-th pick's key; 0: none
     for (int j = 0; j < k; ++j) {
-      uint32_t best = key[0];
-      int at = 0;
-#pragma unroll
-      for (int i = 1; i < NE; ++i)
-        if (key[i] > best) {
-          best = key[i];
-          at = i;
-        }
-      const uint32_t top = __reduce_max_sync(kFull, best);
+      const uint32_t top = __reduce_max_sync(kFull, key[0]);
       if (top <= kKeyMinusInf) break;  // only -inf (or nothing) left
-      const int e = (int)__reduce_min_sync(kFull, best == top ? (unsigned)(lane + 32 * at) : 0xffffffffu);
-      const int owner = e & 31, slot = e >> 5;
-      float picked = 0.0f;
+      const int owner = __ffs(__ballot_sync(kFull, key[0] == top)) - 1;
+      if (lane == j) mine = top;
+      if (lane == owner) {
 #pragma unroll
-      for (int i = 0; i < NE; ++i)
-        if (i == slot) {
-          picked = v[i];
-          if (lane == owner) key[i] = 0u;
-        }
-      picked = __shfl_sync(kFull, picked, owner);
-      if (lane == j) {
-        mine = picked;
-        my_id = e;
+        for (int i = 0; i + 1 < NE; ++i) key[i] = key[i + 1];
+        key[NE - 1] = 0;
       }
     }
-    const float top = __shfl_sync(kFull, mine, 0);
-    const float num = my_id >= 0 ? expf(__fsub_rn(mine, top)) : 0.0f;
-    float den;
-    if (renormalize) {
-      den = warp_sum(num);
-    } else {
-      float s = 0.0f;
+    const uint32_t last = __reduce_min_sync(kFull, mine ? mine : 0xffffffffu);  // the smallest picked
+    const bool any = __any_sync(kFull, mine != 0);
+    int id = -1;
+    float logit = 0.0f;
 #pragma unroll
-      for (int i = 0; i < NE; ++i)
-        if (lane + 32 * i < experts) s = __fadd_rn(s, expf(__fsub_rn(v[i], top)));
-      den = warp_sum(s);
+    for (int i = 0; i < NE; ++i) {
+      const uint32_t own = order_key(v[i]);
+      unsigned found = __ballot_sync(kFull, any && own >= last);
+      while (found) {
+        const int from = __ffs(found) - 1;
+        found &= found - 1;
+        const uint32_t its = __shfl_sync(kFull, own, from);
+        const float value = __shfl_sync(kFull, v[i], from);
+        const unsigned open = __ballot_sync(kFull, mine == its && id < 0);
+        if (open && lane == __ffs(open) - 1) {
+          id = from + 32 * i;
+          logit = value;
+        }
+      }
     }
+    const float top = __shfl_sync(kFull, logit, 0);
+    const float num = id >= 0 ? exp_below(logit, top) : 0.0f;
+    float den = num;
+    if (!renormalize) {
+      den = 0.0f;
+#pragma unroll
+      for (int i = 0; i < NE; ++i) den = __fadd_rn(den, lane + 32 * i < experts ? exp_below(v[i], top) : 0.0f);
+    }
+    den = warp_sum(den);
     if (lane < k) {
-      weights[t * k + lane] = my_id >= 0 ? __fdiv_rn(num, den) : 0.0f;
-      ids[t * k + lane] = my_id;
+      weights[t * k + lane] = id >= 0 ? __fdiv_rn(num, den) : 0.0f;
+      ids[t * k + lane] = id;
     }
   }
 }
@@ -116,57 +155,59 @@ __global__ void __launch_bounds__(256) route_backward_kernel(float *__restrict__
   const int lane = threadIdx.x & 31;
   float *up = rows[threadIdx.x >> 5];
   const int64_t warps = (int64_t)gridDim.x * (blockDim.x >> 5);
-  for (int64_t t = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); t < tokens; t += warps) {
-    int id = -1;
-    float w = 0.0f, dw = 0.0f;
+  int64_t t = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+  float v[NE], next[NE], next_w = 0.0f, next_dw = 0.0f;
+  int next_id = -1;
+  const auto fetch = [&](int64_t at) {
+    if (at >= tokens) return;
+    if (!renormalize) load_row(next, logits + at * experts, lane, experts);
     if (lane < k) {
-      id = ids[t * k + lane];
-      if (id >= 0 && id < experts) {
-        w = weights[t * k + lane];
-        dw = dweights[t * k + lane];
-      } else {
-        id = -1;
-      }
+      next_id = ids[at * k + lane];
+      next_w = weights[at * k + lane];
+      next_dw = dweights[at * k + lane];
     }
-    const float dot = warp_sum(__fmul_rn(w, dw));
-    const bool any = __any_sync(kFull, id >= 0);
+  };
+  fetch(t);
 #pragma unroll
-    for (int i = 0; i < NE; ++i) up[lane + 32 * i] = 0.0f;
+  for (int i = 0; i < NE; ++i) up[lane + 32 * i] = 0.0f;
+  for (; t < tokens; t += warps) {
+    const bool held = next_id >= 0 && next_id < experts;
+    const int id = held ? next_id : -1;
+    const float w = held ? next_w : 0.0f, dw = held ? next_dw : 0.0f;
+    if (!renormalize)
+#pragma unroll
+      for (int i = 0; i < NE; ++i) v[i] = next[i];
+    fetch(t + warps);
+    const float dot = warp_sum(__fmul_rn(w, dw));
+    const bool any = __any_sync(kFull, held);
     __syncwarp();
-    if (id >= 0) up[id] = renormalize ? __fmul_rn(w, __fsub_rn(dw, dot)) : dw;
+    if (held) up[id] = renormalize ? __fmul_rn(w, __fsub_rn(dw, dot)) : dw;
     __syncwarp();
     float *out = dlogits + t * experts;
     if (renormalize || !any) {
 #pragma unroll
-      for (int i = 0; i < NE; ++i) {
-        const int e = lane + 32 * i;
-        if (e < experts) out[e] = up[e];
-      }
+      for (int i = 0; i < NE; ++i)
+        if (lane + 32 * i < experts) out[lane + 32 * i] = up[lane + 32 * i];
     } else {
-      const float *row = logits + t * experts;
-      float v[NE], top = -INFINITY;
+      float top = v[0];
 #pragma unroll
-      for (int i = 0; i < NE; ++i) {
-        const int e = lane + 32 * i;
-        v[i] = e < experts ? row[e] : -INFINITY;
-        top = fmaxf(top, v[i]);
-      }
+      for (int i = 1; i < NE; ++i) top = fmaxf(top, v[i]);
 #pragma unroll
       for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(kFull, top, d));
       float s = 0.0f;
 #pragma unroll
       for (int i = 0; i < NE; ++i) {
-        v[i] = expf(__fsub_rn(v[i], top));
+        v[i] = lane + 32 * i < experts ? exp_below(v[i], top) : 0.0f;
         s = __fadd_rn(s, v[i]);
       }
-      const float den = warp_sum(s);
+      const float inv = __fdiv_rn(1.0f, warp_sum(s));
 #pragma unroll
-      for (int i = 0; i < NE; ++i) {
-        const int e = lane + 32 * i;
-        if (e < experts) out[e] = __fmul_rn(__fdiv_rn(v[i], den), __fsub_rn(up[e], dot));
-      }
+      for (int i = 0; i < NE; ++i)
+        if (lane + 32 * i < experts)
+          out[lane + 32 * i] = __fmul_rn(__fmul_rn(v[i], inv), __fsub_rn(up[lane + 32 * i], dot));
     }
     __syncwarp();
+    if (held) up[id] = 0.0f;  // the row is clean again for the next token
   }
 }
 
@@ -466,10 +507,16 @@ int64_t chunks_of(int64_t width) {
 
 unsigned warps_grid(int64_t pieces) { return fz::grid_for(pieces, 8, 8, 4); }
 
+// Resident warps go through the tokens (their registers allow 6 or 3 CTAs an SM).
+template <int NE>
+unsigned route_grid(int64_t tokens) {
+  return fz::grid_for(tokens, 8, NE <= 8 ? 6 : 3);
+}
+
 template <int NE>
 int launch_route(float *w, int32_t *ids, const float *logits, int64_t tokens, int experts, int k, int renorm,
                  cudaStream_t s) {
-  FZ_CUDA(fz::launch_pdl(route_kernel<NE>, dim3(warps_grid(tokens)), dim3(256), 0, s, w, ids, logits, tokens,
+  FZ_CUDA(fz::launch_pdl(route_kernel<NE>, dim3(route_grid<NE>(tokens)), dim3(256), 0, s, w, ids, logits, tokens,
                          experts, k, renorm));
   FZ_CHECK_LAUNCH();
   return FZ_OK;
@@ -477,7 +524,7 @@ int launch_route(float *w, int32_t *ids, const float *logits, int64_t tokens, in
 template <int NE>
 int launch_route_backward(float *dl, const float *dw, const float *w, const int32_t *ids, const float *logits,
                           int64_t tokens, int experts, int k, int renorm, cudaStream_t s) {
-  FZ_CUDA(fz::launch_pdl(route_backward_kernel<NE>, dim3(warps_grid(tokens)), dim3(256), 0, s, dl, dw, w, ids,
+  FZ_CUDA(fz::launch_pdl(route_backward_kernel<NE>, dim3(route_grid<NE>(tokens)), dim3(256), 0, s, dl, dw, w, ids,
                          logits, tokens, experts, k, renorm));
   FZ_CHECK_LAUNCH();
   return FZ_OK;
