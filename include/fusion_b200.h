@@ -485,7 +485,7 @@ int fz_expert_combine_backward(float *drows, float *dweights, const float *dout,
  *   loss[r] = tau^2 * (sum_i p_i (log p_i - log q_i) + pT (log pT - log qT)),
  * a term with p = 0 counting 0. A row without entries (with teacher_lse NULL also one whose
  * entries are all -inf) has loss 0 whatever its logits hold. For the backward, stats
- * [rows, 4] receives the maximum of z and log sum exp((z - max) / tau), then, with
+ * [rows, 4] (16-byte aligned) receives the maximum of z and log sum exp((z - max) / tau), then, with
  * teacher_lse, the same two over the logits outside the entries.
  * k <= FZ_MAX_TEACHER, vocab <= 2^23; an id named twice counts its p each time. */
 int fz_distill(float *loss, float *stats, const float *logits, int64_t ld, const int32_t *ids,

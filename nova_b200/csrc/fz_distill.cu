@@ -1,13 +1,15 @@
 // Distillation from a teacher's top logits: the loss and its gradient.
 //
-// Per row, one pass over the student's logits keeps a running maximum m and sum of
-// exp((z - m) / tau) per thread, joined over the CTA and, where few rows would leave SMs
-// idle, over a cluster of CTAs that share the row. With the tail bucket the row's entries
-// are marked in a bitmap in shared memory and go to a sum of their own, so that the tail's
-// mass qT is summed directly (1 - sum of q inside would cancel where the student is sure
-// of itself), and an id named twice counts once. The maximum and the log of the sum are
-// kept apart: a large common offset of the logits, or a row of the type's lowest value,
-// costs no digits.
+// Bound by memory: the forward reads the student's logits once (4 bytes a value), the
+// backward reads them once more and writes dz (8 bytes). Per row, a thread keeps a running
+// maximum m and sum of exp((z - m) / tau), 16 values at a time; the sums are joined over
+// the row's team: a warp for small vocabularies, a CTA of 128 or 512 threads for larger
+// ones, a cluster of CTAs where few rows would leave SMs idle (team_of). With the tail
+// bucket the row's entries are marked in a bitmap in shared memory and go to a sum of their
+// own, so that the tail's mass qT is summed directly (1 - sum of q inside would cancel where
+// the student is sure of itself), and an id named twice counts once. The maximum and the
+// log of the sum are kept apart: a large common offset of the logits, or a row of the type's
+// lowest value, costs no digits.
 // The backward streams the row once more, writing dz from the saved statistics, and then
 // overwrites the entries' columns.
 #include <cooperative_groups.h>
@@ -21,7 +23,7 @@ namespace cg = cooperative_groups;
 
 namespace {
 
-constexpr int kThreads = 512;
+constexpr unsigned kFull = 0xffffffffu;
 constexpr float kLog2e = 1.4426950408889634f;
 
 // 2^x to within 2 ulp (results below the normal range flush to 0, next to sums that are
@@ -43,16 +45,14 @@ __device__ __forceinline__ Lse join(Lse p, Lse q, float a) {
   const float m = fmaxf(p.m, q.m), at = floor_of(m);
   return {m, __fmaf_rn(p.s, term(p.m, at, a), __fmul_rn(q.s, term(q.m, at, a)))};
 }
-
 __device__ __forceinline__ Lse warp_join(Lse p, float a) {
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) {
-    const Lse q{__shfl_xor_sync(0xffffffffu, p.m, d), __shfl_xor_sync(0xffffffffu, p.s, d)};
+    const Lse q{__shfl_xor_sync(kFull, p.m, d), __shfl_xor_sync(kFull, p.s, d)};
     p = join(p, q, a);
   }
   return p;
 }
-
 // NaN and +inf logits make the sum NaN.
 template <int N>
 __device__ __forceinline__ void take(Lse &p, const float (&x)[N], float a) {
@@ -64,244 +64,370 @@ __device__ __forceinline__ void take(Lse &p, const float (&x)[N], float a) {
     p.m = top;
   }
   const float at = floor_of(p.m);
+  float s = term(x[0], at, a);
 #pragma unroll
-  for (int i = 0; i < N; ++i) p.s = __fadd_rn(p.s, term(x[i], at, a));
+  for (int i = 1; i < N; ++i) s = __fadd_rn(s, term(x[i], at, a));
+  p.s = __fadd_rn(p.s, s);
 }
 
-// The teacher's side of one row.
+// ---------------------------------------------------------------- teams
+// T threads work on a row: 32 (eight rows a CTA) or a whole CTA.
+__host__ __device__ constexpr int threads_of(int t) { return t == 32 ? 256 : t; }
+
+template <int T>
+__device__ __forceinline__ int team_thread() {
+  return T == 32 ? (int)(threadIdx.x & 31) : (int)threadIdx.x;
+}
+template <int T>
+__device__ __forceinline__ void team_sync() {
+  if constexpr (T == 32) __syncwarp();
+  else __syncthreads();
+}
+template <int T>
+__device__ __forceinline__ bool team_any(bool v) {
+  if constexpr (T == 32) return __any_sync(kFull, v);
+  else return __syncthreads_or(v);
+}
+template <int T, bool MAX>
+__device__ __forceinline__ float team_fold(float v, float *sh) {
+  const auto fold = [](float a, float b) { return MAX ? fmaxf(a, b) : __fadd_rn(a, b); };
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) v = fold(v, __shfl_xor_sync(kFull, v, d));
+  if constexpr (T > 32) {
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = v;
+    __syncthreads();
+    v = sh[0];
+#pragma unroll
+    for (int w = 1; w < T / 32; ++w) v = fold(v, sh[w]);
+  }
+  return v;
+}
+
+// ---------------------------------------------------------------- the teacher's side of a row
+
 struct Teacher {
-  int count;         // nonzero if the row has entries
+  bool some;         // the row has entries
   float mass, tail;  // P = sum p + pT, pT
 };
 
-__device__ __forceinline__ float block_sum(float v, float *sh) {
-#pragma unroll
-  for (int d = 16; d > 0; d >>= 1) v = __fadd_rn(v, __shfl_xor_sync(0xffffffffu, v, d));
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = v;
-  __syncthreads();
-  float s = 0.0f;
-  for (int w = 0; w < kThreads / 32; ++w) s = __fadd_rn(s, sh[w]);
-  return s;
-}
-__device__ __forceinline__ float block_max(float v, float *sh) {
-#pragma unroll
-  for (int d = 16; d > 0; d >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, d));
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = v;
-  __syncthreads();
-  float s = -INFINITY;
-  for (int w = 0; w < kThreads / 32; ++w) s = fmaxf(s, sh[w]);
-  return s;
-}
-
-// Made by the whole CTA in shared memory: id[i] (-1: padding), p[i] and, when asked for,
-// logp[i] = log p[i].
-__device__ Teacher read_teacher(int *id, float *p, float *logp, const int32_t *ids, const float *teacher,
-                                const float *lse, int64_t r, int k, int vocab, float tau, float *sh) {
-  int n = 0;
+// Made by the whole team in shared memory: id[i] (-1: padding), p[i], the student's logit
+// z[i] there and, when asked for, logp[i] = log p[i].
+template <int T>
+__device__ __forceinline__ Teacher read_teacher(int *id, float *p, float *z, float *logp, const float *row,
+                                                const int32_t *ids, const float *teacher, const float *lse,
+                                                int64_t r, int k, int vocab, float tau, float *sh) {
+  const int tid = team_thread<T>();
+  bool some = false;
   float top = -INFINITY;
-  for (int i = threadIdx.x; i < k; i += kThreads) {
+  for (int i = tid; i < k; i += T) {
     const int v = ids[r * k + i];
     const bool ok = v >= 0 && v < vocab;
     const float t = ok ? teacher[r * k + i] : -INFINITY;
     id[i] = ok ? v : -1;
     p[i] = t;
-    n += ok && (lse || t != -INFINITY);
+    if (z) z[i] = ok ? row[v] : 0.0f;
+    some = some || (ok && (lse || t != -INFINITY));
     top = fmaxf(top, t);
   }
-  Teacher T{__syncthreads_or(n), 0.0f, 0.0f};
-  if (!T.count) return T;
-  float shift = 0.0f;
+  Teacher t{team_any<T>(some), 0.0f, 0.0f};
+  if (!t.some) return t;
+  float shift;
   if (!lse) {
-    top = block_max(top, sh);
+    top = team_fold<T, true>(top, sh);
     float s = 0.0f;
-    for (int i = threadIdx.x; i < k; i += kThreads)
+    for (int i = tid; i < k; i += T)
       if (id[i] >= 0) s = __fadd_rn(s, expf(__fdiv_rn(__fsub_rn(p[i], top), tau)));
-    shift = logf(block_sum(s, sh));
+    shift = logf(team_fold<T, false>(s, sh));
   } else {
     top = 0.0f;
     shift = lse[r];
   }
   float s = 0.0f;
-  for (int i = threadIdx.x; i < k; i += kThreads) {
+  for (int i = tid; i < k; i += T) {
     const float l = __fsub_rn(__fdiv_rn(__fsub_rn(p[i], top), tau), shift);
     const float q = id[i] >= 0 ? expf(l) : 0.0f;
     if (logp) logp[i] = l;
     p[i] = q;
     s = __fadd_rn(s, q);
   }
-  s = block_sum(s, sh);
+  s = team_fold<T, false>(s, sh);
   if (lse) {
     const float rest = __fsub_rn(1.0f, s);
-    T.tail = rest < 0.0f ? 0.0f : rest;  // NaN stays
+    t.tail = rest < 0.0f ? 0.0f : rest;  // NaN stays
   }
-  T.mass = __fadd_rn(s, T.tail);
-  return T;
+  t.mass = __fadd_rn(s, t.tail);
+  return t;
 }
 
-// One cluster of CTAs per row; each takes a slice of the columns. Columns are counted
-// from `shift` before the row's start, so that the float4s of an unaligned row begin at
-// multiples of 4.
-template <bool TAIL>
-__global__ void __launch_bounds__(kThreads) distill_kernel(float *__restrict__ loss, float *__restrict__ stats,
-                                                           const float *__restrict__ logits, int64_t ld,
-                                                           const int32_t *__restrict__ ids,
-                                                           const float *__restrict__ teacher,
-                                                           const float *__restrict__ teacher_lse, int vocab, int k,
-                                                           float tau, int slice) {
+// Columns of a row are counted from `shift` before its start, so that 16-byte accesses to an
+// unaligned row begin at multiples of 4: column c of the row lies at c + shift.
+struct Row {
+  const float *aligned;  // 16-byte aligned; the row's first value is aligned[shift]
+  int shift, end;        // end = vocab + shift
+};
+__device__ __forceinline__ Row row_at(const float *row, int vocab) {
+  const int shift = (int)(((uintptr_t)row >> 2) & 3);
+  return {row - shift, shift, vocab + shift};
+}
+__device__ __forceinline__ bool inside(const Row &r, int c) { return c >= r.shift && c + 4 <= r.end; }
+__device__ __forceinline__ void load4(float *x, const Row &r, int c) {
+  if (inside(r, c)) {
+    const float4 q = *reinterpret_cast<const float4 *>(r.aligned + c);
+    x[0] = q.x, x[1] = q.y, x[2] = q.z, x[3] = q.w;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = c + i >= r.shift && c + i < r.end ? r.aligned[c + i] : -INFINITY;
+  }
+}
+constexpr int kUnroll = 4;  // float4s a thread has in flight
+
+template <bool TAIL, int T>
+__global__ void __launch_bounds__(threads_of(T)) distill_kernel(float *__restrict__ loss, float *__restrict__ stats,
+                                                                const float *__restrict__ logits, int64_t ld,
+                                                                const int32_t *__restrict__ ids,
+                                                                const float *__restrict__ teacher,
+                                                                const float *__restrict__ teacher_lse, int64_t rows,
+                                                                int vocab, int k, float tau, int slice) {
   pdl_wait();
+  constexpr int kTeams = threads_of(T) / T, kWarps = T / 32;
   cg::cluster_group cluster = cg::this_cluster();
-  const int rank = (int)cluster.block_rank(), ctas = (int)cluster.num_blocks();
-  const int64_t r = blockIdx.x / ctas;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int rank = T == 512 ? (int)cluster.block_rank() : 0, ctas = T == 512 ? (int)cluster.num_blocks() : 1;
+  const int team = T == 32 ? (int)threadIdx.x / 32 : 0, tid = team_thread<T>(), lane = tid & 31, warp = tid >> 5;
+  const int64_t r = (int64_t)(blockIdx.x / ctas) * kTeams + team;
   extern __shared__ float dyn[];
-  int *id = reinterpret_cast<int *>(dyn);
-  float *p = dyn + k, *logp = dyn + 2 * k;
-  uint32_t *marks = reinterpret_cast<uint32_t *>(dyn + 3 * k);
-  __shared__ float sh[kThreads / 32];
-  __shared__ Lse part[2][kThreads / 32];
+  const int words = TAIL ? slice / 32 : 0;
+  int *id = reinterpret_cast<int *>(dyn) + team * (4 * k + words);
+  float *p = reinterpret_cast<float *>(id + k), *logp = p + k, *z = logp + k;
+  uint32_t *marks = reinterpret_cast<uint32_t *>(z + k);
+  __shared__ float sh[kWarps];
+  __shared__ Lse part[2][kWarps];
   __shared__ Lse whole[2];  // outside the entries (without TAIL: all), inside
+  if (T == 32 && r >= rows) return;
 
   const float a = __fdiv_rn(kLog2e, tau);
-  const float *row = logits + r * ld;
-  const int shift = (int)(((uintptr_t)row >> 2) & 3);
-  const int from = rank * slice, to = min(from + slice, vocab + shift);  // slice: a multiple of 128
-  const Teacher T = read_teacher(id, p, logp, ids, teacher, teacher_lse, r, k, vocab, tau, sh);
-  if (!T.count) {  // the same in every CTA of the cluster
+  const float *start = logits + r * ld;
+  const Row row = row_at(start, vocab);
+  const int from = rank * slice, to = min(from + slice, row.end);  // slice: a multiple of 128
+  const Teacher t = read_teacher<T>(id, p, rank == 0 ? z : nullptr, logp, start, ids, teacher, teacher_lse, r, k,
+                                    vocab, tau, sh);
+  if (!t.some) {  // the same in every CTA of the cluster
     if (rank == 0 && tid == 0) loss[r] = 0.0f;
     if (rank == 0 && tid < 4) stats[r * 4 + tid] = 0.0f;
     return;
   }
   if (TAIL) {
-    for (int i = tid; i < slice / 32; i += kThreads) marks[i] = 0u;
-    __syncthreads();
-    for (int i = tid; i < k; i += kThreads) {
-      const int at = id[i] + shift;
+    for (int i = tid; i < words; i += T) marks[i] = 0u;
+    team_sync<T>();
+    for (int i = tid; i < k; i += T) {
+      const int at = id[i] + row.shift;
       if (id[i] >= 0 && at >= from && at < to) atomicOr(&marks[(at - from) >> 5], 1u << (at & 31));
     }
-    __syncthreads();
+    team_sync<T>();
   }
 
   Lse out{-INFINITY, 0.0f}, in{-INFINITY, 0.0f};
-  const float *aligned = row - shift;
-  for (int c = from + 4 * tid; c < to; c += 4 * kThreads) {
-    float x[4];
-    if (c >= shift && c + 4 <= vocab + shift) {
-      const float4 q = *reinterpret_cast<const float4 *>(aligned + c);
-      x[0] = q.x, x[1] = q.y, x[2] = q.z, x[3] = q.w;
+  for (int c = from + 4 * tid; c < to; c += kUnroll * 4 * T) {
+    float x[kUnroll * 4];
+    const int last = c + (kUnroll - 1) * 4 * T;
+    if (inside(row, c) && last < to && inside(row, last)) {
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) {
+        const float4 q = *reinterpret_cast<const float4 *>(row.aligned + c + u * 4 * T);
+        x[u * 4] = q.x, x[u * 4 + 1] = q.y, x[u * 4 + 2] = q.z, x[u * 4 + 3] = q.w;
+      }
     } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) x[i] = c + i >= shift && c + i < vocab + shift ? aligned[c + i] : -INFINITY;
+      for (int u = 0; u < kUnroll; ++u) {
+        if (c + u * 4 * T < to) {
+          load4(x + u * 4, row, c + u * 4 * T);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) x[u * 4 + i] = -INFINITY;
+        }
+      }
     }
     if (TAIL) {
-      const uint32_t m = marks[(c - from) >> 5] >> (c & 31) & 15u;
-      if (m) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (m >> i & 1) {
-            const float y[1] = {x[i]};
-            take(in, y, a);
-            x[i] = -INFINITY;
-          }
+      for (int u = 0; u < kUnroll; ++u) {
+        const int at = c + u * 4 * T;
+        const uint32_t m = at < to ? marks[(at - from) >> 5] >> (at & 31) & 15u : 0u;
+        if (m) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (m >> i & 1) {
+              const float y[1] = {x[u * 4 + i]};
+              take(in, y, a);
+              x[u * 4 + i] = -INFINITY;
+            }
+        }
       }
     }
     take(out, x, a);
   }
   out = warp_join(out, a);
   if (TAIL) in = warp_join(in, a);
-  if (lane == 0) {
-    part[0][warp] = out;
-    part[1][warp] = in;
+  if constexpr (T > 32) {
+    if (lane == 0) {
+      part[0][warp] = out;
+      part[1][warp] = in;
+    }
+    __syncthreads();
+    if (warp < (TAIL ? 2 : 1)) {
+      const Lse mine = warp_join(lane < kWarps ? part[warp][lane] : Lse{-INFINITY, 0.0f}, a);
+      if (lane == 0) whole[warp] = mine;
+    }
+    if (ctas > 1) cluster.sync();
+    else __syncthreads();
   }
-  __syncthreads();
-  if (warp < (TAIL ? 2 : 1)) {
-    const Lse mine = warp_join(lane < kThreads / 32 ? part[warp][lane] : Lse{-INFINITY, 0.0f}, a);
-    if (lane == 0) whole[warp] = mine;
-  }
-  cluster.sync();
   if (rank == 0 && warp == 0) {
-    Lse sum{-INFINITY, 0.0f}, tail{-INFINITY, 0.0f};
-    for (int q = 0; q < ctas; ++q) {
-      const Lse *theirs = cluster.map_shared_rank(whole, q);
-      if (TAIL) {
-        tail = join(tail, theirs[0], a);
-        sum = join(sum, theirs[1], a);
-      } else {
-        sum = join(sum, theirs[0], a);
+    Lse sum = out, tail = out;
+    if constexpr (T > 32) {
+      sum = tail = whole[0];
+      if (TAIL) in = whole[1];
+      for (int q = 1; q < ctas; ++q) {
+        const Lse *theirs = cluster.map_shared_rank(whole, q);
+        sum = tail = join(sum, theirs[0], a);
+        if (TAIL) in = join(in, theirs[1], a);
       }
     }
-    if (TAIL) sum = join(sum, tail, a);
+    if (TAIL) sum = join(in, tail, a);
     const float log_sum = logf(sum.s);
     float l = 0.0f;
     for (int i = lane; i < k; i += 32) {
       const float w = p[i];
       if (id[i] < 0 || w == 0.0f) continue;
-      const float logq = __fsub_rn(__fdiv_rn(__fsub_rn(row[id[i]], sum.m), tau), log_sum);
+      const float logq = __fsub_rn(__fdiv_rn(__fsub_rn(z[i], sum.m), tau), log_sum);
       l = __fmaf_rn(w, __fsub_rn(logp[i], logq), l);
     }
 #pragma unroll
-    for (int d = 16; d > 0; d >>= 1) l = __fadd_rn(l, __shfl_xor_sync(0xffffffffu, l, d));
+    for (int d = 16; d > 0; d >>= 1) l = __fadd_rn(l, __shfl_xor_sync(kFull, l, d));
     if (lane == 0) {
       const float log_tail = logf(tail.s);
-      if (TAIL && T.tail != 0.0f) {
-        const float logq =
-            __fadd_rn(__fdiv_rn(__fsub_rn(tail.m, sum.m), tau), __fsub_rn(log_tail, log_sum));
-        l = __fmaf_rn(T.tail, __fsub_rn(logf(T.tail), logq), l);
+      if (TAIL && t.tail != 0.0f) {
+        const float logq = __fadd_rn(__fdiv_rn(__fsub_rn(tail.m, sum.m), tau), __fsub_rn(log_tail, log_sum));
+        l = __fmaf_rn(t.tail, __fsub_rn(logf(t.tail), logq), l);
       }
       loss[r] = __fmul_rn(__fmul_rn(tau, tau), l);
-      stats[r * 4] = sum.m;
-      stats[r * 4 + 1] = log_sum;
-      stats[r * 4 + 2] = tail.m;
-      stats[r * 4 + 3] = log_tail;
+      *reinterpret_cast<float4 *>(stats + r * 4) = make_float4(sum.m, log_sum, tail.m, log_tail);
     }
   }
-  cluster.sync();  // no CTA leaves while its sums may be read
+  if (T > 32 && ctas > 1) cluster.sync();  // no CTA leaves while its sums may be read
 }
 
-template <bool TAIL>
-__global__ void __launch_bounds__(kThreads) distill_backward_kernel(
+// dz from z and the row's statistics, without its entries.
+struct Slope {
+  float a, m, l2, inside, tm, t2, outside;
+  template <bool TAIL>
+  __device__ __forceinline__ float at(float z) const {
+    float d = __fmul_rn(inside, ex2(__fmaf_rn(__fsub_rn(z, m), a, -l2)));
+    if (TAIL) d = __fmaf_rn(-outside, ex2(__fmaf_rn(__fsub_rn(z, tm), a, -t2)), d);
+    return d;
+  }
+};
+
+template <bool TAIL, bool VEC, int T>
+__device__ __forceinline__ void stream_slope(float *out, const Row &row, const Slope &s, int from, int to, int tid) {
+  if constexpr (VEC) {  // out and the row are equally far from 16-byte alignment
+    float *aligned = out - row.shift;
+    for (int c = from + 4 * tid; c < to; c += kUnroll * 4 * T) {
+      float x[kUnroll * 4];
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u)
+        if (c + u * 4 * T < to) load4(x + u * 4, row, c + u * 4 * T);
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) {
+        const int at = c + u * 4 * T;
+        if (at >= to) break;
+        float d[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) d[i] = s.at<TAIL>(x[u * 4 + i]);
+        if (inside(row, at)) {
+          *reinterpret_cast<float4 *>(aligned + at) = make_float4(d[0], d[1], d[2], d[3]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (at + i >= row.shift && at + i < row.end) aligned[at + i] = d[i];
+        }
+      }
+    }
+  } else {
+    const int first = max(from, row.shift);
+    for (int c = first + tid; c < to; c += T) out[c - row.shift] = s.at<TAIL>(row.aligned[c]);
+  }
+}
+
+// Whether an id is named twice: a hash table of `size` (a power of two, at least 2 k) slots.
+template <int T>
+__device__ __forceinline__ bool any_twice(const int *id, int *table, int k, int size, int tid) {
+  for (int i = tid; i < size; i += T) table[i] = -1;
+  team_sync<T>();
+  bool twice = false;
+  for (int i = tid; i < k; i += T) {
+    const int v = id[i];
+    if (v < 0) continue;
+    for (int at = (int)((uint32_t)v * 2654435761u >> 16) & (size - 1);; at = (at + 1) & (size - 1)) {
+      const int was = atomicCAS(&table[at], -1, v);
+      twice = twice || was == v;
+      if (was == -1 || was == v) break;
+    }
+  }
+  return team_any<T>(twice);
+}
+
+template <bool TAIL, int T>
+__global__ void __launch_bounds__(threads_of(T)) distill_backward_kernel(
     float *__restrict__ dlogits, int64_t ldd, const float *__restrict__ dloss, const float *__restrict__ stats,
     const float *__restrict__ logits, int64_t ld, const int32_t *__restrict__ ids,
-    const float *__restrict__ teacher, const float *__restrict__ teacher_lse, int vocab, int k, float tau, int slice, int ctas) {
+    const float *__restrict__ teacher, const float *__restrict__ teacher_lse, int64_t rows, int vocab, int k,
+    float tau, int slice, int ctas, int table_size) {
   pdl_wait();
-  const int64_t r = blockIdx.x / ctas;
-  const int rank = (int)(blockIdx.x - r * ctas), tid = threadIdx.x;
+  constexpr int kTeams = threads_of(T) / T;
+  const int team = T == 32 ? (int)threadIdx.x / 32 : 0, tid = team_thread<T>();
+  const int64_t r = (int64_t)(blockIdx.x / ctas) * kTeams + team;
+  const int rank = (int)(blockIdx.x % ctas);
   extern __shared__ float dyn[];
-  int *id = reinterpret_cast<int *>(dyn);
-  float *p = dyn + k;
-  __shared__ float sh[kThreads / 32];
-  const Teacher T = read_teacher(id, p, nullptr, ids, teacher, teacher_lse, r, k, vocab, tau, sh);
-  const float *row = logits + r * ld;
+  int *id = reinterpret_cast<int *>(dyn) + team * (3 * k + table_size);
+  float *p = reinterpret_cast<float *>(id + k), *z = p + k;
+  int *table = reinterpret_cast<int *>(z + k);
+  __shared__ float sh[T / 32];
+  if (T == 32 && r >= rows) return;
+  const float *start = logits + r * ld;
   float *out = dlogits + r * ldd;
-  const int from = rank * slice, to = min(from + slice, vocab);
-  if (!T.count) {
-    for (int c = from + tid; c < to; c += kThreads) out[c] = 0.0f;
+  const Row row = row_at(start, vocab);
+  const int from = rank * slice, to = min(from + slice, row.end);  // slice: a multiple of 128
+  const Teacher t =
+      read_teacher<T>(id, p, z, nullptr, start, ids, teacher, teacher_lse, r, k, vocab, tau, sh);
+  if (!t.some) {
+    for (int c = max(from, row.shift) + tid; c < to; c += T) out[c - row.shift] = 0.0f;
     return;
   }
-  const float a = __fdiv_rn(kLog2e, tau), scale = __fmul_rn(tau, dloss[r]);
-  const float m = stats[r * 4], l2 = __fmul_rn(stats[r * 4 + 1], kLog2e), inside = __fmul_rn(scale, T.mass);
-  const float tm = stats[r * 4 + 2], t2 = __fmul_rn(stats[r * 4 + 3], kLog2e), outside = __fmul_rn(scale, T.tail);
-  for (int c = from + tid; c < to; c += kThreads) {
-    const float x = row[c];
-    float d = __fmul_rn(inside, ex2(__fmaf_rn(__fsub_rn(x, m), a, -l2)));
-    if (TAIL && T.tail != 0.0f) d = __fmaf_rn(-outside, ex2(__fmaf_rn(__fsub_rn(x, tm), a, -t2)), d);
-    out[c] = d;
-  }
-  __syncthreads();
+  const float scale = __fmul_rn(tau, dloss[r]);
+  const float4 st = *reinterpret_cast<const float4 *>(stats + r * 4);
+  const Slope s{__fdiv_rn(kLog2e, tau),        st.x, __fmul_rn(st.y, kLog2e), __fmul_rn(scale, t.mass), st.z,
+                __fmul_rn(st.w, kLog2e), __fmul_rn(scale, t.tail)};
+  const bool vec = (((uintptr_t)out >> 2) & 3) == (uintptr_t)row.shift, tail = TAIL && t.tail != 0.0f;
+  if (vec && tail) stream_slope<true, true, T>(out, row, s, from, to, tid);
+  else if (vec) stream_slope<false, true, T>(out, row, s, from, to, tid);
+  else if (tail) stream_slope<true, false, T>(out, row, s, from, to, tid);
+  else stream_slope<false, false, T>(out, row, s, from, to, tid);
+  const bool twice = any_twice<T>(id, table, k, table_size, tid);  // a barrier, too
   // the entries' columns, each by its first entry
-  for (int i = tid; i < k; i += kThreads) {
-    const int c = id[i];
-    if (c < from || c >= to) continue;
-    float s = 0.0f;
-    bool again = false;
-    for (int j = 0; j < k; ++j)
-      if (id[j] == c) {
-        again = again || j < i;
-        s = __fadd_rn(s, p[j]);
-      }
-    if (again) continue;
-    out[c] = __fmaf_rn(inside, ex2(__fmaf_rn(__fsub_rn(row[c], m), a, -l2)), -__fmul_rn(scale, s));
+  for (int i = tid; i < k; i += T) {
+    const int c = id[i], at = c + row.shift;
+    if (c < 0 || at < from || at >= to) continue;
+    float sum = p[i];
+    if (twice) {
+      bool again = false;
+      sum = 0.0f;
+      for (int j = 0; j < k; ++j)
+        if (id[j] == c) {
+          again = again || j < i;
+          sum = __fadd_rn(sum, p[j]);
+        }
+      if (again) continue;
+    }
+    out[c] = __fsub_rn(s.at<false>(z[i]), __fmul_rn(scale, sum));
   }
 }
 
@@ -316,13 +442,54 @@ int check_distill(const char *who, int64_t rows, int64_t vocab, int64_t k, int64
   return FZ_OK;
 }
 
-// CTAs per row: the fewest (1, 2, 4, 8) that give every SM two, while a slice keeps 4096
-// columns, and enough that a slice's marks fit in shared memory.
-int ctas_per_row(int64_t rows, int64_t vocab) {
-  int n = 1;
-  while (n < 8 && ((rows * n < 2 * (int64_t)fz::num_sms() && vocab / (2 * n) >= 4096) || vocab / n > (1 << 20)))
-    n *= 2;
-  return n;
+// Threads and CTAs a row. A warp for up to 4096 columns, 128 threads for up to 16384, else
+// CTAs of 512, of which a row gets the number that wastes the least: on SMs without work in
+// the last wave (three such CTAs an SM), on a CTA's fixed cost, about that of 3000 columns, and
+// in the forward on the cluster's barriers (4096 rows of 131072: 323 us with one CTA a row, 353
+// with two; 64 rows: 14 us with eight).
+struct Team {
+  int threads, ctas, slice;
+};
+Team team_of(int64_t rows, int64_t vocab, int64_t k, bool backward) {
+  Team t{vocab <= 4096 && k <= 256 ? 32 : vocab <= 16384 ? 128 : 512, 1, 0};
+  if (t.threads == 512) {
+    const double wave = 3.0 * fz::num_sms();
+    double best = 0.0;
+    for (int n = 1; n <= 8; n *= 2) {
+      const double columns = (double)vocab / n, waves = (double)rows * n / wave;
+      if (columns > (1 << 20)) continue;  // a slice's marks have to fit in shared memory
+      if (n > 1 && columns < 4096) break;
+      double use = waves / (double)(int64_t)(waves + 0.999999) * columns / (columns + 3000.0);
+      if (n > 1 && !backward) use *= 0.93;
+      if (use > best) best = use, t.ctas = n;
+    }
+  }
+  t.slice = (int)(((vocab + 3 + t.ctas - 1) / t.ctas + 127) / 128 * 128);
+  return t;
+}
+
+template <typename... KArgs, typename... Args>
+int launch_team(void (*kernel)(KArgs...), int64_t rows, const Team &t, size_t smem, bool cluster, cudaStream_t s,
+                Args... args) {
+  if (smem > 32 * 1024)
+    FZ_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)(t.threads == 32 ? (rows + 7) / 8 : rows * t.ctas));
+  cfg.blockDim = dim3((unsigned)threads_of(t.threads));
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster ? (unsigned)t.ctas : 1u;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  FZ_CUDA(cudaLaunchKernelEx(&cfg, kernel, args...));
+  FZ_CHECK_LAUNCH();
+  return FZ_OK;
 }
 
 }  // namespace
@@ -333,30 +500,17 @@ extern "C" int fz_distill(float *loss, float *stats, const float *logits, int64_
   if (int rc = check_distill("fz_distill", rows, vocab, k, ld, temperature)) return rc;
   if (rows == 0) return FZ_OK;
   FZ_REQUIRE(loss && stats && logits && ids && teacher, "fz_distill: null pointer");
-  const int ctas = ctas_per_row(rows, vocab);
-  const int slice = (int)(((vocab + 3 + ctas - 1) / ctas + 127) / 128 * 128);
-  const size_t smem = (size_t)k * 12 + (teacher_lse ? (size_t)slice / 8 : 0);
-  auto kernel = teacher_lse ? distill_kernel<true> : distill_kernel<false>;
-  if (smem > 48 * 1024)
-    FZ_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)(rows * ctas));
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = fz::resolve(stream);
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = (unsigned)ctas;
-  attr[1].val.clusterDim.y = 1;
-  attr[1].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 2;
-  FZ_CUDA(cudaLaunchKernelEx(&cfg, kernel, loss, stats, logits, ld, ids, teacher, teacher_lse, (int)vocab,
-                             (int)k, temperature, slice));
-  FZ_CHECK_LAUNCH();
-  return FZ_OK;
+  FZ_REQUIRE(((uintptr_t)stats & 15) == 0, "fz_distill: stats must be 16-byte aligned");
+  const Team t = team_of(rows, vocab, k, false);
+  const size_t smem = ((size_t)k * 16 + (teacher_lse ? (size_t)t.slice / 8 : 0)) * (t.threads == 32 ? 8 : 1);
+  const auto kernel = teacher_lse ? (t.threads == 32    ? distill_kernel<true, 32>
+                                     : t.threads == 128 ? distill_kernel<true, 128>
+                                                        : distill_kernel<true, 512>)
+                                  : (t.threads == 32    ? distill_kernel<false, 32>
+                                     : t.threads == 128 ? distill_kernel<false, 128>
+                                                        : distill_kernel<false, 512>);
+  return launch_team(kernel, rows, t, smem, true, fz::resolve(stream), loss, stats, logits, ld, ids, teacher,
+                     teacher_lse, rows, (int)vocab, (int)k, temperature, t.slice);
 }
 
 extern "C" int fz_distill_backward(float *dlogits, int64_t ldd, const float *dloss, const float *stats,
@@ -367,14 +521,18 @@ extern "C" int fz_distill_backward(float *dlogits, int64_t ldd, const float *dlo
   FZ_REQUIRE(ldd >= vocab, "fz_distill_backward: row pitch below vocab");
   if (rows == 0) return FZ_OK;
   FZ_REQUIRE(dlogits && dloss && stats && logits && ids && teacher, "fz_distill_backward: null pointer");
+  FZ_REQUIRE(((uintptr_t)stats & 15) == 0, "fz_distill_backward: stats must be 16-byte aligned");
   FZ_REQUIRE(dlogits != logits, "fz_distill_backward: dlogits may not overlap logits");
-  const int ctas = ctas_per_row(rows, vocab);
-  const int slice = (int)((vocab + ctas - 1) / ctas);
-  const size_t smem = (size_t)k * 8;
-  auto kernel = teacher_lse ? distill_backward_kernel<true> : distill_backward_kernel<false>;
-  FZ_CUDA(fz::launch_pdl(kernel, dim3((unsigned)(rows * ctas)), dim3(kThreads), smem, fz::resolve(stream), dlogits,
-                         ldd, dloss, stats, logits, ld, ids, teacher, teacher_lse, (int)vocab, (int)k,
-                         temperature, slice, ctas));
-  FZ_CHECK_LAUNCH();
-  return FZ_OK;
+  const Team t = team_of(rows, vocab, k, true);
+  int table = 2;
+  while (table < 2 * k) table *= 2;
+  const size_t smem = ((size_t)k * 12 + (size_t)table * 4) * (t.threads == 32 ? 8 : 1);
+  const auto kernel = teacher_lse ? (t.threads == 32    ? distill_backward_kernel<true, 32>
+                                     : t.threads == 128 ? distill_backward_kernel<true, 128>
+                                                        : distill_backward_kernel<true, 512>)
+                                  : (t.threads == 32    ? distill_backward_kernel<false, 32>
+                                     : t.threads == 128 ? distill_backward_kernel<false, 128>
+                                                        : distill_backward_kernel<false, 512>);
+  return launch_team(kernel, rows, t, smem, false, fz::resolve(stream), dlogits, ldd, dloss, stats, logits, ld, ids,
+                     teacher, teacher_lse, rows, (int)vocab, (int)k, temperature, t.slice, t.ctas, table);
 }
