@@ -217,20 +217,23 @@ __global__ void __launch_bounds__(256) route_backward_kernel(float *__restrict__
 // choices and counts them per expert in shared memory; the CTAs exchange their totals
 // through distributed shared memory; then each warp places its run, in order, from its
 // own first place per expert. Equal experts within a warp's 32 choices are ranked by
-// match_any, so the order is stable whatever the scheduling.
+// ballots over the expert's bits, so the order is stable whatever the scheduling.
+// The ids of the next kSortAhead groups of 32 are in flight.
+constexpr int kSortAhead = 4, kMaxSortCtas = 16;
 __global__ void __launch_bounds__(1024) sort_kernel(int32_t *__restrict__ slot, int32_t *__restrict__ src,
                                                     int32_t *__restrict__ counts, int32_t *__restrict__ offsets,
                                                     const int32_t *__restrict__ ids, int n, int experts,
-                                                    int capacity, int rows, int per_warp) {
+                                                    int capacity, int rows, int per_warp, int bits) {
   pdl_wait();
   cg::cluster_group cluster = cg::this_cluster();
   const int rank = (int)cluster.block_rank(), ctas = (int)cluster.num_blocks();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nwarps = blockDim.x >> 5;
   extern __shared__ int32_t sh[];
-  int32_t *hist = sh;                       // [nwarps][experts]: counts, then the next place in the expert
+  int32_t *hist = sh;                       // [nwarps][experts]: counts, then the next place among the CTA's choices
   int32_t *total = sh + nwarps * experts;   // [experts]: this CTA's counts
   int32_t *start = total + experts;         // [experts]: the expert's first row
   int32_t *all = start + experts;           // [experts]: counts over the cluster
+  int32_t *ahead = all + experts;           // [experts]: counts of the CTAs before this one
   __shared__ int32_t scan[32];
 
   for (int i = tid; i < nwarps * experts; i += blockDim.x) hist[i] = 0;
@@ -238,32 +241,49 @@ __global__ void __launch_bounds__(1024) sort_kernel(int32_t *__restrict__ slot, 
   const int64_t first = ((int64_t)rank * nwarps + warp) * per_warp;
   const int end = (int)(first + per_warp < n ? first + per_warp : n);
   int32_t *mine = hist + warp * experts;
-  for (int64_t i = first + lane; i < end; i += 32) {
-    const int e = ids[i];
-    if (e >= 0 && e < experts) atomicAdd(&mine[e], 1);
+  // an id; `experts` if it names none
+  const auto read = [&](int64_t i) {
+    const int e = i < end ? ids[i] : -1;
+    return e >= 0 && e < experts ? e : experts;
+  };
+  for (int64_t i0 = first; i0 < end; i0 += 32 * kSortAhead) {
+    int e[kSortAhead];
+#pragma unroll
+    for (int u = 0; u < kSortAhead; ++u) e[u] = read(i0 + u * 32 + lane);
+#pragma unroll
+    for (int u = 0; u < kSortAhead; ++u)
+      if (e[u] < experts) atomicAdd(&mine[e[u]], 1);
   }
   __syncthreads();
-  // exclusive sums over this CTA's warps
+  // exclusive sums over this CTA's warps, eight loads in flight
   for (int e = tid; e < experts; e += blockDim.x) {
     int s = 0;
-    for (int w = 0; w < nwarps; ++w) {
-      const int c = hist[w * experts + e];
-      hist[w * experts + e] = s;
-      s += c;
+    for (int w0 = 0; w0 < nwarps; w0 += 8) {
+      int c[8];
+#pragma unroll
+      for (int w = 0; w < 8; ++w) c[w] = hist[(w0 + w) * experts + e];
+#pragma unroll
+      for (int w = 0; w < 8; ++w) {
+        hist[(w0 + w) * experts + e] = s;
+        s += c[w];
+      }
     }
     total[e] = s;
   }
-  cluster.sync();
+  if (ctas > 1) cluster.sync();
+  else __syncthreads();
   // counts over the cluster, and those of the CTAs before this one
   for (int e = tid; e < experts; e += blockDim.x) {
-    int s = 0, before = 0;
-    for (int r = 0; r < ctas; ++r) {
-      const int c = cluster.map_shared_rank(total, r)[e];
-      if (r < rank) before += c;
-      s += c;
+    int c[kMaxSortCtas], s = 0, before = 0;
+#pragma unroll
+    for (int r = 0; r < kMaxSortCtas; ++r) c[r] = r < ctas ? cluster.map_shared_rank(total, r)[e] : 0;
+#pragma unroll
+    for (int r = 0; r < kMaxSortCtas; ++r) {
+      before += r < rank ? c[r] : 0;
+      s += c[r];
     }
     all[e] = s;
-    start[e] = before;
+    ahead[e] = before;
   }
   // the experts' first rows: e * capacity, or the exclusive sum of the counts
   // (experts <= 1024 = one value a thread over up to 1024 threads; fewer threads loop)
@@ -287,9 +307,7 @@ __global__ void __launch_bounds__(1024) sort_kernel(int32_t *__restrict__ slot, 
     }
     if (e < experts) {
       const int begin = capacity ? e * capacity : carry + before + x - c;
-      const int ahead = start[e];
       start[e] = begin;
-      for (int w = 0; w < nwarps; ++w) hist[w * experts + e] += ahead;
       if (rank == 0) {
         counts[e] = c;
         offsets[e] = begin;
@@ -307,25 +325,40 @@ __global__ void __launch_bounds__(1024) sort_kernel(int32_t *__restrict__ slot, 
     for (int r = carry + rank * (int)blockDim.x + tid; r < rows; r += ctas * (int)blockDim.x) src[r] = -1;
   }
   // places
-  for (int64_t i0 = first; i0 < end; i0 += 32) {
-    const int64_t i = i0 + lane;
-    int e = i < end ? ids[i] : -1;
-    if (e < 0 || e >= experts) e = -1;
-    const unsigned peers = __match_any_sync(kFull, e);
-    int at = -1;
-    if (e >= 0) {
-      at = mine[e] + __popc(peers & ((1u << lane) - 1u));
-      at = capacity && at >= capacity ? -1 : start[e] + at;
+  int next[kSortAhead];
+#pragma unroll
+  for (int u = 0; u < kSortAhead; ++u) next[u] = read(first + u * 32 + lane);
+  for (int64_t i0 = first; i0 < end; i0 += 32 * kSortAhead) {
+    int e[kSortAhead];
+#pragma unroll
+    for (int u = 0; u < kSortAhead; ++u) {
+      e[u] = next[u];
+      next[u] = read(i0 + (kSortAhead + u) * 32 + lane);
     }
-    __syncwarp();
-    if (e >= 0 && lane == __ffs(peers) - 1) mine[e] += __popc(peers);
-    __syncwarp();
-    if (i < end) {
-      slot[i] = at;
-      if (at >= 0) src[at] = (int)i;
+#pragma unroll
+    for (int u = 0; u < kSortAhead; ++u) {
+      const int64_t i = i0 + u * 32 + lane;
+      unsigned peers = kFull;  // the lanes with this lane's expert
+      for (int b = 0; b < bits; ++b) {
+        const unsigned set = __ballot_sync(kFull, e[u] >> b & 1);
+        peers &= e[u] >> b & 1 ? set : ~set;
+      }
+      const bool has = e[u] < experts;
+      int at = -1;
+      if (has) {
+        at = ahead[e[u]] + mine[e[u]] + __popc(peers & ((1u << lane) - 1u));
+        at = capacity && at >= capacity ? -1 : start[e[u]] + at;
+      }
+      __syncwarp();
+      if (has && lane == __ffs(peers) - 1) mine[e[u]] += __popc(peers);
+      __syncwarp();
+      if (i < end) {
+        slot[i] = at;
+        if (at >= 0) src[at] = (int)i;
+      }
     }
   }
-  cluster.sync();  // no CTA leaves while another may read its totals
+  if (ctas > 1) cluster.sync();  // no CTA leaves while another may read its totals
 }
 
 // ---------------------------------------------------------------- rows to experts and back
@@ -581,14 +614,17 @@ extern "C" int fz_expert_sort(int32_t *slot, int32_t *src, int32_t *counts, int3
   const int64_t n = tokens * k, rows = capacity ? experts * capacity : n;
   FZ_REQUIRE(counts && offsets, "fz_expert_sort: null pointer");
   FZ_REQUIRE((n == 0 || (slot && ids)) && (rows == 0 || src), "fz_expert_sort: null pointer");
-  // Few choices: one CTA of few warps (fewer histograms to scan); many: a cluster of 8.
-  const int ctas = n > 8192 || rows > 65536 ? 8 : 1;
+  // Few choices: one CTA of few warps (fewer histograms to scan); many: a cluster of 8 or 16.
+  const int ctas = n > 131072 ? 16 : n > 8192 || rows > 65536 ? 8 : 1;
   const int threads = n > 1024 || experts > 256 || ctas > 1 ? 1024 : 256;
   const int warps = ctas * threads / 32;
   const int per_warp = (int)((n + warps - 1) / warps);
-  const size_t smem = sizeof(int32_t) * (size_t)experts * (threads / 32 + 3);
+  int bits = 1;  // of numbers up to `experts`
+  while ((experts >> bits) != 0) ++bits;
+  const size_t smem = sizeof(int32_t) * (size_t)experts * (threads / 32 + 4);
   FZ_CUDA(cudaFuncSetAttribute(sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                               (int)(sizeof(int32_t) * FZ_MAX_EXPERTS * (1024 / 32 + 3))));
+                               (int)(sizeof(int32_t) * FZ_MAX_EXPERTS * (1024 / 32 + 4))));
+  if (ctas > 8) FZ_CUDA(cudaFuncSetAttribute(sort_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(ctas);
   cfg.blockDim = dim3(threads);
@@ -604,7 +640,7 @@ extern "C" int fz_expert_sort(int32_t *slot, int32_t *src, int32_t *counts, int3
   cfg.attrs = attr;
   cfg.numAttrs = 2;
   FZ_CUDA(cudaLaunchKernelEx(&cfg, sort_kernel, slot, src, counts, offsets, ids, (int)n, (int)experts,
-                             (int)capacity, (int)rows, per_warp));
+                             (int)capacity, (int)rows, per_warp, bits));
   FZ_CHECK_LAUNCH();
   return FZ_OK;
 }
