@@ -115,13 +115,14 @@ __device__ __forceinline__ Pair phi2(Pair v, Pair *e) {
   return pair(a < 0.0f ? c : g, b < 0.0f ? d : k);  // NaN: both are
 }
 
-__device__ __forceinline__ Pair activate2(int act, Pair v) {
-  if (act == FZ_ACT_SILU) return mul2(v, sigmoid2(v));
-  if (act == FZ_ACT_GELU) {
+template <int ACT>
+__device__ __forceinline__ Pair activate2(Pair v) {
+  if constexpr (ACT == FZ_ACT_SILU) return mul2(v, sigmoid2(v));
+  if constexpr (ACT == FZ_ACT_GELU) {
     Pair e;
     return mul2(v, phi2(v, &e));
   }
-  if (act == FZ_ACT_RELU) {
+  if constexpr (ACT == FZ_ACT_RELU) {
     float a, b;
     unpair(v, a, b);
     return pair(a > 0.0f ? a : 0.0f, b > 0.0f ? b : 0.0f);
@@ -130,23 +131,39 @@ __device__ __forceinline__ Pair activate2(int act, Pair v) {
 }
 
 // d act'(v)
-__device__ __forceinline__ Pair times_slope2(int act, Pair d, Pair v) {
-  if (act == FZ_ACT_SILU) {
+template <int ACT>
+__device__ __forceinline__ Pair times_slope2(Pair d, Pair v) {
+  if constexpr (ACT == FZ_ACT_SILU) {
     const Pair s = sigmoid2(v), rest = fma2(s, both(-1.0f), both(1.0f));
     return mul2(d, mul2(s, fma2(v, rest, both(1.0f))));
   }
-  if (act == FZ_ACT_GELU) {
+  if constexpr (ACT == FZ_ACT_GELU) {
     Pair e;
     const Pair p = phi2(v, &e);
     return mul2(d, fma2(mul2(v, both(0.39894228040143268f)), e, p));
   }
-  if (act == FZ_ACT_RELU) {
+  if constexpr (ACT == FZ_ACT_RELU) {
     float a, b, x, y;
     unpair(v, a, b);
     unpair(d, x, y);
     return pair(a > 0.0f ? x : 0.0f, b > 0.0f ? y : 0.0f);
   }
   return d;
+}
+
+// f(Act<ACT>) for the activation of the call: chosen once around a loop, not in it.
+template <int ACT>
+struct Act {
+  static constexpr int value = ACT;
+};
+template <class F>
+__device__ __forceinline__ void with_activation(int act, F f) {
+  switch (act) {
+    case FZ_ACT_RELU: f(Act<FZ_ACT_RELU>{}); break;
+    case FZ_ACT_SILU: f(Act<FZ_ACT_SILU>{}); break;
+    case FZ_ACT_GELU: f(Act<FZ_ACT_GELU>{}); break;
+    default: f(Act<FZ_ACT_NONE>{}); break;
+  }
 }
 
 // ---------------------------------------------------------------- vectors
@@ -234,23 +251,23 @@ __device__ __forceinline__ void square_into(Vec<V> &s, const Vec<V> &x, Pair min
   }
 }
 // act(gamma (x - mean) rstd + beta)
-template <int V>
-__device__ __forceinline__ Vec<V> normalize(int act, const Vec<V> &x, Pair minus_mean, Pair rstd, const Vec<V> &gamma,
+template <int ACT, int V>
+__device__ __forceinline__ Vec<V> normalize(const Vec<V> &x, Pair minus_mean, Pair rstd, const Vec<V> &gamma,
                                             const Vec<V> &beta) {
   Vec<V> r;
 #pragma unroll
   for (int i = 0; i < Vec<V>::N; ++i)
-    r.p[i] = activate2(act, fma2(mul2(add2(x.p[i], minus_mean), rstd), gamma.p[i], beta.p[i]));
+    r.p[i] = activate2<ACT>(fma2(mul2(add2(x.p[i], minus_mean), rstd), gamma.p[i], beta.p[i]));
   return r;
 }
 // x <- xh, d <- dv gamma; dv and dv xh are added to db and dg
-template <int V>
-__device__ __forceinline__ void gradient(int act, Vec<V> &x, Vec<V> &d, Vec<V> &db, Vec<V> &dg, Pair minus_mean,
-                                         Pair rstd, const Vec<V> &gamma, const Vec<V> &beta) {
+template <int ACT, int V>
+__device__ __forceinline__ void gradient(Vec<V> &x, Vec<V> &d, Vec<V> &db, Vec<V> &dg, Pair minus_mean, Pair rstd,
+                                         const Vec<V> &gamma, const Vec<V> &beta) {
 #pragma unroll
   for (int i = 0; i < Vec<V>::N; ++i) {
     x.p[i] = mul2(add2(x.p[i], minus_mean), rstd);
-    const Pair dv = times_slope2(act, d.p[i], fma2(x.p[i], gamma.p[i], beta.p[i]));
+    const Pair dv = times_slope2<ACT>(d.p[i], fma2(x.p[i], gamma.p[i], beta.p[i]));
     db.p[i] = add2(db.p[i], dv);
     dg.p[i] = fma2(dv, x.p[i], dg.p[i]);
     d.p[i] = mul2(dv, gamma.p[i]);
@@ -439,24 +456,29 @@ __global__ void __launch_bounds__(kRowThreads, row_ctas(false, NV)) norm_rows_ke
       rstd[u] = total(q);
     }
     team_sums<P, U>(rstd, sh, [&](float v) { return rstd_of(v, a.inv_m, a.eps); });
+    with_activation(a.act, [&](auto act) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (b + u * parts < batch) {
+      for (int u = 0; u < U; ++u) {
+        if (b + u * parts < batch) {
 #pragma unroll
-        for (int i = 0; i < NV; ++i)
-          if (t.at[i] >= 0) {
-            Vec<V> ga, be;
-            affine.get(a, t.channel, i, ga, be);
-            store(to + t.at[i], normalize(a.act, x[u][i], both(-mean[u]), both(rstd[u]), ga, be));
-          }
-        if (a.mean && threadIdx.x % P == 0) {
-          a.mean[team] = mean[u];
-          a.rstd[team] = rstd[u];
+          for (int i = 0; i < NV; ++i)
+            if (t.at[i] >= 0) {
+              Vec<V> ga, be;
+              affine.get(a, t.channel, i, ga, be);
+              store(to + u * hop + t.at[i],
+                    normalize<decltype(act)::value>(x[u][i], both(-mean[u]), both(rstd[u]), ga, be));
+            }
         }
       }
-      to += hop;
-      team += stride;
-    }
+    });
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (a.mean && threadIdx.x % P == 0 && b + u * parts < batch) {
+        a.mean[team + (int64_t)u * stride] = mean[u];
+        a.rstd[team + (int64_t)u * stride] = rstd[u];
+      }
+    to += U * hop;
+    team += (int64_t)U * stride;
   }
   copy_wait<0>();
 }
@@ -529,22 +551,24 @@ __global__ void __launch_bounds__(kRowThreads, row_ctas(true, NV))
     }
     fetch(s, b + S * step);
     fetch_stats(b + step);
+    with_activation(a.act, [&](auto act) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      if (t.at[i] < 0) continue;
-      Vec<V> ga, be;
-      affine.get(a, t.channel, i, ga, be);
+      for (int i = 0; i < NV; ++i) {
+        if (t.at[i] < 0) continue;
+        Vec<V> ga, be;
+        affine.get(a, t.channel, i, ga, be);
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        // behind the batch x, d, mean and rstd are 0, and so is all that they give
-        gradient(a.act, x[u][i], d[u][i], db[i], dg[i], minus[u], both(rstd[u]), ga, be);
-        Vec<V> w;
+        for (int u = 0; u < U; ++u) {
+          // behind the batch x, d, mean and rstd are 0, and so is all that they give
+          gradient<decltype(act)::value>(x[u][i], d[u][i], db[i], dg[i], minus[u], both(rstd[u]), ga, be);
+          Vec<V> w;
 #pragma unroll
-        for (int j = 0; j < Vec<V>::N; ++j) w.p[j] = mul2(d[u][i].p[j], x[u][i].p[j]);
-        s1[u] = __fadd_rn(s1[u], total(d[u][i]));
-        s2[u] = __fadd_rn(s2[u], total(w));
+          for (int j = 0; j < Vec<V>::N; ++j) w.p[j] = mul2(d[u][i].p[j], x[u][i].p[j]);
+          s1[u] = __fadd_rn(s1[u], total(d[u][i]));
+          s2[u] = __fadd_rn(s2[u], total(w));
+        }
       }
-    }
+    });
     const auto over_m = [&](float v) { return __fmul_rn(v, -a.inv_m); };
     team_sums<P, U>(s1, sh, over_m);
     team_sums<P, U>(s2, sh, over_m);
@@ -928,11 +952,13 @@ __global__ void __launch_bounds__(kTileThreads, kTileCtas) norm_tile_kernel(cons
       const Vec<V> be = load_or<V>(a.beta ? a.beta + me.channel : nullptr, 0.0f);
       const Pair minus = both(-stats[column].x), rstd = both(stats[column].y);
       float *q = a.y + me.at;
+      with_activation(a.act, [&](auto act) {
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        if (i < me.mine) store(q, normalize(a.act, x[i], minus, rstd, ga, be));
-        q += step;
-      }
+        for (int i = 0; i < N; ++i) {
+          if (i < me.mine) store(q, normalize<decltype(act)::value>(x[i], minus, rstd, ga, be));
+          q += step;
+        }
+      });
     }
   }
   copy_wait<0>();
@@ -1040,9 +1066,11 @@ __global__ void __launch_bounds__(kTileThreads, kTileCtas) norm_tile_backward_ke
       const Vec<V> ga = load_or<V>(a.gamma ? a.gamma + me.channel : nullptr, 1.0f);
       const Vec<V> be = load_or<V>(a.beta ? a.beta + me.channel : nullptr, 0.0f);
       const Pair minus = both(-stat.x);
+      with_activation(a.act, [&](auto act) {
 #pragma unroll
-      for (int i = 0; i < N; ++i)
-        if (i < me.mine) gradient(a.act, x[i], d[i], db, dg, minus, rstd, ga, be);
+        for (int i = 0; i < N; ++i)
+          if (i < me.mine) gradient<decltype(act)::value>(x[i], d[i], db, dg, minus, rstd, ga, be);
+      });
     }
     if (MODE != kWhole) column_sums(db, dg, sh, a, me, t, walk.tx);
     if (joined) {
