@@ -638,6 +638,7 @@ struct Tile {
   int b, chunk, k;
   int g0, q, cols;  // its first group, its groups, its vectors a row
   int rows, mine;   // its rows, and those of this thread (0: none)
+  int most;         // rows of the thread that has most: what runs for all skips only behind it
   int channel;      // this thread's first channel
   int64_t at;       // offset of this thread's first vector
 };
@@ -692,6 +693,7 @@ struct Walk {
     r.rows = (int)min((int64_t)t.rows, a.len - row0);
     r.channel = r.g0 * a.c + (piece * t.cols + tx) * V;
     r.mine = tx < r.cols && ty < r.rows ? ((r.rows - 1 - ty) >> shift) + 1 : 0;
+    r.most = ((r.rows - 1) >> shift) + 1;
     r.at = (r.b * a.len + row0 + ty) * a.channels + r.channel;
     return r;
   }
@@ -947,15 +949,18 @@ __global__ void __launch_bounds__(kTileThreads, kTileCtas) norm_tile_kernel(cons
       }
     }
     __syncthreads();
-    if (MODE != kParts && me.mine) {
-      const Vec<V> ga = load_or<V>(a.gamma ? a.gamma + me.channel : nullptr, 1.0f);
-      const Vec<V> be = load_or<V>(a.beta ? a.beta + me.channel : nullptr, 0.0f);
-      const Pair minus = both(-stats[column].x), rstd = both(stats[column].y);
+    if (MODE != kParts) {
+      const int mine = me.mine ? column : 0;
+      const Vec<V> ga = load_or<V>(a.gamma && me.mine ? a.gamma + me.channel : nullptr, 1.0f);
+      const Vec<V> be = load_or<V>(a.beta && me.mine ? a.beta + me.channel : nullptr, 0.0f);
+      const Pair minus = both(-stats[mine].x), rstd = both(stats[mine].y);
       float *q = a.y + me.at;
       with_activation(a.act, [&](auto act) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-          if (i < me.mine) store(q, normalize<decltype(act)::value>(x[i], minus, rstd, ga, be));
+          if (i >= me.most) break;
+          const Vec<V> r = normalize<decltype(act)::value>(x[i], minus, rstd, ga, be);
+          if (i < me.mine) store(q, r);
           q += step;
         }
       });
@@ -1062,14 +1067,15 @@ __global__ void __launch_bounds__(kTileThreads, kTileCtas) norm_tile_backward_ke
     take_tile(d, fifo + kStage, me);
     fetch();
     const Pair rstd = both(stat.y);
-    if (me.mine) {
-      const Vec<V> ga = load_or<V>(a.gamma ? a.gamma + me.channel : nullptr, 1.0f);
-      const Vec<V> be = load_or<V>(a.beta ? a.beta + me.channel : nullptr, 0.0f);
+    {
+      // behind a thread's rows x and dy are 0, and so is what they add to its columns' sums
+      const Vec<V> ga = load_or<V>(a.gamma && me.mine ? a.gamma + me.channel : nullptr, 1.0f);
+      const Vec<V> be = load_or<V>(a.beta && me.mine ? a.beta + me.channel : nullptr, 0.0f);
       const Pair minus = both(-stat.x);
       with_activation(a.act, [&](auto act) {
 #pragma unroll
         for (int i = 0; i < N; ++i)
-          if (i < me.mine) gradient<decltype(act)::value>(x[i], d[i], db, dg, minus, rstd, ga, be);
+          if (i < me.most) gradient<decltype(act)::value>(x[i], d[i], db, dg, minus, rstd, ga, be);
       });
     }
     if (MODE != kWhole) column_sums(db, dg, sh, a, me, t, walk.tx);
@@ -1103,12 +1109,15 @@ __global__ void __launch_bounds__(kTileThreads, kTileCtas) norm_tile_backward_ke
       if (lane == 0) means[g] = make_float2(u, w);
     }
     __syncthreads();
-    if (MODE != kParts && me.mine) {
-      const Pair k1 = both(means[column].x), k2 = both(means[column].y);
+    if (MODE != kParts) {
+      const int mine = me.mine ? column : 0;
+      const Pair k1 = both(means[mine].x), k2 = both(means[mine].y);
       float *q = a.dx + me.at;
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        if (i < me.mine) store(q, finish(x[i], d[i], k1, k2, rstd));
+        if (i >= me.most) break;
+        const Vec<V> r = finish(x[i], d[i], k1, k2, rstd);
+        if (i < me.mine) store(q, r);
         q += step;
       }
     }
