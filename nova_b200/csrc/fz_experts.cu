@@ -21,12 +21,14 @@ bool aligned16(const void *a, const void *b = nullptr, const void *c = nullptr) 
 
 // ---------------------------------------------------------------- router
 
-// Logits as unsigned keys in the same order: NaN above all, -0 equal to +0, and 0 free
-// to mark what has been taken.
+// Logits as unsigned keys in the same order: NaN above all (an addition gives the canonical,
+// positive NaN), -0 equal to +0, and 0 free to mark what has been taken.
 __device__ __forceinline__ uint32_t order_key(float v) {
-  if (v != v) return 0xffffffffu;
   const uint32_t u = __float_as_uint(__fadd_rn(v, 0.0f));
-  return u ^ ((u >> 31) ? 0xffffffffu : 0x80000000u);
+  return u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ float from_key(uint32_t key) {
+  return __uint_as_float(key ^ ((uint32_t)((int32_t)~key >> 31) | 0x80000000u));
 }
 constexpr uint32_t kKeyMinusInf = 0x007fffffu;
 
@@ -85,11 +87,11 @@ __global__ void __launch_bounds__(256) route_kernel(float *__restrict__ weights,
   float v[NE], next[NE];
   if (t < tokens) load_row(next, logits + t * experts, lane, experts);
   for (; t < tokens; t += warps) {
-    uint32_t key[NE];
+    uint32_t own[NE], key[NE];
 #pragma unroll
     for (int i = 0; i < NE; ++i) {
       v[i] = next[i];
-      key[i] = order_key(v[i]);
+      own[i] = key[i] = order_key(v[i]);
     }
     if (t + warps < tokens) load_row(next, logits + (t + warps) * experts, lane, experts);
     sort_keys(key);
@@ -108,23 +110,18 @@ __global__ void __launch_bounds__(256) route_kernel(float *__restrict__ weights,
     const uint32_t last = __reduce_min_sync(kFull, mine ? mine : 0xffffffffu);  // the smallest picked
     const bool any = __any_sync(kFull, mine != 0);
     int id = -1;
-    float logit = 0.0f;
 #pragma unroll
     for (int i = 0; i < NE; ++i) {
-      const uint32_t own = order_key(v[i]);
-      unsigned found = __ballot_sync(kFull, any && own >= last);
+      unsigned found = __ballot_sync(kFull, any && own[i] >= last);
       while (found) {
         const int from = __ffs(found) - 1;
         found &= found - 1;
-        const uint32_t its = __shfl_sync(kFull, own, from);
-        const float value = __shfl_sync(kFull, v[i], from);
+        const uint32_t its = __shfl_sync(kFull, own[i], from);
         const unsigned open = __ballot_sync(kFull, mine == its && id < 0);
-        if (open && lane == __ffs(open) - 1) {
-          id = from + 32 * i;
-          logit = value;
-        }
+        if (lane == __ffs(open) - 1) id = from + 32 * i;
       }
     }
+    const float logit = from_key(mine);
     const float top = __shfl_sync(kFull, logit, 0);
     const float num = id >= 0 ? exp_below(logit, top) : 0.0f;
     float den = num;
