@@ -68,14 +68,61 @@ __device__ __forceinline__ void load_row(float (&v)[NE], const float *row, int l
   for (int i = 0; i < NE; ++i) v[i] = lane + 32 * i < experts ? row[lane + 32 * i] : -INFINITY;
 }
 
-// One warp per token, expert e = lane + 32 i in register i of lane `lane`, the next token's
-// logits fetched ahead. Bound by instruction issue, so experts are picked by their keys
-// alone: every lane sorts its own keys once, a pick is the largest of the lanes' heads (one
-// warp-wide reduction) and its lane moves its list up. Then the experts whose keys were
-// picked are found in ascending order, each taking the first open pick of its key: ties go
-// to the lowest experts, and those that are too many find none. (Keeping each expert's
-// number with its key, and removing it from an unsorted list, cost 2.4 times as many
-// instructions at 256 experts and 8 picks.)
+// A warp's token, expert e = lane + 32 i in register i of lane `lane`. Experts are picked by
+// their keys alone: every lane sorts its own keys once, a pick is the largest of the lanes'
+// heads (one warp-wide reduction) and its lane moves its list up. Then the experts whose keys
+// were picked are found in ascending order, each taking the first open pick of its key: ties
+// go to the lowest experts, and those that are too many find none.
+template <int NE>
+__device__ __forceinline__ void route_token(float *weights, int32_t *ids, const float (&v)[NE], int64_t t,
+                                            int experts, int k, int renormalize, int lane) {
+  uint32_t own[NE], key[NE];
+#pragma unroll
+  for (int i = 0; i < NE; ++i) own[i] = key[i] = order_key(v[i]);
+  sort_keys(key);
+  uint32_t mine = 0;  // lane j: the j-th pick's key; 0: none
+  for (int j = 0; j < k; ++j) {
+    const uint32_t top = __reduce_max_sync(kFull, key[0]);
+    if (top <= kKeyMinusInf) break;  // only -inf (or nothing) left
+    const int owner = __ffs(__ballot_sync(kFull, key[0] == top)) - 1;
+    if (lane == j) mine = top;
+    if (lane == owner) {
+#pragma unroll
+      for (int i = 0; i + 1 < NE; ++i) key[i] = key[i + 1];
+      key[NE - 1] = 0;
+    }
+  }
+  const uint32_t last = __reduce_min_sync(kFull, mine ? mine : 0xffffffffu);  // the smallest picked
+  const bool any = __any_sync(kFull, mine != 0);
+  int id = -1;
+#pragma unroll
+  for (int i = 0; i < NE; ++i) {
+    unsigned found = __ballot_sync(kFull, any && own[i] >= last);
+    while (found) {
+      const int from = __ffs(found) - 1;
+      found &= found - 1;
+      const uint32_t its = __shfl_sync(kFull, own[i], from);
+      const unsigned open = __ballot_sync(kFull, mine == its && id < 0);
+      if (lane == __ffs(open) - 1) id = from + 32 * i;
+    }
+  }
+  const float logit = from_key(mine);
+  const float top = __shfl_sync(kFull, logit, 0);
+  const float num = id >= 0 ? exp_below(logit, top) : 0.0f;
+  float den = num;
+  if (!renormalize) {
+    den = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NE; ++i) den = __fadd_rn(den, lane + 32 * i < experts ? exp_below(v[i], top) : 0.0f);
+  }
+  den = warp_sum(den);
+  if (lane < k) {
+    weights[t * k + lane] = id >= 0 ? __fdiv_rn(num, den) : 0.0f;
+    ids[t * k + lane] = id;
+  }
+}
+
+// One warp per token, the next token's logits fetched ahead.
 template <int NE>
 __global__ void __launch_bounds__(256) route_kernel(float *__restrict__ weights, int32_t *__restrict__ ids,
                                                     const float *__restrict__ logits, int64_t tokens, int experts,
@@ -87,53 +134,123 @@ __global__ void __launch_bounds__(256) route_kernel(float *__restrict__ weights,
   float v[NE], next[NE];
   if (t < tokens) load_row(next, logits + t * experts, lane, experts);
   for (; t < tokens; t += warps) {
-    uint32_t own[NE], key[NE];
 #pragma unroll
-    for (int i = 0; i < NE; ++i) {
-      v[i] = next[i];
-      own[i] = key[i] = order_key(v[i]);
-    }
+    for (int i = 0; i < NE; ++i) v[i] = next[i];
     if (t + warps < tokens) load_row(next, logits + (t + warps) * experts, lane, experts);
-    sort_keys(key);
-    uint32_t mine = 0;  // lane j: the j-th pick's key; 0: none
-    for (int j = 0; j < k; ++j) {
-      const uint32_t top = __reduce_max_sync(kFull, key[0]);
-      if (top <= kKeyMinusInf) break;  // only -inf (or nothing) left
-      const int owner = __ffs(__ballot_sync(kFull, key[0] == top)) - 1;
-      if (lane == j) mine = top;
-      if (lane == owner) {
+    route_token(weights, ids, v, t, experts, k, renormalize, lane);
+  }
+}
+
+// The K largest of two descending lists of K, descending, in a.
+template <int K>
+__device__ __forceinline__ void merge_keys(uint32_t (&a)[K], const uint32_t (&b)[K]) {
 #pragma unroll
-        for (int i = 0; i + 1 < NE; ++i) key[i] = key[i + 1];
-        key[NE - 1] = 0;
+  for (int i = 0; i < K; ++i) a[i] = max(a[i], b[K - 1 - i]);  // a bitonic sequence
+#pragma unroll
+  for (int d = K / 2; d > 0; d /= 2)
+#pragma unroll
+    for (int i = 0; i < K; ++i)
+      if (!(i & d)) {
+        const uint32_t x = a[i], y = a[i + d];
+        a[i] = max(x, y);
+        a[i + d] = min(x, y);
+      }
+}
+
+// Eight lanes per token, expert e = sub + 8 i in register i (at most 8 N experts, K picks).
+// Bound by instruction issue, which four tokens a warp share: a lane's K largest keys come
+// from sorting networks, the token's from three rounds of merging with another lane's, with
+// no exchange per pick. A pick's place is the number of larger keys, so that each lane
+// writes its own picks. Tokens with equal keys among their picks or at their end, or with
+// a NaN, are left to route_token. (65536 tokens, 256 experts, 8 picks: 49 us with a warp a
+// token throughout.)
+template <int N, int K>
+__global__ void __launch_bounds__(256) route_team_kernel(float *__restrict__ weights, int32_t *__restrict__ ids,
+                                                         const float *__restrict__ logits, int64_t tokens,
+                                                         int experts, int k, int renormalize) {
+  pdl_wait();
+  const int lane = threadIdx.x & 31, sub = lane & 7;
+  const int64_t warps = (int64_t)gridDim.x * (blockDim.x >> 5);
+  for (int64_t w = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); w * 4 < tokens; w += warps) {
+    const int64_t t = w * 4 + (lane >> 3);
+    const bool on = t < tokens;
+    const float *row = logits + t * experts;
+    float v[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = on && sub + 8 * i < experts ? row[sub + 8 * i] : -INFINITY;
+    uint32_t top[K];
+#pragma unroll
+    for (int g = 0; g < N; g += K) {
+      uint32_t key[K];
+#pragma unroll
+      for (int i = 0; i < K; ++i) key[i] = order_key(v[g + i]);
+      sort_keys(key);
+      if (g == 0) {
+#pragma unroll
+        for (int i = 0; i < K; ++i) top[i] = key[i];
+      } else {
+        merge_keys(top, key);
       }
     }
-    const uint32_t last = __reduce_min_sync(kFull, mine ? mine : 0xffffffffu);  // the smallest picked
-    const bool any = __any_sync(kFull, mine != 0);
-    int id = -1;
 #pragma unroll
-    for (int i = 0; i < NE; ++i) {
-      unsigned found = __ballot_sync(kFull, any && own[i] >= last);
-      while (found) {
-        const int from = __ffs(found) - 1;
-        found &= found - 1;
-        const uint32_t its = __shfl_sync(kFull, own[i], from);
-        const unsigned open = __ballot_sync(kFull, mine == its && id < 0);
-        if (lane == __ffs(open) - 1) id = from + 32 * i;
-      }
+    for (int d = 1; d < 8; d *= 2) {
+      uint32_t other[K];
+#pragma unroll
+      for (int i = 0; i < K; ++i) other[i] = __shfl_xor_sync(kFull, top[i], d);
+      merge_keys(top, other);
     }
-    const float logit = from_key(mine);
-    const float top = __shfl_sync(kFull, logit, 0);
-    const float num = id >= 0 ? exp_below(logit, top) : 0.0f;
-    float den = num;
+    int picks = 0;
+    uint32_t last = 0, mine = 0;  // the smallest key picked; lane j's: the j-th
+    bool odd = top[0] == 0xffffffffu;
+#pragma unroll
+    for (int j = 0; j < K; ++j) {
+      const bool picked = j < k && top[j] > kKeyMinusInf;
+      picks += picked;
+      if (picked) odd = odd || (j > 0 && top[j] == last);
+      if (picked) last = top[j];
+      if (picked && j == sub) mine = top[j];
+    }
+    const float end = from_key(last), most = from_key(top[0]);
+    unsigned chosen = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) chosen |= (unsigned)(v[i] >= end) << i;
+    if (picks == 0) chosen = 0;
+    int count = __popc(chosen);
+    float den = mine ? exp_below(from_key(mine), most) : 0.0f;
     if (!renormalize) {
       den = 0.0f;
 #pragma unroll
-      for (int i = 0; i < NE; ++i) den = __fadd_rn(den, lane + 32 * i < experts ? exp_below(v[i], top) : 0.0f);
+      for (int i = 0; i < N; ++i) den = __fadd_rn(den, exp_below(v[i], most));  // -inf: 0
     }
-    den = warp_sum(den);
-    if (lane < k) {
-      weights[t * k + lane] = id >= 0 ? __fdiv_rn(num, den) : 0.0f;
-      ids[t * k + lane] = id;
+#pragma unroll
+    for (int d = 1; d < 8; d *= 2) {
+      count += __shfl_xor_sync(kFull, count, d);
+      den = __fadd_rn(den, __shfl_xor_sync(kFull, den, d));
+    }
+    odd = odd || count != picks;
+    if (odd) chosen = 0;
+    while (__any_sync(kFull, chosen != 0)) {
+      if (chosen) {
+        const int e = sub + 8 * (__ffs(chosen) - 1);
+        chosen &= chosen - 1;
+        const float x = row[e];
+        const uint32_t key = order_key(x);
+        int place = 0;
+#pragma unroll
+        for (int j = 0; j < K; ++j) place += top[j] > key;
+        weights[t * k + place] = __fdiv_rn(exp_below(x, most), den);
+        ids[t * k + place] = e;
+      }
+    }
+    if (on && !odd && sub >= picks && sub < k) {
+      weights[t * k + sub] = 0.0f;
+      ids[t * k + sub] = -1;
+    }
+    for (unsigned left = __ballot_sync(kFull, odd && sub == 0); left; left &= left - 1) {
+      const int64_t its = w * 4 + ((__ffs(left) - 1) >> 3);
+      float u[N / 4];
+      load_row(u, logits + its * experts, lane, experts);
+      route_token(weights, ids, u, its, experts, k, renormalize, lane);
     }
   }
 }
@@ -551,6 +668,14 @@ int launch_route(float *w, int32_t *ids, const float *logits, int64_t tokens, in
   FZ_CHECK_LAUNCH();
   return FZ_OK;
 }
+template <int N, int K>
+int launch_route_team(float *w, int32_t *ids, const float *logits, int64_t tokens, int experts, int k, int renorm,
+                      cudaStream_t s) {
+  FZ_CUDA(fz::launch_pdl(route_team_kernel<N, K>, dim3(fz::grid_for((tokens + 3) / 4, 8, 4)), dim3(256), 0, s, w,
+                         ids, logits, tokens, experts, k, renorm));
+  FZ_CHECK_LAUNCH();
+  return FZ_OK;
+}
 template <int NE>
 int launch_route_backward(float *dl, const float *dw, const float *w, const int32_t *ids, const float *logits,
                           int64_t tokens, int experts, int k, int renorm, cudaStream_t s) {
@@ -578,6 +703,16 @@ extern "C" int fz_route(float *weights, int32_t *ids, const float *logits, int64
   FZ_REQUIRE(weights && ids && logits, "fz_route: null pointer");
   cudaStream_t s = fz::resolve(stream);
   const int e = (int)experts, kk = (int)k, rn = renormalize != 0;
+  // eight lanes a token up to 256 experts and 8 picks, else a warp
+  if (k <= 4) {
+    if (e <= 64) return launch_route_team<8, 4>(weights, ids, logits, tokens, e, kk, rn, s);
+    if (e <= 128) return launch_route_team<16, 4>(weights, ids, logits, tokens, e, kk, rn, s);
+    if (e <= 256) return launch_route_team<32, 4>(weights, ids, logits, tokens, e, kk, rn, s);
+  } else if (k <= 8) {
+    if (e <= 64) return launch_route_team<8, 8>(weights, ids, logits, tokens, e, kk, rn, s);
+    if (e <= 128) return launch_route_team<16, 8>(weights, ids, logits, tokens, e, kk, rn, s);
+    if (e <= 256) return launch_route_team<32, 8>(weights, ids, logits, tokens, e, kk, rn, s);
+  }
   if (e <= 32) return launch_route<1>(weights, ids, logits, tokens, e, kk, rn, s);
   if (e <= 64) return launch_route<2>(weights, ids, logits, tokens, e, kk, rn, s);
   if (e <= 128) return launch_route<4>(weights, ids, logits, tokens, e, kk, rn, s);
