@@ -396,7 +396,8 @@ enum fz_activation { FZ_ACT_NONE = 0, FZ_ACT_RELU = 1, FZ_ACT_SILU = 2, FZ_ACT_G
  * gamma / beta hold `channels` values; NULL means ones / zeros. mean and rstd
  * ([batch, groups], both or neither NULL) are written for the backward. Statistics are
  * held in fp32 and joined by mean and centred sum of squares, so a large common offset
- * of x costs no digits beyond those x itself lost. y may not overlap x.
+ * of x costs no digits beyond those x itself lost. y may not overlap x. At most 2^30
+ * batch * len rows and 2^36 values.
  * workspace: at least fz_group_norm_workspace(..., backward = 0, ...) bytes, 16-byte
  * aligned, free for reuse once the call's work on `stream` is done (calls that overlap
  * need one each); NULL when that is 0. eps >= 0. */

@@ -433,10 +433,10 @@ __global__ void __launch_bounds__(1024) sort_kernel(int32_t *__restrict__ slot, 
   if (rank == 0 && tid == 0) offsets[experts] = capacity ? experts * capacity : carry;
   // empty rows
   if (capacity) {
-    for (int r = rank * (int)blockDim.x + tid; r < rows; r += ctas * (int)blockDim.x)
-      if (r % capacity >= all[r / capacity]) src[r] = -1;
+    for (int64_t r = rank * (int)blockDim.x + tid; r < rows; r += ctas * (int)blockDim.x)
+      if ((int)r % capacity >= all[(int)r / capacity]) src[r] = -1;
   } else {
-    for (int r = carry + rank * (int)blockDim.x + tid; r < rows; r += ctas * (int)blockDim.x) src[r] = -1;
+    for (int64_t r = (int64_t)carry + rank * (int)blockDim.x + tid; r < rows; r += ctas * (int)blockDim.x) src[r] = -1;
   }
   // places
   int next[kSortAhead];

@@ -555,18 +555,20 @@ __global__ void __launch_bounds__(kRowThreads, row_ctas(true, NV))
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
         if (t.at[i] < 0) continue;
-        Vec<V> ga, be;
+        Vec<V> ga, be, b_sum = splat<V>(0.0f), g_sum = b_sum;  // of U teams, then of all
         affine.get(a, t.channel, i, ga, be);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
           // behind the batch x, d, mean and rstd are 0, and so is all that they give
-          gradient<decltype(act)::value>(x[u][i], d[u][i], db[i], dg[i], minus[u], both(rstd[u]), ga, be);
+          gradient<decltype(act)::value>(x[u][i], d[u][i], b_sum, g_sum, minus[u], both(rstd[u]), ga, be);
           Vec<V> w;
 #pragma unroll
           for (int j = 0; j < Vec<V>::N; ++j) w.p[j] = mul2(d[u][i].p[j], x[u][i].p[j]);
           s1[u] = __fadd_rn(s1[u], total(d[u][i]));
           s2[u] = __fadd_rn(s2[u], total(w));
         }
+        sum_into(db[i], b_sum);
+        sum_into(dg[i], g_sum);
       }
     });
     const auto over_m = [&](float v) { return __fmul_rn(v, -a.inv_m); };
@@ -1395,8 +1397,10 @@ int check_sizes(const char *who, int64_t batch, int64_t len, int64_t channels, i
   const std::string name(who);
   FZ_REQUIRE(batch >= 0 && len >= 0 && channels >= 1 && groups >= 1, name + ": negative or zero size");
   FZ_REQUIRE(channels % groups == 0, name + ": channels must be a multiple of groups");
-  FZ_REQUIRE(channels <= INT_MAX && len <= INT_MAX && batch <= INT_MAX, name + ": too many elements");
-  FZ_REQUIRE(len == 0 || batch == 0 || (batch <= INT_MAX / len && batch * len <= ((int64_t)1 << 36) / channels),
+  // 2^36 values in at most 2^30 rows of channels (batch numbers are 32-bit in the kernels)
+  const int64_t rows = (int64_t)1 << 30, values = (int64_t)1 << 36;
+  FZ_REQUIRE(channels <= rows && len <= rows && batch <= rows, name + ": too many elements");
+  FZ_REQUIRE(len == 0 || batch == 0 || (batch <= rows / len && batch * len <= values / channels),
              name + ": too many elements");
   return FZ_OK;
 }

@@ -87,6 +87,12 @@ Indices indices_from_array(py::object values, Device dev) {
   const char kind = a.dtype().kind();
   if (kind != 'i' && kind != 'u')
     throw std::invalid_argument("Indices: an array of whole numbers is needed");
+  if (kind == 'u' && a.itemsize() == 8) {  // would not fit the int64 that the values are read as
+    auto u = py::array_t<uint64_t, py::array::c_style | py::array::forcecast>::ensure(a);
+    if (!u) throw py::error_already_set();
+    for (ssize_t i = 0; i < u.size(); ++i)
+      if (u.data()[i] > (uint64_t)INT32_MAX) throw std::invalid_argument("Indices: a value does not fit int32");
+  }
   auto v = py::array_t<int64_t, py::array::c_style | py::array::forcecast>::ensure(a);
   if (!v) throw py::error_already_set();
   std::vector<size_t> shape;

@@ -280,6 +280,8 @@ def refusals(F):
         lambda: F.route(T(F, np.ones((1, 1025))), 2),
         lambda: F.Indices(np.zeros((2, 2))),                          # not whole numbers
         lambda: F.Indices(np.array([1 << 31])),
+        lambda: F.Indices(np.array([2 ** 64 - 1], np.uint64)),
+        lambda: F.Indices([[1, 2], [3]]),
         lambda: F.Indices(np.int64(3)),                               # no axis
         lambda: F.ExpertPlan(ids, 0, 4),
         lambda: F.ExpertPlan(ids, 1025, 4),

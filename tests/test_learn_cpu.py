@@ -46,6 +46,9 @@ BAD_CALLS = [
     ("fz_group_norm", [P, None, None, P, None, None, 1, 1, 4, 2, 1e-5, 0, None, 0, None], "overlap"),
     ("fz_group_norm", [None, None, None, P, None, None, 1, 1, 4, 2, 1e-5, 0, None, 0, None], "null"),
     ("fz_group_norm", [P, None, None, P, None, None, 1 << 40, 1 << 40, 4, 2, 1e-5, 0, None, 0, None], "too many"),
+    ("fz_group_norm", [P, None, None, P, None, None, (1 << 30) + 1, 1, 4, 2, 1e-5, 0, None, 0, None], "too many"),
+    ("fz_group_norm", [C.c_void_p(8192), None, None, P, None, None, 1, 1 << 24, 8, 2, 1e-5, 0, None, 0, None], "workspace"),
+    ("fz_group_norm_backward", [C.c_void_p(8192), P, P, C.c_void_p(12288), P, P, P, None, None, 4, 1, 4, 2, 0, P, 3, None], "workspace"),
     ("fz_group_norm_backward", [P, None, None, None, P, P, P, None, None, 1, 1, 4, 2, 0, None, 0, None], "null"),
     ("fz_group_norm_backward", [P, None, None, P, P, P, P, None, None, 1, 1, 4, 2, 0, None, 0, None], "overlap"),
     ("fz_route", [P, P, P, 4, 1025, 2, 1, None], "FZ_MAX_EXPERTS"),
