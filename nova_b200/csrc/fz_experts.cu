@@ -477,8 +477,13 @@ __global__ void __launch_bounds__(1024) sort_kernel(int32_t *__restrict__ slot, 
 
 // ---------------------------------------------------------------- rows to experts and back
 
-// Work is cut into pieces of one token and kChunk vectors a lane; a warp takes a piece.
-// VEC = 4: rows of float4 (width a multiple of 4, 16-byte aligned buffers), else 1.
+// Work is cut into pieces of one token and kUnroll vectors a lane, taken by a team of P
+// lanes: a warp (rows of many vectors: several pieces), or 8 or 2 lanes where a row has at
+// most 32 or 8 vectors, so that narrow rows do not leave a warp's lanes idle (32768 tokens of
+// 16 floats, 8 choices: combine 32 us with a warp a token, 11 us so). VEC = 4: rows of float4
+// (width a multiple of 4, 16-byte aligned buffers), else 1. Every value is read or written
+// once: the token's row once for its k copies, each expert's row once; the next choice's
+// row number is fetched ahead.
 constexpr int kUnroll = 4;
 
 template <int VEC>
@@ -525,7 +530,7 @@ __device__ __forceinline__ void zero_empty(typename Vec<VEC>::T *rows, const int
   }
 }
 
-template <int VEC>
+template <int VEC, int P>
 __global__ void __launch_bounds__(256) dispatch_kernel(typename Vec<VEC>::T *__restrict__ rows,
                                                        const typename Vec<VEC>::T *__restrict__ x,
                                                        const int32_t *__restrict__ slot,
@@ -533,35 +538,35 @@ __global__ void __launch_bounds__(256) dispatch_kernel(typename Vec<VEC>::T *__r
                                                        int64_t num_rows, int64_t nvec, int64_t chunks) {
   using V = Vec<VEC>;
   pdl_wait();
-  const int lane = threadIdx.x & 31;
-  const int64_t work = tokens * chunks, all = work + (num_rows + 31) / 32 * chunks;
+  constexpr int kTeams = 32 / P;
+  const int lane = threadIdx.x & 31, sub = lane % P;
+  // warps' pieces: of kTeams tokens each, then groups of 32 rows to look for empty ones in
+  const int64_t work = (tokens * chunks + kTeams - 1) / kTeams;
+  const int64_t zero_chunks = (nvec + 32 * kUnroll - 1) / (32 * kUnroll);
+  const int64_t all = work + (num_rows + 31) / 32 * zero_chunks;
   const int64_t warps = (int64_t)gridDim.x * (blockDim.x >> 5);
   for (int64_t p = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); p < all; p += warps) {
     if (p >= work) {
-      const int64_t q = p - work, g = q / chunks;
-      zero_empty<VEC>(rows, src, g * 32, num_rows, nvec, (q - g * chunks) * 32 * kUnroll, lane);
+      const int64_t q = p - work, g = q / zero_chunks;
+      zero_empty<VEC>(rows, src, g * 32, num_rows, nvec, (q - g * zero_chunks) * 32 * kUnroll, lane);
       continue;
     }
-    const int64_t t = p / chunks, c0 = (p - t * chunks) * 32 * kUnroll;
+    const int64_t piece = p * kTeams + lane / P, t = piece / chunks, c0 = (piece - t * chunks) * P * kUnroll + sub;
+    if (t >= tokens) continue;
     typename V::T v[kUnroll];
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      const int64_t c = c0 + u * 32 + lane;
-      v[u] = c < nvec ? x[t * nvec + c] : V::zero();
-    }
+    for (int u = 0; u < kUnroll; ++u) v[u] = c0 + u * P < nvec ? x[t * nvec + c0 + u * P] : V::zero();
     for (int64_t j = 0; j < k; ++j) {
       const int64_t r = slot[t * k + j];
       if (r < 0 || r >= num_rows) continue;
 #pragma unroll
-      for (int u = 0; u < kUnroll; ++u) {
-        const int64_t c = c0 + u * 32 + lane;
-        if (c < nvec) rows[r * nvec + c] = v[u];
-      }
+      for (int u = 0; u < kUnroll; ++u)
+        if (c0 + u * P < nvec) rows[r * nvec + c0 + u * P] = v[u];
     }
   }
 }
 
-template <int VEC>
+template <int VEC, int P>
 __global__ void __launch_bounds__(256) combine_kernel(typename Vec<VEC>::T *__restrict__ out,
                                                       const typename Vec<VEC>::T *__restrict__ rows,
                                                       const float *__restrict__ weights,
@@ -569,10 +574,12 @@ __global__ void __launch_bounds__(256) combine_kernel(typename Vec<VEC>::T *__re
                                                       int64_t num_rows, int64_t nvec, int64_t chunks) {
   using V = Vec<VEC>;
   pdl_wait();
-  const int lane = threadIdx.x & 31;
-  const int64_t work = tokens * chunks, warps = (int64_t)gridDim.x * (blockDim.x >> 5);
+  constexpr int kTeams = 32 / P;
+  const int lane = threadIdx.x & 31, sub = lane % P;
+  const int64_t work = (tokens * chunks + kTeams - 1) / kTeams, warps = (int64_t)gridDim.x * (blockDim.x >> 5);
   for (int64_t p = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); p < work; p += warps) {
-    const int64_t t = p / chunks, c0 = (p - t * chunks) * 32 * kUnroll;
+    const int64_t piece = p * kTeams + lane / P, t = piece / chunks, c0 = (piece - t * chunks) * P * kUnroll + sub;
+    if (t >= tokens) continue;
     typename V::T acc[kUnroll];
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) acc[u] = V::zero();
@@ -581,46 +588,45 @@ __global__ void __launch_bounds__(256) combine_kernel(typename Vec<VEC>::T *__re
       if (r < 0 || r >= num_rows) continue;
       const float w = weights ? weights[t * k + j] : 1.0f;
 #pragma unroll
-      for (int u = 0; u < kUnroll; ++u) {
-        const int64_t c = c0 + u * 32 + lane;
-        if (c < nvec) acc[u] = V::fma(w, rows[r * nvec + c], acc[u]);
-      }
+      for (int u = 0; u < kUnroll; ++u)
+        if (c0 + u * P < nvec) acc[u] = V::fma(w, rows[r * nvec + c0 + u * P], acc[u]);
     }
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      const int64_t c = c0 + u * 32 + lane;
-      if (c < nvec) out[t * nvec + c] = acc[u];
-    }
+    for (int u = 0; u < kUnroll; ++u)
+      if (c0 + u * P < nvec) out[t * nvec + c0 + u * P] = acc[u];
   }
 }
 
-// A warp takes one choice: its row of drows and its dweight.
-template <int VEC>
+// A team takes one choice: its row of drows and its dweight.
+template <int VEC, int P>
 __global__ void __launch_bounds__(256) combine_backward_kernel(
     typename Vec<VEC>::T *__restrict__ drows, float *__restrict__ dweights,
     const typename Vec<VEC>::T *__restrict__ dout, const typename Vec<VEC>::T *__restrict__ rows,
     const float *__restrict__ weights, const int32_t *__restrict__ slot, const int32_t *__restrict__ src,
-    int64_t tokens, int64_t k, int64_t num_rows, int64_t nvec, int64_t chunks) {
+    int64_t tokens, int64_t k, int64_t num_rows, int64_t nvec) {
   using V = Vec<VEC>;
   pdl_wait();
-  const int lane = threadIdx.x & 31;
-  const int64_t work = tokens * k, all = work + (num_rows + 31) / 32 * chunks;
+  constexpr int kTeams = 32 / P;
+  const int lane = threadIdx.x & 31, sub = lane % P;
+  const int64_t choices = tokens * k, work = (choices + kTeams - 1) / kTeams;
+  const int64_t zero_chunks = (nvec + 32 * kUnroll - 1) / (32 * kUnroll);
+  const int64_t all = work + (num_rows + 31) / 32 * zero_chunks;
   const int64_t warps = (int64_t)gridDim.x * (blockDim.x >> 5);
   for (int64_t p = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); p < all; p += warps) {
     if (p >= work) {
-      const int64_t q = p - work, g = q / chunks;
-      zero_empty<VEC>(drows, src, g * 32, num_rows, nvec, (q - g * chunks) * 32 * kUnroll, lane);
+      const int64_t q = p - work, g = q / zero_chunks;
+      zero_empty<VEC>(drows, src, g * 32, num_rows, nvec, (q - g * zero_chunks) * 32 * kUnroll, lane);
       continue;
     }
-    const int64_t r = slot[p];
+    const int64_t choice = p * kTeams + lane / P, r = choice < choices ? slot[choice] : -1;
     float s = 0.0f;
     if (r >= 0 && r < num_rows) {
-      const float w = weights ? weights[p] : 1.0f;
-      const typename V::T *g = dout + p / k * nvec;
-      for (int64_t c0 = 0; c0 < nvec; c0 += 32 * kUnroll) {
+      const float w = weights ? weights[choice] : 1.0f;
+      const typename V::T *g = dout + choice / k * nvec;
+      for (int64_t c0 = sub; c0 < nvec; c0 += P * kUnroll) {
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u) {
-          const int64_t c = c0 + u * 32 + lane;
+          const int64_t c = c0 + u * P;
           if (c < nvec) {
             const typename V::T d = g[c];
             if (dweights) s = V::dot(d, rows[r * nvec + c], s);
@@ -630,8 +636,9 @@ __global__ void __launch_bounds__(256) combine_backward_kernel(
       }
     }
     if (dweights) {
-      s = warp_sum(s);
-      if (lane == 0) dweights[p] = s;
+#pragma unroll
+      for (int d = P / 2; d > 0; d >>= 1) s = __fadd_rn(s, __shfl_xor_sync(kFull, s, d));
+      if (sub == 0 && choice < choices) dweights[choice] = s;
     }
   }
 }
@@ -646,11 +653,21 @@ int check_rows(const char *who, int64_t tokens, int64_t k, int64_t num_rows, int
   return FZ_OK;
 }
 
-template <int VEC>
-int64_t chunks_of(int64_t width) {
-  const int64_t per = (int64_t)32 * kUnroll * VEC;
-  return (width + per - 1) / per;
+// Lanes a row of nvec vectors, and f(Lanes<P>) for them.
+template <int P>
+struct Lanes {
+  static constexpr int value = P;
+};
+template <class F>
+int with_lanes(int64_t nvec, F f) {
+  if (nvec <= 2 * kUnroll) return f(Lanes<2>{});
+  if (nvec <= 8 * kUnroll) return f(Lanes<8>{});
+  return f(Lanes<32>{});
 }
+int64_t chunks_of(int64_t nvec, int lanes) { return (nvec + lanes * kUnroll - 1) / (lanes * kUnroll); }
+// Pieces of `tokens` rows for warps, and of the rows that may be empty.
+int64_t warp_pieces(int64_t tokens, int64_t chunks, int lanes) { return (tokens * chunks * lanes + 31) / 32; }
+int64_t zero_pieces(int64_t num_rows, int64_t nvec) { return (num_rows + 31) / 32 * chunks_of(nvec, 32); }
 
 unsigned warps_grid(int64_t pieces) { return fz::grid_for(pieces, 8, 8, 4); }
 
@@ -783,18 +800,20 @@ extern "C" int fz_expert_dispatch(float *rows, const float *x, const int32_t *sl
   if (num_rows == 0 || width == 0) return FZ_OK;
   FZ_REQUIRE(rows && src && (tokens == 0 || (x && slot)), "fz_expert_dispatch: null pointer");
   cudaStream_t s = fz::resolve(stream);
-  const int64_t groups = (num_rows + 31) / 32;
-  if (width % 4 == 0 && aligned16(rows, x)) {
-    const int64_t chunks = chunks_of<4>(width);
-    FZ_CUDA(fz::launch_pdl(dispatch_kernel<4>, dim3(warps_grid((tokens + groups) * chunks)), dim3(256), 0, s,
-                           (float4 *)rows, (const float4 *)x, slot, src, tokens, k, num_rows, width / 4, chunks));
-  } else {
-    const int64_t chunks = chunks_of<1>(width);
-    FZ_CUDA(fz::launch_pdl(dispatch_kernel<1>, dim3(warps_grid((tokens + groups) * chunks)), dim3(256), 0, s,
-                           rows, x, slot, src, tokens, k, num_rows, width, chunks));
-  }
-  FZ_CHECK_LAUNCH();
-  return FZ_OK;
+  const auto launch = [&](auto vec, int64_t nvec) {
+    constexpr int kVec = decltype(vec)::value;
+    using T = typename Vec<kVec>::T;
+    return with_lanes(nvec, [&](auto lanes) {
+      constexpr int P = decltype(lanes)::value;
+      const int64_t chunks = chunks_of(nvec, P);
+      const unsigned grid = warps_grid(warp_pieces(tokens, chunks, P) + zero_pieces(num_rows, nvec));
+      FZ_CUDA(fz::launch_pdl(dispatch_kernel<kVec, P>, dim3(grid), dim3(256), 0, s, (T *)rows, (const T *)x, slot,
+                             src, tokens, k, num_rows, nvec, chunks));
+      FZ_CHECK_LAUNCH();
+      return (int)FZ_OK;
+    });
+  };
+  return width % 4 == 0 && aligned16(rows, x) ? launch(Lanes<4>{}, width / 4) : launch(Lanes<1>{}, width);
 }
 
 extern "C" int fz_expert_combine(float *out, const float *rows, const float *weights, const int32_t *slot,
@@ -803,17 +822,19 @@ extern "C" int fz_expert_combine(float *out, const float *rows, const float *wei
   if (tokens == 0 || width == 0) return FZ_OK;
   FZ_REQUIRE(out && slot && (num_rows == 0 || rows), "fz_expert_combine: null pointer");
   cudaStream_t s = fz::resolve(stream);
-  if (width % 4 == 0 && aligned16(out, rows)) {
-    const int64_t chunks = chunks_of<4>(width);
-    FZ_CUDA(fz::launch_pdl(combine_kernel<4>, dim3(warps_grid(tokens * chunks)), dim3(256), 0, s, (float4 *)out,
-                           (const float4 *)rows, weights, slot, tokens, k, num_rows, width / 4, chunks));
-  } else {
-    const int64_t chunks = chunks_of<1>(width);
-    FZ_CUDA(fz::launch_pdl(combine_kernel<1>, dim3(warps_grid(tokens * chunks)), dim3(256), 0, s, out, rows,
-                           weights, slot, tokens, k, num_rows, width, chunks));
-  }
-  FZ_CHECK_LAUNCH();
-  return FZ_OK;
+  const auto launch = [&](auto vec, int64_t nvec) {
+    constexpr int kVec = decltype(vec)::value;
+    using T = typename Vec<kVec>::T;
+    return with_lanes(nvec, [&](auto lanes) {
+      constexpr int P = decltype(lanes)::value;
+      const int64_t chunks = chunks_of(nvec, P);
+      FZ_CUDA(fz::launch_pdl(combine_kernel<kVec, P>, dim3(warps_grid(warp_pieces(tokens, chunks, P))), dim3(256), 0,
+                             s, (T *)out, (const T *)rows, weights, slot, tokens, k, num_rows, nvec, chunks));
+      FZ_CHECK_LAUNCH();
+      return (int)FZ_OK;
+    });
+  };
+  return width % 4 == 0 && aligned16(out, rows) ? launch(Lanes<4>{}, width / 4) : launch(Lanes<1>{}, width);
 }
 
 extern "C" int fz_expert_combine_backward(float *drows, float *dweights, const float *dout, const float *rows,
@@ -827,18 +848,17 @@ extern "C" int fz_expert_combine_backward(float *drows, float *dweights, const f
                  (!dweights || !data || tokens == 0 || rows),
              "fz_expert_combine_backward: null pointer");
   cudaStream_t s = fz::resolve(stream);
-  const int64_t groups = (num_rows + 31) / 32;
-  if (width % 4 == 0 && aligned16(drows, dout, rows)) {
-    const int64_t chunks = chunks_of<4>(width);
-    FZ_CUDA(fz::launch_pdl(combine_backward_kernel<4>, dim3(warps_grid(tokens * k + groups * chunks)), dim3(256),
-                           0, s, (float4 *)drows, dweights, (const float4 *)dout, (const float4 *)rows, weights,
-                           slot, src, tokens, k, num_rows, width / 4, chunks));
-  } else {
-    const int64_t chunks = chunks_of<1>(width);
-    FZ_CUDA(fz::launch_pdl(combine_backward_kernel<1>, dim3(warps_grid(tokens * k + groups * chunks)), dim3(256),
-                           0, s, drows, dweights, dout, rows, weights, slot, src, tokens, k, num_rows, width,
-                           chunks));
-  }
-  FZ_CHECK_LAUNCH();
-  return FZ_OK;
+  const auto launch = [&](auto vec, int64_t nvec) {
+    constexpr int kVec = decltype(vec)::value;
+    using T = typename Vec<kVec>::T;
+    return with_lanes(nvec, [&](auto lanes) {
+      constexpr int P = decltype(lanes)::value;
+      const unsigned grid = warps_grid(warp_pieces(tokens * k, 1, P) + zero_pieces(num_rows, nvec));
+      FZ_CUDA(fz::launch_pdl(combine_backward_kernel<kVec, P>, dim3(grid), dim3(256), 0, s, (T *)drows, dweights,
+                             (const T *)dout, (const T *)rows, weights, slot, src, tokens, k, num_rows, nvec));
+      FZ_CHECK_LAUNCH();
+      return (int)FZ_OK;
+    });
+  };
+  return width % 4 == 0 && aligned16(drows, dout, rows) ? launch(Lanes<4>{}, width / 4) : launch(Lanes<1>{}, width);
 }
