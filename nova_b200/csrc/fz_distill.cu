@@ -12,6 +12,10 @@
 // lowest value, costs no digits.
 // The backward streams the row once more, writing dz from the saved statistics, and then
 // overwrites the entries' columns.
+// Measured (B200, copy bandwidth 6.55 TB/s), 64 entries a row: 4096 rows of 131072, forward
+// 324 us (1.01 of the copy bandwidth), backward 660 us (0.99); 2048 rows of 50001 (no two
+// alike aligned) 80 and 141 us (0.78, 0.89: the last wave of CTAs and their fixed cost); 8192
+// rows of 2000, a warp each, 21 and 29 us (90 and 91 with a CTA of 512 threads a row).
 #include <cooperative_groups.h>
 
 #include <climits>
@@ -438,7 +442,8 @@ int check_distill(const char *who, int64_t rows, int64_t vocab, int64_t k, int64
   FZ_REQUIRE(k <= FZ_MAX_TEACHER, name + ": more than FZ_MAX_TEACHER entries");
   FZ_REQUIRE(ld >= vocab, name + ": row pitch below vocab");
   FZ_REQUIRE(rows <= INT_MAX / 8, name + ": too many rows");
-  FZ_REQUIRE(temperature > 0.0f && temperature < INFINITY, name + ": temperature must be positive and finite");
+  // (its square, the loss's factor, has to be a normal number)
+  FZ_REQUIRE(temperature >= 1e-18f && temperature < INFINITY, name + ": temperature must be in [1e-18, inf)");
   return FZ_OK;
 }
 

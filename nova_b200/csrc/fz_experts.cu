@@ -2,6 +2,10 @@
 // gradients. All are bound by memory (or, for a handful of tokens, by launch latency):
 // every kernel reads its inputs once and writes its outputs once, with no atomics on
 // floating-point values, so results do not depend on scheduling.
+// Measured (B200, copy bandwidth 6.55 TB/s): router, 65536 tokens, 256 experts, 8 picks, all
+// logits normalised: 32 us (0.34 of the copy bandwidth: instruction issue), backward 28 us
+// (0.77). 16384 tokens of 4096 floats, 4 of 64 experts, capacity 1280: sort 12 us (latency of
+// its three steps), dispatch 268 us (0.92), combine 178 us, its backward 426 us (0.96).
 #include <cooperative_groups.h>
 
 #include <climits>
