@@ -9,7 +9,12 @@
 //     allows) is held by 4 to 32 lanes of a warp, of at most 2048 vectors by a CTA;
 //   * tile kernels: a tile of rows x columns (several whole groups wide, or a part of
 //     one) a CTA; the tiles of a team exchange their statistics through distributed
-//     shared memory in one cluster, of up to 16 CTAs;
+//     shared memory in one cluster, of up to 16 CTAs. Where c is odd but a row of channels
+//     is whole vectors, they may lie across two groups ("mixed": statistics per channel,
+//     two groups' values spread over a vector). Against single floats, SiLU, forward and
+//     backward: [64, 1024, 264] / 8 104 -> 69 and 214 -> 141 us, [64, 1024, 120] / 8
+//     32 -> 24 and 55 -> 34 us. Where c is 2 modulo 4 the vectors are of 2: mixed ones of 4
+//     took 27 and 40 us against 21 and 38 at [16, 1369, 320] / 32;
 //   * larger teams: the tile kernels in two launches that leave the statistics in the
 //     workspace and read x (and dy) twice; the second launch takes the tiles in reverse,
 //     so it finds the last of what the first read in L2. (Taking the batch a few samples at
@@ -17,9 +22,9 @@
 //     [8, 16384, 512] 205 against 161 us.)
 // Measured (B200, copy bandwidth 6.55 TB/s): rows, [65536, 4096] in 32 groups, GELU: forward
 // 378 us, backward 563 us (0.87 of the copy bandwidth both). Clusters, [64, 4096, 256] in 32
-// groups, SiLU: forward 100 us (0.82), backward 198 us (0.62: the tiles of x and dy fill the
-// registers, and a cluster's CTAs wait for one another). Two launches, [8, 16384, 512]: 161
-// and 264 us. A first version with one CTA a team, reading x three times: 566 us for the
+// groups, SiLU: forward 100 us (0.82), backward 211 us (0.58: the tiles of x and dy fill the
+// registers, and a cluster's CTAs wait for one another). Two launches, [8, 16384, 512]: 158
+// and 250 us. A first version with one CTA a team, reading x three times: 566 us for the
 // maps' forward, 16.6 ms for the rows' two passes.
 // Statistics: the mean, then the sum of squares about it, so that a common offset of x
 // does not cancel; parts are joined as (n, mean, M2) (Chan, Golub and LeVeque). Everything
@@ -185,8 +190,9 @@ struct Vec {
 template <int V>
 __device__ __forceinline__ Vec<V> splat(float a) {
   Vec<V> r;
+  const Pair p = V == 1 ? pair(a, 0.0f) : both(a);
 #pragma unroll
-  for (int i = 0; i < Vec<V>::N; ++i) r.p[i] = V == 1 ? pair(a, 0.0f) : both(a);
+  for (int i = 0; i < Vec<V>::N; ++i) r.p[i] = p;
   return r;
 }
 template <int V>
@@ -251,30 +257,30 @@ __device__ __forceinline__ void sum_into(Vec<V> &s, const Vec<V> &x) {
   for (int i = 0; i < Vec<V>::N; ++i) s.p[i] = add2(s.p[i], x.p[i]);
 }
 template <int V>
-__device__ __forceinline__ void square_into(Vec<V> &s, const Vec<V> &x, Pair minus_mean) {
+__device__ __forceinline__ void square_into(Vec<V> &s, const Vec<V> &x, const Vec<V> &minus_mean) {
 #pragma unroll
   for (int i = 0; i < Vec<V>::N; ++i) {
-    const Pair d = add2(x.p[i], minus_mean);
+    const Pair d = add2(x.p[i], minus_mean.p[i]);
     s.p[i] = fma2(d, d, s.p[i]);
   }
 }
 // act(gamma (x - mean) rstd + beta)
 template <int ACT, int V>
-__device__ __forceinline__ Vec<V> normalize(const Vec<V> &x, Pair minus_mean, Pair rstd, const Vec<V> &gamma,
-                                            const Vec<V> &beta) {
+__device__ __forceinline__ Vec<V> normalize(const Vec<V> &x, const Vec<V> &minus_mean, const Vec<V> &rstd,
+                                            const Vec<V> &gamma, const Vec<V> &beta) {
   Vec<V> r;
 #pragma unroll
   for (int i = 0; i < Vec<V>::N; ++i)
-    r.p[i] = activate2<ACT>(fma2(mul2(add2(x.p[i], minus_mean), rstd), gamma.p[i], beta.p[i]));
+    r.p[i] = activate2<ACT>(fma2(mul2(add2(x.p[i], minus_mean.p[i]), rstd.p[i]), gamma.p[i], beta.p[i]));
   return r;
 }
 // x <- xh, d <- dv gamma; dv and dv xh are added to db and dg
 template <int ACT, int V>
-__device__ __forceinline__ void gradient(Vec<V> &x, Vec<V> &d, Vec<V> &db, Vec<V> &dg, Pair minus_mean, Pair rstd,
-                                         const Vec<V> &gamma, const Vec<V> &beta) {
+__device__ __forceinline__ void gradient(Vec<V> &x, Vec<V> &d, Vec<V> &db, Vec<V> &dg, const Vec<V> &minus_mean,
+                                         const Vec<V> &rstd, const Vec<V> &gamma, const Vec<V> &beta) {
 #pragma unroll
   for (int i = 0; i < Vec<V>::N; ++i) {
-    x.p[i] = mul2(add2(x.p[i], minus_mean), rstd);
+    x.p[i] = mul2(add2(x.p[i], minus_mean.p[i]), rstd.p[i]);
     const Pair dv = times_slope2<ACT>(d.p[i], fma2(x.p[i], gamma.p[i], beta.p[i]));
     db.p[i] = add2(db.p[i], dv);
     dg.p[i] = fma2(dv, x.p[i], dg.p[i]);
@@ -283,10 +289,12 @@ __device__ __forceinline__ void gradient(Vec<V> &x, Vec<V> &d, Vec<V> &db, Vec<V
 }
 // rstd (d - k1 - xh k2)
 template <int V>
-__device__ __forceinline__ Vec<V> finish(const Vec<V> &xh, const Vec<V> &d, Pair minus_k1, Pair minus_k2, Pair rstd) {
+__device__ __forceinline__ Vec<V> finish(const Vec<V> &xh, const Vec<V> &d, const Vec<V> &minus_k1,
+                                         const Vec<V> &minus_k2, const Vec<V> &rstd) {
   Vec<V> r;
 #pragma unroll
-  for (int i = 0; i < Vec<V>::N; ++i) r.p[i] = mul2(rstd, fma2(xh.p[i], minus_k2, add2(d.p[i], minus_k1)));
+  for (int i = 0; i < Vec<V>::N; ++i)
+    r.p[i] = mul2(rstd.p[i], fma2(xh.p[i], minus_k2.p[i], add2(d.p[i], minus_k1.p[i])));
   return r;
 }
 
@@ -457,7 +465,7 @@ __global__ void __launch_bounds__(kRowThreads, row_ctas(false, NV)) norm_rows_ke
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       Vec<V> q = splat<V>(0.0f);
-      const Pair minus = V == 1 ? pair(-mean[u], 0.0f) : both(-mean[u]);
+      const Vec<V> minus = splat<V>(-mean[u]);
 #pragma unroll
       for (int i = 0; i < NV; ++i)
         if (t.at[i] >= 0) square_into(q, x[u][i], minus);
@@ -474,7 +482,7 @@ __global__ void __launch_bounds__(kRowThreads, row_ctas(false, NV)) norm_rows_ke
               Vec<V> ga, be;
               affine.get(a, t.channel, i, ga, be);
               store(to + u * hop + t.at[i],
-                    normalize<decltype(act)::value>(x[u][i], both(-mean[u]), both(rstd[u]), ga, be));
+                    normalize<decltype(act)::value>(x[u][i], splat<V>(-mean[u]), splat<V>(rstd[u]), ga, be));
             }
         }
       }
@@ -543,11 +551,11 @@ __global__ void __launch_bounds__(kRowThreads, row_ctas(true, NV))
     const int b = b0 + t.part;
     Vec<V> x[U][NV], d[U][NV];
     float rstd[U], s1[U], s2[U];
-    Pair minus[U];
+    float minus[U];
     copy_wait<S - 1>();
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      minus[u] = both(-next_mean[u]);
+      minus[u] = -next_mean[u];
       rstd[u] = next_rstd[u];
       s1[u] = s2[u] = 0.0f;
 #pragma unroll
@@ -568,7 +576,7 @@ __global__ void __launch_bounds__(kRowThreads, row_ctas(true, NV))
 #pragma unroll
         for (int u = 0; u < U; ++u) {
           // behind the batch x, d, mean and rstd are 0, and so is all that they give
-          gradient<decltype(act)::value>(x[u][i], d[u][i], b_sum, g_sum, minus[u], both(rstd[u]), ga, be);
+          gradient<decltype(act)::value>(x[u][i], d[u][i], b_sum, g_sum, splat<V>(minus[u]), splat<V>(rstd[u]), ga, be);
           Vec<V> w;
 #pragma unroll
           for (int j = 0; j < Vec<V>::N; ++j) w.p[j] = mul2(d[u][i].p[j], x[u][i].p[j]);
@@ -588,7 +596,7 @@ __global__ void __launch_bounds__(kRowThreads, row_ctas(true, NV))
 #pragma unroll
         for (int i = 0; i < NV; ++i)
           if (t.at[i] >= 0)
-            store(to + t.at[i], finish(x[u][i], d[u][i], both(s1[u]), both(s2[u]), both(rstd[u])));
+            store(to + t.at[i], finish(x[u][i], d[u][i], splat<V>(s1[u]), splat<V>(s2[u]), splat<V>(rstd[u])));
       to += hop;
     }
   }
@@ -648,14 +656,41 @@ struct Tile {
   int b, chunk, k;
   int g0, q, cols;  // its first group, its groups, its vectors a row
   int rows, mine;   // its rows, and those of this thread (0: none)
-  int most;         // rows of the thread that has most: what runs for all skips only behind it
+  int most;         // rows of the thread that has most
   int channel;      // this thread's first channel
   int64_t at;       // offset of this thread's first vector
 };
 
+// The groups (counted from the tile's first) of a thread's vector: values before `from` belong
+// to lo, the others to hi. Only mixed vectors (V = 4, c >= 3) have two.
+template <int V, bool MIXED>
+struct Place {
+  int lo, hi, from;
+  __device__ Place(const Norm &a, const Tiling &t, int tx) {
+    if (MIXED) {
+      lo = tx * V / a.c;
+      hi = (tx * V + V - 1) / a.c;
+      from = hi * a.c - tx * V;  // 0 or less: the whole vector is hi's
+    } else {
+      lo = hi = t.split > 1 ? 0 : tx / (a.c / V);
+      from = V;
+    }
+  }
+  __device__ __forceinline__ Vec<V> spread(float l, float h) const {
+    if constexpr (MIXED) {
+      Vec<V> r;
+      r.p[0] = pair(0 < from ? l : h, 1 < from ? l : h);
+      r.p[Vec<V>::N - 1] = pair(2 < from ? l : h, 3 < from ? l : h);
+      return r;
+    } else {
+      return splat<V>(l);
+    }
+  }
+};
+
 // A CTA's walk over the tiles: (b, bundle, share) counted in mixed radix, since a division
 // a tile costs as much as a good part of its arithmetic. kWhole walks from the last tile.
-template <int V, int MODE>
+template <int V, int MODE, bool MIXED>
 struct Walk {
   int b, bundle, share, db, dbundle, dshare, left;
   int tx, ty, shift;  // thread column and row, log2 of the thread rows
@@ -691,14 +726,14 @@ struct Walk {
   __device__ Tile<V> get(const Norm &a, const Tiling &t) const {
     Tile<V> r;
     const bool back = MODE == kWhole;
-    const int cv = a.c / V, at = back ? t.bundles - 1 - bundle : bundle;
+    const int at = back ? t.bundles - 1 - bundle : bundle;
     r.b = back ? (int)a.batch - 1 - b : b;
     r.k = back ? t.k - 1 - share : share;
     r.chunk = t.split > 1 ? r.k / t.split : r.k;
     const int piece = r.k - r.chunk * t.split;
     r.g0 = at * t.q;
     r.q = min(t.q, a.groups - r.g0);
-    r.cols = t.split > 1 ? min(t.cols, cv - piece * t.cols) : r.q * cv;
+    r.cols = t.split > 1 ? min(t.cols, a.c / V - piece * t.cols) : MIXED ? r.q * a.c / V : r.q * (a.c / V);
     const int64_t row0 = (int64_t)r.chunk * t.rows;
     r.rows = (int)min((int64_t)t.rows, a.len - row0);
     r.channel = r.g0 * a.c + (piece * t.cols + tx) * V;
@@ -717,12 +752,24 @@ __device__ __forceinline__ float count_of(const Norm &a, const Tiling &t, int k)
   return rows * (float)(t.split > 1 ? min(t.cols, a.c / V - piece * t.cols) * V : a.c);
 }
 
+// The loops over a thread's rows end, four rows at a time, behind the tile's last, so that a
+// short tile costs what it has: [2048, 64, 40] / 4, vectors of 2, forward 57 -> 40 us, backward
+// 69 -> 44 us; [16, 1369, 320] / 32, backward 38 -> 35 us (full tiles, [64, 4096, 256] / 32:
+// 204 -> 211 us). A forward of vectors of 4 runs all of its rows: with the branches between its
+// loads and sums, full tiles took 105.7 us instead of 102.0.
+template <int V, int N>
+__device__ __forceinline__ bool behind(int i, const Tile<V> &me) {
+  return (V < 4 || N < held(4, false)) && i % 4 == 0 && i >= me.most;
+}
+
 // A tile's vectors to a thread's place in shared memory ([held][threads] vectors), and back.
+// Behind a thread's rows x is 0.
 template <int V, int N>
 __device__ __forceinline__ void fetch_tile(float *fifo, const float *p, const Tile<V> &me, int64_t step) {
   const float *q = p + me.at;
 #pragma unroll
   for (int i = 0; i < N; ++i) {
+    if (behind<V, N>(i, me)) break;
     if (i < me.mine) copy_async<V>(fifo + (i * kTileThreads + (int)threadIdx.x) * V, q);
     q += step;
   }
@@ -730,8 +777,10 @@ __device__ __forceinline__ void fetch_tile(float *fifo, const float *p, const Ti
 template <int V, int N>
 __device__ __forceinline__ void take_tile(Vec<V> (&x)[N], const float *fifo, const Tile<V> &me) {
 #pragma unroll
-  for (int i = 0; i < N; ++i)
+  for (int i = 0; i < N; ++i) {
+    if (behind<V, N>(i, me)) break;
     x[i] = i < me.mine ? load<V>(fifo + (i * kTileThreads + (int)threadIdx.x) * V) : splat<V>(0.0f);
+  }
 }
 
 __device__ __forceinline__ float warp_sum(float v) {
@@ -754,47 +803,82 @@ __device__ __forceinline__ int rows_of_slice(int y, int rows, int wide, int shif
   return (rows >> shift) * tall + min(max(rest - y * tall, 0), tall);
 }
 
-// The tile's own moments. column_moments: each slice reduces a column to its mean and the sum
-// of squares about it, with a barrier at the end. group_moments: (mean, M2) of group g in
-// every lane of the warp that asks, M2 = sum of theirs + n_column (mean_column - mean)^2.
-template <int V, int N>
+// The tile's own moments. column_moments: each slice reduces a column (mixed: each of its
+// channels) to its mean and the sum of squares about it, with a barrier at the end.
+// group_moments: (mean, M2) of group g in every lane of the warp that asks, M2 = sum of theirs
+// + n_column (mean_column - mean)^2. sh: [slices][wide] columns, mixed [slices][wide * V].
+template <int V, bool MIXED, int N>
 __device__ __forceinline__ void column_moments(const Vec<V> (&x)[N], float2 *sh, const Tile<V> &me, const Tiling &t,
                                                int shift) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int slice = t.wide < 32 ? warp : (int)threadIdx.x / t.wide;
   Vec<V> s = x[0];
 #pragma unroll
-  for (int i = 1; i < N; ++i) sum_into(s, x[i]);
-  const float n = (float)(rows_of_slice(slice, me.rows, t.wide, shift) * V);
-  const float mean = __fdiv_rn(over_rows(total(s), t.wide), n);  // n = 0: not read
-  const Pair minus = V == 1 ? pair(-mean, 0.0f) : both(-mean);
-  s = splat<V>(0.0f);
+  for (int i = 1; i < N; ++i) {
+    if (behind<V, N>(i, me)) break;
+    sum_into(s, x[i]);
+  }
+  const int rows = rows_of_slice(slice, me.rows, t.wide, shift);  // 0: nothing of this slice is read
+  const int at = t.wide < 32 ? warp * t.wide + lane : (int)threadIdx.x;
+  const bool puts = t.wide >= 32 || lane < t.wide;
+  if constexpr (MIXED) {
+    float mean[4], m2[4];
+    unpair(s.p[0], mean[0], mean[1]);
+    unpair(s.p[Vec<V>::N - 1], mean[2], mean[3]);
 #pragma unroll
-  for (int i = 0; i < N; ++i)
-    if (i < me.mine) square_into(s, x[i], minus);
-  const float m2 = over_rows(total(s), t.wide);
-  if (t.wide >= 32) sh[threadIdx.x] = make_float2(mean, m2);
-  else if (lane < t.wide) sh[warp * t.wide + lane] = make_float2(mean, m2);
+    for (int j = 0; j < 4; ++j) mean[j] = __fdiv_rn(over_rows(mean[j], t.wide), (float)rows);
+    Vec<V> minus;
+    minus.p[0] = pair(-mean[0], -mean[1]);
+    minus.p[Vec<V>::N - 1] = pair(-mean[2], -mean[3]);
+    s = splat<V>(0.0f);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      if (behind<V, N>(i, me)) break;
+      if (i < me.mine) square_into(s, x[i], minus);
+    }
+    unpair(s.p[0], m2[0], m2[1]);
+    unpair(s.p[Vec<V>::N - 1], m2[2], m2[3]);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) m2[j] = over_rows(m2[j], t.wide);
+    if (puts) {
+      float4 *q = reinterpret_cast<float4 *>(sh + at * 4);
+      q[0] = make_float4(mean[0], m2[0], mean[1], m2[1]);
+      q[1] = make_float4(mean[2], m2[2], mean[3], m2[3]);
+    }
+  } else {
+    const float mean = __fdiv_rn(over_rows(total(s), t.wide), (float)(rows * V));
+    const Vec<V> minus = splat<V>(-mean);
+    s = splat<V>(0.0f);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      if (behind<V, N>(i, me)) break;
+      if (i < me.mine) square_into(s, x[i], minus);
+    }
+    const float m2 = over_rows(total(s), t.wide);
+    if (puts) sh[at] = make_float2(mean, m2);
+  }
   __syncthreads();
 }
-template <int V>
+template <int V, bool MIXED>
 __device__ __forceinline__ float2 group_moments(const float2 *sh, int g, const Norm &a, const Tile<V> &me,
                                                 const Tiling &t, int shift) {
-  const int lane = threadIdx.x & 31, cv = a.c / V, width = t.split > 1 ? me.cols : cv;
+  constexpr int kEach = MIXED ? 1 : V;  // values a row that an entry of sh stands for
+  const int lane = threadIdx.x & 31, row = MIXED ? t.wide * V : t.wide;
+  const int per = MIXED ? a.c : a.c / V, width = t.split > 1 ? me.cols : per;
   const int total = slices_of(t.wide) * width, dy = 32 / width, dc = 32 - dy * width;
   const int y0 = lane / width, c0 = lane - y0 * width;
   float u = 0.0f, w = 0.0f;
   for (int i = lane, y = y0, c = c0; i < total; i += 32) {
-    const int n = rows_of_slice(y, me.rows, t.wide, shift) * V;
-    if (n) u = __fmaf_rn((float)n, sh[y * t.wide + g * cv + c].x, u);
+    const int n = rows_of_slice(y, me.rows, t.wide, shift) * kEach;
+    if (n) u = __fmaf_rn((float)n, sh[y * row + g * per + c].x, u);
     y += dy, c += dc;
     if (c >= width) c -= width, ++y;
   }
-  const float mean = __fdiv_rn(warp_sum(u), (float)me.rows * (float)(width * V));
+  const float mean = __fdiv_rn(warp_sum(u), (float)me.rows * (float)(width * kEach));
   for (int i = lane, y = y0, c = c0; i < total; i += 32) {
-    const int n = rows_of_slice(y, me.rows, t.wide, shift) * V;
+    const int n = rows_of_slice(y, me.rows, t.wide, shift) * kEach;
     if (n) {
-      const float2 p = sh[y * t.wide + g * cv + c];
+      const float2 p = sh[y * row + g * per + c];
       const float d = __fsub_rn(p.x, mean);
       w = __fadd_rn(w, __fmaf_rn(__fmul_rn(d, d), (float)n, p.y));
     }
@@ -876,26 +960,26 @@ __device__ __forceinline__ void exchange_wait(Exchange &x, int parity, int phase
   }
 }
 
-template <int V, int MODE>
+template <int V, int MODE, bool MIXED>
 __global__ void __launch_bounds__(kTileThreads, kTileCtas) norm_tile_kernel(const Norm a, const Tiling t) {
   pdl_wait();
   constexpr int N = held(V, false);
   cg::cluster_group cluster = cg::this_cluster();
   extern __shared__ __align__(16) float fifo[];
-  __shared__ float2 sh[kTileThreads];
+  __shared__ __align__(16) float2 sh[kTileThreads * (MIXED ? V : 1)];
   // by parity of the tile: a warp may be a tile ahead of one that still reads
   __shared__ float2 stats_by[2][kMaxTileGroups];
   __shared__ Exchange exchange;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, cv = a.c / V;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const bool joined = MODE == kInCluster && t.k > 1;
-  Walk<V, MODE> walk(t, MODE == kInCluster ? (int)cluster.block_rank() : 0);
+  Walk<V, MODE, MIXED> walk(t, MODE == kInCluster ? (int)cluster.block_rank() : 0);
   if (joined) {
     exchange_init(exchange);
     __syncthreads();
     cluster.barrier_arrive();
   }
   const int64_t step = (int64_t)(kTileThreads / t.wide) * a.channels;
-  const int column = t.split > 1 ? 0 : walk.tx / cv;  // this thread's group in the tile
+  const Place<V, MIXED> place(a, t, walk.tx);
   const float share = joined && lane < t.k ? count_of<V>(a, t, lane) : 0.0f;
   Tile<V> me, next;
   if (walk.left) {
@@ -916,11 +1000,11 @@ __global__ void __launch_bounds__(kTileThreads, kTileCtas) norm_tile_kernel(cons
       fetch_tile<V, N>(fifo, a.x, next, step);
     }
     copy_commit();
-    if (MODE != kWhole) column_moments(x, sh, me, t, walk.shift);
+    if (MODE != kWhole) column_moments<V, MIXED>(x, sh, me, t, walk.shift);
     if (joined) {
       if (threadIdx.x == kTileThreads - 1) exchange_expect(exchange, n, t.k * me.q * (int)sizeof(float2));
       for (int g = warp; g < me.q; g += kTileThreads / 32) {
-        const float2 m = group_moments(sh, g, a, me, t, walk.shift);
+        const float2 m = group_moments<V, MIXED>(sh, g, a, me, t, walk.shift);
         if (lane < t.k) exchange_push(exchange, n, me.k, g, lane, m);
       }
       if (warp < me.q) exchange_wait(exchange, n, i >> 1 & 1, a.err);
@@ -929,7 +1013,7 @@ __global__ void __launch_bounds__(kTileThreads, kTileCtas) norm_tile_kernel(cons
     for (int g = warp; g < me.q; g += kTileThreads / 32) {
       const int64_t team = (int64_t)me.b * a.groups + me.g0 + g;
       if (MODE == kParts) {
-        const float2 m = group_moments(sh, g, a, me, t, walk.shift);
+        const float2 m = group_moments<V, MIXED>(sh, g, a, me, t, walk.shift);
         if (lane == 0) reinterpret_cast<float2 *>(a.stat)[team * t.k + me.k] = m;
         continue;
       }
@@ -937,7 +1021,7 @@ __global__ void __launch_bounds__(kTileThreads, kTileCtas) norm_tile_kernel(cons
       if (joined) {
         r = join_lanes(share, lane < t.k ? exchange.all[n][lane][g] : make_float2(0.0f, 0.0f), a);
       } else if (MODE == kInCluster) {
-        r = group_moments(sh, g, a, me, t, walk.shift);
+        r = group_moments<V, MIXED>(sh, g, a, me, t, walk.shift);
         r.y = rstd_of(r.y, a.inv_m, a.eps);
       } else {
         const float2 *q = reinterpret_cast<const float2 *>(a.stat) + team * t.k;
@@ -960,10 +1044,10 @@ __global__ void __launch_bounds__(kTileThreads, kTileCtas) norm_tile_kernel(cons
     }
     __syncthreads();
     if (MODE != kParts) {
-      const int mine = me.mine ? column : 0;
+      const float2 lo = stats[me.mine ? place.lo : 0], hi = stats[me.mine ? place.hi : 0];
       const Vec<V> ga = load_or<V>(a.gamma && me.mine ? a.gamma + me.channel : nullptr, 1.0f);
       const Vec<V> be = load_or<V>(a.beta && me.mine ? a.beta + me.channel : nullptr, 0.0f);
-      const Pair minus = both(-stats[mine].x), rstd = both(stats[mine].y);
+      const Vec<V> minus = place.spread(-lo.x, -hi.x), rstd = place.spread(lo.y, hi.y);
       float *q = a.y + me.at;
       with_activation(a.act, [&](auto act) {
 #pragma unroll
@@ -1034,7 +1118,7 @@ __device__ __forceinline__ float2 group_sums(const float *sh, int g, const Norm 
   return make_float2(warp_sum(u), warp_sum(w));
 }
 
-template <int V, int MODE>
+template <int V, int MODE, bool MIXED>
 __global__ void __launch_bounds__(kTileThreads, kTileCtas) norm_tile_backward_kernel(const Norm a, const Tiling t) {
   pdl_wait();
   constexpr int N = held(V, true), kStage = N * kTileThreads * V;
@@ -1043,25 +1127,27 @@ __global__ void __launch_bounds__(kTileThreads, kTileCtas) norm_tile_backward_ke
   __shared__ __align__(16) float sh[2 * V * kTileThreads];
   __shared__ float2 means_by[2][kMaxTileGroups];
   __shared__ Exchange exchange;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, cv = a.c / V;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const bool joined = MODE == kInCluster && t.k > 1;
-  Walk<V, MODE> walk(t, MODE == kInCluster ? (int)cluster.block_rank() : 0);
+  Walk<V, MODE, MIXED> walk(t, MODE == kInCluster ? (int)cluster.block_rank() : 0);
   if (joined) {
     exchange_init(exchange);
     __syncthreads();
     cluster.barrier_arrive();
   }
   const int64_t step = (int64_t)(kTileThreads / t.wide) * a.channels;
-  const int column = t.split > 1 ? 0 : walk.tx / cv;
+  const Place<V, MIXED> place(a, t, walk.tx);
   Tile<V> me, next;
-  float2 stat, next_stat = make_float2(0.0f, 0.0f);  // mean and rstd of this thread's group
+  float2 lo, hi, next_lo = make_float2(0.0f, 0.0f), next_hi = next_lo;  // mean and rstd of the vector's groups
   const auto fetch = [&]() {
     if (walk.left) {
       next = walk.get(a, t);
       fetch_tile<V, N>(fifo, a.x, next, step);
       fetch_tile<V, N>(fifo + kStage, a.dy, next, step);
-      const int64_t team = (int64_t)next.b * a.groups + next.g0 + (next.mine ? column : 0);
-      next_stat = make_float2(a.mean_in[team], a.rstd_in[team]);
+      const int64_t team = (int64_t)next.b * a.groups + next.g0;
+      const int l = next.mine ? place.lo : 0, h = next.mine ? place.hi : 0;
+      next_lo = make_float2(a.mean_in[team + l], a.rstd_in[team + l]);
+      if (MIXED) next_hi = make_float2(a.mean_in[team + h], a.rstd_in[team + h]);
     }
     copy_commit();
   };
@@ -1070,23 +1156,26 @@ __global__ void __launch_bounds__(kTileThreads, kTileCtas) norm_tile_backward_ke
   for (int i = 0; walk.left; ++i) {
     const int n = i & 1;
     me = next;
-    stat = next_stat;
+    lo = next_lo;
+    hi = next_hi;
     walk.advance(t);
     Vec<V> x[N], d[N], db = splat<V>(0.0f), dg = db;
     copy_wait<0>();
     take_tile(x, fifo, me);
     take_tile(d, fifo + kStage, me);
     fetch();
-    const Pair rstd = both(stat.y);
+    const Vec<V> rstd = place.spread(lo.y, hi.y);
     {
       // behind a thread's rows x and dy are 0, and so is what they add to its columns' sums
       const Vec<V> ga = load_or<V>(a.gamma && me.mine ? a.gamma + me.channel : nullptr, 1.0f);
       const Vec<V> be = load_or<V>(a.beta && me.mine ? a.beta + me.channel : nullptr, 0.0f);
-      const Pair minus = both(-stat.x);
+      const Vec<V> minus = place.spread(-lo.x, -hi.x);
       with_activation(a.act, [&](auto act) {
 #pragma unroll
-        for (int i = 0; i < N; ++i)
-          if (i < me.most) gradient<decltype(act)::value>(x[i], d[i], db, dg, minus, rstd, ga, be);
+        for (int i = 0; i < N; ++i) {
+          if (behind<V, N>(i, me)) break;
+          gradient<decltype(act)::value>(x[i], d[i], db, dg, minus, rstd, ga, be);
+        }
       });
     }
     if (MODE != kWhole) column_sums(db, dg, sh, a, me, t, walk.tx);
@@ -1121,12 +1210,12 @@ __global__ void __launch_bounds__(kTileThreads, kTileCtas) norm_tile_backward_ke
     }
     __syncthreads();
     if (MODE != kParts) {
-      const int mine = me.mine ? column : 0;
-      const Pair k1 = both(means[mine].x), k2 = both(means[mine].y);
+      const float2 l = means[me.mine ? place.lo : 0], h = means[me.mine ? place.hi : 0];
+      const Vec<V> k1 = place.spread(l.x, h.x), k2 = place.spread(l.y, h.y);
       float *q = a.dx + me.at;
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        if (i >= me.most) break;
+        if (behind<V, N>(i, me)) break;
         const Vec<V> r = finish(x[i], d[i], k1, k2, rstd);
         if (i < me.mine) store(q, r);
         q += step;
@@ -1191,6 +1280,7 @@ struct Plan {
   unsigned grid;
   Tiling t;
   bool cluster;          // tile kernels: statistics within a cluster
+  bool mixed;            // tile kernels: vectors of 4 across groups
   int parts;             // rows of the per-channel partial sums (backward)
   int fold;              // row kernels: teams a CTA adds up
   size_t part_floats, stat_floats;
@@ -1206,13 +1296,16 @@ int64_t power_of_two(int64_t a) {
 Plan norm_plan(int64_t batch, int64_t len, int64_t channels, int64_t groups, int v, bool backward) {
   Plan p{};
   const int64_t c = channels / groups;
-  while (c % v) v /= 2;
+  // Mixed vectors where the tile kernels would move single floats. A tile then holds a
+  // multiple of 4 groups, and has at least 32 rows for its thread rows.
+  p.mixed = v == 4 && c % 2 && c >= 3 && channels % 4 == 0 && c <= kTileThreads && len >= 32 && len * c > 256;
+  while (!p.mixed && c % v) v /= 2;
   p.v = v;
   const int64_t cv = c / v, vectors = len * cv, teams = batch * groups;
   // Row kernels up to 2048 vectors; above 256 (a CTA's worth) only where a row's piece of
   // a group is at least 512 bytes, else the tile kernels, which take several groups' pieces
   // of a row together.
-  if (len * channels <= INT_MAX && (vectors <= 256 || (vectors <= 2048 && c >= 128))) {
+  if (!p.mixed && len * channels <= INT_MAX && (vectors <= 256 || (vectors <= 2048 && c >= 128))) {
     p.lanes = vectors <= 4 ? 4 : vectors <= 8 ? 8 : vectors <= 16 ? 16 : vectors <= 256 ? 32 : kRowThreads;
     p.nv = 1;
     while ((int64_t)p.nv * p.lanes < vectors) p.nv *= 2;
@@ -1235,21 +1328,22 @@ Plan norm_plan(int64_t batch, int64_t len, int64_t channels, int64_t groups, int
   // CTA has threads.
   Tiling &t = p.t;
   t.q = 1;
-  t.split = (int)up(cv, kTileThreads);
+  t.split = p.mixed ? 1 : (int)up(cv, kTileThreads);
   if (t.split == 1) {
     // Of the numbers of groups that give 48 to 192 bytes a row, the one that wastes the fewest
     // thread columns (their number is a power of two), the larger of equals; tiles of less
     // than 96 bytes only where they bring the cluster to 8 CTAs.
     double best = 0.0;
-    for (int64_t q = 1; q <= groups && q <= kMaxTileGroups && q * cv <= kTileThreads; ++q) {
-      if (q > 1 && q * c > 48) break;
-      const int64_t wide = power_of_two(q * cv), tall = kTileThreads / wide * held(v, backward);
-      double use = (double)(q * cv) / wide;
+    const int64_t some = p.mixed ? 4 : 1;
+    for (int64_t q = some; q <= groups && q <= kMaxTileGroups && q * c <= kTileThreads * v; q += some) {
+      if (q > some && q * c > (p.mixed ? 64 : 48)) break;
+      const int64_t wide = power_of_two(q * c / v), tall = kTileThreads / wide * held(v, backward);
+      double use = (double)(q * c / v) / wide;
       if (q * c < 24) use *= q * c / 24.0;
       if (up(len, tall) > 8 && up(len, tall) <= 2 * kMaxCluster) use *= 0.6;
       if (use >= best) best = use, t.q = (int)q;
     }
-    t.cols = (int)(t.q * cv);
+    t.cols = (int)(t.q * c / v);
   } else {
     t.cols = (int)up(cv, t.split);
   }
@@ -1375,7 +1469,7 @@ int run_rows(const Norm &a, const Plan &p, bool backward, cudaStream_t s) {
   }
 }
 
-template <int V, int MODE>
+template <int V, int MODE, bool MIXED>
 int run_tile(Norm a, const Plan &p, bool backward, cudaStream_t s) {
   // the word for waits that give up; not allocated while the stream is being captured
   a.err = fz::device_error_word_if_any();
@@ -1385,7 +1479,7 @@ int run_tile(Norm a, const Plan &p, bool backward, cudaStream_t s) {
     if (capture == cudaStreamCaptureStatusNone)
       if (int rc = fz::device_error_word(&a.err)) return rc;
   }
-  const auto kernel = backward ? norm_tile_backward_kernel<V, MODE> : norm_tile_kernel<V, MODE>;
+  const auto kernel = backward ? norm_tile_backward_kernel<V, MODE, MIXED> : norm_tile_kernel<V, MODE, MIXED>;
   const int smem = held(V, backward) * kTileThreads * V * 4 * (backward ? 2 : 1);
   const int k = MODE == kInCluster ? p.t.k : 1;
   int resident = 0;
@@ -1395,12 +1489,22 @@ int run_tile(Norm a, const Plan &p, bool backward, cudaStream_t s) {
   return launch_cluster(kernel, (unsigned)grid, kTileThreads, smem, k, s, a, p.t);
 }
 
-template <int V>
+template <int V, bool MIXED>
+int run_tiles(const Norm &a, const Plan &p, bool backward, cudaStream_t s) {
+  if (p.cluster) return run_tile<V, kInCluster, MIXED>(a, p, backward, s);
+  if (int rc = run_tile<V, kParts, MIXED>(a, p, backward, s)) return rc;
+  return run_tile<V, kWhole, MIXED>(a, p, backward, s);
+}
+
 int run(const Norm &a, const Plan &p, bool backward, cudaStream_t s) {
-  if (p.lanes) return run_rows<V>(a, p, backward, s);
-  if (p.cluster) return run_tile<V, kInCluster>(a, p, backward, s);
-  if (int rc = run_tile<V, kParts>(a, p, backward, s)) return rc;
-  return run_tile<V, kWhole>(a, p, backward, s);
+  if (p.mixed) return run_tiles<4, true>(a, p, backward, s);
+  if (p.lanes)
+    return p.v == 4   ? run_rows<4>(a, p, backward, s)
+           : p.v == 2 ? run_rows<2>(a, p, backward, s)
+                      : run_rows<1>(a, p, backward, s);
+  return p.v == 4   ? run_tiles<4, false>(a, p, backward, s)
+         : p.v == 2 ? run_tiles<2, false>(a, p, backward, s)
+                    : run_tiles<1, false>(a, p, backward, s);
 }
 
 int check_sizes(const char *who, int64_t batch, int64_t len, int64_t channels, int64_t groups) {
@@ -1453,7 +1557,7 @@ extern "C" int fz_group_norm(float *y, float *mean, float *rstd, const float *x,
   a.batch = batch, a.len = len, a.channels = channels, a.groups = (int)groups, a.c = (int)(channels / groups);
   a.m = (float)(len * a.c), a.inv_m = (float)(1.0 / (double)(len * a.c)), a.eps = eps, a.act = act;
   cudaStream_t s = fz::resolve(stream);
-  return p.v == 4 ? run<4>(a, p, false, s) : p.v == 2 ? run<2>(a, p, false, s) : run<1>(a, p, false, s);
+  return run(a, p, false, s);
 }
 
 extern "C" int fz_group_norm_backward(float *dx, float *dgamma, float *dbeta, const float *dy, const float *x,
@@ -1480,8 +1584,7 @@ extern "C" int fz_group_norm_backward(float *dx, float *dgamma, float *dbeta, co
   a.part = dgamma || dbeta ? (float *)workspace + p.stat_floats : nullptr;
   a.batch = batch, a.len = len, a.channels = channels, a.groups = (int)groups, a.c = (int)(channels / groups);
   a.m = (float)(len * a.c), a.inv_m = (float)(1.0 / (double)(len * a.c)), a.act = act;
-  if (int rc = p.v == 4 ? run<4>(a, p, true, s) : p.v == 2 ? run<2>(a, p, true, s) : run<1>(a, p, true, s))
-    return rc;
+  if (int rc = run(a, p, true, s)) return rc;
   if (!a.part) return FZ_OK;
   // CTAs a block of 32 channels: as many as have 4 rows a warp, until the SMs are filled
   const int64_t blocks = up(channels, 32);

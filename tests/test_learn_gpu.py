@@ -160,6 +160,41 @@ def test_group_norm(capi, shape, act, affine, off):
         np.testing.assert_array_equal(g.view(np.uint32), h.view(np.uint32))
 
 
+# groups of odd channels while a row is whole vectors of 4 (and of 2 modulo 4), up to a tile of
+# 1020 channels; one tile a sample, a cluster's, and two launches
+MIXED_SHAPES = [(3, 64, 12, 4), (2, 100, 20, 4), (2, 300, 12, 2), (1, 33, 1020, 4), (2, 50, 1020, 2), (1, 9000, 40, 8),
+                (1, 40000, 28, 4), (3, 1369, 264, 8), (2, 65, 500, 20), (1, 20000, 140, 4), (5, 70, 104, 8),
+                (3, 90, 12, 4)]
+
+
+@pytest.mark.parametrize("shape", MIXED_SHAPES, ids=str)
+@pytest.mark.parametrize("act,affine,off", [("silu", True, 0), ("gelu", True, 1), ("none", False, 0)])
+def test_group_norm_vectors_across_groups(capi, shape, act, affine, off):
+    test_group_norm(capi, shape, act, affine, off)
+
+
+@pytest.mark.parametrize("shape,at", [((3, 64, 12, 4), 1), ((2, 100, 20, 4), 2), ((1, 9000, 40, 8), 3),
+                                      ((1, 40000, 28, 4), 1), ((3, 130, 264, 8), 5)], ids=str)
+def test_group_norm_neighbours_in_a_vector_stay_apart(capi, shape, at):
+    """NaN in one group's last channel and 1e18 in the next one's first: the groups around them,
+    whose values share vectors with theirs, come out bit for bit as without them."""
+    b, n, c, groups = shape
+    per = c // groups
+    rng = np.random.default_rng(16)
+    x, dy = rng.standard_normal(shape[:3]).astype(np.float32), rng.standard_normal(shape[:3]).astype(np.float32)
+    clean = run_norm(capi, x, None, None, groups, 1e-5, "silu", dy)
+    bad = x.copy()
+    bad[0, n // 2, at * per - 1] = np.nan
+    bad[0, n - 1, at * per] = 1e18
+    got = run_norm(capi, bad, None, None, groups, 1e-5, "silu", dy)
+    hit = np.zeros((b, n, c), bool)
+    hit[0, :, (at - 1) * per:(at + 1) * per] = True
+    for which in (0, 3):
+        np.testing.assert_array_equal(got[which][~hit], clean[which][~hit])
+    assert np.isnan(got[0][0, :, (at - 1) * per:at * per]).all()
+    assert np.isfinite(got[0][0, :, at * per:(at + 1) * per]).all()
+
+
 @pytest.mark.parametrize("shape", [(4, 1, 4096, 32), (2, 37, 320, 32), (1, 16384, 8, 2)], ids=str)
 def test_group_norm_relu(capi, shape):
     """ReLU's slope jumps at zero: the inputs keep away from it by more than v's error."""
