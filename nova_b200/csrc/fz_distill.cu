@@ -13,9 +13,9 @@
 // The backward streams the row once more, writing dz from the saved statistics, and then
 // overwrites the entries' columns.
 // Measured (B200, copy bandwidth 6.55 TB/s), 64 entries a row: 4096 rows of 131072, forward
-// 324 us (1.01 of the copy bandwidth), backward 660 us (0.99); 2048 rows of 50001 (no two
+// 324 us (1.01 of the copy bandwidth), backward 650 us (1.01); 2048 rows of 50001 (no two
 // alike aligned) 80 and 141 us (0.78, 0.89: the last wave of CTAs and their fixed cost); 8192
-// rows of 2000, a warp each, 21 and 29 us (90 and 91 with a CTA of 512 threads a row).
+// rows of 2000, a warp each, 25 and 37 us.
 #include <cooperative_groups.h>
 
 #include <climits>
@@ -361,22 +361,32 @@ __device__ __forceinline__ void stream_slope(float *out, const Row &row, const S
   }
 }
 
-// Whether an id is named twice: a hash table of `size` (a power of two, at least 2 k) slots.
+// The ids that are named, and which of them twice: a hash table of `size` (a power of two, at
+// least 2 k) slots.
+constexpr int kTwice = 1 << 30;  // ids are below 2^23
+__device__ __forceinline__ int hash(int id, int size) { return (int)((uint32_t)id * 2654435761u >> 16) & (size - 1); }
 template <int T>
-__device__ __forceinline__ bool any_twice(const int *id, int *table, int k, int size, int tid) {
+__device__ __forceinline__ void name_ids(const int *id, int *table, int k, int size, int tid) {
   for (int i = tid; i < size; i += T) table[i] = -1;
   team_sync<T>();
-  bool twice = false;
   for (int i = tid; i < k; i += T) {
     const int v = id[i];
     if (v < 0) continue;
-    for (int at = (int)((uint32_t)v * 2654435761u >> 16) & (size - 1);; at = (at + 1) & (size - 1)) {
+    for (int at = hash(v, size);; at = (at + 1) & (size - 1)) {
       const int was = atomicCAS(&table[at], -1, v);
-      twice = twice || was == v;
-      if (was == -1 || was == v) break;
+      if (was == -1) break;
+      if ((was & (kTwice - 1)) == v) {
+        atomicOr(&table[at], kTwice);
+        break;
+      }
     }
   }
-  return team_any<T>(twice);
+  team_sync<T>();
+}
+__device__ __forceinline__ bool named_twice(const int *table, int size, int id) {
+  int at = hash(id, size);
+  while ((table[at] & (kTwice - 1)) != id) at = (at + 1) & (size - 1);
+  return table[at] & kTwice;
 }
 
 template <bool TAIL, int T>
@@ -415,23 +425,33 @@ __global__ void __launch_bounds__(threads_of(T)) distill_backward_kernel(
   else if (vec) stream_slope<false, true, T>(out, row, s, from, to, tid);
   else if (tail) stream_slope<true, false, T>(out, row, s, from, to, tid);
   else stream_slope<false, false, T>(out, row, s, from, to, tid);
-  const bool twice = any_twice<T>(id, table, k, table_size, tid);  // a barrier, too
-  // the entries' columns, each by its first entry
-  for (int i = tid; i < k; i += T) {
-    const int c = id[i], at = c + row.shift;
-    if (c < 0 || at < from || at >= to) continue;
-    float sum = p[i];
-    if (twice) {
-      bool again = false;
-      sum = 0.0f;
-      for (int j = 0; j < k; ++j)
-        if (id[j] == c) {
-          again = again || j < i;
-          sum = __fadd_rn(sum, p[j]);
+  name_ids<T>(id, table, k, table_size, tid);  // a barrier, too
+  // the entries' columns, each by its first entry; the entries of an id that is named twice
+  // are looked for by a warp (300 rows of 1000 entries, a few named twice: 450 us with a thread
+  // for each and no account of which ids were, 38 so)
+  const int lane = tid & 31;
+  for (int i0 = tid - lane; i0 < k; i0 += T) {
+    const int i = i0 + lane, c = i < k ? id[i] : -1, at = c + row.shift;
+    bool mine = c >= 0 && at >= from && at < to;
+    float sum = mine ? p[i] : 0.0f;
+    for (unsigned todo = __ballot_sync(kFull, mine && named_twice(table, table_size, c)); todo; todo &= todo - 1) {
+      const int who = __ffs(todo) - 1, v = __shfl_sync(kFull, c, who);
+      bool before = false;
+      float all = 0.0f;
+      for (int j = lane; j < k; j += 32)
+        if (id[j] == v) {
+          before = before || j < i0 + who;
+          all = __fadd_rn(all, p[j]);
         }
-      if (again) continue;
+#pragma unroll
+      for (int d = 16; d > 0; d >>= 1) all = __fadd_rn(all, __shfl_xor_sync(kFull, all, d));
+      before = __any_sync(kFull, before);
+      if (lane == who) {
+        sum = all;
+        mine = !before;
+      }
     }
-    out[c] = __fsub_rn(s.at<false>(z[i]), __fmul_rn(scale, sum));
+    if (mine) out[c] = __fsub_rn(s.at<false>(z[i]), __fmul_rn(scale, sum));
   }
 }
 
@@ -447,27 +467,32 @@ int check_distill(const char *who, int64_t rows, int64_t vocab, int64_t k, int64
   return FZ_OK;
 }
 
-// Threads and CTAs a row. A warp for up to 4096 columns, 128 threads for up to 16384, else
-// CTAs of 512, of which a row gets the number that wastes the least: on SMs without work in
-// the last wave (three such CTAs an SM), on a CTA's fixed cost, about that of 3000 columns, and
-// in the forward on the cluster's barriers (4096 rows of 131072: 323 us with one CTA a row, 353
-// with two; 64 rows: 14 us with eight).
+// Threads and CTAs a row (times with 64 entries).
+// A warp a row where that gives every SM more than 8 CTAs' worth of rows: 4096 rows of 2000,
+// 14 and 23 us forward and backward against 22 and 28 with 128 threads and 56 and 61 with 512;
+// 100 rows of 4096, 9 and 13 against 5 and 7. 128 threads where rows are short, or of medium
+// length and more than 3 an SM: 1024 of 16384, 18 and 29 us against 26 and 31 with 512; 148,
+// 12 and 14 against 7 and 9. Else 512.
+// More than one CTA (in the forward a cluster, whose barriers and repeated reading of the
+// entries cost more than the last wave's idle SMs once there are two CTAs an SM): while no more
+// than two an SM result; 8 rows of 131072, 7.9 us forward with 8 against 15.0 with one, 464
+// rows, 101 against 55. The backward's CTAs know nothing of one another, so it also splits
+// many rows of many columns, which shortens the last wave: 4096 rows of 131072, 648 us with 4
+// against 682 with one; 1024 of 50000, 77 with one, 89 with 4.
 struct Team {
   int threads, ctas, slice;
 };
 Team team_of(int64_t rows, int64_t vocab, int64_t k, bool backward) {
-  Team t{vocab <= 4096 && k <= 256 ? 32 : vocab <= 16384 ? 128 : 512, 1, 0};
+  const int64_t sms = fz::num_sms();
+  Team t{512, 1, 0};
+  if (vocab <= 4096) t.threads = k <= 256 && rows > 8 * sms ? 32 : 128;
+  else if (vocab <= 16384 && rows > 3 * sms) t.threads = 128;
   if (t.threads == 512) {
-    const double wave = 3.0 * fz::num_sms();
-    double best = 0.0;
-    for (int n = 1; n <= 8; n *= 2) {
-      const double columns = (double)vocab / n, waves = (double)rows * n / wave;
-      if (columns > (1 << 20)) continue;  // a slice's marks have to fit in shared memory
-      if (n > 1 && columns < 4096) break;
-      double use = waves / (double)(int64_t)(waves + 0.999999) * columns / (columns + 3000.0);
-      if (n > 1 && !backward) use *= 0.93;
-      if (use > best) best = use, t.ctas = n;
-    }
+    const int64_t least = backward ? 4096 : 8192;  // columns a CTA
+    while (t.ctas < 8 && ((rows * t.ctas * 2 <= 2 * sms && vocab >= least * t.ctas * 2) ||
+                          (backward && rows > 2 * sms && vocab >= 32768 * (int64_t)t.ctas * 2) ||
+                          vocab > ((int64_t)t.ctas << 20)))  // a slice's marks have to fit in shared memory
+      t.ctas *= 2;
   }
   t.slice = (int)(((vocab + 3 + t.ctas - 1) / t.ctas + 127) / 128 * 128);
   return t;

@@ -623,6 +623,36 @@ def test_distill_repeated_ids(capi, tail):
         np.testing.assert_array_equal(dz.view(np.uint32), again[1].view(np.uint32))
 
 
+# enough rows for a warp a row (short rows), 128 threads (medium ones), and for a backward that
+# splits long rows
+@pytest.mark.parametrize("r,v,k,tau,off,pitch", [(1300, 515, 20, 2.0, 3, 2), (1250, 90, 64, 1.0, 0, 0), (1190, 4096, 9, 1.0, 1, 0),
+                                                 (460, 9000, 33, 0.5, 1, 1), (300, 66001, 9, 1.0, 0, 0)])
+@pytest.mark.parametrize("tail", [False, True])
+def test_distill_many_rows(capi, r, v, k, tau, off, pitch, tail):
+    test_distill(capi, r, v, k, tau, off, pitch, tail)
+
+
+@pytest.mark.parametrize("r,v,k", [(1200, 300, 40), (1200, 300, 256), (450, 5000, 40), (9, 40000, 1000), (1, 20000, 1024)])
+@pytest.mark.parametrize("tail", [False, True])
+def test_distill_repeated_ids_of_each_team(capi, r, v, k, tail):
+    """One id named by all of a row, by half of it, by two entries at its ends; none."""
+    rng = np.random.default_rng(23)
+    z, ids, t, lse, g = distill_inputs(rng, r, v, k, 1.0, False)
+    ids = np.stack([rng.permutation(v) for _ in range(r)])[:, :k]
+    ids[::4] = v - 1
+    ids[1::4, ::2] = 0
+    ids[2::4, 0] = ids[2::4, -1]
+    if tail:
+        lse = np.log(np.exp(t.astype(np.float64)).sum(1) / 0.8).astype(np.float32)
+    loss, dz = run_distill(capi, z, ids, t, 1.0, lse, g)
+    loss64, dz64 = O.distill(z, ids, t, 1.0, lse, g)
+    e_loss, e_dz = distill_bounds(z, ids, t, 1.0, lse, g)
+    close(loss, loss64, e_loss, "loss")
+    close(dz, dz64, e_dz, "dz")
+    again = run_distill(capi, z, ids, t, 1.0, lse, g)
+    np.testing.assert_array_equal(dz.view(np.uint32), again[1].view(np.uint32))
+
+
 @pytest.mark.parametrize("tail", [False, True])
 def test_distill_masks(capi, tail):
     """Masked columns at -inf and at the type's lowest value; a row of nothing but the lowest
