@@ -5,7 +5,7 @@
 // Measured (B200, copy bandwidth 6.55 TB/s): router, 65536 tokens, 256 experts, 8 picks, all
 // logits normalised: 32 us (0.34 of the copy bandwidth: instruction issue), backward 28 us
 // (0.77). 16384 tokens of 4096 floats, 4 of 64 experts, capacity 1280: sort 12 us (latency of
-// its three steps), dispatch 268 us (0.92), combine 178 us, its backward 426 us (0.96).
+// its three steps), dispatch 268 us (0.92), combine 178 us, its backward 416 us (0.98).
 #include <cooperative_groups.h>
 
 #include <climits>
@@ -610,19 +610,23 @@ __global__ void __launch_bounds__(256) combine_backward_kernel(
     int64_t tokens, int64_t k, int64_t num_rows, int64_t nvec) {
   using V = Vec<VEC>;
   pdl_wait();
-  constexpr int kTeams = 32 / P;
-  const int lane = threadIdx.x & 31, sub = lane % P;
+  // threads that go through the pieces together, a warp or a CTA, and their teams
+  constexpr int kUnit = P > 32 ? P : 32, kTeams = kUnit / P, kWarps = kUnit / 32;
+  const int lane = threadIdx.x & 31, sub = threadIdx.x % P, warp = threadIdx.x % kUnit / 32;
   const int64_t choices = tokens * k, work = (choices + kTeams - 1) / kTeams;
   const int64_t zero_chunks = (nvec + 32 * kUnroll - 1) / (32 * kUnroll);
-  const int64_t all = work + (num_rows + 31) / 32 * zero_chunks;
-  const int64_t warps = (int64_t)gridDim.x * (blockDim.x >> 5);
-  for (int64_t p = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); p < all; p += warps) {
+  const int64_t zeros = (num_rows + 31) / 32 * zero_chunks, all = work + (zeros + kWarps - 1) / kWarps;
+  const int64_t units = (int64_t)gridDim.x * (blockDim.x / kUnit);
+  __shared__ float sums[2][kWarps];
+  int parity = 0;
+  for (int64_t p = (int64_t)blockIdx.x * (blockDim.x / kUnit) + threadIdx.x / kUnit; p < all; p += units) {
     if (p >= work) {
-      const int64_t q = p - work, g = q / zero_chunks;
-      zero_empty<VEC>(drows, src, g * 32, num_rows, nvec, (q - g * zero_chunks) * 32 * kUnroll, lane);
+      const int64_t q = (p - work) * kWarps + warp, g = q / zero_chunks;
+      if (q < zeros)
+        zero_empty<VEC>(drows, src, g * 32, num_rows, nvec, (q - g * zero_chunks) * 32 * kUnroll, lane);
       continue;
     }
-    const int64_t choice = p * kTeams + lane / P, r = choice < choices ? slot[choice] : -1;
+    const int64_t choice = p * kTeams + threadIdx.x % kUnit / P, r = choice < choices ? slot[choice] : -1;
     float s = 0.0f;
     if (r >= 0 && r < num_rows) {
       const float w = weights ? weights[choice] : 1.0f;
@@ -641,7 +645,15 @@ __global__ void __launch_bounds__(256) combine_backward_kernel(
     }
     if (dweights) {
 #pragma unroll
-      for (int d = P / 2; d > 0; d >>= 1) s = __fadd_rn(s, __shfl_xor_sync(kFull, s, d));
+      for (int d = (P > 32 ? 32 : P) / 2; d > 0; d >>= 1) s = __fadd_rn(s, __shfl_xor_sync(kFull, s, d));
+      if constexpr (P > 32) {
+        if (lane == 0) sums[parity][warp] = s;
+        __syncthreads();  // one a choice: the next one's sums go to the other half
+        s = sums[parity][0];
+#pragma unroll
+        for (int i = 1; i < kWarps; ++i) s = __fadd_rn(s, sums[parity][i]);
+        parity ^= 1;
+      }
       if (sub == 0 && choice < choices) dweights[choice] = s;
     }
   }
@@ -667,6 +679,14 @@ int with_lanes(int64_t nvec, F f) {
   if (nvec <= 2 * kUnroll) return f(Lanes<2>{});
   if (nvec <= 8 * kUnroll) return f(Lanes<8>{});
   return f(Lanes<32>{});
+}
+// Whether a choice's gradients are a CTA's work, not a warp's: where a row is at least three
+// passes of the CTA, or of two of a warp's and there are fewer choices than warps. Warps are slow
+// on few rows (288 tokens of 6843 floats, 2 choices, 121 us against 11; 600 of 4096, 4 choices,
+// 27 against 17) and a little on many (8192 of 4096, 2 choices, 108 against 103); CTAs on many
+// shorter rows (16384 of 2400, 2 choices, 142 us against 131).
+bool wide_choices(int64_t choices, int64_t nvec) {
+  return nvec >= 768 || (nvec > 256 && choices < (int64_t)32 * fz::num_sms());
 }
 int64_t chunks_of(int64_t nvec, int lanes) { return (nvec + lanes * kUnroll - 1) / (lanes * kUnroll); }
 // Pieces of `tokens` rows for warps, and of the rows that may be empty.
@@ -855,14 +875,15 @@ extern "C" int fz_expert_combine_backward(float *drows, float *dweights, const f
   const auto launch = [&](auto vec, int64_t nvec) {
     constexpr int kVec = decltype(vec)::value;
     using T = typename Vec<kVec>::T;
-    return with_lanes(nvec, [&](auto lanes) {
+    const auto with = [&](auto lanes) {
       constexpr int P = decltype(lanes)::value;
       const unsigned grid = warps_grid(warp_pieces(tokens * k, 1, P) + zero_pieces(num_rows, nvec));
       FZ_CUDA(fz::launch_pdl(combine_backward_kernel<kVec, P>, dim3(grid), dim3(256), 0, s, (T *)drows, dweights,
                              (const T *)dout, (const T *)rows, weights, slot, src, tokens, k, num_rows, nvec));
       FZ_CHECK_LAUNCH();
       return (int)FZ_OK;
-    });
+    };
+    return wide_choices(tokens * k, nvec) ? with(Lanes<256>{}) : with_lanes(nvec, with);
   };
   return width % 4 == 0 && aligned16(drows, dout, rows) ? launch(Lanes<4>{}, width / 4) : launch(Lanes<1>{}, width);
 }

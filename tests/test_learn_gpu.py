@@ -444,6 +444,13 @@ def test_dispatch_and_combine(capi, t, k, e, cap, width, off):
     np.testing.assert_array_equal(only.get(), O.dispatch(g, slot, n).astype(np.float32))
 
 
+# rows of several passes of a warp, and of a CTA; empty rows beside them
+@pytest.mark.parametrize("t,k,e,cap,width,off", [(1300, 4, 6, 0, 301, 0), (40, 2, 3, 35, 2500, 1), (3, 2, 4, 5, 9000, 0),
+                                                 (700, 2, 5, 0, 770, 2), (20, 1, 4, 8, 1030, 0)])
+def test_dispatch_and_combine_of_wide_rows(capi, t, k, e, cap, width, off):
+    test_dispatch_and_combine(capi, t, k, e, cap, width, off)
+
+
 def test_combine_passes_over_foreign_slots(capi):
     """A slot outside the rows is no choice: nothing is read or written for it."""
     L = capi.lib()
