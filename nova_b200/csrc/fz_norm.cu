@@ -9,12 +9,12 @@
 //     allows) is held by 4 to 32 lanes of a warp, of at most 2048 vectors by a CTA;
 //   * tile kernels: a tile of rows x columns (several whole groups wide, or a part of
 //     one) a CTA; the tiles of a team exchange their statistics through distributed
-//     shared memory in one cluster, of up to 16 CTAs. Where c is odd but a row of channels
-//     is whole vectors, they may lie across two groups ("mixed": statistics per channel,
-//     two groups' values spread over a vector). Against single floats, SiLU, forward and
-//     backward: [64, 1024, 264] / 8 104 -> 69 and 214 -> 141 us, [64, 1024, 120] / 8
-//     32 -> 24 and 55 -> 34 us. Where c is 2 modulo 4 the vectors are of 2: mixed ones of 4
-//     took 27 and 40 us against 21 and 38 at [16, 1369, 320] / 32;
+//     shared memory in one cluster, of up to 16 CTAs. Where c is no multiple of 4 but a row
+//     of channels is whole vectors of 4, they may lie across two groups ("mixed":
+//     statistics per vector and group, two groups' values spread over a vector). Against
+//     vectors that stay in a group, SiLU, forward and backward: [64, 1024, 264] / 8 104 -> 37
+//     and 214 -> 88 us, [64, 1024, 120] / 8 32 -> 21 and 55 -> 34 us, [16, 1369, 320] / 32
+//     21.5 -> 19 and 37 -> 32 us, [64, 4096, 256] / 128 140 -> 123 and 263 -> 208 us;
 //   * larger teams: the tile kernels in two launches that leave the statistics in the
 //     workspace and read x (and dy) twice; the second launch takes the tiles in reverse,
 //     so it finds the last of what the first read in L2. (Taking the batch a few samples at
@@ -22,9 +22,9 @@
 //     [8, 16384, 512] 205 against 161 us.)
 // Measured (B200, copy bandwidth 6.55 TB/s): rows, [65536, 4096] in 32 groups, GELU: forward
 // 378 us, backward 563 us (0.87 of the copy bandwidth both). Clusters, [64, 4096, 256] in 32
-// groups, SiLU: forward 100 us (0.82), backward 211 us (0.58: the tiles of x and dy fill the
-// registers, and a cluster's CTAs wait for one another). Two launches, [8, 16384, 512]: 158
-// and 250 us. A first version with one CTA a team, reading x three times: 566 us for the
+// groups, SiLU: forward 98 us (0.84), backward 198 us (0.62: the tiles of x and dy fill the
+// registers, and a cluster's CTAs wait for one another). Two launches, [8, 16384, 512]: 152
+// and 258 us. A first version with one CTA a team, reading x three times: 566 us for the
 // maps' forward, 16.6 ms for the rows' two passes.
 // Statistics: the mean, then the sum of squares about it, so that a common offset of x
 // does not cancel; parts are joined as (n, mean, M2) (Chan, Golub and LeVeque). Everything
@@ -633,7 +633,10 @@ __global__ void __launch_bounds__(kRowThreads, row_ctas(true, NV))
 // How a launch cuts samples into tiles (see norm_plan).
 struct Tiling {
   int cols;      // vectors a tile is wide
-  int wide;      // the next power of two: thread columns
+  int wide;      // thread columns: cols, or the next power of two
+  int tall;      // thread rows: as many as fit
+  int slices;    // of the thread rows: those of a warp where it holds whole ones (wide
+  int each;      // divides 32), else one thread row each; the thread rows of a slice
   int q;         // whole groups a tile holds (1 where a group is split)
   int split;     // tiles a group's columns are split into
   int bundles;   // tiles side by side over a sample's groups (without the split)
@@ -657,12 +660,13 @@ struct Tile {
   int g0, q, cols;  // its first group, its groups, its vectors a row
   int rows, mine;   // its rows, and those of this thread (0: none)
   int most;         // rows of the thread that has most
+  int full, rest;   // rows = full * thread rows + rest
   int channel;      // this thread's first channel
   int64_t at;       // offset of this thread's first vector
 };
 
 // The groups (counted from the tile's first) of a thread's vector: values before `from` belong
-// to lo, the others to hi. Only mixed vectors (V = 4, c >= 3) have two.
+// to lo, the others to hi. Only mixed vectors (V = 4, c >= 2) have two.
 template <int V, bool MIXED>
 struct Place {
   int lo, hi, from;
@@ -674,6 +678,18 @@ struct Place {
     } else {
       lo = hi = t.split > 1 ? 0 : tx / (a.c / V);
       from = V;
+    }
+  }
+  // the sums over a vector's values of each group
+  __device__ __forceinline__ void gather(const Vec<V> &x, float &l, float &h) const {
+    float f[4];
+    unpair(x.p[0], f[0], f[1]);
+    unpair(x.p[Vec<V>::N - 1], f[2], f[3]);
+    l = h = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      l = __fadd_rn(l, j < from ? f[j] : 0.0f);
+      h = __fadd_rn(h, j < from ? 0.0f : f[j]);
     }
   }
   __device__ __forceinline__ Vec<V> spread(float l, float h) const {
@@ -693,7 +709,10 @@ struct Place {
 template <int V, int MODE, bool MIXED>
 struct Walk {
   int b, bundle, share, db, dbundle, dshare, left;
-  int tx, ty, shift;  // thread column and row, log2 of the thread rows
+  int tx, ty;       // thread column and row; past the last row: a row that no tile has
+  int slice;        // its thread row's
+  bool leaves;      // this thread leaves its column's share of its slice
+  unsigned invert;  // by which to multiply instead of dividing by the thread rows
   __device__ Walk(const Tiling &t, int rank) {
     const int k = MODE == kInCluster ? 1 : t.k;
     const int first = MODE == kInCluster ? (int)blockIdx.x / t.k : (int)blockIdx.x;
@@ -706,10 +725,15 @@ struct Walk {
     dshare = MODE == kInCluster ? 0 : step % k;
     dbundle = step / k % t.bundles;
     db = step / k / t.bundles;
-    tx = (int)threadIdx.x & (t.wide - 1);
     ty = (int)threadIdx.x / t.wide;
-    shift = __ffs(kTileThreads / t.wide) - 1;
+    tx = (int)threadIdx.x - ty * t.wide;
+    slice = ty / t.each;
+    leaves = ty < t.tall && ty == slice * t.each;
+    if (ty >= t.tall) ty = INT_MAX;
+    invert = (1u << 22) / t.tall + 1;
   }
+  // x / tall: exact, since x <= 32 tall and 32 tall^2 <= 2^21
+  __device__ int over_tall(int x) const { return (int)((unsigned)x * invert >> 22); }
   __device__ void advance(const Tiling &t) {
     --left;
     int carry = 0;
@@ -737,8 +761,10 @@ struct Walk {
     const int64_t row0 = (int64_t)r.chunk * t.rows;
     r.rows = (int)min((int64_t)t.rows, a.len - row0);
     r.channel = r.g0 * a.c + (piece * t.cols + tx) * V;
-    r.mine = tx < r.cols && ty < r.rows ? ((r.rows - 1 - ty) >> shift) + 1 : 0;
-    r.most = ((r.rows - 1) >> shift) + 1;
+    r.mine = tx < r.cols && ty < r.rows ? over_tall(r.rows - 1 - ty) + 1 : 0;
+    r.full = over_tall(r.rows);
+    r.rest = r.rows - r.full * t.tall;
+    r.most = r.full + (r.rest > 0);
     r.at = (r.b * a.len + row0 + ty) * a.channels + r.channel;
     return r;
   }
@@ -754,9 +780,9 @@ __device__ __forceinline__ float count_of(const Norm &a, const Tiling &t, int k)
 
 // The loops over a thread's rows end, four rows at a time, behind the tile's last, so that a
 // short tile costs what it has: [2048, 64, 40] / 4, vectors of 2, forward 57 -> 40 us, backward
-// 69 -> 44 us; [16, 1369, 320] / 32, backward 38 -> 35 us (full tiles, [64, 4096, 256] / 32:
-// 204 -> 211 us). A forward of vectors of 4 runs all of its rows: with the branches between its
-// loads and sums, full tiles took 105.7 us instead of 102.0.
+// 69 -> 44 us; [16, 1369, 320] / 32, backward 38 -> 35 us. A forward of vectors of 4
+// runs all of its rows: with the branches between its loads and sums, [64, 1024, 264] / 8 took
+// 43 us instead of 37, [4096, 40, 52] / 4 49 instead of 57.
 template <int V, int N>
 __device__ __forceinline__ bool behind(int i, const Tile<V> &me) {
   return (V < 4 || N < held(4, false)) && i % 4 == 0 && i >= me.most;
@@ -789,64 +815,50 @@ __device__ __forceinline__ float warp_sum(float v) {
   return v;
 }
 
-// A tile's thread rows come in slices: the thread rows of a warp where a warp holds several
-// (wide < 32), else one thread row each.
-__device__ __forceinline__ int slices_of(int wide) { return wide < 32 ? kTileThreads / 32 : kTileThreads / wide; }
-// The sum of v over the lanes of a warp that share a thread column.
-__device__ __forceinline__ float over_rows(float v, int wide) {
-  for (int d = 16; d >= wide; d >>= 1) v = __fadd_rn(v, __shfl_xor_sync(kFull, v, d));
+// The sum of v over the thread rows of a slice that is a warp's.
+__device__ __forceinline__ float over_rows(float v, int each) {
+  for (int d = 16; d * each > 16; d >>= 1) v = __fadd_rn(v, __shfl_xor_sync(kFull, v, d));
   return v;
 }
 // Rows of the tile that slice y holds.
-__device__ __forceinline__ int rows_of_slice(int y, int rows, int wide, int shift) {
-  const int tall = wide < 32 ? 32 / wide : 1, rest = rows & ((1 << shift) - 1);
-  return (rows >> shift) * tall + min(max(rest - y * tall, 0), tall);
+template <int V>
+__device__ __forceinline__ int rows_of_slice(int y, const Tile<V> &me, const Tiling &t) {
+  return me.full * t.each + min(max(me.rest - y * t.each, 0), t.each);
 }
 
-// The tile's own moments. column_moments: each slice reduces a column (mixed: each of its
-// channels) to its mean and the sum of squares about it, with a barrier at the end.
+// The tile's own moments. column_moments: each slice reduces a column (mixed: its values of
+// each group) to its mean and the sum of squares about it, with a barrier at the end.
 // group_moments: (mean, M2) of group g in every lane of the warp that asks, M2 = sum of theirs
-// + n_column (mean_column - mean)^2. sh: [slices][wide] columns, mixed [slices][wide * V].
-template <int V, bool MIXED, int N>
+// + n_column (mean_column - mean)^2. sh: [slices][wide], mixed [slices][wide][2].
+template <int V, int MODE, bool MIXED, int N>
 __device__ __forceinline__ void column_moments(const Vec<V> (&x)[N], float2 *sh, const Tile<V> &me, const Tiling &t,
-                                               int shift) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int slice = t.wide < 32 ? warp : (int)threadIdx.x / t.wide;
+                                               const Walk<V, MODE, MIXED> &walk, const Place<V, MIXED> &place) {
   Vec<V> s = x[0];
 #pragma unroll
   for (int i = 1; i < N; ++i) {
     if (behind<V, N>(i, me)) break;
     sum_into(s, x[i]);
   }
-  const int rows = rows_of_slice(slice, me.rows, t.wide, shift);  // 0: nothing of this slice is read
-  const int at = t.wide < 32 ? warp * t.wide + lane : (int)threadIdx.x;
-  const bool puts = t.wide >= 32 || lane < t.wide;
+  const int rows = rows_of_slice(walk.slice, me, t);  // 0: nothing of this slice is read
+  const int at = walk.slice * t.wide + walk.tx;
   if constexpr (MIXED) {
-    float mean[4], m2[4];
-    unpair(s.p[0], mean[0], mean[1]);
-    unpair(s.p[Vec<V>::N - 1], mean[2], mean[3]);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) mean[j] = __fdiv_rn(over_rows(mean[j], t.wide), (float)rows);
-    Vec<V> minus;
-    minus.p[0] = pair(-mean[0], -mean[1]);
-    minus.p[Vec<V>::N - 1] = pair(-mean[2], -mean[3]);
+    float lo, hi;
+    place.gather(s, lo, hi);
+    const float mean_lo = __fdiv_rn(over_rows(lo, t.each), (float)(rows * max(place.from, 1)));
+    const float mean_hi = __fdiv_rn(over_rows(hi, t.each), (float)(rows * (V - max(place.from, 0))));
+    const Vec<V> minus = place.spread(-mean_lo, -mean_hi);
     s = splat<V>(0.0f);
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       if (behind<V, N>(i, me)) break;
       if (i < me.mine) square_into(s, x[i], minus);
     }
-    unpair(s.p[0], m2[0], m2[1]);
-    unpair(s.p[Vec<V>::N - 1], m2[2], m2[3]);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) m2[j] = over_rows(m2[j], t.wide);
-    if (puts) {
-      float4 *q = reinterpret_cast<float4 *>(sh + at * 4);
-      q[0] = make_float4(mean[0], m2[0], mean[1], m2[1]);
-      q[1] = make_float4(mean[2], m2[2], mean[3], m2[3]);
-    }
+    place.gather(s, lo, hi);
+    lo = over_rows(lo, t.each);
+    hi = over_rows(hi, t.each);
+    if (walk.leaves) *reinterpret_cast<float4 *>(sh + at * 2) = make_float4(mean_lo, lo, mean_hi, hi);
   } else {
-    const float mean = __fdiv_rn(over_rows(total(s), t.wide), (float)(rows * V));
+    const float mean = __fdiv_rn(over_rows(total(s), t.each), (float)(rows * V));
     const Vec<V> minus = splat<V>(-mean);
     s = splat<V>(0.0f);
 #pragma unroll
@@ -854,37 +866,36 @@ __device__ __forceinline__ void column_moments(const Vec<V> (&x)[N], float2 *sh,
       if (behind<V, N>(i, me)) break;
       if (i < me.mine) square_into(s, x[i], minus);
     }
-    const float m2 = over_rows(total(s), t.wide);
-    if (puts) sh[at] = make_float2(mean, m2);
+    const float m2 = over_rows(total(s), t.each);
+    if (walk.leaves) sh[at] = make_float2(mean, m2);
   }
   __syncthreads();
 }
 template <int V, bool MIXED>
 __device__ __forceinline__ float2 group_moments(const float2 *sh, int g, const Norm &a, const Tile<V> &me,
-                                                const Tiling &t, int shift) {
-  constexpr int kEach = MIXED ? 1 : V;  // values a row that an entry of sh stands for
-  const int lane = threadIdx.x & 31, row = MIXED ? t.wide * V : t.wide;
-  const int per = MIXED ? a.c : a.c / V, width = t.split > 1 ? me.cols : per;
-  const int total = slices_of(t.wide) * width, dy = 32 / width, dc = 32 - dy * width;
+                                                const Tiling &t) {
+  const int lane = threadIdx.x & 31, begin = g * a.c, end = begin + a.c;  // channels
+  const int first = begin / V, width = t.split > 1 ? me.cols : MIXED ? (end - 1) / V - first + 1 : a.c / V;
+  const int total = t.slices * width, dy = 32 / width, dc = 32 - dy * width;
   const int y0 = lane / width, c0 = lane - y0 * width;
-  float u = 0.0f, w = 0.0f;
-  for (int i = lane, y = y0, c = c0; i < total; i += 32) {
-    const int n = rows_of_slice(y, me.rows, t.wide, shift) * kEach;
-    if (n) u = __fmaf_rn((float)n, sh[y * row + g * per + c].x, u);
-    y += dy, c += dc;
-    if (c >= width) c -= width, ++y;
-  }
-  const float mean = __fdiv_rn(warp_sum(u), (float)me.rows * (float)(width * kEach));
-  for (int i = lane, y = y0, c = c0; i < total; i += 32) {
-    const int n = rows_of_slice(y, me.rows, t.wide, shift) * kEach;
-    if (n) {
-      const float2 p = sh[y * row + g * per + c];
-      const float d = __fsub_rn(p.x, mean);
-      w = __fadd_rn(w, __fmaf_rn(__fmul_rn(d, d), (float)n, p.y));
+  const auto each = [&](auto f) {  // f(values, their mean and M2) for this lane's entries
+    for (int i = lane, y = y0, c = c0; i < total; i += 32) {
+      const int col = first + c;
+      const int values = MIXED ? min(col * V + V, end) - max(col * V, begin) : V;
+      const int n = rows_of_slice(y, me, t) * values;
+      // a mixed column's values of the group that ends in it stand first
+      if (n) f((float)n, sh[MIXED ? (y * t.wide + col) * 2 + (end >= col * V + V) : y * t.wide + col]);
+      y += dy, c += dc;
+      if (c >= width) c -= width, ++y;
     }
-    y += dy, c += dc;
-    if (c >= width) c -= width, ++y;
-  }
+  };
+  float u = 0.0f, w = 0.0f;
+  each([&](float n, float2 p) { u = __fmaf_rn(n, p.x, u); });
+  const float mean = __fdiv_rn(warp_sum(u), (float)me.rows * (float)(t.split > 1 ? me.cols * V : a.c));
+  each([&](float n, float2 p) {
+    const float d = __fsub_rn(p.x, mean);
+    w = __fadd_rn(w, __fmaf_rn(__fmul_rn(d, d), n, p.y));
+  });
   return make_float2(mean, warp_sum(w));
 }
 
@@ -966,7 +977,7 @@ __global__ void __launch_bounds__(kTileThreads, kTileCtas) norm_tile_kernel(cons
   constexpr int N = held(V, false);
   cg::cluster_group cluster = cg::this_cluster();
   extern __shared__ __align__(16) float fifo[];
-  __shared__ __align__(16) float2 sh[kTileThreads * (MIXED ? V : 1)];
+  __shared__ __align__(16) float2 sh[kTileThreads * (MIXED ? 2 : 1)];
   // by parity of the tile: a warp may be a tile ahead of one that still reads
   __shared__ float2 stats_by[2][kMaxTileGroups];
   __shared__ Exchange exchange;
@@ -978,7 +989,7 @@ __global__ void __launch_bounds__(kTileThreads, kTileCtas) norm_tile_kernel(cons
     __syncthreads();
     cluster.barrier_arrive();
   }
-  const int64_t step = (int64_t)(kTileThreads / t.wide) * a.channels;
+  const int64_t step = (int64_t)t.tall * a.channels;
   const Place<V, MIXED> place(a, t, walk.tx);
   const float share = joined && lane < t.k ? count_of<V>(a, t, lane) : 0.0f;
   Tile<V> me, next;
@@ -1000,11 +1011,11 @@ __global__ void __launch_bounds__(kTileThreads, kTileCtas) norm_tile_kernel(cons
       fetch_tile<V, N>(fifo, a.x, next, step);
     }
     copy_commit();
-    if (MODE != kWhole) column_moments<V, MIXED>(x, sh, me, t, walk.shift);
+    if (MODE != kWhole) column_moments(x, sh, me, t, walk, place);
     if (joined) {
       if (threadIdx.x == kTileThreads - 1) exchange_expect(exchange, n, t.k * me.q * (int)sizeof(float2));
       for (int g = warp; g < me.q; g += kTileThreads / 32) {
-        const float2 m = group_moments<V, MIXED>(sh, g, a, me, t, walk.shift);
+        const float2 m = group_moments<V, MIXED>(sh, g, a, me, t);
         if (lane < t.k) exchange_push(exchange, n, me.k, g, lane, m);
       }
       if (warp < me.q) exchange_wait(exchange, n, i >> 1 & 1, a.err);
@@ -1013,7 +1024,7 @@ __global__ void __launch_bounds__(kTileThreads, kTileCtas) norm_tile_kernel(cons
     for (int g = warp; g < me.q; g += kTileThreads / 32) {
       const int64_t team = (int64_t)me.b * a.groups + me.g0 + g;
       if (MODE == kParts) {
-        const float2 m = group_moments<V, MIXED>(sh, g, a, me, t, walk.shift);
+        const float2 m = group_moments<V, MIXED>(sh, g, a, me, t);
         if (lane == 0) reinterpret_cast<float2 *>(a.stat)[team * t.k + me.k] = m;
         continue;
       }
@@ -1021,7 +1032,7 @@ __global__ void __launch_bounds__(kTileThreads, kTileCtas) norm_tile_kernel(cons
       if (joined) {
         r = join_lanes(share, lane < t.k ? exchange.all[n][lane][g] : make_float2(0.0f, 0.0f), a);
       } else if (MODE == kInCluster) {
-        r = group_moments<V, MIXED>(sh, g, a, me, t, walk.shift);
+        r = group_moments<V, MIXED>(sh, g, a, me, t);
         r.y = rstd_of(r.y, a.inv_m, a.eps);
       } else {
         const float2 *q = reinterpret_cast<const float2 *>(a.stat) + team * t.k;
@@ -1067,27 +1078,27 @@ __global__ void __launch_bounds__(kTileThreads, kTileCtas) norm_tile_kernel(cons
 // The tile's sums of dv and dv xh. column_sums: per slice and channel to sh[slices][2][wide * V],
 // with a barrier at the end. Then, a warp a group, group_sums adds up the slices, leaves the
 // channels' sums in `part` and gives the gamma-weighted sums over the group to every lane.
-// Groups of many channels are added up over the slices by all threads first.
-constexpr int kNarrow = 32;  // channels a group up to which a warp adds up the slices alone
-template <int V>
+// Many channels a group, or many slices, are added up over the slices by all threads first.
+__device__ __forceinline__ bool together(const Norm &a, const Tiling &t) { return a.c > 32 || t.slices > 8; }
+template <int V, int MODE, bool MIXED>
 __device__ __forceinline__ void column_sums(Vec<V> db, Vec<V> dg, float *sh, const Norm &a, const Tile<V> &me,
-                                            const Tiling &t, int tx) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, row = t.wide * V;
-  for (int d = 16; d >= t.wide; d >>= 1) {
+                                            const Tiling &t, const Walk<V, MODE, MIXED> &walk) {
+  const int row = t.wide * V;
+  for (int d = 16; d * t.each > 16; d >>= 1) {
 #pragma unroll
     for (int i = 0; i < Vec<V>::N; ++i) {
       db.p[i] = add2(db.p[i], __shfl_xor_sync(kFull, db.p[i], d));
       dg.p[i] = add2(dg.p[i], __shfl_xor_sync(kFull, dg.p[i], d));
     }
   }
-  if (t.wide >= 32 || lane < t.wide) {
-    float *q = sh + (t.wide >= 32 ? (int)threadIdx.x / t.wide : warp) * 2 * row + tx * V;
+  if (walk.leaves) {
+    float *q = sh + walk.slice * 2 * row + walk.tx * V;
     store(q, db);
     store(q + row, dg);
   }
   __syncthreads();
-  if (a.c > kNarrow) {
-    const int n = me.cols * V, slices = slices_of(t.wide);
+  if (together(a, t)) {
+    const int n = me.cols * V, slices = t.slices;
     for (int i = threadIdx.x; i < 2 * n; i += kTileThreads) {
       const int which = i >= n, ch = i - (which ? n : 0);
       float *q = sh + which * row + ch;
@@ -1101,7 +1112,7 @@ __device__ __forceinline__ void column_sums(Vec<V> db, Vec<V> dg, float *sh, con
 template <int V>
 __device__ __forceinline__ float2 group_sums(const float *sh, int g, const Norm &a, const Tile<V> &me,
                                              const Tiling &t, int tx) {
-  const int lane = threadIdx.x & 31, row = t.wide * V, slices = a.c > kNarrow ? 1 : slices_of(t.wide);
+  const int lane = threadIdx.x & 31, row = t.wide * V, slices = together(a, t) ? 1 : t.slices;
   const int width = t.split > 1 ? me.cols * V : a.c, first = me.channel - tx * V + g * a.c;
   float *part = a.part ? a.part + ((int64_t)me.b * t.chunks + me.chunk) * 2 * a.channels + first : nullptr;
   float u = 0.0f, w = 0.0f;
@@ -1135,7 +1146,7 @@ __global__ void __launch_bounds__(kTileThreads, kTileCtas) norm_tile_backward_ke
     __syncthreads();
     cluster.barrier_arrive();
   }
-  const int64_t step = (int64_t)(kTileThreads / t.wide) * a.channels;
+  const int64_t step = (int64_t)t.tall * a.channels;
   const Place<V, MIXED> place(a, t, walk.tx);
   Tile<V> me, next;
   float2 lo, hi, next_lo = make_float2(0.0f, 0.0f), next_hi = next_lo;  // mean and rstd of the vector's groups
@@ -1178,7 +1189,7 @@ __global__ void __launch_bounds__(kTileThreads, kTileCtas) norm_tile_backward_ke
         }
       });
     }
-    if (MODE != kWhole) column_sums(db, dg, sh, a, me, t, walk.tx);
+    if (MODE != kWhole) column_sums(db, dg, sh, a, me, t, walk);
     if (joined) {
       if (threadIdx.x == kTileThreads - 1) exchange_expect(exchange, n, t.k * me.q * (int)sizeof(float2));
       for (int g = warp; g < me.q; g += kTileThreads / 32) {
@@ -1293,12 +1304,22 @@ int64_t power_of_two(int64_t a) {
   return p;
 }
 
+// Thread columns for tiles of `cols` vectors: the next power of two where a warp then holds whole
+// rows and more columns cost at most a ninth of the thread rows, else just as many
+// ([16, 1024, 640] in 32 groups, 10 vectors: 25 and 44 us against 28 and 52 with 16 columns;
+// [8, 4096, 1920], 15 vectors: 133 us with 16 columns, 146 with 15).
+int64_t columns_for(int64_t cols) {
+  const int64_t wide = power_of_two(cols);
+  return wide <= 32 && kTileThreads / wide * 9 >= kTileThreads / cols * 8 ? wide : cols;
+}
+
 Plan norm_plan(int64_t batch, int64_t len, int64_t channels, int64_t groups, int v, bool backward) {
   Plan p{};
   const int64_t c = channels / groups;
-  // Mixed vectors where the tile kernels would move single floats. A tile then holds a
-  // multiple of 4 groups, and has at least 32 rows for its thread rows.
-  p.mixed = v == 4 && c % 2 && c >= 3 && channels % 4 == 0 && c <= kTileThreads && len >= 32 && len * c > 256;
+  // Mixed vectors where the tile kernels would move floats or pairs of them, from a few rows on:
+  // a tile of one row has a vector a thread at most.
+  const int64_t unit = c % 2 ? 4 : 2;  // groups that make whole vectors
+  p.mixed = v == 4 && c % 4 && c >= 2 && channels % 4 == 0 && unit * c <= 4 * kTileThreads && len >= 8 && len * c > 256;
   while (!p.mixed && c % v) v /= 2;
   p.v = v;
   const int64_t cv = c / v, vectors = len * cv, teams = batch * groups;
@@ -1334,25 +1355,37 @@ Plan norm_plan(int64_t batch, int64_t len, int64_t channels, int64_t groups, int
     // thread columns (their number is a power of two), the larger of equals; tiles of less
     // than 96 bytes only where they bring the cluster to 8 CTAs.
     double best = 0.0;
-    const int64_t some = p.mixed ? 4 : 1;
+    const int64_t some = p.mixed ? unit : 1;
     for (int64_t q = some; q <= groups && q <= kMaxTileGroups && q * c <= kTileThreads * v; q += some) {
       if (q > some && q * c > (p.mixed ? 64 : 48)) break;
-      const int64_t wide = power_of_two(q * c / v), tall = kTileThreads / wide * held(v, backward);
-      double use = (double)(q * c / v) / wide;
+      const int64_t cols = q * c / v, thread_rows = kTileThreads / columns_for(cols);
+      const int64_t tall = thread_rows * held(v, backward);
+      double use = (double)(cols * thread_rows) / kTileThreads * groups / (double)(up(groups, q) * q);
       if (q * c < 24) use *= q * c / 24.0;
       if (up(len, tall) > 8 && up(len, tall) <= 2 * kMaxCluster) use *= 0.6;
       if (use >= best) best = use, t.q = (int)q;
     }
     t.cols = (int)(t.q * c / v);
   } else {
+    // Of the numbers of pieces that a cluster holds, the one whose tiles take the least, each four
+    // rows of a thread beside its own; two launches cost as much again.
+    double best = 0.0;
+    for (int64_t n = t.split; n <= kMaxCluster || n == up(cv, kTileThreads); ++n) {
+      const int64_t rows = kTileThreads / columns_for(up(cv, n)), chunks = up(len, rows * held(v, backward));
+      const double cost = (double)(n * chunks) * (up(up(len, chunks), rows) + 4) * (n * chunks > kMaxCluster ? 1.6 : 1.0);
+      if (best == 0.0 || cost < best) best = cost, t.split = (int)n;
+    }
     t.cols = (int)up(cv, t.split);
   }
-  t.wide = (int)power_of_two(t.cols);
+  t.wide = (int)columns_for(t.cols);
+  t.tall = kTileThreads / t.wide;
+  t.each = 32 % t.wide == 0 ? 32 / t.wide : 1;
+  t.slices = t.tall / t.each;
   t.bundles = (int)up(groups, t.q);
   t.sets = (int)(batch * t.bundles);
   // Rows: as few tiles one below the other as hold the sample, or, where those would leave
   // SMs idle, as many as a cluster takes and that keep four rows a thread.
-  const int64_t ty = kTileThreads / t.wide, most = ty * held(v, backward);
+  const int64_t ty = t.tall, most = ty * held(v, backward);
   int64_t chunks = up(len, most);
   const int64_t idle = up((int64_t)fz::num_sms() * kTileCtas, (int64_t)t.sets * t.split);
   int64_t room = kMaxCluster / t.split;

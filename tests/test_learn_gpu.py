@@ -160,11 +160,11 @@ def test_group_norm(capi, shape, act, affine, off):
         np.testing.assert_array_equal(g.view(np.uint32), h.view(np.uint32))
 
 
-# groups of odd channels while a row is whole vectors of 4 (and of 2 modulo 4), up to a tile of
-# 1020 channels; one tile a sample, a cluster's, and two launches
+# channels a group that no vector of 4 divides while a row of them is whole vectors, up to a
+# tile of 1020 channels; one tile a sample, a cluster's, and two launches
 MIXED_SHAPES = [(3, 64, 12, 4), (2, 100, 20, 4), (2, 300, 12, 2), (1, 33, 1020, 4), (2, 50, 1020, 2), (1, 9000, 40, 8),
                 (1, 40000, 28, 4), (3, 1369, 264, 8), (2, 65, 500, 20), (1, 20000, 140, 4), (5, 70, 104, 8),
-                (3, 90, 12, 4)]
+                (3, 90, 12, 4), (2, 500, 64, 32), (1, 3000, 8, 4), (3, 9, 140, 4), (2, 70, 1000, 4)]
 
 
 @pytest.mark.parametrize("shape", MIXED_SHAPES, ids=str)
@@ -173,7 +173,15 @@ def test_group_norm_vectors_across_groups(capi, shape, act, affine, off):
     test_group_norm(capi, shape, act, affine, off)
 
 
-@pytest.mark.parametrize("shape,at", [((3, 64, 12, 4), 1), ((2, 100, 20, 4), 2), ((1, 9000, 40, 8), 3),
+# thread columns that are no power of two; groups in pieces
+@pytest.mark.parametrize("shape", [(2, 300, 300, 5), (3, 500, 150, 1), (2, 51, 271, 1), (1, 90, 1031, 1), (2, 40, 9000, 2),
+                                   (1, 700, 777, 1), (3, 2000, 80, 4), (2, 12, 1100, 2), (1, 5000, 1036, 1)], ids=str)
+@pytest.mark.parametrize("act,affine,off", [("silu", True, 0), ("gelu", True, 1), ("none", False, 0)])
+def test_group_norm_tiles_of_each_width(capi, shape, act, affine, off):
+    test_group_norm(capi, shape, act, affine, off)
+
+
+@pytest.mark.parametrize("shape,at", [((3, 64, 12, 4), 1), ((2, 100, 20, 4), 2), ((1, 9000, 40, 8), 3), ((2, 1369, 320, 32), 13),
                                       ((1, 40000, 28, 4), 1), ((3, 130, 264, 8), 5)], ids=str)
 def test_group_norm_neighbours_in_a_vector_stay_apart(capi, shape, at):
     """NaN in one group's last channel and 1e18 in the next one's first: the groups around them,
