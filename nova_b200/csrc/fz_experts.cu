@@ -161,27 +161,27 @@ __device__ __forceinline__ void merge_keys(uint32_t (&a)[K], const uint32_t (&b)
       }
 }
 
-// Eight lanes per token, expert e = sub + 8 i in register i (at most 8 N experts, K picks).
-// Bound by instruction issue, which four tokens a warp share: a lane's K largest keys come
-// from sorting networks, the token's from three rounds of merging with another lane's, with
+// L lanes per token, expert e = sub + L i in register i (at most L N experts, K <= L picks).
+// Bound by instruction issue, which the 32 / L tokens of a warp share: a lane's K largest keys come
+// from sorting networks, the token's from rounds of merging with another lane's, with
 // no exchange per pick. A pick's place is the number of larger keys, so that each lane
 // writes its own picks. Tokens with equal keys among their picks or at their end, or with
-// a NaN, are left to route_token. (65536 tokens, 256 experts, 8 picks: 49 us with a warp a
-// token throughout.)
-template <int N, int K>
+// a NaN, are left to route_token. (With a warp a token throughout: 65536 tokens, 256 experts, 8
+// picks 49 us, 32 so; 16384 tokens, 1024 experts, 8 picks 110 us, 39 so.)
+template <int L, int N, int K>
 __global__ void __launch_bounds__(256) route_team_kernel(float *__restrict__ weights, int32_t *__restrict__ ids,
                                                          const float *__restrict__ logits, int64_t tokens,
                                                          int experts, int k, int renormalize) {
   pdl_wait();
-  const int lane = threadIdx.x & 31, sub = lane & 7;
+  const int lane = threadIdx.x & 31, sub = lane % L;
   const int64_t warps = (int64_t)gridDim.x * (blockDim.x >> 5);
-  for (int64_t w = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); w * 4 < tokens; w += warps) {
-    const int64_t t = w * 4 + (lane >> 3);
+  for (int64_t w = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); w * (32 / L) < tokens; w += warps) {
+    const int64_t t = w * (32 / L) + lane / L;
     const bool on = t < tokens;
     const float *row = logits + t * experts;
     float v[N];
 #pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = on && sub + 8 * i < experts ? row[sub + 8 * i] : -INFINITY;
+    for (int i = 0; i < N; ++i) v[i] = on && sub + L * i < experts ? row[sub + L * i] : -INFINITY;
     uint32_t top[K];
 #pragma unroll
     for (int g = 0; g < N; g += K) {
@@ -197,7 +197,7 @@ __global__ void __launch_bounds__(256) route_team_kernel(float *__restrict__ wei
       }
     }
 #pragma unroll
-    for (int d = 1; d < 8; d *= 2) {
+    for (int d = 1; d < L; d *= 2) {
       uint32_t other[K];
 #pragma unroll
       for (int i = 0; i < K; ++i) other[i] = __shfl_xor_sync(kFull, top[i], d);
@@ -227,7 +227,7 @@ __global__ void __launch_bounds__(256) route_team_kernel(float *__restrict__ wei
       for (int i = 0; i < N; ++i) den = __fadd_rn(den, exp_below(v[i], most));  // -inf: 0
     }
 #pragma unroll
-    for (int d = 1; d < 8; d *= 2) {
+    for (int d = 1; d < L; d *= 2) {
       count += __shfl_xor_sync(kFull, count, d);
       den = __fadd_rn(den, __shfl_xor_sync(kFull, den, d));
     }
@@ -235,7 +235,7 @@ __global__ void __launch_bounds__(256) route_team_kernel(float *__restrict__ wei
     if (odd) chosen = 0;
     while (__any_sync(kFull, chosen != 0)) {
       if (chosen) {
-        const int e = sub + 8 * (__ffs(chosen) - 1);
+        const int e = sub + L * (__ffs(chosen) - 1);
         chosen &= chosen - 1;
         const float x = row[e];
         const uint32_t key = order_key(x);
@@ -251,8 +251,8 @@ __global__ void __launch_bounds__(256) route_team_kernel(float *__restrict__ wei
       ids[t * k + sub] = -1;
     }
     for (unsigned left = __ballot_sync(kFull, odd && sub == 0); left; left &= left - 1) {
-      const int64_t its = w * 4 + ((__ffs(left) - 1) >> 3);
-      float u[N / 4];
+      const int64_t its = w * (32 / L) + (__ffs(left) - 1) / L;
+      float u[N * L / 32];
       load_row(u, logits + its * experts, lane, experts);
       route_token(weights, ids, u, its, experts, k, renormalize, lane);
     }
@@ -709,10 +709,10 @@ int launch_route(float *w, int32_t *ids, const float *logits, int64_t tokens, in
   FZ_CHECK_LAUNCH();
   return FZ_OK;
 }
-template <int N, int K>
+template <int L, int N, int K>
 int launch_route_team(float *w, int32_t *ids, const float *logits, int64_t tokens, int experts, int k, int renorm,
                       cudaStream_t s) {
-  FZ_CUDA(fz::launch_pdl(route_team_kernel<N, K>, dim3(fz::grid_for((tokens + 3) / 4, 8, 4)), dim3(256), 0, s, w,
+  FZ_CUDA(fz::launch_pdl(route_team_kernel<L, N, K>, dim3(fz::grid_for((tokens * L + 31) / 32, 8, 4)), dim3(256), 0, s, w,
                          ids, logits, tokens, experts, k, renorm));
   FZ_CHECK_LAUNCH();
   return FZ_OK;
@@ -744,15 +744,22 @@ extern "C" int fz_route(float *weights, int32_t *ids, const float *logits, int64
   FZ_REQUIRE(weights && ids && logits, "fz_route: null pointer");
   cudaStream_t s = fz::resolve(stream);
   const int e = (int)experts, kk = (int)k, rn = renormalize != 0;
-  // eight lanes a token up to 256 experts and 8 picks, else a warp
+  // Up to 8 picks, the fewest lanes a token whose registers hold the experts: 262144 tokens of 64
+  // experts, 26 us with 4 lanes, 36 with 8; 65536 of 256, 32 with 8, 39 with 16; 16384 of 512, 17
+  // with 16, 21 with 32.
   if (k <= 4) {
-    if (e <= 64) return launch_route_team<8, 4>(weights, ids, logits, tokens, e, kk, rn, s);
-    if (e <= 128) return launch_route_team<16, 4>(weights, ids, logits, tokens, e, kk, rn, s);
-    if (e <= 256) return launch_route_team<32, 4>(weights, ids, logits, tokens, e, kk, rn, s);
-  } else if (k <= 8) {
-    if (e <= 64) return launch_route_team<8, 8>(weights, ids, logits, tokens, e, kk, rn, s);
-    if (e <= 128) return launch_route_team<16, 8>(weights, ids, logits, tokens, e, kk, rn, s);
-    if (e <= 256) return launch_route_team<32, 8>(weights, ids, logits, tokens, e, kk, rn, s);
+    if (e <= 64) return launch_route_team<4, 16, 4>(weights, ids, logits, tokens, e, kk, rn, s);
+    if (e <= 128) return launch_route_team<4, 32, 4>(weights, ids, logits, tokens, e, kk, rn, s);
+    if (e <= 256) return launch_route_team<8, 32, 4>(weights, ids, logits, tokens, e, kk, rn, s);
+    if (e <= 512) return launch_route_team<16, 32, 4>(weights, ids, logits, tokens, e, kk, rn, s);
+    return launch_route_team<32, 32, 4>(weights, ids, logits, tokens, e, kk, rn, s);
+  }
+  if (k <= 8) {
+    if (e <= 64) return launch_route_team<8, 8, 8>(weights, ids, logits, tokens, e, kk, rn, s);
+    if (e <= 128) return launch_route_team<8, 16, 8>(weights, ids, logits, tokens, e, kk, rn, s);
+    if (e <= 256) return launch_route_team<8, 32, 8>(weights, ids, logits, tokens, e, kk, rn, s);
+    if (e <= 512) return launch_route_team<16, 32, 8>(weights, ids, logits, tokens, e, kk, rn, s);
+    return launch_route_team<32, 32, 8>(weights, ids, logits, tokens, e, kk, rn, s);
   }
   if (e <= 32) return launch_route<1>(weights, ids, logits, tokens, e, kk, rn, s);
   if (e <= 64) return launch_route<2>(weights, ids, logits, tokens, e, kk, rn, s);

@@ -340,6 +340,29 @@ def test_route(capi, t, e, k, renorm):
         assert not dz[dz64 == 0].any()
 
 
+# more experts than eight lanes hold: half the tokens with ties, one without experts
+@pytest.mark.parametrize("t,e,k", [(61, 300, 8), (64, 512, 4), (33, 512, 8), (31, 700, 3), (40, 1024, 8), (5, 257, 1), (1500, 384, 6)])
+@pytest.mark.parametrize("renorm", [True, False])
+def test_route_many_experts(capi, t, e, k, renorm):
+    test_route(capi, t, e, k, renorm)
+
+
+@pytest.mark.parametrize("e", [40, 300, 1000])
+def test_route_nan_stays_with_its_token(capi, e):
+    """A NaN, or a tie, among the tokens that share a warp."""
+    rng = np.random.default_rng(31)
+    z = rng.standard_normal((50, e)).astype(np.float32)
+    clean, clean_ids = run_route(capi, z, 4, False)
+    z[7, e - 1], z[20, 3], z[21] = np.nan, np.nan, 0.5
+    w, ids = run_route(capi, z, 4, False)
+    others = np.delete(np.arange(50), [7, 20, 21])
+    np.testing.assert_array_equal(ids[others], clean_ids[others])
+    np.testing.assert_array_equal(w[others], clean[others])
+    assert ids[7, 0] == e - 1 and ids[20, 0] == 3 and np.isnan(w[[7, 20]]).all()
+    np.testing.assert_array_equal(ids[21], np.arange(4))
+    close(w[21], np.full(4, 1 / e), (e / 32 + 30) * U / e, "uniform")
+
+
 def test_route_specials(capi):
     """NaN ranks first and makes its token's weights NaN, other tokens keep theirs; the
     type's lowest value is a number like others; equal logits go to the lowest experts."""
