@@ -13,7 +13,7 @@
 // The backward streams the row once more, writing dz from the saved statistics, and then
 // overwrites the entries' columns.
 // Measured (B200, copy bandwidth 6.55 TB/s), 64 entries a row: 4096 rows of 131072, forward
-// 324 us (1.01 of the copy bandwidth), backward 650 us (1.01); 2048 rows of 50001 (no two
+// 324 us (1.01 of the copy bandwidth), backward 662 us (0.99); 2048 rows of 50001 (no two
 // alike aligned) 80 and 141 us (0.78, 0.89: the last wave of CTAs and their fixed cost); 8192
 // rows of 2000, a warp each, 25 and 37 us.
 #include <cooperative_groups.h>
@@ -477,8 +477,9 @@ int check_distill(const char *who, int64_t rows, int64_t vocab, int64_t k, int64
 // entries cost more than the last wave's idle SMs once there are two CTAs an SM): while no more
 // than two an SM result; 8 rows of 131072, 7.9 us forward with 8 against 15.0 with one, 464
 // rows, 101 against 55. The backward's CTAs know nothing of one another, so it also splits
-// many rows of many columns, which shortens the last wave: 4096 rows of 131072, 648 us with 4
-// against 682 with one; 1024 of 50000, 77 with one, 89 with 4.
+// many rows of many columns, which shortens the last wave: 4096 rows of 131072, 662 us with 2
+// against 682 with one (with 4, 648, but 20 us more than with 2 right after the forward, of which
+// L2 then holds the last rows); 1024 of 50000, 77 with one, 89 with 4.
 struct Team {
   int threads, ctas, slice;
 };
@@ -490,7 +491,7 @@ Team team_of(int64_t rows, int64_t vocab, int64_t k, bool backward) {
   if (t.threads == 512) {
     const int64_t least = backward ? 4096 : 8192;  // columns a CTA
     while (t.ctas < 8 && ((rows * t.ctas * 2 <= 2 * sms && vocab >= least * t.ctas * 2) ||
-                          (backward && rows > 2 * sms && vocab >= 32768 * (int64_t)t.ctas * 2) ||
+                          (backward && rows > 2 * sms && vocab >= 65536 * (int64_t)t.ctas * 2) ||
                           vocab > ((int64_t)t.ctas << 20)))  // a slice's marks have to fit in shared memory
       t.ctas *= 2;
   }

@@ -664,7 +664,7 @@ def test_distill_repeated_ids(capi, tail):
 # enough rows for a warp a row (short rows), 128 threads (medium ones), and for a backward that
 # splits long rows
 @pytest.mark.parametrize("r,v,k,tau,off,pitch", [(1300, 515, 20, 2.0, 3, 2), (1250, 90, 64, 1.0, 0, 0), (1190, 4096, 9, 1.0, 1, 0),
-                                                 (460, 9000, 33, 0.5, 1, 1), (300, 66001, 9, 1.0, 0, 0)])
+                                                 (460, 9000, 33, 0.5, 1, 1), (300, 131100, 9, 1.0, 0, 0)])
 @pytest.mark.parametrize("tail", [False, True])
 def test_distill_many_rows(capi, r, v, k, tau, off, pitch, tail):
     test_distill(capi, r, v, k, tau, off, pitch, tail)
