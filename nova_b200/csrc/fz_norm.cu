@@ -40,6 +40,7 @@
 #include <climits>
 #include <cstdint>
 #include <mutex>
+#include <type_traits>
 
 #include "fz_common.cuh"
 
@@ -77,7 +78,6 @@ __device__ __forceinline__ Pair pair(float a, float b) {
   asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
   return r;
 }
-__device__ __forceinline__ Pair both(float a) { return pair(a, a); }
 __device__ __forceinline__ void unpair(Pair p, float &a, float &b) {
   asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p));
 }
@@ -97,70 +97,94 @@ __device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
   return r;
 }
 
-__device__ __forceinline__ Pair sigmoid2(Pair v) {
+__device__ __forceinline__ Pair from_lane(Pair a, int mask) { return __shfl_xor_sync(kFull, a, mask); }
+template <class F>
+__device__ __forceinline__ Pair each(F f, Pair v) {
   float a, b;
-  unpair(mul2(v, both(-1.4426950408889634f)), a, b);
-  unpair(add2(pair(ex2(a), ex2(b)), both(1.0f)), a, b);
-  return pair(rcp(a), rcp(b));
+  unpair(v, a, b);
+  return pair(f(a), f(b));
+}
+template <class F>
+__device__ __forceinline__ Pair each(F f, Pair v, Pair w, Pair x) {
+  float a, b, c, d, g, h;
+  unpair(v, a, b);
+  unpair(w, c, d);
+  unpair(x, g, h);
+  return pair(f(a, c, g), f(b, d, h));
+}
+// The same for a value of its own, where no vector of two is possible.
+struct One {
+  float f;
+};
+__device__ __forceinline__ One add2(One a, One b) { return {__fadd_rn(a.f, b.f)}; }
+__device__ __forceinline__ One mul2(One a, One b) { return {__fmul_rn(a.f, b.f)}; }
+__device__ __forceinline__ One fma2(One a, One b, One c) { return {__fmaf_rn(a.f, b.f, c.f)}; }
+__device__ __forceinline__ One from_lane(One a, int mask) { return {__shfl_xor_sync(kFull, a.f, mask)}; }
+template <class F>
+__device__ __forceinline__ One each(F f, One v) {
+  return {f(v.f)};
+}
+template <class F>
+__device__ __forceinline__ One each(F f, One v, One w, One x) {
+  return {f(v.f, w.f, x.f)};
+}
+template <class E>
+__device__ __forceinline__ E both(float a) {
+  if constexpr (std::is_same_v<E, One>) return {a};
+  else return pair(a, a);
+}
+
+template <class E>
+__device__ __forceinline__ E sigmoid2(E v) {
+  const E e = each([](float a) { return ex2(a); }, mul2(v, both<E>(-1.4426950408889634f)));
+  return each([](float a) { return rcp(a); }, add2(e, both<E>(1.0f)));
 }
 
 // Phi(v) and exp(-v^2 / 2). With h = Phi(-|v|) = exp(-v^2 / 2) R(t), t = 1 / (1 + 0.3 |v|):
 // R is a polynomial of degree 8 without constant term, fitted to the least largest relative
 // error on |v| <= 14 (Remez; 1.5e-7).
-__device__ __forceinline__ Pair phi2(Pair v, Pair *e) {
-  float a, b, c, d;
-  unpair(v, a, b);
-  unpair(fma2(pair(fabsf(a), fabsf(b)), both(0.3f), both(1.0f)), c, d);
-  const Pair t = pair(rcp(c), rcp(d));
-  unpair(mul2(mul2(v, v), both(-0.72134752044448170f)), c, d);
-  *e = pair(ex2(c), ex2(d));
-  Pair r = fma2(both(0.035674769431352615f), t, both(-0.1572030633687973f));
-  r = fma2(r, t, both(0.20635347068309784f));
-  r = fma2(r, t, both(-0.05368361622095108f));
-  r = fma2(r, t, both(0.1285616159439087f));
-  r = fma2(r, t, both(0.09991349279880524f));
-  r = fma2(r, t, both(0.12075395882129669f));
-  r = fma2(r, t, both(0.11962930113077164f));
-  const Pair h = mul2(mul2(r, t), *e);
-  float g, k;
-  unpair(h, c, d);
-  unpair(fma2(h, both(-1.0f), both(1.0f)), g, k);
-  return pair(a < 0.0f ? c : g, b < 0.0f ? d : k);  // NaN: both are
+template <class E>
+__device__ __forceinline__ E phi2(E v, E *e) {
+  const E c = fma2(each([](float a) { return fabsf(a); }, v), both<E>(0.3f), both<E>(1.0f));
+  const E t = each([](float a) { return rcp(a); }, c);
+  *e = each([](float a) { return ex2(a); }, mul2(mul2(v, v), both<E>(-0.72134752044448170f)));
+  E r = fma2(both<E>(0.035674769431352615f), t, both<E>(-0.1572030633687973f));
+  r = fma2(r, t, both<E>(0.20635347068309784f));
+  r = fma2(r, t, both<E>(-0.05368361622095108f));
+  r = fma2(r, t, both<E>(0.1285616159439087f));
+  r = fma2(r, t, both<E>(0.09991349279880524f));
+  r = fma2(r, t, both<E>(0.12075395882129669f));
+  r = fma2(r, t, both<E>(0.11962930113077164f));
+  const E h = mul2(mul2(r, t), *e);
+  // NaN: both are
+  return each([](float a, float low, float high) { return a < 0.0f ? low : high; }, v, h,
+              fma2(h, both<E>(-1.0f), both<E>(1.0f)));
 }
 
-template <int ACT>
-__device__ __forceinline__ Pair activate2(Pair v) {
+template <int ACT, class E>
+__device__ __forceinline__ E activate2(E v) {
   if constexpr (ACT == FZ_ACT_SILU) return mul2(v, sigmoid2(v));
   if constexpr (ACT == FZ_ACT_GELU) {
-    Pair e;
+    E e;
     return mul2(v, phi2(v, &e));
   }
-  if constexpr (ACT == FZ_ACT_RELU) {
-    float a, b;
-    unpair(v, a, b);
-    return pair(a > 0.0f ? a : 0.0f, b > 0.0f ? b : 0.0f);
-  }
+  if constexpr (ACT == FZ_ACT_RELU) return each([](float a) { return a > 0.0f ? a : 0.0f; }, v);
   return v;
 }
 
 // d act'(v)
-template <int ACT>
-__device__ __forceinline__ Pair times_slope2(Pair d, Pair v) {
+template <int ACT, class E>
+__device__ __forceinline__ E times_slope2(E d, E v) {
   if constexpr (ACT == FZ_ACT_SILU) {
-    const Pair s = sigmoid2(v), rest = fma2(s, both(-1.0f), both(1.0f));
-    return mul2(d, mul2(s, fma2(v, rest, both(1.0f))));
+    const E s = sigmoid2(v), rest = fma2(s, both<E>(-1.0f), both<E>(1.0f));
+    return mul2(d, mul2(s, fma2(v, rest, both<E>(1.0f))));
   }
   if constexpr (ACT == FZ_ACT_GELU) {
-    Pair e;
-    const Pair p = phi2(v, &e);
-    return mul2(d, fma2(mul2(v, both(0.39894228040143268f)), e, p));
+    E e;
+    const E p = phi2(v, &e);
+    return mul2(d, fma2(mul2(v, both<E>(0.39894228040143268f)), e, p));
   }
-  if constexpr (ACT == FZ_ACT_RELU) {
-    float a, b, x, y;
-    unpair(v, a, b);
-    unpair(d, x, y);
-    return pair(a > 0.0f ? x : 0.0f, b > 0.0f ? y : 0.0f);
-  }
+  if constexpr (ACT == FZ_ACT_RELU) return each([](float a, float x, float) { return a > 0.0f ? x : 0.0f; }, v, d, d);
   return d;
 }
 
@@ -181,16 +205,18 @@ __device__ __forceinline__ void with_activation(int act, F f) {
 
 // ---------------------------------------------------------------- vectors
 
-// V floats in registers as pairs (V = 1: a pair whose second value is zero and never stored).
+// V floats in registers as pairs, or a float. ([2922, 1082, 31] in one group, SiLU: 374 and 751 us
+// with a float as a pair with an idle half, 322 and 464 so.)
 template <int V>
 struct Vec {
+  using E = std::conditional_t<V == 1, One, Pair>;
   static constexpr int N = V == 4 ? 2 : 1;
-  Pair p[N];
+  E p[N];
 };
 template <int V>
 __device__ __forceinline__ Vec<V> splat(float a) {
   Vec<V> r;
-  const Pair p = V == 1 ? pair(a, 0.0f) : both(a);
+  const auto p = both<typename Vec<V>::E>(a);
 #pragma unroll
   for (int i = 0; i < Vec<V>::N; ++i) r.p[i] = p;
   return r;
@@ -206,21 +232,23 @@ __device__ __forceinline__ Vec<V> load(const float *q) {
     const float2 f = *reinterpret_cast<const float2 *>(q);
     r.p[0] = pair(f.x, f.y);
   } else {
-    r.p[0] = pair(*q, 0.0f);
+    r.p[0] = {*q};
   }
   return r;
 }
 template <int V>
 __device__ __forceinline__ void store(float *q, const Vec<V> &r) {
-  float a, b, c, d;
-  unpair(r.p[0], a, b);
-  if constexpr (V == 4) {
-    unpair(r.p[1], c, d);
-    *reinterpret_cast<float4 *>(q) = make_float4(a, b, c, d);
-  } else if constexpr (V == 2) {
-    *reinterpret_cast<float2 *>(q) = make_float2(a, b);
+  if constexpr (V == 1) {
+    *q = r.p[0].f;
   } else {
-    *q = a;
+    float a, b, c, d;
+    unpair(r.p[0], a, b);
+    if constexpr (V == 4) {
+      unpair(r.p[1], c, d);
+      *reinterpret_cast<float4 *>(q) = make_float4(a, b, c, d);
+    } else {
+      *reinterpret_cast<float2 *>(q) = make_float2(a, b);
+    }
   }
 }
 template <int V>
@@ -246,9 +274,13 @@ __device__ __forceinline__ void copy_wait() {
 // The sum of a vector's values.
 template <int V>
 __device__ __forceinline__ float total(const Vec<V> &r) {
-  float a, b;
-  unpair(V == 4 ? add2(r.p[0], r.p[Vec<V>::N - 1]) : r.p[0], a, b);
-  return V == 1 ? a : __fadd_rn(a, b);
+  if constexpr (V == 1) {
+    return r.p[0].f;
+  } else {
+    float a, b;
+    unpair(V == 4 ? add2(r.p[0], r.p[Vec<V>::N - 1]) : r.p[0], a, b);
+    return __fadd_rn(a, b);
+  }
 }
 // s += x; s += (x - mean)^2
 template <int V>
@@ -260,7 +292,7 @@ template <int V>
 __device__ __forceinline__ void square_into(Vec<V> &s, const Vec<V> &x, const Vec<V> &minus_mean) {
 #pragma unroll
   for (int i = 0; i < Vec<V>::N; ++i) {
-    const Pair d = add2(x.p[i], minus_mean.p[i]);
+    const auto d = add2(x.p[i], minus_mean.p[i]);
     s.p[i] = fma2(d, d, s.p[i]);
   }
 }
@@ -281,7 +313,7 @@ __device__ __forceinline__ void gradient(Vec<V> &x, Vec<V> &d, Vec<V> &db, Vec<V
 #pragma unroll
   for (int i = 0; i < Vec<V>::N; ++i) {
     x.p[i] = mul2(add2(x.p[i], minus_mean.p[i]), rstd.p[i]);
-    const Pair dv = times_slope2<ACT>(d.p[i], fma2(x.p[i], gamma.p[i], beta.p[i]));
+    const auto dv = times_slope2<ACT>(d.p[i], fma2(x.p[i], gamma.p[i], beta.p[i]));
     db.p[i] = add2(db.p[i], dv);
     dg.p[i] = fma2(dv, x.p[i], dg.p[i]);
     d.p[i] = mul2(dv, gamma.p[i]);
@@ -1087,8 +1119,8 @@ __device__ __forceinline__ void column_sums(Vec<V> db, Vec<V> dg, float *sh, con
   for (int d = 16; d * t.each > 16; d >>= 1) {
 #pragma unroll
     for (int i = 0; i < Vec<V>::N; ++i) {
-      db.p[i] = add2(db.p[i], __shfl_xor_sync(kFull, db.p[i], d));
-      dg.p[i] = add2(dg.p[i], __shfl_xor_sync(kFull, dg.p[i], d));
+      db.p[i] = add2(db.p[i], from_lane(db.p[i], d));
+      dg.p[i] = add2(dg.p[i], from_lane(dg.p[i], d));
     }
   }
   if (walk.leaves) {
