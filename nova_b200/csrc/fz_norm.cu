@@ -55,6 +55,11 @@ constexpr int kMaxTileGroups = 16;  // groups side by side in a tile
 // Vectors of x (backward: of x and of dy) a tile kernel's thread holds: what the registers of
 // two CTAs an SM leave.
 __host__ __device__ constexpr int held(int v, bool backward) { return (v == 4 ? 16 : 32) / (backward ? 2 : 1); }
+// Tiles of at most a half or a quarter of that run in kernels made for it, SHORT = 1 and 2, with 3
+// and 4 CTAs an SM: what a tile costs beside its rows is then spread over more of them.
+// [1024, 64, 640] / 32, SiLU, 3 rows a thread: forward 222 us with the kernels for 16 rows, 163
+// with those for 8, 134 with those for 4; backward 178 with those for 8, 145 with those for 4.
+constexpr int kShortest = 2;
 constexpr int kMaxCluster = 16;
 
 // ---------------------------------------------------------------- activations
@@ -811,7 +816,7 @@ __device__ __forceinline__ float count_of(const Norm &a, const Tiling &t, int k)
 }
 
 // The loops over a thread's rows end, four rows at a time, behind the tile's last, so that a
-// short tile costs what it has: [2048, 64, 40] / 4, vectors of 2, forward 57 -> 40 us, backward
+// short tile costs what it has: [2048, 64, 40] / 4 in vectors of 2, forward 57 -> 40 us, backward
 // 69 -> 44 us; [16, 1369, 320] / 32, backward 38 -> 35 us. A forward of vectors of 4
 // runs all of its rows: with the branches between its loads and sums, [64, 1024, 264] / 8 took
 // 43 us instead of 37, [4096, 40, 52] / 4 49 instead of 57.
@@ -1003,10 +1008,10 @@ __device__ __forceinline__ void exchange_wait(Exchange &x, int parity, int phase
   }
 }
 
-template <int V, int MODE, bool MIXED>
-__global__ void __launch_bounds__(kTileThreads, kTileCtas) norm_tile_kernel(const Norm a, const Tiling t) {
+template <int V, int MODE, bool MIXED, int SHORT>
+__global__ void __launch_bounds__(kTileThreads, kTileCtas + SHORT) norm_tile_kernel(const Norm a, const Tiling t) {
   pdl_wait();
-  constexpr int N = held(V, false);
+  constexpr int N = held(V, false) >> SHORT;
   cg::cluster_group cluster = cg::this_cluster();
   extern __shared__ __align__(16) float fifo[];
   __shared__ __align__(16) float2 sh[kTileThreads * (MIXED ? 2 : 1)];
@@ -1161,10 +1166,10 @@ __device__ __forceinline__ float2 group_sums(const float *sh, int g, const Norm 
   return make_float2(warp_sum(u), warp_sum(w));
 }
 
-template <int V, int MODE, bool MIXED>
-__global__ void __launch_bounds__(kTileThreads, kTileCtas) norm_tile_backward_kernel(const Norm a, const Tiling t) {
+template <int V, int MODE, bool MIXED, int SHORT>
+__global__ void __launch_bounds__(kTileThreads, kTileCtas + SHORT) norm_tile_backward_kernel(const Norm a, const Tiling t) {
   pdl_wait();
-  constexpr int N = held(V, true), kStage = N * kTileThreads * V;
+  constexpr int N = held(V, true) >> SHORT, kStage = N * kTileThreads * V;
   cg::cluster_group cluster = cg::this_cluster();
   extern __shared__ __align__(16) float fifo[];  // x and dy of one tile
   __shared__ __align__(16) float sh[2 * V * kTileThreads];
@@ -1324,6 +1329,7 @@ struct Plan {
   Tiling t;
   bool cluster;          // tile kernels: statistics within a cluster
   bool mixed;            // tile kernels: vectors of 4 across groups
+  int shorter;           // tile kernels in a cluster: those for short tiles
   int parts;             // rows of the per-channel partial sums (backward)
   int fold;              // row kernels: teams a CTA adds up
   size_t part_floats, stat_floats;
@@ -1348,17 +1354,22 @@ int64_t columns_for(int64_t cols) {
 Plan norm_plan(int64_t batch, int64_t len, int64_t channels, int64_t groups, int v, bool backward) {
   Plan p{};
   const int64_t c = channels / groups;
-  // Mixed vectors where the tile kernels would move floats or pairs of them, from a few rows on:
-  // a tile of one row has a vector a thread at most.
-  const int64_t unit = c % 2 ? 4 : 2;  // groups that make whole vectors
-  p.mixed = v == 4 && c % 4 && c >= 2 && channels % 4 == 0 && unit * c <= 4 * kTileThreads && len >= 8 && len * c > 256;
-  while (!p.mixed && c % v) v /= 2;
-  p.v = v;
-  const int64_t cv = c / v, vectors = len * cv, teams = batch * groups;
+  int whole = v;  // floats a vector that stays in a group
+  while (c % whole) whole /= 2;
+  int64_t cv = c / whole, vectors = len * cv;
+  const int64_t teams = batch * groups;
   // Row kernels up to 2048 vectors; above 256 (a CTA's worth) only where a row's piece of
   // a group is at least 512 bytes, else the tile kernels, which take several groups' pieces
   // of a row together.
-  if (!p.mixed && len * channels <= INT_MAX && (vectors <= 256 || (vectors <= 2048 && c >= 128))) {
+  const bool rows = len * channels <= INT_MAX && (vectors <= 256 || (vectors <= 2048 && c >= 128));
+  // Else tiles, of mixed vectors where others would be floats or pairs of them. (Tiles where row
+  // kernels would do: [8192, 3, 680] / 4 forward 135 us against 31, [2048, 48, 40] / 4 20 against 12.)
+  const int64_t unit = c % 2 ? 4 : 2;  // groups that make whole vectors
+  p.mixed = !rows && v == 4 && c % 4 && c >= 2 && channels % 4 == 0 && unit * c <= 4 * kTileThreads;
+  if (!p.mixed) v = whole;
+  cv = c / v, vectors = len * cv;
+  p.v = v;
+  if (rows) {
     p.lanes = vectors <= 4 ? 4 : vectors <= 8 ? 8 : vectors <= 16 ? 16 : vectors <= 256 ? 32 : kRowThreads;
     p.nv = 1;
     while ((int64_t)p.nv * p.lanes < vectors) p.nv *= 2;
@@ -1429,6 +1440,7 @@ Plan norm_plan(int64_t batch, int64_t len, int64_t channels, int64_t groups, int
   const int64_t k = (int64_t)t.split * t.chunks;
   t.k = (int)k;
   p.cluster = k <= kMaxCluster;
+  while (p.shorter < kShortest && up(t.rows, t.tall) <= held(v, backward) >> (p.shorter + 1)) ++p.shorter;
   if (backward) {
     p.parts = (int)(batch * t.chunks);
     p.part_floats = (size_t)p.parts * 2 * channels;
@@ -1534,7 +1546,7 @@ int run_rows(const Norm &a, const Plan &p, bool backward, cudaStream_t s) {
   }
 }
 
-template <int V, int MODE, bool MIXED>
+template <int V, int MODE, bool MIXED, int SHORT = 0>
 int run_tile(Norm a, const Plan &p, bool backward, cudaStream_t s) {
   // the word for waits that give up; not allocated while the stream is being captured
   a.err = fz::device_error_word_if_any();
@@ -1544,8 +1556,8 @@ int run_tile(Norm a, const Plan &p, bool backward, cudaStream_t s) {
     if (capture == cudaStreamCaptureStatusNone)
       if (int rc = fz::device_error_word(&a.err)) return rc;
   }
-  const auto kernel = backward ? norm_tile_backward_kernel<V, MODE, MIXED> : norm_tile_kernel<V, MODE, MIXED>;
-  const int smem = held(V, backward) * kTileThreads * V * 4 * (backward ? 2 : 1);
+  const auto kernel = backward ? norm_tile_backward_kernel<V, MODE, MIXED, SHORT> : norm_tile_kernel<V, MODE, MIXED, SHORT>;
+  const int smem = (held(V, backward) >> SHORT) * kTileThreads * V * 4 * (backward ? 2 : 1);
   const int k = MODE == kInCluster ? p.t.k : 1;
   int resident = 0;
   if (int rc = resident_clusters((const void *)kernel, kTileThreads, smem, k, &resident)) return rc;
@@ -1556,7 +1568,10 @@ int run_tile(Norm a, const Plan &p, bool backward, cudaStream_t s) {
 
 template <int V, bool MIXED>
 int run_tiles(const Norm &a, const Plan &p, bool backward, cudaStream_t s) {
-  if (p.cluster) return run_tile<V, kInCluster, MIXED>(a, p, backward, s);
+  if (p.cluster)
+    return p.shorter == 2   ? run_tile<V, kInCluster, MIXED, 2>(a, p, backward, s)
+           : p.shorter == 1 ? run_tile<V, kInCluster, MIXED, 1>(a, p, backward, s)
+                            : run_tile<V, kInCluster, MIXED>(a, p, backward, s);
   if (int rc = run_tile<V, kParts, MIXED>(a, p, backward, s)) return rc;
   return run_tile<V, kWhole, MIXED>(a, p, backward, s);
 }

@@ -173,9 +173,10 @@ def test_group_norm_vectors_across_groups(capi, shape, act, affine, off):
     test_group_norm(capi, shape, act, affine, off)
 
 
-# thread columns that are no power of two; groups in pieces
+# thread columns that are no power of two; groups in pieces; many tiles of a few rows
 @pytest.mark.parametrize("shape", [(2, 300, 300, 5), (3, 500, 150, 1), (2, 51, 271, 1), (1, 90, 1031, 1), (2, 40, 9000, 2),
-                                   (1, 700, 777, 1), (3, 2000, 80, 4), (2, 12, 1100, 2), (1, 5000, 1036, 1)], ids=str)
+                                   (1, 700, 777, 1), (3, 2000, 80, 4), (2, 12, 1100, 2), (1, 5000, 1036, 1), (40, 64, 640, 32),
+                                   (37, 18, 264, 4), (700, 7, 148, 2), (5, 232, 4, 2), (30, 30, 1040, 8)], ids=str)
 @pytest.mark.parametrize("act,affine,off", [("silu", True, 0), ("gelu", True, 1), ("none", False, 0)])
 def test_group_norm_tiles_of_each_width(capi, shape, act, affine, off):
     test_group_norm(capi, shape, act, affine, off)
