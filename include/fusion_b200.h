@@ -484,8 +484,11 @@ int fz_expert_combine_backward(float *drows, float *dweights, const float *dout,
  *   vocabulary over tau), the rest pT = max(0, 1 - sum p) on one bucket, against the
  *   student's qT = sum of q outside the row's entries;
  *   loss[r] = tau^2 * (sum_i p_i (log p_i - log q_i) + pT (log pT - log qT)),
- * a term with p = 0 counting 0. A row without entries (with teacher_lse NULL also one whose
- * entries are all -inf) has loss 0 whatever its logits hold. For the backward, stats
+ * a term with p = 0 counting 0. A pT that fp32 rounding explains (at most 2^-24 (48 +
+ * 4 |teacher_lse[r]|)) is 0 where qT is below 2^-126: no columns outside the entries, or masked
+ * ones; a larger one there makes the loss infinite (or as large as the masks are low).
+ * A row without entries (with teacher_lse NULL also one whose entries are all -inf) has
+ * loss 0 whatever its logits hold. For the backward, stats
  * [rows, 4] (16-byte aligned) receives the maximum of z and log sum exp((z - max) / tau), then, with
  * teacher_lse, the same two over the logits outside the entries.
  * k <= FZ_MAX_TEACHER, vocab <= 2^23; an id named twice counts its p each time. */
@@ -495,7 +498,8 @@ int fz_distill(float *loss, float *stats, const float *logits, int64_t ld, const
 /* dlogits (row pitch ldd >= vocab; columns from vocab on are left alone) from dloss [rows]
  * and the stats that fz_distill wrote. With P = sum p + pT and c = tau * dloss[r]:
  * c * (P q_v - sum of p of the entries that name v), and for v outside the entries
- * c * (P - pT / qT) q_v; rows without entries get zeros. dlogits may not overlap logits. */
+ * c * (P - pT / qT) q_v (0 where z_v is -inf); rows without entries get zeros. dlogits may
+ * not overlap logits. */
 int fz_distill_backward(float *dlogits, int64_t ldd, const float *dloss, const float *stats,
                         const float *logits, int64_t ld, const int32_t *ids, const float *teacher,
                         const float *teacher_lse, int64_t rows, int64_t vocab, int64_t k,

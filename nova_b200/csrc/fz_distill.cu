@@ -111,9 +111,21 @@ __device__ __forceinline__ float team_fold(float v, float *sh) {
 // ---------------------------------------------------------------- the teacher's side of a row
 
 struct Teacher {
-  bool some;         // the row has entries
-  float mass, tail;  // P = sum p + pT, pT
+  bool some;           // the row has entries
+  float listed, tail;  // sum p, pT
+  float slack;         // what rounding alone may leave in pT
+  __device__ __forceinline__ float mass() const { return __fadd_rn(listed, tail); }
+  // Where the student gives the columns outside the entries no mass that fp32 holds (there are
+  // none, or all are masked), pT (log pT - log qT) would turn a rounding of pT into an infinite
+  // loss: a pT that is no larger than its rounding is 0 there.
+  __device__ __forceinline__ void settle(float log_q_tail) {
+    if (log_q_tail < -87.0f && tail <= slack) tail = 0.0f;  // below 2^-126 or so
+  }
 };
+// log qT from the maximum and log sum of all logits and of those outside the entries
+__device__ __forceinline__ float log_tail_mass(float m, float log_sum, float tail_m, float log_tail, float tau) {
+  return __fadd_rn(__fdiv_rn(__fsub_rn(tail_m, m), tau), __fsub_rn(log_tail, log_sum));
+}
 
 // Made by the whole team in shared memory: id[i] (-1: padding), p[i], the student's logit
 // z[i] there and, when asked for, logp[i] = log p[i].
@@ -134,7 +146,7 @@ __device__ __forceinline__ Teacher read_teacher(int *id, float *p, float *z, flo
     some = some || (ok && (lse || t != -INFINITY));
     top = fmaxf(top, t);
   }
-  Teacher t{team_any<T>(some), 0.0f, 0.0f};
+  Teacher t{team_any<T>(some), 0.0f, 0.0f, 0.0f};
   if (!t.some) return t;
   float shift;
   if (!lse) {
@@ -155,12 +167,16 @@ __device__ __forceinline__ Teacher read_teacher(int *id, float *p, float *z, flo
     p[i] = q;
     s = __fadd_rn(s, q);
   }
-  s = team_fold<T, false>(s, sh);
+  t.listed = team_fold<T, false>(s, sh);
   if (lse) {
-    const float rest = __fsub_rn(1.0f, s);
+    const float rest = __fsub_rn(1.0f, t.listed);
     t.tail = rest < 0.0f ? 0.0f : rest;  // NaN stays
+    // To first order, with u = 2^-24 and L = |lse|: the sum of p, at most 24 additions deep
+    // (k <= 1024), 24 u; expf 4 u; p's argument, t / tau and the difference rounded, (L + 2 H) u
+    // with the entries' entropy H <= log 1024; the caller's lse, 2 roundings of it and as much
+    // again of its sum, (3 L + 6) u.
+    t.slack = __fmul_rn(__fmaf_rn(fabsf(shift), 4.0f, 48.0f), 1.0f / (1 << 24));
   }
-  t.mass = __fadd_rn(s, t.tail);
   return t;
 }
 
@@ -213,7 +229,7 @@ __global__ void __launch_bounds__(threads_of(T)) distill_kernel(float *__restric
   const float *start = logits + r * ld;
   const Row row = row_at(start, vocab);
   const int from = rank * slice, to = min(from + slice, row.end);  // slice: a multiple of 128
-  const Teacher t = read_teacher<T>(id, p, rank == 0 ? z : nullptr, logp, start, ids, teacher, teacher_lse, r, k,
+  Teacher t = read_teacher<T>(id, p, rank == 0 ? z : nullptr, logp, start, ids, teacher, teacher_lse, r, k,
                                     vocab, tau, sh);
   if (!t.some) {  // the same in every CTA of the cluster
     if (rank == 0 && tid == 0) loss[r] = 0.0f;
@@ -308,9 +324,10 @@ __global__ void __launch_bounds__(threads_of(T)) distill_kernel(float *__restric
     for (int d = 16; d > 0; d >>= 1) l = __fadd_rn(l, __shfl_xor_sync(kFull, l, d));
     if (lane == 0) {
       const float log_tail = logf(tail.s);
-      if (TAIL && t.tail != 0.0f) {
-        const float logq = __fadd_rn(__fdiv_rn(__fsub_rn(tail.m, sum.m), tau), __fsub_rn(log_tail, log_sum));
-        l = __fmaf_rn(t.tail, __fsub_rn(logf(t.tail), logq), l);
+      if (TAIL) {
+        const float logq = log_tail_mass(sum.m, log_sum, tail.m, log_tail, tau);
+        t.settle(logq);
+        if (t.tail != 0.0f) l = __fmaf_rn(t.tail, __fsub_rn(logf(t.tail), logq), l);
       }
       loss[r] = __fmul_rn(__fmul_rn(tau, tau), l);
       *reinterpret_cast<float4 *>(stats + r * 4) = make_float4(sum.m, log_sum, tail.m, log_tail);
@@ -410,7 +427,7 @@ __global__ void __launch_bounds__(threads_of(T)) distill_backward_kernel(
   float *out = dlogits + r * ldd;
   const Row row = row_at(start, vocab);
   const int from = rank * slice, to = min(from + slice, row.end);  // slice: a multiple of 128
-  const Teacher t =
+  Teacher t =
       read_teacher<T>(id, p, z, nullptr, start, ids, teacher, teacher_lse, r, k, vocab, tau, sh);
   if (!t.some) {
     for (int c = max(from, row.shift) + tid; c < to; c += T) out[c - row.shift] = 0.0f;
@@ -418,9 +435,12 @@ __global__ void __launch_bounds__(threads_of(T)) distill_backward_kernel(
   }
   const float scale = __fmul_rn(tau, dloss[r]);
   const float4 st = *reinterpret_cast<const float4 *>(stats + r * 4);
-  const Slope s{__fdiv_rn(kLog2e, tau),        st.x, __fmul_rn(st.y, kLog2e), __fmul_rn(scale, t.mass), st.z,
+  if (TAIL) t.settle(log_tail_mass(st.x, st.y, st.z, st.w, tau));
+  const Slope s{__fdiv_rn(kLog2e, tau),        st.x, __fmul_rn(st.y, kLog2e), __fmul_rn(scale, t.mass()), st.z,
                 __fmul_rn(st.w, kLog2e), __fmul_rn(scale, t.tail)};
-  const bool vec = (((uintptr_t)out >> 2) & 3) == (uintptr_t)row.shift, tail = TAIL && t.tail != 0.0f;
+  const bool vec = (((uintptr_t)out >> 2) & 3) == (uintptr_t)row.shift;
+  // (outside maximum -inf: every column outside is masked, and 0 - 0)
+  const bool tail = TAIL && t.tail != 0.0f && st.z != -INFINITY;
   if (vec && tail) stream_slope<true, true, T>(out, row, s, from, to, tid);
   else if (vec) stream_slope<false, true, T>(out, row, s, from, to, tid);
   else if (tail) stream_slope<true, false, T>(out, row, s, from, to, tid);

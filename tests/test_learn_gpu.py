@@ -730,6 +730,62 @@ def test_distill_masks(capi, tail):
         assert loss[7] == 0 and not dz[7].any()
 
 
+# a warp, 128 threads, a CTA and a cluster a row; every column named, or the others masked
+@pytest.mark.parametrize("r,v,k", [(1200, 64, 64), (1200, 256, 256), (300, 64, 64), (300, 1000, 1000), (3, 2000, 1024), (460, 6000, 100),
+                                   (150, 6000, 64), (3, 40000, 64), (2, 40000, 1024)])
+@pytest.mark.parametrize("mask", [-np.inf, np.finfo(np.float32).min, -1e6])
+def test_distill_list_with_the_whole_mass(capi, r, v, k, mask):
+    """The teacher's list holds its whole mass, and the student has none outside it: what rounding
+    leaves of 1 - sum p is no mass. The result is that of the list alone; masked columns have no
+    gradient."""
+    rng = np.random.default_rng(r + v + k)
+    z = (rng.standard_normal((r, v)) * 2).astype(np.float32)
+    ids = np.stack([rng.permutation(v)[:k] for _ in range(r)])
+    t = (rng.standard_normal((r, k)) * 2 + rng.uniform(-20, 20, (r, 1))).astype(np.float32)
+    g = rng.standard_normal(r).astype(np.float32)
+    outside = np.ones((r, v), bool)
+    np.put_along_axis(outside, ids, False, 1)
+    z[outside] = mask
+    t64 = t.astype(np.float64)
+    lse = (np.log(np.exp(t64 - t64.max(1, keepdims=True)).sum(1)) + t64.max(1)).astype(np.float32)
+    loss, dz = run_distill(capi, z, ids, t, 1.0, lse, g)
+    loss64, dz64 = O.distill(z, ids, t, 1.0, None, g)
+    e_loss, e_dz = distill_bounds(z, ids, t, 1.0, None, g)
+    # p from lse in place of the list's own sum: lse is rounded, and so is the argument
+    m = z.max(1, keepdims=True).astype(np.float64)
+    logq = z - m - np.log(np.exp(z - m).sum(1, keepdims=True))
+    logp = t64 - lse[:, None].astype(np.float64)
+    p, at = np.exp(logp), np.take_along_axis(logq, ids, 1)
+    e_p = p * (3 * U * (np.abs(t64) + np.abs(lse[:, None])) + 4 * U)
+    e_loss = e_loss + (e_p * (np.abs(logp - at) + 1)).sum(1)
+    more = np.exp(logq) * e_p.sum(1, keepdims=True)
+    np.put_along_axis(more, ids, np.take_along_axis(more, ids, 1) + e_p, 1)
+    close(loss, loss64, e_loss, "loss")
+    close(dz, dz64, e_dz + np.abs(g[:, None]) * more, "dz")
+    assert not dz[outside].any()
+
+
+@pytest.mark.parametrize("r,v,k", [(1200, 300, 20), (5, 300, 20), (150, 6000, 20), (3, 40000, 64)])
+def test_distill_mass_outside_that_the_student_lacks(capi, r, v, k):
+    """A tail of the teacher where the student's columns are all at -inf: the loss is infinite, the
+    entries' gradient is q - p, and the masked columns have none."""
+    rng = np.random.default_rng(v + k)
+    z = np.full((r, v), -np.inf, np.float32)
+    ids = np.stack([rng.permutation(v)[:k] for _ in range(r)])
+    np.put_along_axis(z, ids, (rng.standard_normal((r, k)) * 2).astype(np.float32), 1)
+    t = rng.standard_normal((r, k)).astype(np.float32)
+    lse = np.log(np.exp(t.astype(np.float64)).sum(1) / 0.7).astype(np.float32)
+    g = rng.standard_normal(r).astype(np.float32)
+    loss, dz = run_distill(capi, z, ids, t, 1.0, lse, g)
+    assert (loss == np.inf).all()
+    z64 = np.take_along_axis(z, ids, 1).astype(np.float64)
+    q, p = np.exp(z64) / np.exp(z64).sum(1, keepdims=True), np.exp(t.astype(np.float64) - lse[:, None])
+    want = np.zeros((r, v))
+    np.put_along_axis(want, ids, (q - p) * g[:, None], 1)
+    # q: its argument |z - max| + log sum <= 20, 2^x, the sum; P and p as in distill_bounds
+    close(dz, want, 200 * U * np.abs(g[:, None]) * (want != 0), "dz")
+
+
 def test_distill_student_without_mass(capi):
     """The student gives a teacher's entry no probability: the loss is infinite, the gradient
     q - p is not."""
