@@ -478,7 +478,7 @@ int fz_expert_combine_backward(float *drows, float *dweights, const float *dout,
 /* Distillation from a teacher's top logits; no reference counterpart (Nova's only loss is
  * the mean squared error). Per row r: z = logits[r, 0..vocab) (row pitch ld >= vocab), the
  * teacher's k entries (ids[r, i], teacher[r, i]); an entry whose id lies outside
- * [0, vocab) is padding. With tau = temperature >= 1e-18, q = softmax(z / tau) and
+ * [0, vocab) is padding. With tau = temperature in [1e-18, 1e18], q = softmax(z / tau) and
  *   teacher_lse NULL: p = softmax(teacher / tau) over the row's entries;
  *   else: p = exp(teacher / tau - teacher_lse[r]) (the logsumexp of the teacher's whole
  *   vocabulary over tau), the rest pT = max(0, 1 - sum p) on one bucket, against the

@@ -483,7 +483,7 @@ int check_distill(const char *who, int64_t rows, int64_t vocab, int64_t k, int64
   FZ_REQUIRE(ld >= vocab, name + ": row pitch below vocab");
   FZ_REQUIRE(rows <= INT_MAX / 8, name + ": too many rows");
   // (its square, the loss's factor, has to be a normal number)
-  FZ_REQUIRE(temperature >= 1e-18f && temperature < INFINITY, name + ": temperature must be in [1e-18, inf)");
+  FZ_REQUIRE(temperature >= 1e-18f && temperature <= 1e18f, name + ": temperature must be in [1e-18, 1e18]");
   return FZ_OK;
 }
 

@@ -8,7 +8,6 @@
 #include <pybind11/pybind11.h>
 #include <pybind11/stl.h>
 
-#include <cmath>
 #include <numeric>
 #include <optional>
 #include <random>
@@ -158,8 +157,8 @@ ADTensor expert_combine(ADTensor &rows, std::shared_ptr<ExpertPlan> plan, ADTens
 // The teacher's values are constants: no gradient reaches them.
 ADTensor distill(ADTensor &logits, const Indices &ids, const ADTensor &teacher, float temperature,
                  const ADTensor *teacher_lse) {
-  if (!(temperature > 0.0f) || std::isinf(temperature))
-    throw std::invalid_argument("distill: temperature must be positive and finite");
+  if (!(temperature >= 1e-18f && temperature <= 1e18f))  // its square is a normal number
+    throw std::invalid_argument("distill: temperature must be in [1e-18, 1e18]");
   auto value = [](const ADTensor &t) { return RawTensor(t.raw().expr(), t.raw().dtype(), t.raw().device()); };
   LearnParam l;
   l.ids = ids;

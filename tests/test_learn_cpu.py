@@ -88,6 +88,24 @@ def test_c_abi_refuses(name, args, says):
     assert says in lib.fz_last_error().decode()
 
 
+@pytest.mark.parametrize("tau", [-1.0, 9e-19, 1.1e18, 1.9e19, 3e38, float("inf")])
+def test_distill_refuses_temperatures_without_a_square(F, tau):
+    """The loss's factor tau^2 has to be a normal number: outside [1e-18, 1e18] both directions and
+    the module refuse, at the ends they go on to their other checks."""
+    from nova_b200 import capi
+
+    lib = capi.lib()
+    for name, args in (("fz_distill", lambda t: [P, None, P, 8, P, P, None, 2, 8, 3, t, None]),
+                       ("fz_distill_backward", lambda t: [P, 8, P, None, P, 8, P, P, None, 2, 8, 3, t, None])):
+        assert getattr(lib, name)(*args(tau)) == 1
+        assert "temperature must be in [1e-18, 1e18]" in lib.fz_last_error().decode()
+        for end in (1e-18, 1e18):
+            assert getattr(lib, name)(*args(end)) == 1 and "null" in lib.fz_last_error().decode()
+    T = learn_cases.T
+    with pytest.raises(ValueError, match="temperature"):
+        F.distill(T(F, np.ones((4, 6))), F.Indices(np.zeros((4, 2), np.int64)), T(F, np.ones((4, 2))), temperature=tau)
+
+
 def test_empty_calls_launch_nothing():
     """No tokens, rows or elements: nothing to do, and no pointers needed."""
     from nova_b200 import capi
