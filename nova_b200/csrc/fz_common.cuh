@@ -25,10 +25,8 @@ void note_launch(int n = 1);
 
 cudaStream_t resolve(void *stream);
 // Per-device int in global memory where kernels with bounded waits record a
-// nonzero code when a wait expires; read and cleared by fz_kernel_status.
+// nonzero code when a wait expires; read and cleared by fz_kernel_status. Allocates nothing.
 int device_error_word(int **word);
-// The same without allocating: null if this device has none yet.
-int *device_error_word_if_any();
 int num_sms();
 
 // Fused-program support shared by the elementwise and GEMM-epilogue compilers

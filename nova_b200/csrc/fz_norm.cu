@@ -350,7 +350,7 @@ struct Norm {
   int groups, c;  // c: channels a group
   float m, inv_m, eps;  // inv_m = 1 / m
   int act;
-  int *err;  // where a wait that gave up is recorded, or null
+  int *err;  // tiles in a cluster: where a wait that gave up is recorded
 };
 
 // ---------------------------------------------------------------- row kernels
@@ -1003,7 +1003,7 @@ __device__ __forceinline__ void exchange_wait(Exchange &x, int parity, int phase
     asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
     if (t - t0 > kWaitNs) {
       *gave_up = 1;
-      if (err) atomicCAS(err, 0, kErrNormExchange);
+      atomicCAS(err, 0, kErrNormExchange);
     }
   }
 }
@@ -1548,14 +1548,8 @@ int run_rows(const Norm &a, const Plan &p, bool backward, cudaStream_t s) {
 
 template <int V, int MODE, bool MIXED, int SHORT = 0>
 int run_tile(Norm a, const Plan &p, bool backward, cudaStream_t s) {
-  // the word for waits that give up; not allocated while the stream is being captured
-  a.err = fz::device_error_word_if_any();
-  if (!a.err && MODE == kInCluster) {
-    cudaStreamCaptureStatus capture;
-    FZ_CUDA(cudaStreamIsCapturing(s, &capture));
-    if (capture == cudaStreamCaptureStatusNone)
-      if (int rc = fz::device_error_word(&a.err)) return rc;
-  }
+  if (MODE == kInCluster)
+    if (int rc = fz::device_error_word(&a.err)) return rc;
   const auto kernel = backward ? norm_tile_backward_kernel<V, MODE, MIXED, SHORT> : norm_tile_kernel<V, MODE, MIXED, SHORT>;
   const int smem = (held(V, backward) >> SHORT) * kTileThreads * V * 4 * (backward ? 2 : 1);
   const int k = MODE == kInCluster ? p.t.k : 1;

@@ -90,6 +90,9 @@ cudaStream_t resolve(void *stream) {
   return t_stream[d];
 }
 
+// Part of the library's image on each device: an allocation on first use would fail, and spoil
+// the capture, while any stream of the process is being captured in the global mode.
+__device__ int g_error_word;
 static int *g_err_word[kMaxDevices] = {};
 static std::mutex g_err_mu;
 
@@ -97,21 +100,13 @@ int device_error_word(int **word) {
   int d = current_device();
   std::lock_guard<std::mutex> lk(g_err_mu);
   if (!g_err_word[d]) {
-    int *p = nullptr;
-    cudaError_t e = cudaMalloc(&p, sizeof(int));
-    if (e != cudaSuccess) return cuda_fail(e, "cudaMalloc(error word)", __FILE__, __LINE__);
-    e = cudaMemset(p, 0, sizeof(int));
-    if (e != cudaSuccess) return cuda_fail(e, "cudaMemset(error word)", __FILE__, __LINE__);
-    g_err_word[d] = p;
+    void *p = nullptr;
+    cudaError_t e = cudaGetSymbolAddress(&p, g_error_word);
+    if (e != cudaSuccess) return cuda_fail(e, "cudaGetSymbolAddress(error word)", __FILE__, __LINE__);
+    g_err_word[d] = (int *)p;
   }
   *word = g_err_word[d];
   return FZ_OK;
-}
-
-int *device_error_word_if_any() {
-  int d = current_device();
-  std::lock_guard<std::mutex> lk(g_err_mu);
-  return g_err_word[d];
 }
 
 int num_sms() {

@@ -923,6 +923,64 @@ def test_two_streams_and_graph_replay(capi):
     del graph  # nothing captured outlives its buffers
 
 
+FIRST_CALLS = """
+import sys
+import torch
+from nova_b200 import capi
+L = capi.lib()
+b, n, c, g = 2, 4096, 64, 8  # a cluster a sample
+x = torch.randn(b, n, c, device="cuda")
+size = capi.group_norm_workspace(b, n, c, g, True)
+work, stats, gb = torch.empty(size // 4 + 4, device="cuda"), torch.empty(2, b, g, device="cuda"), torch.empty(2, c, device="cuda")
+y, dx, other = torch.empty_like(x), torch.empty_like(x), torch.zeros(4, device="cuda")
+p = lambda t: t.data_ptr()
+def call(s):
+    capi.check(L.fz_group_norm(p(y), p(stats[0]), p(stats[1]), p(x), None, None, b, n, c, g, 1e-5, 2, p(work), size, s))
+    capi.check(L.fz_group_norm_backward(p(dx), p(gb[0]), p(gb[1]), p(x), p(x), p(stats[0]), p(stats[1]), None, None, b, n, c, g, 2,
+                                        p(work), size, s))
+side, cap = torch.cuda.Stream(), torch.cuda.Stream()
+graph = torch.cuda.CUDAGraph()
+torch.cuda.synchronize()
+with torch.cuda.graph(graph, stream=cap, capture_error_mode="global"):
+    other += 1
+    if sys.argv[1] == "beside":
+        call(side.cuda_stream)
+    else:
+        call(cap.cuda_stream)
+torch.cuda.synchronize()
+graph.replay()
+torch.cuda.synchronize()
+assert (other == 1).all()
+first = [t.clone() for t in (y, dx, gb)]
+for t in (y, dx, gb):
+    t.zero_()
+torch.cuda.synchronize()
+call(side.cuda_stream)
+torch.cuda.synchronize()
+assert all(torch.equal(u, v) for u, v in zip(first, (y, dx, gb)))
+want = torch.nn.functional.silu(torch.nn.functional.group_norm(x.double().transpose(1, 2), g, eps=1e-5)).transpose(1, 2)
+assert (y - want).abs().max() < 1e-4  # values up to 5: some 300 roundings, of sums at most 100 deep
+capi.check(L.fz_kernel_status())
+del graph
+"""
+
+
+@pytest.mark.parametrize("where", ["beside", "captured"])
+def test_first_norm_of_a_process_during_a_capture(capi, where):
+    """The first group norm of a process, while another stream is captured in the global mode
+    (which forbids allocations in the whole process), and captured itself."""
+    import os
+    import pathlib
+    import subprocess
+    import sys
+
+    pytest.importorskip("torch")
+    root = pathlib.Path(__file__).resolve().parent.parent
+    r = subprocess.run([sys.executable, "-c", FIRST_CALLS, where], cwd=root, capture_output=True, text=True, timeout=300,
+                       env={**os.environ, "PYTHONPATH": str(root)})
+    assert r.returncode == 0, r.stderr[-2000:]
+
+
 def test_norm_and_distill_past_32_bit_offsets(capi):
     """More than 2^31 values: the last rows and samples come out as they do in a small call."""
     torch = pytest.importorskip("torch")
