@@ -826,7 +826,7 @@ __device__ __forceinline__ bool behind(int i, const Tile<V> &me) {
 }
 
 // A tile's vectors to a thread's place in shared memory ([held][threads] vectors), and back.
-// Behind a thread's rows x is 0.
+// Behind a thread's rows they are `none`.
 template <int V, int N>
 __device__ __forceinline__ void fetch_tile(float *fifo, const float *p, const Tile<V> &me, int64_t step) {
   const float *q = p + me.at;
@@ -838,11 +838,12 @@ __device__ __forceinline__ void fetch_tile(float *fifo, const float *p, const Ti
   }
 }
 template <int V, int N>
-__device__ __forceinline__ void take_tile(Vec<V> (&x)[N], const float *fifo, const Tile<V> &me) {
+__device__ __forceinline__ void take_tile(Vec<V> (&x)[N], const float *fifo, const Tile<V> &me,
+                                          const Vec<V> &none) {
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     if (behind<V, N>(i, me)) break;
-    x[i] = i < me.mine ? load<V>(fifo + (i * kTileThreads + (int)threadIdx.x) * V) : splat<V>(0.0f);
+    x[i] = i < me.mine ? load<V>(fifo + (i * kTileThreads + (int)threadIdx.x) * V) : none;
   }
 }
 
@@ -1042,7 +1043,7 @@ __global__ void __launch_bounds__(kTileThreads, kTileCtas + SHORT) norm_tile_ker
     walk.advance(t);
     Vec<V> x[N];
     copy_wait<0>();
-    take_tile(x, fifo, me);
+    take_tile(x, fifo, me, splat<V>(0.0f));
     if (walk.left) {
       next = walk.get(a, t);
       fetch_tile<V, N>(fifo, a.x, next, step);
@@ -1193,9 +1194,12 @@ __global__ void __launch_bounds__(kTileThreads, kTileCtas + SHORT) norm_tile_bac
       fetch_tile<V, N>(fifo, a.x, next, step);
       fetch_tile<V, N>(fifo + kStage, a.dy, next, step);
       const int64_t team = (int64_t)next.b * a.groups + next.g0;
-      const int l = next.mine ? place.lo : 0, h = next.mine ? place.hi : 0;
-      next_lo = make_float2(a.mean_in[team + l], a.rstd_in[team + l]);
-      if (MIXED) next_hi = make_float2(a.mean_in[team + h], a.rstd_in[team + h]);
+      // a thread without rows takes part in its column's sums all the same: no group's statistics
+      next_lo = next_hi = make_float2(0.0f, 0.0f);
+      if (next.mine) {
+        next_lo = make_float2(a.mean_in[team + place.lo], a.rstd_in[team + place.lo]);
+        if (MIXED) next_hi = make_float2(a.mean_in[team + place.hi], a.rstd_in[team + place.hi]);
+      }
     }
     copy_commit();
   };
@@ -1209,12 +1213,13 @@ __global__ void __launch_bounds__(kTileThreads, kTileCtas + SHORT) norm_tile_bac
     walk.advance(t);
     Vec<V> x[N], d[N], db = splat<V>(0.0f), dg = db;
     copy_wait<0>();
-    take_tile(x, fifo, me);
-    take_tile(d, fifo + kStage, me);
+    // behind a thread's rows x is the mean and dy 0: xh is 0 there (a mean without x, times rstd,
+    // may be infinite), and so is what they add to their column's sums
+    take_tile(x, fifo, me, place.spread(lo.x, hi.x));
+    take_tile(d, fifo + kStage, me, splat<V>(0.0f));
     fetch();
     const Vec<V> rstd = place.spread(lo.y, hi.y);
     {
-      // behind a thread's rows x and dy are 0, and so is what they add to its columns' sums
       const Vec<V> ga = load_or<V>(a.gamma && me.mine ? a.gamma + me.channel : nullptr, 1.0f);
       const Vec<V> be = load_or<V>(a.beta && me.mine ? a.beta + me.channel : nullptr, 0.0f);
       const Vec<V> minus = place.spread(-lo.x, -hi.x);

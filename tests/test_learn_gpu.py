@@ -258,6 +258,56 @@ def test_group_norm_nan_stays_in_its_group(capi, shape):
     np.testing.assert_array_equal(y[~hit], clean[~hit])
 
 
+# the last of a sample's tiles, in a cluster and in two launches, has fewer rows than a CTA's threads
+@pytest.mark.parametrize("shape", [(1, 181, 260, 4), (1, 961, 260, 4), (2, 181, 260, 4), (3, 64, 1020, 4), (2, 300, 300, 5),
+                                   (1, 40000, 28, 4)], ids=str)
+@pytest.mark.parametrize("act", ["none", "relu", "silu", "gelu"])
+@pytest.mark.parametrize("off", [0, 1])
+def test_group_norm_gradients_of_a_bad_group_stay_in_it(capi, shape, act, off):
+    """NaN in each of the groups in turn: dx, dgamma and dbeta of the others are bit for bit what they
+    are without it."""
+    b, n, c, groups = shape
+    per = c // groups
+    rng = np.random.default_rng(17)
+    x, dy = rng.standard_normal(shape[:3]).astype(np.float32), rng.standard_normal(shape[:3]).astype(np.float32)
+    clean = run_norm(capi, x, None, None, groups, 1e-5, act, dy, off)
+    for g in range(groups):
+        bad = x.copy()
+        bad[b - 1, n // 2, g * per] = np.nan
+        got = run_norm(capi, bad, None, None, groups, 1e-5, act, dy, off)
+        hit = np.zeros((b, n, c), bool)
+        hit[b - 1, :, g * per:(g + 1) * per] = True
+        np.testing.assert_array_equal(got[3][~hit], clean[3][~hit])
+        assert np.isnan(got[3][hit]).all()
+        for which in (4, 5):
+            np.testing.assert_array_equal(np.delete(got[which], np.s_[g * per:(g + 1) * per]),
+                                          np.delete(clean[which], np.s_[g * per:(g + 1) * per]))
+
+
+@pytest.mark.parametrize("shape,value", [((2, 300, 1, 1), 1e36), ((3, 181, 260, 4), 2e34), ((2, 2000, 12, 2), 3e33)], ids=str)
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+def test_group_norm_gradients_of_a_large_constant(capi, shape, value, act):
+    """Equal values so large that value * rstd overflows: x - mean is 0, and the gradients are finite.
+    (eps is chosen so that it does, while no sum of the values does.)"""
+    b, n, c, groups = shape
+    rng = np.random.default_rng(18)
+    x = np.full(shape[:3], value, np.float32)
+    x = np.float32(2.0 ** np.floor(np.log2(x)))  # a power of two: its sums and mean are exact
+    eps = np.float32((float(x.flat[0]) / 1e39) ** 2)
+    dy = rng.standard_normal(shape[:3]).astype(np.float32)
+    got = run_norm(capi, x, None, None, groups, eps, act, dy)
+    rstd = 1 / np.sqrt(np.float64(eps))
+    # xh = 0 and v = 0: dv = dy / 2, dx = rstd (dv - mean dv), dgamma = 0, dbeta = sum dv
+    dv = dy.astype(np.float64) / 2
+    g4 = dv.reshape(b, n, groups, c // groups)
+    mean, size = g4.mean(axis=(1, 3), keepdims=True), np.abs(g4).mean(axis=(1, 3), keepdims=True)
+    m = n * c // groups
+    want = rstd * (g4 - mean).reshape(x.shape)
+    close(got[3], want, rstd * U * (16 * np.abs(g4) + (m / 32 + 48) * size).reshape(x.shape), "dx")
+    assert not got[4].any()
+    close(got[5], dv.sum(axis=(0, 1)), (b * n / 8 + 64) * U * np.abs(dv).sum(axis=(0, 1)), "dbeta")
+
+
 def test_group_norm_partial_results(capi):
     """mean and rstd, and the parameters' gradients, are optional; an empty batch has zero
     gradients."""
