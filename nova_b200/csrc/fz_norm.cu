@@ -536,6 +536,10 @@ __global__ void __launch_bounds__(kRowThreads, row_ctas(false, NV)) norm_rows_ke
   copy_wait<0>();
 }
 
+// Sums of many terms are taken in two levels, so that their rounding errors grow with the number of
+// blocks of kNear terms and not with that of the terms.
+constexpr int kNear = 16;
+
 // fold: teams of a CTA that share a group and whose channel sums are added up in the CTA.
 template <int V, int P, int NV>
 __global__ void __launch_bounds__(kRowThreads, row_ctas(true, NV))
@@ -583,62 +587,92 @@ __global__ void __launch_bounds__(kRowThreads, row_ctas(true, NV))
   Vec<V> db[NV], dg[NV];
 #pragma unroll
   for (int i = 0; i < NV; ++i) db[i] = dg[i] = splat<V>(0.0f);
-  int s = 0;
-  for (int b0 = 0; b0 < (int)a.batch; b0 += step, s = s + 1 < S ? s + 1 : 0) {
-    const int b = b0 + t.part;
-    Vec<V> x[U][NV], d[U][NV];
-    float rstd[U], s1[U], s2[U];
-    float minus[U];
-    copy_wait<S - 1>();
+  // The sums of earlier blocks of steps. Four and eight vectors of 4 a lane leave no registers for
+  // them: there they stay in memory (the asm hides where `sums` points), and a block has 64 steps,
+  // for a block's end stops the stream of loads for 5 us ([16384, 8192] in one group: 463 us with
+  // one block, 507 with blocks of 16).
+  constexpr bool kInMemory = V == 4 && NV > 2;
+  constexpr int kBlock = kInMemory ? 64 : kNear;
+  Vec<V> blocks[2 * NV], *sums = blocks;
+  if constexpr (kInMemory) asm volatile("" : "+l"(sums)::"memory");
+  bool carried = false;
+  const auto carry = [&](bool last) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      minus[u] = -next_mean[u];
-      rstd[u] = next_rstd[u];
-      s1[u] = s2[u] = 0.0f;
-#pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        const bool in = b + u * parts < batch && t.at[i] >= 0;
-        x[u][i] = in ? load<V>(mine + ((s * 2 * U + u) * NV + i) * kRowThreads * V) : splat<V>(0.0f);
-        d[u][i] = in ? load<V>(mine + (((s * 2 + 1) * U + u) * NV + i) * kRowThreads * V) : splat<V>(0.0f);
+    for (int i = 0; i < NV; ++i) {
+      if (carried) {
+        sum_into(db[i], sums[2 * i]);
+        sum_into(dg[i], sums[2 * i + 1]);
+      }
+      if (!last) {
+        sums[2 * i] = db[i];
+        sums[2 * i + 1] = dg[i];
+        db[i] = dg[i] = splat<V>(0.0f);
       }
     }
-    fetch(s, b + S * step);
-    fetch_stats(b + step);
-    with_activation(a.act, [&](auto act) {
+    carried = true;
+  };
+  int s = 0;
+  for (int b0 = 0; b0 < (int)a.batch;) {
+    if (b0) carry(false);
+    const int end = (int)min((int64_t)a.batch, b0 + (int64_t)kBlock * step);
+#pragma unroll 1
+    for (; b0 < end; b0 += step, s = s + 1 < S ? s + 1 : 0) {
+      const int b = b0 + t.part;
+      Vec<V> x[U][NV], d[U][NV];
+      float rstd[U], s1[U], s2[U];
+      float minus[U];
+      copy_wait<S - 1>();
 #pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        if (t.at[i] < 0) continue;
-        Vec<V> ga, be, b_sum = splat<V>(0.0f), g_sum = b_sum;  // of U teams, then of all
-        affine.get(a, t.channel, i, ga, be);
+      for (int u = 0; u < U; ++u) {
+        minus[u] = -next_mean[u];
+        rstd[u] = next_rstd[u];
+        s1[u] = s2[u] = 0.0f;
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-          // behind the batch x, d, mean and rstd are 0, and so is all that they give
-          gradient<decltype(act)::value>(x[u][i], d[u][i], b_sum, g_sum, splat<V>(minus[u]), splat<V>(rstd[u]), ga, be);
-          Vec<V> w;
-#pragma unroll
-          for (int j = 0; j < Vec<V>::N; ++j) w.p[j] = mul2(d[u][i].p[j], x[u][i].p[j]);
-          s1[u] = __fadd_rn(s1[u], total(d[u][i]));
-          s2[u] = __fadd_rn(s2[u], total(w));
+        for (int i = 0; i < NV; ++i) {
+          const bool in = b + u * parts < batch && t.at[i] >= 0;
+          x[u][i] = in ? load<V>(mine + ((s * 2 * U + u) * NV + i) * kRowThreads * V) : splat<V>(0.0f);
+          d[u][i] = in ? load<V>(mine + (((s * 2 + 1) * U + u) * NV + i) * kRowThreads * V) : splat<V>(0.0f);
         }
-        sum_into(db[i], b_sum);
-        sum_into(dg[i], g_sum);
       }
-    });
-    const auto over_m = [&](float v) { return __fmul_rn(v, -a.inv_m); };
-    team_sums<P, U>(s1, sh, over_m);
-    team_sums<P, U>(s2, sh, over_m);
+      fetch(s, b + S * step);
+      fetch_stats(b + step);
+      with_activation(a.act, [&](auto act) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (b + u * parts < batch)
+        for (int i = 0; i < NV; ++i) {
+          if (t.at[i] < 0) continue;
+          Vec<V> ga, be, b_sum = splat<V>(0.0f), g_sum = b_sum;  // of U teams, then of all
+          affine.get(a, t.channel, i, ga, be);
 #pragma unroll
-        for (int i = 0; i < NV; ++i)
-          if (t.at[i] >= 0)
-            store(to + t.at[i], finish(x[u][i], d[u][i], splat<V>(s1[u]), splat<V>(s2[u]), splat<V>(rstd[u])));
-      to += hop;
+          for (int u = 0; u < U; ++u) {
+            // behind the batch x, d, mean and rstd are 0, and so is all that they give
+            gradient<decltype(act)::value>(x[u][i], d[u][i], b_sum, g_sum, splat<V>(minus[u]), splat<V>(rstd[u]), ga, be);
+            Vec<V> w;
+#pragma unroll
+            for (int j = 0; j < Vec<V>::N; ++j) w.p[j] = mul2(d[u][i].p[j], x[u][i].p[j]);
+            s1[u] = __fadd_rn(s1[u], total(d[u][i]));
+            s2[u] = __fadd_rn(s2[u], total(w));
+          }
+          sum_into(db[i], b_sum);
+          sum_into(dg[i], g_sum);
+        }
+      });
+      const auto over_m = [&](float v) { return __fmul_rn(v, -a.inv_m); };
+      team_sums<P, U>(s1, sh, over_m);
+      team_sums<P, U>(s2, sh, over_m);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (b + u * parts < batch)
+#pragma unroll
+          for (int i = 0; i < NV; ++i)
+            if (t.at[i] >= 0)
+              store(to + t.at[i], finish(x[u][i], d[u][i], splat<V>(s1[u]), splat<V>(s2[u]), splat<V>(rstd[u])));
+        to += hop;
+      }
     }
   }
   copy_wait<0>();
   if (!a.part) return;
+  carry(true);
   // Per channel, over the rows of the sample and the CTA's `fold` teams of the group, in
   // order: part[row][2][channels]. The teams' sums (at most 8192 floats) take the place of
   // the first stage.
@@ -1194,12 +1228,9 @@ __global__ void __launch_bounds__(kTileThreads, kTileCtas + SHORT) norm_tile_bac
       fetch_tile<V, N>(fifo, a.x, next, step);
       fetch_tile<V, N>(fifo + kStage, a.dy, next, step);
       const int64_t team = (int64_t)next.b * a.groups + next.g0;
-      // a thread without rows takes part in its column's sums all the same: no group's statistics
-      next_lo = next_hi = make_float2(0.0f, 0.0f);
-      if (next.mine) {
-        next_lo = make_float2(a.mean_in[team + place.lo], a.rstd_in[team + place.lo]);
-        if (MIXED) next_hi = make_float2(a.mean_in[team + place.hi], a.rstd_in[team + place.hi]);
-      }
+      const int l = next.mine ? place.lo : 0, h = next.mine ? place.hi : 0;
+      next_lo = make_float2(a.mean_in[team + l], a.rstd_in[team + l]);
+      if (MIXED) next_hi = make_float2(a.mean_in[team + h], a.rstd_in[team + h]);
     }
     copy_commit();
   };
@@ -1230,6 +1261,7 @@ __global__ void __launch_bounds__(kTileThreads, kTileCtas + SHORT) norm_tile_bac
           gradient<decltype(act)::value>(x[i], d[i], db, dg, minus, rstd, ga, be);
         }
       });
+      if (!me.mine) db = dg = splat<V>(0.0f);  // no rows: the statistics were another group's
     }
     if (MODE != kWhole) column_sums(db, dg, sh, a, me, t, walk);
     if (joined) {
@@ -1283,7 +1315,7 @@ __global__ void __launch_bounds__(kTileThreads, kTileCtas + SHORT) norm_tile_bac
 
 // dbeta[c] and dgamma[c] from part[rows][2][channels]: 32 channels a CTA, the rows over its
 // warps and over the CTAs of a cluster, which fold their sums through distributed shared
-// memory in order.
+// memory in order; a warp's rows in blocks of kNear.
 constexpr int kFoldWarps = 16;
 __global__ void __launch_bounds__(kFoldWarps * 32) norm_fold_kernel(float *__restrict__ dgamma,
                                                                     float *__restrict__ dbeta,
@@ -1298,12 +1330,28 @@ __global__ void __launch_bounds__(kFoldWarps * 32) norm_fold_kernel(float *__res
   const int64_t ch = (int64_t)(blockIdx.x / ctas) * 32 + lane;
   float u = 0.0f, w = 0.0f;
   if (ch < channels) {
-#pragma unroll 8
-    for (int r = rank * kFoldWarps + warp; r < rows; r += ctas * kFoldWarps) {
-      const float *at = part + (int64_t)r * 2 * channels + ch;
-      u = __fadd_rn(u, at[0]);
-      w = __fadd_rn(w, at[channels]);
+    const int step = ctas * kFoldWarps;
+    const int64_t hop = (int64_t)step * 2 * channels;
+    int r = rank * kFoldWarps + warp;
+    const float *at = part + (int64_t)r * 2 * channels + ch;
+    for (; r < rows - (kNear - 1) * step; r += kNear * step) {
+      float us = 0.0f, ws = 0.0f;
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        float x[kNear / 2], y[kNear / 2];  // in flight together
+#pragma unroll
+        for (int i = 0; i < kNear / 2; ++i, at += hop) x[i] = at[0], y[i] = at[channels];
+#pragma unroll
+        for (int i = 0; i < kNear / 2; ++i) us = __fadd_rn(us, x[i]), ws = __fadd_rn(ws, y[i]);
+      }
+      u = __fadd_rn(u, us);
+      w = __fadd_rn(w, ws);
     }
+    float us = 0.0f, ws = 0.0f;
+#pragma unroll 8
+    for (; r < rows; r += step, at += hop) us = __fadd_rn(us, at[0]), ws = __fadd_rn(ws, at[channels]);
+    u = __fadd_rn(u, us);
+    w = __fadd_rn(w, ws);
   }
   sh[0][warp][lane] = u;
   sh[1][warp][lane] = w;

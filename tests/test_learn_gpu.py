@@ -308,6 +308,47 @@ def test_group_norm_gradients_of_a_large_constant(capi, shape, value, act):
     close(got[5], dv.sum(axis=(0, 1)), (b * n / 8 + 64) * U * np.abs(dv).sum(axis=(0, 1)), "dbeta")
 
 
+# 1, 2, 4 and 8 vectors a lane of a warp, 2 a thread of a CTA, so that each thread adds up some 250
+# steps; how many teams of a group are in flight on 148 SMs, how many of them a step takes, and the
+# steps of a block
+@pytest.mark.parametrize("shape,parts,at_once,block", [((65536, 1, 4096, 32), 74, 4, 16), ((40000, 1, 8192, 32), 74, 2, 16),
+                                                       ((20000, 1, 16384, 32), 74, 1, 64), ((10000, 1, 32768, 32), 37, 1, 64),
+                                                       ((40000, 1, 4096, 2), 148, 1, 16), ((300000, 1, 512, 64), 296, 4, 16)], ids=str)
+def test_group_norm_parameter_sums_keep_their_digits(capi, shape, parts, at_once, block):
+    """One large dy before many ones: a chain of additions to it loses each of them, blocks of
+    steps do not. x is +-1, so xh is too (eps = 0) and every product is exact. The bound: the
+    teams of a step, the steps of a block, a thread's blocks, and the fold over the teams in flight:
+    16 rows a block, their blocks, 16 warps, 8 CTAs."""
+    torch = pytest.importorskip("torch")
+    L = capi.lib()
+    b, n, c, groups = shape
+    x = torch.ones(b, n, c, device="cuda")
+    x[:, :, 1::2] = -1
+    dy = torch.ones_like(x)
+    big = 2.0 ** 24 * at_once
+    dy[0] = big
+    dy[0, :, c // 2:] = 1
+    dy[b - 1, :, c // 2:] = big
+    y, dx = torch.empty_like(x), torch.empty_like(x)
+    stats, gb = torch.empty(2, b, groups, device="cuda"), torch.empty(2, c, device="cuda")
+    size = capi.group_norm_workspace(b, n, c, groups, True)
+    work = torch.empty(size // 4 + 4, device="cuda")
+    at = lambda t: t.data_ptr()  # noqa: E731
+    capi.check(L.fz_group_norm(at(y), at(stats[0]), at(stats[1]), at(x), None, None, b, n, c, groups, 0.0, 0, at(work), size, 1))
+    capi.check(L.fz_group_norm_backward(at(dx), at(gb[0]), at(gb[1]), at(dy), at(x), at(stats[0]), at(stats[1]), None, None, b, n, c,
+                                        groups, 0, at(work), size, 1))
+    torch.cuda.synchronize()
+    assert torch.equal(y, x)
+    sign = x[0, 0].double().cpu().numpy()
+    got = gb.double().cpu().numpy()
+    want = big + b * n - 1
+    bound = (at_once + block + b / parts / at_once / block + 1 + 16 + 16 + 16 + 8) * U * want
+    close(got[0], sign * want, bound, "dgamma")
+    close(got[1], np.full(c, want), bound, "dbeta")
+    del x, y, dx, dy, work
+    torch.cuda.empty_cache()
+
+
 def test_group_norm_partial_results(capi):
     """mean and rstd, and the parameters' gradients, are optional; an empty batch has zero
     gradients."""
