@@ -33,8 +33,10 @@
 // Backward: with xh and v recomputed from x, dv = dy act'(v) and, per channel,
 // sum dv and sum dv xh: these give dbeta and dgamma, and weighted by gamma and summed over
 // the group's channels the two sums that dx needs. A thread sees only few channels, whose
-// sums it keeps in registers; per-CTA (or, in the row kernels, per-team) partial sums go to
-// the workspace and a last launch adds them up.
+// sums it keeps in registers; partial sums (in the row kernels a row a CTA's teams, in the tile
+// kernels a row a run of samples and row of tiles) go to the workspace and a last launch adds
+// them up: 16 more bytes a value, divided by the rows that a row of sums stands for (at least 16
+// once there are many samples).
 #include <cooperative_groups.h>
 
 #include <climits>
@@ -714,7 +716,8 @@ struct Tiling {
   int rows;      // rows a tile
   int chunks;    // tiles one below the other
   int k;         // tiles that share statistics: split * chunks
-  int sets;      // sets of k tiles: batch * bundles
+  int run;       // samples whose tiles at one place a CTA takes one after the other
+  int units;     // the pieces of work that leaves: runs of a set's tiles (in a cluster) or of one
 };
 
 // How a tile kernel gets the statistics of a set of tiles: kInCluster, one cluster a set
@@ -734,6 +737,8 @@ struct Tile {
   int full, rest;   // rows = full * thread rows + rest
   int channel;      // this thread's first channel
   int64_t at;       // offset of this thread's first vector
+  int row;          // where the run's parameter sums go
+  bool begins, ends;  // the run
 };
 
 // The groups (counted from the tile's first) of a thread's vector: values before `from` belong
@@ -775,11 +780,13 @@ struct Place {
   }
 };
 
-// A CTA's walk over the tiles: (b, bundle, share) counted in mixed radix, since a division
-// a tile costs as much as a good part of its arithmetic. kWhole walks from the last tile.
-template <int V, int MODE, bool MIXED>
+// A CTA's walk over the tiles: (run of samples, bundle, share) counted in mixed radix, since a
+// division a tile costs as much as a good part of its arithmetic, and the samples of each run.
+// kWhole walks from the last tile. RUNS: runs may be of more than one sample; kernels for those are
+// apart ([1024, 64, 640] / 32, backward: 149 us with their walk and sums and runs of one, 140 so).
+template <int V, int MODE, bool MIXED, bool RUNS = false>
 struct Walk {
-  int b, bundle, share, db, dbundle, dshare, left;
+  int block, in_run, bundle, share, dblock, dbundle, dshare, left;  // left: units, this one included
   int tx, ty;       // thread column and row; past the last row: a row that no tile has
   int slice;        // its thread row's
   bool leaves;      // this thread leaves its column's share of its slice
@@ -788,14 +795,14 @@ struct Walk {
     const int k = MODE == kInCluster ? 1 : t.k;
     const int first = MODE == kInCluster ? (int)blockIdx.x / t.k : (int)blockIdx.x;
     const int step = MODE == kInCluster ? (int)gridDim.x / t.k : (int)gridDim.x;
-    const int units = t.sets * k;
-    left = first < units ? (units - 1 - first) / step + 1 : 0;
+    left = first < t.units ? (t.units - 1 - first) / step + 1 : 0;
     share = MODE == kInCluster ? rank : first % k;
     bundle = first / k % t.bundles;
-    b = first / k / t.bundles;
+    block = first / k / t.bundles;
+    in_run = 0;
     dshare = MODE == kInCluster ? 0 : step % k;
     dbundle = step / k % t.bundles;
-    db = step / k / t.bundles;
+    dblock = step / k / t.bundles;
     ty = (int)threadIdx.x / t.wide;
     tx = (int)threadIdx.x - ty * t.wide;
     slice = ty / t.each;
@@ -805,7 +812,11 @@ struct Walk {
   }
   // x / tall: exact, since x <= 32 tall and 32 tall^2 <= 2^21
   __device__ int over_tall(int x) const { return (int)((unsigned)x * invert >> 22); }
-  __device__ void advance(const Tiling &t) {
+  __device__ void advance(const Norm &a, const Tiling &t) {
+    if (RUNS) {
+      if (++in_run < t.run && block * t.run + in_run < (int)a.batch) return;
+      in_run = 0;
+    }
     --left;
     int carry = 0;
     if (MODE != kInCluster) {
@@ -816,15 +827,18 @@ struct Walk {
     bundle += dbundle + carry;
     carry = bundle >= t.bundles;
     bundle -= carry ? t.bundles : 0;
-    b += db + carry;
+    block += dblock + carry;
   }
   __device__ Tile<V> get(const Norm &a, const Tiling &t) const {
     Tile<V> r;
     const bool back = MODE == kWhole;
-    const int at = back ? t.bundles - 1 - bundle : bundle;
+    const int at = back ? t.bundles - 1 - bundle : bundle, b = RUNS ? block * t.run + in_run : block;
     r.b = back ? (int)a.batch - 1 - b : b;
+    r.begins = !RUNS || in_run == 0;
+    r.ends = !RUNS || in_run + 1 == t.run || b + 1 == (int)a.batch;
     r.k = back ? t.k - 1 - share : share;
     r.chunk = t.split > 1 ? r.k / t.split : r.k;
+    r.row = block * t.chunks + r.chunk;
     const int piece = r.k - r.chunk * t.split;
     r.g0 = at * t.q;
     r.q = min(t.q, a.groups - r.g0);
@@ -1074,7 +1088,7 @@ __global__ void __launch_bounds__(kTileThreads, kTileCtas + SHORT) norm_tile_ker
   for (int i = 0; walk.left; ++i) {
     const int n = i & 1;
     me = next;
-    walk.advance(t);
+    walk.advance(a, t);
     Vec<V> x[N];
     copy_wait<0>();
     take_tile(x, fifo, me, splat<V>(0.0f));
@@ -1152,9 +1166,20 @@ __global__ void __launch_bounds__(kTileThreads, kTileCtas + SHORT) norm_tile_ker
 // channels' sums in `part` and gives the gamma-weighted sums over the group to every lane.
 // Many channels a group, or many slices, are added up over the slices by all threads first.
 __device__ __forceinline__ bool together(const Norm &a, const Tiling &t) { return a.c > 32 || t.slices > 8; }
-template <int V, int MODE, bool MIXED>
-__device__ __forceinline__ void column_sums(Vec<V> db, Vec<V> dg, float *sh, const Norm &a, const Tile<V> &me,
-                                            const Tiling &t, const Walk<V, MODE, MIXED> &walk) {
+// A channel's sum over a tile of a run: added up in `run_sums` ([2][wide * V], each value the same
+// thread's in all of the run's tiles), it leaves for `part` at the run's end.
+template <int V>
+__device__ __forceinline__ void run_sum(float s, int which, int ch, float *run_sums, const Norm &a,
+                                        const Tile<V> &me, const Tiling &t, int tx) {
+  if (!a.part) return;
+  float *sum = run_sums + which * t.wide * V + ch;
+  if (!me.begins) s = __fadd_rn(*sum, s);
+  if (me.ends) a.part[((int64_t)me.row * 2 + which) * a.channels + (me.channel - tx * V + ch)] = s;
+  else *sum = s;
+}
+template <int V, int MODE, bool MIXED, bool RUNS>
+__device__ __forceinline__ void column_sums(Vec<V> db, Vec<V> dg, float *sh, float *run_sums, const Norm &a,
+                                            const Tile<V> &me, const Tiling &t, const Walk<V, MODE, MIXED, RUNS> &walk) {
   const int row = t.wide * V;
   for (int d = 16; d * t.each > 16; d >>= 1) {
 #pragma unroll
@@ -1177,23 +1202,26 @@ __device__ __forceinline__ void column_sums(Vec<V> db, Vec<V> dg, float *sh, con
       float s = q[0];
       for (int y = 1; y < slices; ++y) s = __fadd_rn(s, q[y * 2 * row]);
       q[0] = s;
+      if (RUNS) run_sum(s, which, ch, run_sums, a, me, t, walk.tx);
     }
     __syncthreads();
   }
 }
-template <int V>
-__device__ __forceinline__ float2 group_sums(const float *sh, int g, const Norm &a, const Tile<V> &me,
-                                             const Tiling &t, int tx) {
-  const int lane = threadIdx.x & 31, row = t.wide * V, slices = together(a, t) ? 1 : t.slices;
+template <int V, bool RUNS>
+__device__ __forceinline__ float2 group_sums(const float *sh, float *run_sums, int g, const Norm &a,
+                                             const Tile<V> &me, const Tiling &t, int tx) {
+  const bool whole = together(a, t);
+  const int lane = threadIdx.x & 31, row = t.wide * V, slices = whole ? 1 : t.slices;
   const int width = t.split > 1 ? me.cols * V : a.c, first = me.channel - tx * V + g * a.c;
-  float *part = a.part ? a.part + ((int64_t)me.b * t.chunks + me.chunk) * 2 * a.channels + first : nullptr;
+  float *part = !RUNS && a.part ? a.part + (int64_t)me.row * 2 * a.channels + first : nullptr;
   float u = 0.0f, w = 0.0f;
   for (int i = lane; i < 2 * width; i += 32) {
     const int which = i >= width, ch = i - (which ? width : 0);
     const float *q = sh + which * row + g * a.c + ch;
     float s = q[0];
     for (int y = 1; y < slices; ++y) s = __fadd_rn(s, q[y * 2 * row]);
-    if (part) part[which * a.channels + ch] = s;
+    if (RUNS && !whole) run_sum(s, which, g * a.c + ch, run_sums, a, me, t, tx);
+    if (!RUNS && part) part[which * a.channels + ch] = s;
     s = __fmul_rn(a.gamma ? a.gamma[first + ch] : 1.0f, s);
     if (which) w = __fadd_rn(w, s);
     else u = __fadd_rn(u, s);
@@ -1201,18 +1229,19 @@ __device__ __forceinline__ float2 group_sums(const float *sh, int g, const Norm 
   return make_float2(warp_sum(u), warp_sum(w));
 }
 
-template <int V, int MODE, bool MIXED, int SHORT>
+template <int V, int MODE, bool MIXED, int SHORT, bool RUNS>
 __global__ void __launch_bounds__(kTileThreads, kTileCtas + SHORT) norm_tile_backward_kernel(const Norm a, const Tiling t) {
   pdl_wait();
   constexpr int N = held(V, true) >> SHORT, kStage = N * kTileThreads * V;
   cg::cluster_group cluster = cg::this_cluster();
   extern __shared__ __align__(16) float fifo[];  // x and dy of one tile
   __shared__ __align__(16) float sh[2 * V * kTileThreads];
+  __shared__ float run_sums[RUNS ? 2 * V * kTileThreads : 1];
   __shared__ float2 means_by[2][kMaxTileGroups];
   __shared__ Exchange exchange;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const bool joined = MODE == kInCluster && t.k > 1;
-  Walk<V, MODE, MIXED> walk(t, MODE == kInCluster ? (int)cluster.block_rank() : 0);
+  Walk<V, MODE, MIXED, RUNS> walk(t, MODE == kInCluster ? (int)cluster.block_rank() : 0);
   if (joined) {
     exchange_init(exchange);
     __syncthreads();
@@ -1241,7 +1270,7 @@ __global__ void __launch_bounds__(kTileThreads, kTileCtas + SHORT) norm_tile_bac
     me = next;
     lo = next_lo;
     hi = next_hi;
-    walk.advance(t);
+    walk.advance(a, t);
     Vec<V> x[N], d[N], db = splat<V>(0.0f), dg = db;
     copy_wait<0>();
     // behind a thread's rows x is the mean and dy 0: xh is 0 there (a mean without x, times rstd,
@@ -1263,11 +1292,11 @@ __global__ void __launch_bounds__(kTileThreads, kTileCtas + SHORT) norm_tile_bac
       });
       if (!me.mine) db = dg = splat<V>(0.0f);  // no rows: the statistics were another group's
     }
-    if (MODE != kWhole) column_sums(db, dg, sh, a, me, t, walk);
+    if (MODE != kWhole) column_sums(db, dg, sh, run_sums, a, me, t, walk);
     if (joined) {
       if (threadIdx.x == kTileThreads - 1) exchange_expect(exchange, n, t.k * me.q * (int)sizeof(float2));
       for (int g = warp; g < me.q; g += kTileThreads / 32) {
-        const float2 m = group_sums(sh, g, a, me, t, walk.tx);
+        const float2 m = group_sums<V, RUNS>(sh, run_sums, g, a, me, t, walk.tx);
         if (lane < t.k) exchange_push(exchange, n, me.k, g, lane, m);
       }
       if (warp < me.q) exchange_wait(exchange, n, i >> 1 & 1, a.err);
@@ -1276,7 +1305,7 @@ __global__ void __launch_bounds__(kTileThreads, kTileCtas + SHORT) norm_tile_bac
     for (int g = warp; g < me.q; g += kTileThreads / 32) {
       const int64_t team = (int64_t)me.b * a.groups + me.g0 + g;
       float2 m = make_float2(0.0f, 0.0f);
-      if (MODE == kParts || (MODE == kInCluster && !joined)) m = group_sums(sh, g, a, me, t, walk.tx);
+      if (MODE == kParts || (MODE == kInCluster && !joined)) m = group_sums<V, RUNS>(sh, run_sums, g, a, me, t, walk.tx);
       if (MODE == kParts) {
         if (lane == 0) reinterpret_cast<float2 *>(a.stat)[team * t.k + me.k] = m;
         continue;
@@ -1478,12 +1507,11 @@ Plan norm_plan(int64_t batch, int64_t len, int64_t channels, int64_t groups, int
   t.each = 32 % t.wide == 0 ? 32 / t.wide : 1;
   t.slices = t.tall / t.each;
   t.bundles = (int)up(groups, t.q);
-  t.sets = (int)(batch * t.bundles);
   // Rows: as few tiles one below the other as hold the sample, or, where those would leave
   // SMs idle, as many as a cluster takes and that keep four rows a thread.
   const int64_t ty = t.tall, most = ty * held(v, backward);
   int64_t chunks = up(len, most);
-  const int64_t idle = up((int64_t)fz::num_sms() * kTileCtas, (int64_t)t.sets * t.split);
+  const int64_t idle = up((int64_t)fz::num_sms() * kTileCtas, batch * t.bundles * t.split);
   int64_t room = kMaxCluster / t.split;
   if (room > up(len, ty * 4)) room = up(len, ty * 4);
   if (room > idle) room = idle;
@@ -1494,8 +1522,19 @@ Plan norm_plan(int64_t batch, int64_t len, int64_t channels, int64_t groups, int
   t.k = (int)k;
   p.cluster = k <= kMaxCluster;
   while (p.shorter < kShortest && up(t.rows, t.tall) <= held(v, backward) >> (p.shorter + 1)) ++p.shorter;
+  // The backward leaves 2 floats a channel, row of tiles and run of samples: with runs of one, as
+  // much as x for tiles of two rows, and twice that for one. So a CTA takes the tiles of up to 16
+  // samples at one place in turn, until the sums are an eighth of x, as long as every CTA still has
+  // 16 such runs (a run more or less than the others' then costs little). [65536, 16384] in one
+  // group: 25.4 ms and 0.5 GB of sums with runs of 16, 36.6 ms and 8.6 GB with runs of one.
+  const int64_t ctas = (int64_t)fz::num_sms() * (kTileCtas + (p.cluster ? p.shorter : 0));
+  const auto units = [&](int64_t run) { return up(batch, run) * t.bundles * k; };  // in tiles
+  int64_t run = 1;
+  while (backward && t.rows * run < 16 && units(2 * run) >= 16 * ctas) run *= 2;
+  t.run = (int)run;
+  t.units = (int)(p.cluster ? units(run) / k : units(run));
   if (backward) {
-    p.parts = (int)(batch * t.chunks);
+    p.parts = (int)(up(batch, run) * t.chunks);
     p.part_floats = (size_t)p.parts * 2 * channels;
   }
   if (!p.cluster) p.stat_floats = (size_t)(teams * k * 2);
@@ -1603,14 +1642,17 @@ template <int V, int MODE, bool MIXED, int SHORT = 0>
 int run_tile(Norm a, const Plan &p, bool backward, cudaStream_t s) {
   if (MODE == kInCluster)
     if (int rc = fz::device_error_word(&a.err)) return rc;
-  const auto kernel = backward ? norm_tile_backward_kernel<V, MODE, MIXED, SHORT> : norm_tile_kernel<V, MODE, MIXED, SHORT>;
+  const auto kernel = !backward                          ? norm_tile_kernel<V, MODE, MIXED, SHORT>
+                      : MODE != kWhole && p.t.run > 1 ? norm_tile_backward_kernel<V, MODE, MIXED, SHORT, MODE != kWhole>
+                                                      : norm_tile_backward_kernel<V, MODE, MIXED, SHORT, false>;
   const int smem = (held(V, backward) >> SHORT) * kTileThreads * V * 4 * (backward ? 2 : 1);
   const int k = MODE == kInCluster ? p.t.k : 1;
   int resident = 0;
   if (int rc = resident_clusters((const void *)kernel, kTileThreads, smem, k, &resident)) return rc;
-  const int64_t units = (int64_t)p.t.sets * (MODE == kInCluster ? 1 : p.t.k);
-  const int64_t grid = (units < resident ? units : resident) * k;
-  return launch_cluster(kernel, (unsigned)grid, kTileThreads, smem, k, s, a, p.t);
+  Tiling t = p.t;
+  if (MODE == kWhole) t.run = 1, t.units = (int)(a.batch * t.bundles * t.k);
+  const int64_t grid = (int64_t)(t.units < resident ? t.units : resident) * k;
+  return launch_cluster(kernel, (unsigned)grid, kTileThreads, smem, k, s, a, t);
 }
 
 template <int V, bool MIXED>

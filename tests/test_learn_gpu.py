@@ -349,6 +349,66 @@ def test_group_norm_parameter_sums_keep_their_digits(capi, shape, parts, at_once
     torch.cuda.empty_cache()
 
 
+def test_group_norm_workspace_stays_below_the_input(capi):
+    """Samples of one row whose groups need several CTAs: the parameters' partial sums are an eighth
+    of x, not twice x, once there are many; beside them two launches leave 2 floats a tile."""
+    for shape in ((65536, 1, 16384, 1), (100000, 1, 4097, 1), (65536, 1, 131072, 8), (200000, 2, 5000, 1), (1000000, 1, 2100, 1)):
+        b, n, c, _ = shape
+        assert capi.group_norm_workspace(*shape, True) <= 4 * b * n * c * (1 / 8 + 1 / 64), shape
+
+
+# runs of samples at one place of a sample: clusters (vectors of 4 and single floats), two launches,
+# vectors across groups, several bundles; a last run that is shorter
+@pytest.mark.parametrize("shape,off", [((2503, 1, 8200, 1), 0), ((5003, 1, 2100, 1), 1), ((3001, 1, 20000, 1), 0),
+                                       ((40011, 5, 508, 4), 0), ((9001, 9, 516, 12), 0), ((6007, 1, 4097, 1), 0),
+                                       ((2000, 3, 5000, 1), 2)], ids=str)
+def test_group_norm_parameter_sums_of_many_samples(capi, shape, off):
+    """dbeta of small whole numbers is exact in every order of summation: no row is left out or counted
+    twice. dgamma within the roundings of a thread's rows (32), the tile's tree (8), a run (16), the
+    fold (56), and of xh (64)."""
+    torch = pytest.importorskip("torch")
+    L = capi.lib()
+    b, n, c, groups = shape
+    gen = torch.Generator("cuda").manual_seed(3)
+    flat = torch.empty(b * n * c + 4, device="cuda")
+    x = flat[off:off + b * n * c].view(b, n, c).normal_(generator=gen)
+    dy = torch.randint(-8, 9, (b, n, c), generator=gen, device="cuda").float()
+    y, dx = torch.empty_like(flat), torch.full((b * n * c + 8,), 7.0, device="cuda")
+    stats, gb = torch.empty(2, b, groups, device="cuda"), torch.empty(2, c, device="cuda")
+    size = capi.group_norm_workspace(b, n, c, groups, True)
+    work = torch.empty(size // 4 + 4, device="cuda")
+    work.fill_(float("nan"))
+    at = lambda t: t.data_ptr()  # noqa: E731
+    capi.check(L.fz_group_norm(at(y[off:]), at(stats[0]), at(stats[1]), at(x), None, None, b, n, c, groups, 1e-5, 0, at(work), size, 1))
+    work.fill_(float("nan"))
+    capi.check(L.fz_group_norm_backward(at(dx[off:]), at(gb[0]), at(gb[1]), at(dy), at(x), at(stats[0]), at(stats[1]), None, None, b, n,
+                                        c, groups, 0, at(work), size, 1))
+    torch.cuda.synchronize()
+    assert torch.equal(gb[1].double(), dy.double().sum((0, 1)))
+    total, size_of = torch.zeros(c, dtype=torch.float64, device="cuda"), torch.zeros(c, dtype=torch.float64, device="cuda")
+    for lo in range(0, b, 500):
+        part = x[lo:lo + 500].double()
+        grouped = part.view(-1, n, groups, c // groups)
+        var, mean = torch.var_mean(grouped, dim=(1, 3), keepdim=True, correction=0)
+        xh = ((grouped - mean) / torch.sqrt(var + 1e-5)).view(part.shape)
+        d = dy[lo:lo + 500].double()
+        total += (d * xh).sum((0, 1))
+        size_of += (d.abs() * (xh.abs() + 1)).sum((0, 1))
+        if lo == 0 or lo + 500 >= b:
+            a = d.view(grouped.shape)
+            h = xh.view(grouped.shape)
+            r = 1 / torch.sqrt(var + 1e-5)
+            want = r * (a - a.mean((1, 3), keepdim=True) - h * (a * h).mean((1, 3), keepdim=True))
+            got = dx[off + lo * n * c:off + (lo + part.shape[0]) * n * c].view(grouped.shape).double()
+            # sums of up to 32 rows, 8 levels and 16 tiles; values of at most 8
+            bound = 100 * U * r * (a.abs() + 8 * (1 + h.abs()))
+            assert ((got - want).abs() <= bound).all()
+    assert ((gb[0].double() - total).abs() <= (32 + 8 + 16 + 56 + 64) * U * size_of).all()
+    assert (dx[:off] == 7).all() and (dx[off + b * n * c:] == 7).all()
+    del flat, x, dy, y, dx, work
+    torch.cuda.empty_cache()
+
+
 def test_group_norm_partial_results(capi):
     """mean and rstd, and the parameters' gradients, are optional; an empty batch has zero
     gradients."""
