@@ -16,7 +16,7 @@
 //     and 214 -> 88 us, [64, 1024, 120] / 8 32 -> 21 and 55 -> 34 us, [16, 1369, 320] / 32
 //     21.5 -> 19 and 37 -> 32 us, [64, 4096, 256] / 128 140 -> 123 and 263 -> 208 us;
 //   * larger teams: the tile kernels in two launches that leave the statistics in the
-//     workspace and read x (and dy) twice; the second launch takes the tiles in reverse,
+//     workspace (of very many tiles, joined by a launch between them) and read x (and dy) twice; the second launch takes the tiles in reverse,
 //     so it finds the last of what the first read in L2. (Taking the batch a few samples at
 //     a time instead, so that all of it is found there, cost more in launches than it saved:
 //     [8, 16384, 512] 205 against 161 us.)
@@ -63,6 +63,11 @@ __host__ __device__ constexpr int held(int v, bool backward) { return (v == 4 ? 
 // with those for 8, 134 with those for 4; backward 178 with those for 8, 145 with those for 4.
 constexpr int kShortest = 2;
 constexpr int kMaxCluster = 16;
+// Tiles of a group whose statistics every tile of the second launch joins for itself; those of more
+// are joined once, by a launch between the two (one group of 32 channels: 131072 rows, 256 tiles,
+// 14.8 us without and 15.8 with it; 262144 rows, 24.5 and 23.9; 2^22 rows, 683 and 275; 2^24 rows,
+// 14.4 and 1.05 ms).
+constexpr int kMostTiles = 256;
 
 // ---------------------------------------------------------------- activations
 
@@ -348,6 +353,7 @@ struct Norm {
   float *dx;
   float *part;  // per-channel partial sums, or null: [part][2][...]
   float *stat;  // two-launch tiles: statistics of a group's tiles
+  float2 *whole;  // and, of many tiles, those of the group, or null
   int64_t batch, len, channels;
   int groups, c;  // c: channels a group
   float m, inv_m, eps;  // inv_m = 1 / m
@@ -856,11 +862,10 @@ struct Walk {
 };
 
 // Values of one group in tile `k` of a set.
-template <int V>
-__device__ __forceinline__ float count_of(const Norm &a, const Tiling &t, int k) {
+__device__ __forceinline__ float count_of(const Norm &a, const Tiling &t, int k, int v) {
   const int chunk = t.split > 1 ? k / t.split : k, piece = k - chunk * t.split;
   const float rows = (float)min((int64_t)t.rows, a.len - (int64_t)chunk * t.rows);
-  return rows * (float)(t.split > 1 ? min(t.cols, a.c / V - piece * t.cols) * V : a.c);
+  return rows * (float)(t.split > 1 ? min(t.cols, a.c / v - piece * t.cols) * v : a.c);
 }
 
 // The loops over a thread's rows end, four rows at a time, behind the tile's last, so that a
@@ -1077,7 +1082,7 @@ __global__ void __launch_bounds__(kTileThreads, kTileCtas + SHORT) norm_tile_ker
   }
   const int64_t step = (int64_t)t.tall * a.channels;
   const Place<V, MIXED> place(a, t, walk.tx);
-  const float share = joined && lane < t.k ? count_of<V>(a, t, lane) : 0.0f;
+  const float share = joined && lane < t.k ? count_of(a, t, lane, V) : 0.0f;
   Tile<V> me, next;
   if (walk.left) {
     next = walk.get(a, t);
@@ -1120,14 +1125,16 @@ __global__ void __launch_bounds__(kTileThreads, kTileCtas + SHORT) norm_tile_ker
       } else if (MODE == kInCluster) {
         r = group_moments<V, MIXED>(sh, g, a, me, t);
         r.y = rstd_of(r.y, a.inv_m, a.eps);
+      } else if (a.whole) {
+        r = a.whole[team];
       } else {
         const float2 *q = reinterpret_cast<const float2 *>(a.stat) + team * t.k;
         float u = 0.0f, w = 0.0f;
-        for (int i = lane; i < t.k; i += 32) u = __fmaf_rn(count_of<V>(a, t, i), q[i].x, u);
+        for (int i = lane; i < t.k; i += 32) u = __fmaf_rn(count_of(a, t, i, V), q[i].x, u);
         const float mean = __fdiv_rn(warp_sum(u), a.m);
         for (int i = lane; i < t.k; i += 32) {
           const float d = __fsub_rn(q[i].x, mean);
-          w = __fadd_rn(w, __fmaf_rn(__fmul_rn(d, d), count_of<V>(a, t, i), q[i].y));
+          w = __fadd_rn(w, __fmaf_rn(__fmul_rn(d, d), count_of(a, t, i, V), q[i].y));
         }
         r = make_float2(mean, rstd_of(warp_sum(w), a.inv_m, a.eps));
       }
@@ -1311,7 +1318,9 @@ __global__ void __launch_bounds__(kTileThreads, kTileCtas + SHORT) norm_tile_bac
         continue;
       }
       float u = m.x, w = m.y;
-      if (MODE == kWhole) {
+      if (MODE == kWhole && a.whole) {
+        if (lane == 0) u = a.whole[team].x, w = a.whole[team].y;
+      } else if (MODE == kWhole) {
         const float2 *q = reinterpret_cast<const float2 *>(a.stat) + team * t.k;
         for (int i = lane; i < t.k; i += 32) u = __fadd_rn(u, q[i].x), w = __fadd_rn(w, q[i].y);
       } else if (joined && lane < t.k) {
@@ -1338,6 +1347,51 @@ __global__ void __launch_bounds__(kTileThreads, kTileCtas + SHORT) norm_tile_bac
   }
   copy_wait<0>();
   if (joined) cluster.sync();
+}
+
+// ---------------------------------------------------------------- many tiles a group
+
+// Between the two launches: a group's k pairs, by a CTA, in place of every tile's joining all of
+// them, which is quadratic in k. (mean, rstd), or of the backward's sums their totals; in 64 bits,
+// since a thread may have thousands.
+constexpr int kJoinThreads = 512;
+__device__ __forceinline__ double join_sum(double v, double *sh) {
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(kFull, v, d);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = v;
+  __syncthreads();
+  v = sh[0];
+#pragma unroll
+  for (int w = 1; w < kJoinThreads / 32; ++w) v += sh[w];
+  return v;
+}
+template <bool BACKWARD>
+__global__ void __launch_bounds__(kJoinThreads) norm_join_kernel(const Norm a, const Tiling t, int v) {
+  pdl_wait();
+  __shared__ double sh[kJoinThreads / 32];
+  const int64_t team = blockIdx.x;
+  const float2 *q = reinterpret_cast<const float2 *>(a.stat) + team * t.k;
+  double u = 0.0, w = 0.0;
+#pragma unroll 4
+  for (int i = threadIdx.x; i < t.k; i += kJoinThreads) {
+    u += BACKWARD ? (double)q[i].x : (double)count_of(a, t, i, v) * q[i].x;
+    if (BACKWARD) w += q[i].y;
+  }
+  u = join_sum(u, sh);
+  if (BACKWARD) {
+    w = join_sum(w, sh);
+    if (threadIdx.x == 0) a.whole[team] = make_float2((float)u, (float)w);
+    return;
+  }
+  const double m = (double)a.len * a.c, mean = u / m;
+#pragma unroll 4
+  for (int i = threadIdx.x; i < t.k; i += kJoinThreads) {
+    const double d = q[i].x - mean;
+    w += d * d * count_of(a, t, i, v) + q[i].y;
+  }
+  w = join_sum(w, sh);
+  if (threadIdx.x == 0) a.whole[team] = make_float2((float)mean, (float)(1.0 / sqrt(w / m + a.eps)));
 }
 
 // ---------------------------------------------------------------- the parameters' gradients
@@ -1410,6 +1464,7 @@ struct Plan {
   unsigned grid;
   Tiling t;
   bool cluster;          // tile kernels: statistics within a cluster
+  bool join;             // two-launch tiles: statistics joined by a launch between them
   bool mixed;            // tile kernels: vectors of 4 across groups
   int shorter;           // tile kernels in a cluster: those for short tiles
   int parts;             // rows of the per-channel partial sums (backward)
@@ -1537,7 +1592,8 @@ Plan norm_plan(int64_t batch, int64_t len, int64_t channels, int64_t groups, int
     p.parts = (int)(up(batch, run) * t.chunks);
     p.part_floats = (size_t)p.parts * 2 * channels;
   }
-  if (!p.cluster) p.stat_floats = (size_t)(teams * k * 2);
+  p.join = !p.cluster && k > kMostTiles;
+  if (!p.cluster) p.stat_floats = (size_t)(teams * (k + p.join) * 2);
   return p;
 }
 
@@ -1656,12 +1712,19 @@ int run_tile(Norm a, const Plan &p, bool backward, cudaStream_t s) {
 }
 
 template <int V, bool MIXED>
-int run_tiles(const Norm &a, const Plan &p, bool backward, cudaStream_t s) {
+int run_tiles(Norm a, const Plan &p, bool backward, cudaStream_t s) {
   if (p.cluster)
     return p.shorter == 2   ? run_tile<V, kInCluster, MIXED, 2>(a, p, backward, s)
            : p.shorter == 1 ? run_tile<V, kInCluster, MIXED, 1>(a, p, backward, s)
                             : run_tile<V, kInCluster, MIXED>(a, p, backward, s);
   if (int rc = run_tile<V, kParts, MIXED>(a, p, backward, s)) return rc;
+  if (p.join) {
+    const int64_t teams = a.batch * a.groups;
+    a.whole = reinterpret_cast<float2 *>(a.stat) + teams * p.t.k;
+    if (int rc = launch_cluster(backward ? norm_join_kernel<true> : norm_join_kernel<false>, (unsigned)teams, kJoinThreads,
+                                0, 1, s, a, p.t, V))
+      return rc;
+  }
   return run_tile<V, kWhole, MIXED>(a, p, backward, s);
 }
 

@@ -409,6 +409,93 @@ def test_group_norm_parameter_sums_of_many_samples(capi, shape, off):
     torch.cuda.empty_cache()
 
 
+# more than 256 tiles a group: vectors of 4, across groups, single floats
+@pytest.mark.parametrize("shape,off", [((1, 1 << 20, 8, 2), 0), ((2, 500001, 12, 4), 0), ((1, 200003, 31, 1), 0), ((1, 400000, 32, 4), 1),
+                                       ((3, 300000, 32, 1), 0)], ids=str)
+def test_group_norm_of_long_samples(capi, shape, off):
+    """Bounds: sums of at most 32 rows, 8 levels and a tile's 16 columns in fp32 (the tiles' are joined in
+    64 bits), so D = 64 with what is rounded beside them; a common offset of 50 costs x's own digits."""
+    torch = pytest.importorskip("torch")
+    L = capi.lib()
+    b, n, c, groups = shape
+    gen = torch.Generator("cuda").manual_seed(5)
+    flat = torch.empty(b * n * c + 4, device="cuda")
+    x = flat[off:off + b * n * c].view(b, n, c).normal_(generator=gen)
+    x += 50
+    x[:, -1, -1] += 1000  # the last value of each sample counts
+    dy = torch.randint(-8, 9, (b, n, c), generator=gen, device="cuda").float()
+    y, dx = torch.empty_like(flat), torch.empty_like(flat)
+    stats, gb = torch.empty(2, b, groups, device="cuda"), torch.empty(2, c, device="cuda")
+    size = capi.group_norm_workspace(b, n, c, groups)
+    assert size > 8 * b * groups * 257  # a pair a tile and one of the group
+    size = capi.group_norm_workspace(b, n, c, groups, True)
+    work = torch.full((size // 4 + 4,), float("nan"), device="cuda")
+    at = lambda t: t.data_ptr()  # noqa: E731
+    capi.check(L.fz_group_norm(at(y[off:]), at(stats[0]), at(stats[1]), at(x), None, None, b, n, c, groups, 1e-5, 0, at(work), size, 1))
+    work.fill_(float("nan"))
+    capi.check(L.fz_group_norm_backward(at(dx[off:]), at(gb[0]), at(gb[1]), at(dy), at(x), at(stats[0]), at(stats[1]), None, None, b, n,
+                                        c, groups, 0, at(work), size, 1))
+    torch.cuda.synchronize()
+    g4 = lambda t: t.view(b, n, groups, c // groups).double()  # noqa: E731
+    X, A, Y, DX = g4(x), g4(dy), g4(y[off:off + b * n * c]), g4(dx[off:off + b * n * c])
+    E = lambda t: t.mean((1, 3), keepdim=True)  # noqa: E731
+    mean = E(X)
+    var = E((X - mean) ** 2)
+    rstd = 1 / torch.sqrt(var + 1e-5)
+    H = (X - mean) * rstd
+    D = 64 * U
+    e_mean = D * E(X.abs())
+    e_rstd = D + e_mean * rstd  # relative
+    assert ((stats[0].view_as(mean).double() - mean).abs() <= e_mean).all()
+    assert ((stats[1].view_as(mean).double() - rstd).abs() <= rstd * e_rstd).all()
+    e_h = rstd * e_mean + H.abs() * (e_rstd + 4 * U)
+    assert ((Y - H).abs() <= e_h).all()
+    k1, k2 = E(A), E(A * H)
+    e_k1, e_k2 = D * E(A.abs()), D * E((A * H).abs()) + E(A.abs() * e_h)
+    want = rstd * (A - k1 - H * k2)
+    size_of = A.abs() + k1.abs() + H.abs() * k2.abs()
+    assert ((DX - want).abs() <= rstd * (e_k1 + H.abs() * e_k2 + e_h * k2.abs() + size_of * (e_rstd + 6 * U))).all()
+    assert torch.equal(gb[1].double(), dy.double().sum((0, 1)))
+    e_g = (A.abs() * e_h + (A * H).abs() * (D + 56 * U)).sum((0, 1)).view(c)
+    assert ((gb[0].double() - (A * H).sum((0, 1)).view(c)).abs() <= e_g).all()
+    del flat, x, dy, y, dx, work, X, A, Y, DX, H
+    torch.cuda.empty_cache()
+
+
+def test_group_norm_of_a_long_sample_takes_no_longer(capi):
+    """One sample of 2^23 rows of 32 channels (up to 32768 tiles) against 16 of 2^19, the same bytes. Each
+    tile's joining all tiles' statistics took 6 times as long; 3 times is the most allowed here."""
+    torch = pytest.importorskip("torch")
+    L = capi.lib()
+    n = 1 << 28
+    x, y, dx = (torch.ones(n, device="cuda") for _ in range(3))
+    at = lambda t: t.data_ptr()  # noqa: E731
+    times = []
+    for b in (16, 1):
+        s = (b, n // 32 // b, 32, 1)
+        stats, gb = torch.empty(2, b, device="cuda"), torch.empty(2, 32, device="cuda")
+        size = capi.group_norm_workspace(*s, True)
+        work = torch.empty(size // 4 + 4, device="cuda")
+
+        def call():
+            capi.check(L.fz_group_norm(at(y), at(stats[0]), at(stats[1]), at(x), None, None, *s, 1e-5, 0, at(work), size, 1))
+            capi.check(L.fz_group_norm_backward(at(dx), at(gb[0]), at(gb[1]), at(x), at(x), at(stats[0]), at(stats[1]), None, None, *s, 0,
+                                                at(work), size, 1))
+
+        best = float("inf")
+        for i in range(4):
+            begin, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            begin.record()
+            call()
+            end.record()
+            torch.cuda.synchronize()
+            best = min(best, begin.elapsed_time(end)) if i else best
+        times.append(best)
+    del x, y, dx
+    torch.cuda.empty_cache()
+    assert times[1] <= 3 * times[0], times
+
+
 def test_group_norm_partial_results(capi):
     """mean and rstd, and the parameters' gradients, are optional; an empty batch has zero
     gradients."""
