@@ -1488,7 +1488,8 @@ int64_t columns_for(int64_t cols) {
   return wide <= 32 && kTileThreads / wide * 9 >= kTileThreads / cols * 8 ? wide : cols;
 }
 
-Plan norm_plan(int64_t batch, int64_t len, int64_t channels, int64_t groups, int v, bool backward) {
+// tiles: not the row kernels.
+Plan norm_plan(int64_t batch, int64_t len, int64_t channels, int64_t groups, int v, bool backward, bool tiles = false) {
   Plan p{};
   const int64_t c = channels / groups;
   int whole = v;  // floats a vector that stays in a group
@@ -1498,11 +1499,23 @@ Plan norm_plan(int64_t batch, int64_t len, int64_t channels, int64_t groups, int
   // Row kernels up to 2048 vectors; above 256 (a CTA's worth) only where a row's piece of
   // a group is at least 512 bytes, else the tile kernels, which take several groups' pieces
   // of a row together.
-  const bool rows = len * channels <= INT_MAX && (vectors <= 256 || (vectors <= 2048 && c >= 128));
+  const bool rows = !tiles && len * channels <= INT_MAX && (vectors <= 256 || (vectors <= 2048 && c >= 128));
   // Else tiles, of mixed vectors where others would be floats or pairs of them. (Tiles where row
   // kernels would do: [8192, 3, 680] / 4 forward 135 us against 31, [2048, 48, 40] / 4 20 against 12.)
   const int64_t unit = c % 2 ? 4 : 2;  // groups that make whole vectors
-  p.mixed = !rows && v == 4 && c % 4 && c >= 2 && channels % 4 == 0 && unit * c <= 4 * kTileThreads;
+  const bool can_mix = v == 4 && c % 4 && c >= 2 && channels % 4 == 0 && unit * c <= 4 * kTileThreads;
+  // But a backward whose row kernel holds 8 vectors of 1 or 2 floats a thread (one CTA an SM) takes
+  // mixed tiles that hold a sample's rows whole and enough values: of odd c, 1200 ([2941, 8, 1020]
+  // / 4, 138 us by rows, 95 so; [4096, 8, 1048] / 8, 275 and 171; of 960 values [25000, 48, 20] / 4, 132
+  // and 187); of even c, with 10 rows, 2400 ([1470, 24, 680] / 4, 105 and 83; of 1200 [20000, 30, 40] / 4,
+  // 107 and 147), or 1900 where a warp gets few groups ([2048, 48, 40] / 4, 26 and 21; [12500, 48, 40] / 4,
+  // 91 and 98).
+  if (rows && backward && can_mix && (vectors > 1024 || (vectors > 128 && vectors <= 256))) {
+    const Plan m = norm_plan(batch, len, channels, groups, v, true, true);
+    const int64_t values = m.t.q * c * len, few = (int64_t)fz::num_sms() * 8 * 16;
+    if (m.t.k == 1 && (c % 2 ? values >= 1200 : len >= 10 && values >= (teams <= few ? 1900 : 2400))) return m;
+  }
+  p.mixed = !rows && can_mix;
   if (!p.mixed) v = whole;
   cv = c / v, vectors = len * cv;
   p.v = v;

@@ -173,6 +173,14 @@ def test_group_norm_vectors_across_groups(capi, shape, act, affine, off):
     test_group_norm(capi, shape, act, affine, off)
 
 
+# a backward in vectors across groups after a forward by rows, beside sizes of the rows' own
+@pytest.mark.parametrize("shape", [(5, 8, 1048, 8), (3, 5, 1020, 4), (7, 8, 1020, 4), (6, 48, 40, 4), (4, 24, 680, 4), (5, 48, 40, 8),
+                                   (3, 11, 888, 4), (3, 9, 1048, 8), (3, 8, 2040, 4), (300, 48, 40, 4), (4, 80, 48, 8)], ids=str)
+@pytest.mark.parametrize("act,affine,off", [("silu", True, 0), ("gelu", True, 1), ("none", False, 0)])
+def test_group_norm_backward_in_other_tiles(capi, shape, act, affine, off):
+    test_group_norm(capi, shape, act, affine, off)
+
+
 # thread columns that are no power of two; groups in pieces; many tiles of a few rows
 @pytest.mark.parametrize("shape", [(2, 300, 300, 5), (3, 500, 150, 1), (2, 51, 271, 1), (1, 90, 1031, 1), (2, 40, 9000, 2),
                                    (1, 700, 777, 1), (3, 2000, 80, 4), (2, 12, 1100, 2), (1, 5000, 1036, 1), (40, 64, 640, 32),
