@@ -497,9 +497,11 @@ int check_distill(const char *who, int64_t rows, int64_t vocab, int64_t k, int64
 // entries cost more than the last wave's idle SMs once there are two CTAs an SM): while no more
 // than two an SM result; 8 rows of 131072, 7.9 us forward with 8 against 15.0 with one, 464
 // rows, 101 against 55. The backward's CTAs know nothing of one another, so it also splits
-// many rows of many columns, which shortens the last wave: 4096 rows of 131072, 662 us with 2
-// against 682 with one (with 4, 648, but 20 us more than with 2 right after the forward, of which
-// L2 then holds the last rows); 1024 of 50000, 77 with one, 89 with 4.
+// many rows into pieces of 40000 columns and more, which shortens the last wave. 4096 rows, alone
+// and with the forward before it (of which L2 then holds the last rows), us with 1, 2, 4 and 8 CTAs:
+// 50000 columns, 268 282 349 499 and 424 439 506 658; 80000, 421 403 462 622 and 636 620 680 853;
+// 131072, 685 663 671 843 and 1016 992 1012 1177; 165000, 883 855 832 979 and 1297 1267 1254 1401;
+// 1500 rows of 320000, 625 610 596 580 and 922 905 891 878. (Fewer rows in between differ by 2 %.)
 struct Team {
   int threads, ctas, slice;
 };
@@ -511,7 +513,7 @@ Team team_of(int64_t rows, int64_t vocab, int64_t k, bool backward) {
   if (t.threads == 512) {
     const int64_t least = backward ? 4096 : 8192;  // columns a CTA
     while (t.ctas < 8 && ((rows * t.ctas * 2 <= 2 * sms && vocab >= least * t.ctas * 2) ||
-                          (backward && rows > 2 * sms && vocab >= 65536 * (int64_t)t.ctas * 2) ||
+                          (backward && rows > 2 * sms && vocab >= 40000 * (int64_t)t.ctas * 2) ||
                           vocab > ((int64_t)t.ctas << 20)))  // a slice's marks have to fit in shared memory
       t.ctas *= 2;
   }

@@ -917,6 +917,46 @@ def test_distill_many_rows(capi, r, v, k, tau, off, pitch, tail):
     test_distill(capi, r, v, k, tau, off, pitch, tail)
 
 
+# rows whose backward is cut into 1, 2, 4 and 8 pieces
+@pytest.mark.parametrize("r,v,k,tau,off,pitch", [(300, 79999, 9, 1.0, 1, 0), (300, 80000, 9, 1.0, 0, 0), (300, 160001, 5, 2.0, 3, 2),
+                                                 (297, 320003, 40, 1.0, 1, 1)])
+def test_distill_pieces_of_many_rows(capi, r, v, k, tau, off, pitch):
+    """Every 40th row against 64 bits; the columns behind a row stay as they were."""
+    torch = pytest.importorskip("torch")
+    L = capi.lib()
+    gen = torch.Generator("cuda").manual_seed(9)
+    ld, at = v + pitch, lambda t: t.data_ptr()  # noqa: E731
+    flat = torch.randn(r * ld + off, generator=gen, device="cuda") * 2
+    z = flat[off:].view(r, ld)
+    ids = torch.stack([torch.randperm(v, generator=gen, device="cuda")[:k] for _ in range(r)]).to(torch.int32)
+    ids[:, 0] = v - 1
+    t = torch.randn(r, k, generator=gen, device="cuda")
+    lse = (t / tau).logsumexp(1) + 0.4
+    loss, stats, one = torch.empty(r, device="cuda"), torch.empty(r, 4, device="cuda"), torch.ones(r, device="cuda")
+    out = torch.full((r * ld + off,), 7.0, device="cuda")
+    dz = out[off:].view(r, ld)
+    capi.check(L.fz_distill(at(loss), at(stats), at(z), ld, at(ids), at(t), at(lse), r, v, k, tau, 1))
+    capi.check(L.fz_distill_backward(at(dz), ld, at(one), at(stats), at(z), ld, at(ids), at(t), at(lse), r, v, k, tau, 1))
+    torch.cuda.synchronize()
+    for i in range(0, r, 40):
+        q = torch.log_softmax(z[i, :v].double() / tau, 0)
+        p = torch.exp(t[i].double() / tau - lse[i].double())
+        rest = 1 - p.sum()
+        inside = torch.zeros(v, dtype=torch.bool, device="cuda")
+        inside[ids[i].long()] = True
+        tail = torch.logsumexp(q.masked_fill(inside, -torch.inf), 0)
+        want = torch.where(inside, q.exp(), q.exp() * (1 - rest / tail.exp()))
+        want[ids[i].long()] -= p
+        # exp's argument (up to 20, twice rounded), a sum of up to v / 512 additions a thread, p and its rest
+        bound = U * (4 * 20 + 3 * v / 512 + 100) * (want.abs() + q.exp() + p.sum() * inside)
+        assert ((dz[i, :v].double() - want * tau).abs() <= tau * bound).all()
+    if pitch:
+        assert (dz[:, v:] == 7).all()
+    assert (out[:off] == 7).all()
+    del flat, out
+    torch.cuda.empty_cache()
+
+
 @pytest.mark.parametrize("r,v,k", [(1200, 300, 40), (1200, 300, 256), (450, 5000, 40), (9, 40000, 1000), (1, 20000, 1024)])
 @pytest.mark.parametrize("tail", [False, True])
 def test_distill_repeated_ids_of_each_team(capi, r, v, k, tail):
