@@ -357,6 +357,41 @@ def test_group_norm_parameter_sums_keep_their_digits(capi, shape, parts, at_once
     torch.cuda.empty_cache()
 
 
+SPIKE_SHAPES = [(65, 1, 100, 1), (4, 1, 4096, 32), (2, 4096, 64, 8), (1, 16384, 8, 2), (1, 65536, 32, 1), (1, 30011, 16, 4),
+                (1, 40000, 28, 4), (1, 9000, 40, 8), (1, 20000, 140, 4), (1, 5000, 1036, 1), (2, 1024, 256, 32), (1, 2, 40000, 1),
+                (700, 7, 148, 2), (1, 181, 260, 4), (1, 961, 260, 4), (5, 7, 2368, 32), (3, 257, 68, 17), (2, 40, 9000, 2),
+                (1, 300001, 32, 1), (300, 2, 2048, 1), (5, 8, 1048, 8)]
+
+
+@pytest.mark.parametrize("shape", SPIKE_SHAPES, ids=str)
+@pytest.mark.parametrize("off", [0, 1])
+@pytest.mark.parametrize("where", ["first", "last", "inside"])
+def test_group_norm_counts_each_value_once(capi, shape, off, where):
+    """One value other than 0: it alone makes mean and rstd, which show it left out, counted twice or
+    counted for another group. dy of small whole numbers: dbeta is exact. (The sums' zeros are exact, so
+    the bounds are a few dozen roundings of divisions and joins, whatever the length.)"""
+    b, n, c, groups = shape
+    per, m = c // groups, n * c // groups
+    rng = np.random.default_rng(b + n + c)
+    at = {"first": (0, 0, 0), "last": (b - 1, n - 1, c - 1), "inside": tuple(int(rng.integers(s)) for s in (b, n, c))}[where]
+    x = np.zeros((b, n, c), np.float32)
+    x[at] = 1000.0
+    dy = rng.integers(-8, 9, (b, n, c)).astype(np.float32)
+    eps = 2.0 ** -20
+    y, mean, rstd, dx, dg, db = run_norm(capi, x, None, None, groups, eps, "none", dy, off)
+    want_mean, want_rstd = np.zeros((b, groups)), np.full((b, groups), 1 / np.sqrt(eps))
+    want_mean[at[0], at[2] // per] = 1000.0 / m
+    var = 1e6 / m * (1 - 1 / m)
+    want_rstd[at[0], at[2] // per] = 1 / np.sqrt(var + eps)
+    close(mean, want_mean, 64 * U * np.abs(want_mean), "mean")
+    close(rstd, want_rstd, 64 * U * want_rstd, "rstd")
+    np.testing.assert_array_equal(db, dy.sum(axis=(0, 1), dtype=np.float64))
+    xh = (x - np.repeat(want_mean, per, axis=1)[:, None]) * np.repeat(want_rstd, per, axis=1)[:, None]
+    # xh = s (x - mean) of a group of zeros and one 1000: the roundings of mean and rstd (64 each), and
+    # sums of equal magnitudes: at most 32 rows, 16 levels, a run of 16 and the fold's 56
+    close(dg, (dy * xh).sum(axis=(0, 1)), (2 * 64 + 4 + 32 + 16 + 16 + 56) * U * (np.abs(dy * xh)).sum(axis=(0, 1)), "dgamma")
+
+
 def test_group_norm_workspace_stays_below_the_input(capi):
     """Samples of one row whose groups need several CTAs: the parameters' partial sums are an eighth
     of x, not twice x, once there are many; beside them two launches leave 2 floats a tile."""
@@ -1316,6 +1351,72 @@ def test_norm_and_distill_past_32_bit_offsets(capi):
     assert torch.allclose(dz[-600:], dz_few, rtol=1e-4, atol=1e-9)
     del z, dz, dz_few
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("shape", [(530000, 1, 4096, 32), (36, 250000, 256, 8), (131073, 1, 16400, 2)], ids=str)
+def test_norm_parameter_sums_past_32_bit_offsets(capi, shape):
+    """More than 2^31 values: dbeta of ones is the number of rows, exactly; dgamma against 64 bits, within
+    xh's roundings (sums of at most 32 rows, 16 levels and 16 joins, and its own) and the sum's
+    (16 steps a block, at most 128 blocks, the fold's 56)."""
+    torch = pytest.importorskip("torch")
+    L = capi.lib()
+    b, n, c, g = shape
+    at = lambda t: t.data_ptr()  # noqa: E731
+    x = torch.randn(b, n, c, generator=torch.Generator("cuda").manual_seed(4), device="cuda")
+    dy, y = torch.ones_like(x), torch.empty_like(x)
+    stats, gb = torch.empty(2, b, g, device="cuda"), torch.empty(2, c, device="cuda")
+    size = capi.group_norm_workspace(b, n, c, g, True)
+    work = torch.empty(size // 4 + 4, device="cuda")
+    capi.check(L.fz_group_norm(at(y), at(stats[0]), at(stats[1]), at(x), None, None, b, n, c, g, 1e-5, 0, at(work), size, 1))
+    # dx goes where y was
+    capi.check(L.fz_group_norm_backward(at(y), at(gb[0]), at(gb[1]), at(dy), at(x), at(stats[0]), at(stats[1]), None, None, b, n, c, g, 0,
+                                        at(work), size, 1))
+    torch.cuda.synchronize()
+    assert (gb[1] == b * n).all()
+    del dy, y, work
+    torch.cuda.empty_cache()
+    total, size_of = torch.zeros(c, dtype=torch.float64, device="cuda"), torch.zeros(c, dtype=torch.float64, device="cuda")
+    step = max(1, (1 << 27) // (n * c))
+    for lo in range(0, b, step):
+        part = x[lo:lo + step].double().view(-1, n, g, c // g)
+        var, mean = torch.var_mean(part, dim=(1, 3), keepdim=True, correction=0)
+        xh = (part - mean) / torch.sqrt(var + 1e-5)
+        total += xh.sum((0, 1)).view(c)
+        size_of += xh.abs().sum((0, 1)).view(c)
+    rows = b * n
+    bound = (64 + 64 + 16 + 128 + 56) * U * (size_of + rows)  # rows: xh's error from the mean's
+    assert ((gb[0].double() - total).abs() <= bound).all()
+    del x
+    torch.cuda.empty_cache()
+
+
+def test_norms_from_two_threads(capi):
+    """Two host threads, each on its own stream, whose first calls of several of the norm's kernels meet
+    in the table of resident clusters."""
+    import threading
+
+    rng = np.random.default_rng(32)
+    jobs = [[(rng.standard_normal(s[:3]).astype(np.float32), s[3]) for s in shapes] for shapes in
+            ([(3, 1100, 36, 3), (2, 333, 72, 6), (1, 9001, 52, 4), (4, 77, 1000, 1), (2, 2, 9000, 1)],
+             [(2, 2, 9004, 1), (4, 79, 1000, 1), (1, 9003, 52, 4), (2, 331, 72, 6), (3, 1102, 36, 3)])]
+    got, errors = [[], []], []
+
+    def work(q):
+        try:
+            capi.check(capi.lib().fz_set_device(0))
+            for _ in range(5):
+                got[q] = [run_norm(capi, x, None, None, g, 1e-5, "silu", x) for x, g in jobs[q]]
+        except Exception as err:  # pragma: no cover
+            errors.append(err)
+
+    threads = [threading.Thread(target=work, args=(q,)) for q in range(2)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    assert not errors
+    for q in range(2):
+        for (x, g), res in zip(jobs[q], got[q]):
+            for a, e in zip(res, run_norm(capi, x, None, None, g, 1e-5, "silu", x)):
+                np.testing.assert_array_equal(a, e)
 
 
 def test_calls_from_two_threads(capi):
