@@ -42,7 +42,11 @@ __device__ __forceinline__ float warp_sum(float v) {
   return v;
 }
 
-__device__ __forceinline__ float exp_below(float v, float top) {  // e^(v - top)
+// e^(v - top), at most 1: the hardware's 2^x (2 ulp) of (v - top) log2(e). With d = top - v that
+// argument's roundings make the relative error up to 2^-24 (4 + 2.2 d): small weights have fewer
+// digits, in proportion to their logarithm. (expf would hold 2 ulp for all; its instructions would
+// add to what the forward is bound by.)
+__device__ __forceinline__ float exp_below(float v, float top) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(__fmul_rn(__fsub_rn(v, top), 1.4426950408889634f)));
   return y;
@@ -486,8 +490,7 @@ __global__ void __launch_bounds__(1024) sort_kernel(int32_t *__restrict__ slot, 
 // most 32 or 8 vectors, so that narrow rows do not leave a warp's lanes idle (32768 tokens of
 // 16 floats, 8 choices: combine 32 us with a warp a token, 11 us so). VEC = 4: rows of float4
 // (width a multiple of 4, 16-byte aligned buffers), else 1. Every value is read or written
-// once: the token's row once for its k copies, each expert's row once; the next choice's
-// row number is fetched ahead.
+// once: the token's row once for its k copies, each expert's row once.
 constexpr int kUnroll = 4;
 
 template <int VEC>

@@ -16,16 +16,20 @@
 //     and 214 -> 88 us, [64, 1024, 120] / 8 32 -> 21 and 55 -> 34 us, [16, 1369, 320] / 32
 //     21.5 -> 19 and 37 -> 32 us, [64, 4096, 256] / 128 140 -> 123 and 263 -> 208 us;
 //   * larger teams: the tile kernels in two launches that leave the statistics in the
-//     workspace (of very many tiles, joined by a launch between them) and read x (and dy) twice; the second launch takes the tiles in reverse,
-//     so it finds the last of what the first read in L2. (Taking the batch a few samples at
-//     a time instead, so that all of it is found there, cost more in launches than it saved:
-//     [8, 16384, 512] 205 against 161 us.)
+//     workspace (of very many tiles, joined by a launch between them) and read x (and dy)
+//     twice; the second launch takes the tiles in reverse, so it finds the last of what the
+//     first read in L2. (Taking the batch a few samples at a time instead, so that all of it
+//     is found there, cost more in launches than it saved: [8, 16384, 512] 205 against 161 us.)
 // Measured (B200, copy bandwidth 6.55 TB/s): rows, [65536, 4096] in 32 groups, GELU: forward
 // 378 us, backward 563 us (0.87 of the copy bandwidth both). Clusters, [64, 4096, 256] in 32
 // groups, SiLU: forward 98 us (0.84), backward 198 us (0.62: the tiles of x and dy fill the
 // registers, and a cluster's CTAs wait for one another). Two launches, [8, 16384, 512]: 152
-// and 258 us. A first version with one CTA a team, reading x three times: 566 us for the
+// and 257 us. A first version with one CTA a team, reading x three times: 566 us for the
 // maps' forward, 16.6 ms for the rows' two passes.
+// Far from that: short samples, whose tiles are small ([1990, 7, 2368] / 32: 263 and 254 us, 6.5
+// and 4.2 times what their bytes take), above all one row of a group of more than 2048 vectors
+// ([8192, 16384] in one group 1.20 and 3.21 ms, 7 and 13 times; [20000, 4097] 5.0 ms both ways, 50
+// and 33 times), and widths that no vector divides (2 to 5 times).
 // Statistics: the mean, then the sum of squares about it, so that a common offset of x
 // does not cancel; parts are joined as (n, mean, M2) (Chan, Golub and LeVeque). Everything
 // is summed in a fixed order.
@@ -71,6 +75,13 @@ constexpr int kMostTiles = 256;
 
 // ---------------------------------------------------------------- activations
 
+// They use the hardware's 2^x and reciprocal (2 and 1 ulp) without correcting the argument's
+// rounding, and for Phi a polynomial (1.5e-7), because the row kernels issue instructions on 60 % of
+// cycles with these alone. Measured against 64 bits, for standard normal v, norm-wise (and with CUDA's
+// expf, erfcf and IEEE division in their place): SiLU 4.8e-8 (4.0e-8), its slope 4.9e-8 (4.9e-8), GELU
+// 4.4e-8 (3.5e-8), its slope 7.3e-8 (4.6e-8). Far out on the negative side, where the results vanish,
+// the exponent's rounding shows: SiLU is off by 9e-7 of itself at -12 (1.9e-7), GELU by 1.5e-6 at -5
+// (1.5e-6).
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
