@@ -417,8 +417,8 @@ int fz_group_norm_backward(float *dx, float *dgamma, float *dbeta, const float *
                            void *stream);
 /* Bytes of workspace that fz_group_norm (backward = 0) or fz_group_norm_backward (1) needs
  * on the current device for these sizes (0: none). A backward's holds partial sums of the
- * parameters' gradients: at most an eighth of x, 160 MB or 2 floats a channel, whichever is
- * most. Samples that take two launches add 2 floats for each of their tiles (of thousands of
+ * parameters' gradients: at most two thirds of x (an eighth where a group has more than
+ * 512 channels), 160 MB or 2 floats a channel, whichever is most. Samples that take two launches add 2 floats for each of their tiles (of thousands of
  * values). */
 int fz_group_norm_workspace(int64_t batch, int64_t len, int64_t channels, int64_t groups,
                             int backward, size_t *bytes);

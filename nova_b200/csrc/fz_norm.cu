@@ -39,8 +39,8 @@
 // the group's channels the two sums that dx needs. A thread sees only few channels, whose
 // sums it keeps in registers; partial sums (in the row kernels a row a CTA's teams, in the tile
 // kernels a row a run of samples and row of tiles) go to the workspace and a last launch adds
-// them up: 16 more bytes a value, divided by the rows that a row of sums stands for (at least 16
-// once there are many samples).
+// them up: 16 more bytes a value, divided by the rows that a row of sums stands for (three or
+// more, and at least 16 for wide groups, once there are many samples).
 #include <cooperative_groups.h>
 
 #include <climits>
@@ -1605,11 +1605,14 @@ Plan norm_plan(int64_t batch, int64_t len, int64_t channels, int64_t groups, int
   // much as x for tiles of two rows, and twice that for one. So a CTA takes the tiles of up to 16
   // samples at one place in turn, until the sums are an eighth of x, as long as every CTA still has
   // 16 such runs (a run more or less than the others' then costs little). [65536, 16384] in one
-  // group: 25.4 ms and 0.5 GB of sums with runs of 16, 36.6 ms and 8.6 GB with runs of one.
+  // group: 25.4 ms and 0.5 GB of sums with runs of 16, 36.6 ms and 8.6 GB with runs of one;
+  // [4000, 9, 4096] / 4, 954 and 1545 us. Narrow groups' tiles have three rows and more, and runs
+  // cost them more than they save: [20000, 11, 400] / 4, 576 and 544 us, [1990, 7, 2368] / 32 (mixed)
+  // 295 and 248.
   const int64_t ctas = (int64_t)fz::num_sms() * (kTileCtas + (p.cluster ? p.shorter : 0));
   const auto units = [&](int64_t run) { return up(batch, run) * t.bundles * k; };  // in tiles
   int64_t run = 1;
-  while (backward && t.rows * run < 16 && units(2 * run) >= 16 * ctas) run *= 2;
+  while (backward && !p.mixed && c >= 128 && t.rows * run < 16 && units(2 * run) >= 16 * ctas) run *= 2;
   t.run = (int)run;
   t.units = (int)(p.cluster ? units(run) / k : units(run));
   if (backward) {
@@ -1722,9 +1725,10 @@ template <int V, int MODE, bool MIXED, int SHORT = 0>
 int run_tile(Norm a, const Plan &p, bool backward, cudaStream_t s) {
   if (MODE == kInCluster)
     if (int rc = fz::device_error_word(&a.err)) return rc;
-  const auto kernel = !backward                          ? norm_tile_kernel<V, MODE, MIXED, SHORT>
-                      : MODE != kWhole && p.t.run > 1 ? norm_tile_backward_kernel<V, MODE, MIXED, SHORT, MODE != kWhole>
-                                                      : norm_tile_backward_kernel<V, MODE, MIXED, SHORT, false>;
+  constexpr bool kRuns = MODE != kWhole && !MIXED;
+  const auto kernel = !backward                ? norm_tile_kernel<V, MODE, MIXED, SHORT>
+                      : kRuns && p.t.run > 1 ? norm_tile_backward_kernel<V, MODE, MIXED, SHORT, kRuns>
+                                             : norm_tile_backward_kernel<V, MODE, MIXED, SHORT, false>;
   const int smem = (held(V, backward) >> SHORT) * kTileThreads * V * 4 * (backward ? 2 : 1);
   const int k = MODE == kInCluster ? p.t.k : 1;
   int resident = 0;

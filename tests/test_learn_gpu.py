@@ -394,10 +394,15 @@ def test_group_norm_counts_each_value_once(capi, shape, off, where):
 
 def test_group_norm_workspace_stays_below_the_input(capi):
     """Samples of one row whose groups need several CTAs: the parameters' partial sums are an eighth
-    of x, not twice x, once there are many; beside them two launches leave 2 floats a tile."""
+    of x, not twice x, once there are many; beside them two launches leave 2 floats a tile. Narrow
+    groups: two thirds at most."""
     for shape in ((65536, 1, 16384, 1), (100000, 1, 4097, 1), (65536, 1, 131072, 8), (200000, 2, 5000, 1), (1000000, 1, 2100, 1)):
         b, n, c, _ = shape
         assert capi.group_norm_workspace(*shape, True) <= 4 * b * n * c * (1 / 8 + 1 / 64), shape
+    for shape in ((100000, 3, 508, 4), (100000, 5, 504, 4), (50000, 11, 400, 4), (30000, 3, 2368, 32), (70000, 5, 1020, 4),
+                  (400000, 2, 255, 1), (300000, 3, 127, 1)):
+        b, n, c, _ = shape
+        assert capi.group_norm_workspace(*shape, True) <= 4 * b * n * c * 2 / 3, shape
 
 
 # runs of samples at one place of a sample: clusters (vectors of 4 and single floats), two launches,
