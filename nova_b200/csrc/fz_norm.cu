@@ -26,10 +26,10 @@
 // registers, and a cluster's CTAs wait for one another). Two launches, [8, 16384, 512]: 152
 // and 257 us. A first version with one CTA a team, reading x three times: 566 us for the
 // maps' forward, 16.6 ms for the rows' two passes.
-// Far from that: short samples, whose tiles are small ([1990, 7, 2368] / 32: 263 and 254 us, 6.5
+// Far from that: short samples, whose tiles are small ([1990, 7, 2368] / 32: 264 and 252 us, 6.6
 // and 4.2 times what their bytes take), above all one row of a group of more than 2048 vectors
-// ([8192, 16384] in one group 1.20 and 3.21 ms, 7 and 13 times; [20000, 4097] 5.0 ms both ways, 50
-// and 33 times), and widths that no vector divides (2 to 5 times).
+// ([8192, 16384] in one group 1.23 and 3.22 ms, 7.5 and 13 times; [20000, 4097] 5.05 ms both ways,
+// 50 and 34 times), and widths that no vector divides (2.5 to 4 times).
 // Statistics: the mean, then the sum of squares about it, so that a common offset of x
 // does not cancel; parts are joined as (n, mean, M2) (Chan, Golub and LeVeque). Everything
 // is summed in a fixed order.
