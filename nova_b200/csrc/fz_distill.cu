@@ -119,7 +119,7 @@ struct Teacher {
   // none, or all are masked), pT (log pT - log qT) would turn a rounding of pT into an infinite
   // loss: a pT that is no larger than its rounding is 0 there.
   __device__ __forceinline__ void settle(float log_q_tail) {
-    if (log_q_tail < -87.0f && tail <= slack) tail = 0.0f;  // below 2^-126 or so
+    if (log_q_tail < -87.336545f && tail <= slack) tail = 0.0f;  // log 2^-126
   }
 };
 // log qT from the maximum and log sum of all logits and of those outside the entries
